@@ -46,7 +46,9 @@ typedef enum {
     NNVB_LAYER_FC = 2,       /* code/nnv/engine/nn/layers/FullyConnectedLayer.m */
     NNVB_LAYER_BN = 3,       /* code/nnv/engine/nn/layers/BatchNormalizationLayer.m */
     NNVB_LAYER_AVGPOOL2D = 4,/* code/nnv/engine/nn/layers/AveragePooling2DLayer.m */
-    NNVB_LAYER_RELU = 5      /* code/nnv/engine/nn/layers/ReluLayer.m */
+    NNVB_LAYER_RELU = 5,     /* code/nnv/engine/nn/layers/ReluLayer.m */
+    NNVB_LAYER_LAYERNORM = 6,/* layerNormalizationLayer; concrete evaluation only */
+    NNVB_LAYER_ATTENTION = 7 /* attentionLayer over fixed states; concrete evaluation only */
 } nnvb_layer_type;
 
 /* One layer.  Parameter layouts are the reference's own:
@@ -66,6 +68,18 @@ typedef enum {
  *            NNVB_POOL_DIV_INSIDE (1) = entries inside the image.  Without
  *            padding the two agree.
  *   RELU     no parameters
+ *   LAYERNORM  bn_scale, bn_offset [cout] (either may be NULL), bn_eps.  The
+ *            input is a sequence [cout, T, 1] (one column of cout channels per
+ *            position) or a vector of cout entries; every column is normalised
+ *            over its channels.
+ *   ATTENTION  the input is a sequence [kh*cin, T, 1] (or a vector: one position)
+ *            of queries, kh heads of cin channels; W holds the keys and b the
+ *            values of cout fixed states, each [cin, kw, cout] column-major (kw
+ *            state heads; kh must be a multiple of kw, query head h reads state
+ *            head h / (kh/kw)); bn_eps is the factor on the scores, 0 for
+ *            1/sqrt(cin).  Output: the attended values, shaped like the input.
+ * LAYERNORM and ATTENTION exist for nnvb_net_evaluate: they have no approx-star
+ * reach here, and nnvb_batch_create refuses a network that holds one.
  * Unused fields are ignored. */
 #define NNVB_POOL_DIV_WINDOW 0
 #define NNVB_POOL_DIV_INSIDE 1
@@ -413,6 +427,72 @@ int nnvb_estimate_ranges(nnvb_ctx* ctx, int64_t N, int64_t P, const double* V,
 #define NNVB_NOALLOC_SCRATCH_DOUBLES 524288
 int nnvb_estimate_ranges_noalloc(void* stream, int64_t N, int64_t P, const double* V_dev, int64_t ld,
                                  const double* pl_dev, const double* pu_dev, double* lb_dev, double* ub_dev);
+
+/* ---- operators of transformer networks on device tensors -------------------- */
+
+/* The layers of NNVB_LAYER_LAYERNORM / NNVB_LAYER_ATTENTION and their gradients on
+ * the caller's device memory, for hosts that keep activations on the GPU.  As
+ * with nnvb_estimate_ranges_noalloc every pointer is a DEVICE pointer on the
+ * current device, nothing is allocated, and the call returns after enqueueing its
+ * kernels on `stream` (a cudaStream_t; NULL = default stream).  The calls keep no
+ * state: any number may run at once on any streams, and they can be captured
+ * into CUDA graphs; a workspace belongs to one call until that call has run.
+ * Tensors must be aligned to their element type; 16-byte aligned rows are read
+ * with wide accesses.  Inputs and outputs must not overlap.
+ *
+ * `dtype` is the element type of every tensor of a call except the statistics
+ * (mean, rstd, lse), which are float for the 16- and 32-bit types and double for
+ * NNVB_F64.  Sums are held in the type of the statistics; a result is rounded
+ * once when it is stored. */
+typedef enum { NNVB_F64 = 0, NNVB_F32 = 1, NNVB_BF16 = 2, NNVB_F16 = 3 } nnvb_dtype;
+
+/* y = (x - mean) * rstd * scale + offset for each of `rows` rows of `cols`
+ * contiguous elements; mean over the row, rstd = 1/sqrt(mean((x - mean)^2) + eps).
+ * ldx, ldy >= cols: elements from row to row.  scale, offset [cols] may be NULL
+ * (1 and 0); mean, rstd [rows] receive the statistics unless NULL. */
+int nnvb_layer_norm_forward(void* stream, int dtype, int64_t rows, int64_t cols, const void* x, int64_t ldx,
+                            const void* scale, const void* offset, double eps, void* y, int64_t ldy, void* mean,
+                            void* rstd);
+/* Gradients of the same: dx [rows, cols], dscale and doffset [cols] (each may be
+ * NULL).  mean, rstd are the forward call's.  With dscale or doffset the call needs
+ * nnvb_layer_norm_workspace bytes of 16-byte aligned workspace; its contents need
+ * no preparation.  The sums over rows are added in a fixed order. */
+int64_t nnvb_layer_norm_workspace(int dtype, int64_t rows, int64_t cols);
+int nnvb_layer_norm_backward(void* stream, int dtype, int64_t rows, int64_t cols, const void* dy, int64_t lddy,
+                             const void* x, int64_t ldx, const void* scale, const void* mean, const void* rstd, void* dx,
+                             int64_t lddx, void* dscale, void* doffset, void* workspace, int64_t workspace_bytes);
+
+/* Attention of q_len positions over kv_len states (an encoder's output): for batch
+ * entry b and query head h, with state head h / (q_heads / kv_heads),
+ *   S = scale * q k^T over the states j < n_b,  P = softmax(S),  out = P v,
+ *   lse = log(sum(exp(S))),
+ * where n_b = lengths[b] clipped to 0..kv_len (lengths NULL: kv_len).  States from
+ * n_b on are not read into any result, whatever they hold; with n_b = 0 the rows of
+ * `out` are 0 and lse is -inf.  A tensor's element (b, token, head, d) lies at
+ * b*stride[0] + token*stride[1] + head*stride[2] + d; strides are in elements and
+ * not negative; inputs may have any (0 broadcasts), `out` must not overlap itself.
+ * head_dim 1..256; q_heads a multiple of kv_heads. */
+typedef struct {
+    int32_t dtype;
+    int32_t reserved;
+    int64_t batch, q_len, kv_len, q_heads, kv_heads, head_dim;
+    double scale;                 /* factor on the scores, finite and > 0 */
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3], dout_stride[3];
+} nnvb_attention_desc;
+
+/* lengths: int32 [batch] on the device or NULL; lse [batch, q_heads, q_len] or NULL. */
+int nnvb_cross_attention_forward(void* stream, const nnvb_attention_desc* d, const void* q, const void* k, const void* v,
+                                 const int32_t* lengths, void* out, void* lse);
+/* Gradients: dq [batch, q_len, q_heads, head_dim], dk, dv [batch, kv_len, kv_heads,
+ * head_dim], all dense.  out, lse are the forward call's.  dk and dv are sums over
+ * the query heads that share a state head, added in a fixed order; they are 0 for
+ * states from lengths[b] on.  Needs nnvb_cross_attention_workspace bytes of 16-byte
+ * aligned workspace, which needs no preparation. */
+int64_t nnvb_cross_attention_workspace(const nnvb_attention_desc* d);
+int nnvb_cross_attention_backward(void* stream, const nnvb_attention_desc* d, const void* dout, const void* q,
+                                  const void* k, const void* v, const void* out, const void* lse,
+                                  const int32_t* lengths, void* dq, void* dk, void* dv, void* workspace,
+                                  int64_t workspace_bytes);
 
 #ifdef __cplusplus
 }

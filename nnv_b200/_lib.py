@@ -21,6 +21,9 @@ NNVB_E_STATE = 4
 NNVB_E_UNSUPPORTED = 5
 
 LAYER_CONV2D, LAYER_FC, LAYER_BN, LAYER_AVGPOOL2D, LAYER_RELU = 1, 2, 3, 4, 5
+LAYER_LAYERNORM, LAYER_ATTENTION = 6, 7
+
+F64, F32, BF16, F16 = 0, 1, 2, 3
 
 POOL_DIV_WINDOW, POOL_DIV_INSIDE = 0, 1
 NCCL_ID_BYTES = 128
@@ -58,6 +61,15 @@ class Opts(C.Structure):
 
 class ReluStats(C.Structure):
     _fields_ = [("n_neurons", C.c_int64), ("n_cross", C.c_int64), ("n_dead", C.c_int64), ("cols_after", C.c_int64)]
+
+
+class AttentionDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("reserved", C.c_int32),
+                ("batch", C.c_int64), ("q_len", C.c_int64), ("kv_len", C.c_int64),
+                ("q_heads", C.c_int64), ("kv_heads", C.c_int64), ("head_dim", C.c_int64),
+                ("scale", C.c_double),
+                ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+                ("out_stride", C.c_int64 * 3), ("dout_stride", C.c_int64 * 3)]
 
 
 # int (*nnvb_allreduce_fn)(void* user, double* dev_buf, int64_t count, void* stream)
@@ -132,6 +144,18 @@ SIGNATURES = {
     # device pointers travel as integers (c_void_p)
     "nnvb_estimate_ranges_noalloc": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
                                                C.c_void_p, C.c_void_p, C.c_void_p]),
+    "nnvb_layer_norm_forward": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
+                                          C.c_void_p, C.c_double, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
+    "nnvb_layer_norm_workspace": (C.c_int64, [C.c_int, C.c_int64, C.c_int64]),
+    "nnvb_layer_norm_backward": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
+                                           C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
+                                           C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64]),
+    "nnvb_cross_attention_forward": (C.c_int, [C.c_void_p, C.POINTER(AttentionDesc), C.c_void_p, C.c_void_p, C.c_void_p,
+                                               C.c_void_p, C.c_void_p, C.c_void_p]),
+    "nnvb_cross_attention_workspace": (C.c_int64, [C.POINTER(AttentionDesc)]),
+    "nnvb_cross_attention_backward": (C.c_int, [C.c_void_p, C.POINTER(AttentionDesc), C.c_void_p, C.c_void_p, C.c_void_p,
+                                                C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                                C.c_void_p, C.c_void_p, C.c_int64]),
 }
 
 _lib = None

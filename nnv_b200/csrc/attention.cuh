@@ -1,0 +1,41 @@
+// Attention of a batch of positions over an encoder's states: what its kernel families share.
+#pragma once
+#include "common.cuh"
+#include "tensor_types.cuh"
+
+namespace nnvb {
+
+// A call's sizes, strides (elements) and pointers, as the kernels take them.
+struct AttnArgs {
+    int64_t qs[3], ks[3], vs[3], os[3], dos[3];    // batch, token, head
+    const void *q, *k, *v, *dout;
+    const void* o;                 // forward: written; backward: the forward call's output
+    void* lse;
+    const int32_t* lengths;
+    void *dq, *dk, *dv;
+    void* delta;                   // [B, Hq, Lq] sum_d dout * out
+    double scale;
+    int B, Lq, Lk, Hq, Hkv, D;
+    int dtype;
+};
+
+// valid states of batch entry b
+__device__ __forceinline__ int attn_len(const AttnArgs& a, int b) {
+    if (!a.lengths) return a.Lk;
+    const int n = a.lengths[b];
+    return n < 0 ? 0 : (n < a.Lk ? n : a.Lk);
+}
+
+__device__ __forceinline__ float exp_acc(float x) { return exp2f(x); }     // callers scale by log2(e)
+__device__ __forceinline__ double exp_acc(double x) { return exp2(x); }
+__device__ __forceinline__ float log_acc(float x) { return logf(x); }
+__device__ __forceinline__ double log_acc(double x) { return log(x); }
+
+constexpr double LOG2E = 1.4426950408889634074;
+
+// any type, head size up to 256, any strides
+int attn_forward_simt(cudaStream_t st, const AttnArgs& a);
+int attn_backward_simt(cudaStream_t st, const AttnArgs& a);
+int attn_delta(cudaStream_t st, const AttnArgs& a);
+
+}  // namespace nnvb

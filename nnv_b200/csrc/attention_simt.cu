@@ -1,0 +1,454 @@
+// Attention over an encoder's states on the CUDA cores: double and float tensors, and the 16-bit layouts the
+// tensor-core kernels do not take (head sizes over 128, rows that are not 16-byte aligned).
+//
+//   forward   one pass over the states with the running maximum m and sum l of each row's softmax:
+//             m' = max(m, max_j S_j), p_j = exp(S_j - m'), l' = l exp(m - m') + sum p_j, O' = O exp(m - m') + p V
+//   backward  P = exp(S - lse), dP = dO V^T, dS = P (dP - delta), delta = sum_d dO O;  dQ = scale dS K (a block per
+//             tile of positions, walking over the states), dK = scale dS^T Q and dV = P^T dO (a block per tile of
+//             states, walking over the positions of every query head that shares it): nothing is added atomically
+//
+// A block of 256 threads holds TILE x TILE scores, 16 x 16 threads with (TILE/16)^2 scores each, operands in shared
+// memory in the type sums are held in, rows padded by 16 bytes so that the 16-byte loads of neighbouring rows
+// fall on different banks.  Bound by the FMA pipe: a 4 x 4 register tile needs 8 16-byte loads for 64 FMAs.
+#include <algorithm>
+
+#include "attention.cuh"
+
+namespace nnvb {
+namespace {
+
+constexpr int THREADS = 256;
+
+template <typename A> struct VecOf;
+template <> struct VecOf<float> { static constexpr int N = 4; };
+template <> struct VecOf<double> { static constexpr int N = 2; };
+
+template <typename A>
+__device__ __forceinline__ Pack<A, VecOf<A>::N> lds(const A* p) {
+    return *reinterpret_cast<const Pack<A, VecOf<A>::N>*>(p);
+}
+
+// rows [r0, r0 + TILE) of a [token] x D slab into s[TILE][DP + pad]; rows at or past n_rows and columns past D are zero
+template <typename T, typename A, int TILE, int DP>
+__device__ void load_tile(A* s, const T* g, int64_t stride, int r0, int n_rows, int D, bool vec) {
+    constexpr int LD = DP + VecOf<A>::N;
+    constexpr int V = 16 / sizeof(T);
+    if (vec) {
+        for (int i = threadIdx.x; i < TILE * (DP / V); i += THREADS) {
+            const int r = i / (DP / V), c = i % (DP / V) * V;
+            Pack<T, V> p;
+            const bool in = r0 + r < n_rows && c < D;          // D is a multiple of V here
+            if (in) p = *reinterpret_cast<const Pack<T, V>*>(g + int64_t(r0 + r) * stride + c);
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[r * LD + c + e] = in ? to_acc(p.v[e]) : A(0);
+        }
+    } else {
+        for (int i = threadIdx.x; i < TILE * DP; i += THREADS) {
+            const int r = i / DP, c = i % DP;
+            s[r * LD + c] = r0 + r < n_rows && c < D ? A(to_acc(g[int64_t(r0 + r) * stride + c])) : A(0);
+        }
+    }
+}
+
+// acc[i][j] += sum_d X[(ty*M + i)][d] * Y[tx + 16 j][d]
+template <typename A, int TILE, int DP>
+__device__ __forceinline__ void mul_rows(A (&acc)[TILE / 16][TILE / 16], const A* X, const A* Y, int ty, int tx) {
+    constexpr int M = TILE / 16, V = VecOf<A>::N, LD = DP + V;
+#pragma unroll 4
+    for (int d = 0; d < DP; d += V) {
+        Pack<A, V> x[M], y[M];
+#pragma unroll
+        for (int i = 0; i < M; ++i) x[i] = lds<A>(X + (ty * M + i) * LD + d);
+#pragma unroll
+        for (int j = 0; j < M; ++j) y[j] = lds<A>(Y + (tx + 16 * j) * LD + d);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+#pragma unroll
+            for (int i = 0; i < M; ++i)
+#pragma unroll
+                for (int j = 0; j < M; ++j) acc[i][j] += x[i].v[e] * y[j].v[e];
+    }
+}
+
+// acc[i][c] += sum_k P[ty*M + i][k] * Y[k][column c of this thread];  thread columns: V at tx*V + 16*V*c
+template <typename A, int TILE, int DP>
+__device__ __forceinline__ void mul_cols(A (&acc)[TILE / 16][DP / 16], const A* P, const A* Y, int ty, int tx) {
+    constexpr int M = TILE / 16, V = VecOf<A>::N, LD = DP + V, LP = TILE + V, NC = DP / (16 * V);
+#pragma unroll 2
+    for (int k = 0; k < TILE; k += V) {
+        Pack<A, V> p[M];
+#pragma unroll
+        for (int i = 0; i < M; ++i) p[i] = lds<A>(P + (ty * M + i) * LP + k);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const Pack<A, V> y = lds<A>(Y + (k + e) * LD + tx * V + 16 * V * c);
+#pragma unroll
+                for (int i = 0; i < M; ++i)
+#pragma unroll
+                    for (int f = 0; f < V; ++f) acc[i][c * V + f] += p[i].v[e] * y.v[f];
+            }
+    }
+}
+
+// acc[i][c] += sum_q P[q][ty*M + i] * Y[q][column c of this thread]
+template <typename A, int TILE, int DP>
+__device__ __forceinline__ void mul_cols_t(A (&acc)[TILE / 16][DP / 16], const A* P, const A* Y, int ty, int tx) {
+    constexpr int M = TILE / 16, V = VecOf<A>::N, LD = DP + V, LP = TILE + V, NC = DP / (16 * V);
+#pragma unroll 4
+    for (int q = 0; q < TILE; ++q) {
+        A p[M];
+#pragma unroll
+        for (int i = 0; i < M; ++i) p[i] = P[q * LP + ty * M + i];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const Pack<A, V> y = lds<A>(Y + q * LD + tx * V + 16 * V * c);
+#pragma unroll
+            for (int i = 0; i < M; ++i)
+#pragma unroll
+                for (int f = 0; f < V; ++f) acc[i][c * V + f] += p[i] * y.v[f];
+        }
+    }
+}
+
+template <typename T, typename A, int TILE, int DP>
+__device__ __forceinline__ void store_rows(T* g, int64_t stride, int r0, int n_rows, int D, const A (&acc)[TILE / 16][DP / 16],
+                                           const A (&f)[TILE / 16], int ty, int tx) {
+    constexpr int M = TILE / 16, V = VecOf<A>::N, NC = DP / (16 * V);
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        const int r = r0 + ty * M + i;
+        if (r < n_rows)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const int d = tx * V + 16 * V * c + e;
+                    if (d < D) g[int64_t(r) * stride + d] = from_acc<T, A>(acc[i][c * V + e] * f[i]);
+                }
+    }
+}
+
+template <typename A>
+__device__ __forceinline__ A max16(A x) {
+    for (int o = 8; o > 0; o >>= 1) {
+        const A y = __shfl_xor_sync(0xffffffffu, x, o, 32);
+        x = y > x ? y : x;
+    }
+    return x;
+}
+template <typename A>
+__device__ __forceinline__ A sum16(A x) {
+    for (int o = 8; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o, 32);
+    return x;
+}
+
+template <typename T, int TILE, int DP>
+__global__ void __launch_bounds__(THREADS)
+attn_fwd_simt_kernel(AttnArgs a, bool vec) {
+    using A = typename AccOf<T>::type;
+    constexpr int M = TILE / 16, V = VecOf<A>::N, LD = DP + V, LP = TILE + V;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    A* Qs = reinterpret_cast<A*>(smem_raw);
+    A* Ks = Qs + TILE * LD;
+    A* Vs = Ks + TILE * LD;
+    A* Ps = Vs + TILE * LD;
+    const int tiles = (a.Lq + TILE - 1) / TILE;
+    const int q0 = int(blockIdx.x % tiles) * TILE;
+    const int h = int(blockIdx.x / tiles % a.Hq), b = int(blockIdx.x / tiles / a.Hq);
+    const int g = h / (a.Hq / a.Hkv);
+    const int n = attn_len(a, b);
+    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+    const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2];
+    const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + g * a.ks[2];
+    const T* v = static_cast<const T*>(a.v) + b * a.vs[0] + g * a.vs[2];
+    const A c = A(a.scale * LOG2E), ninf = -INFINITY;
+    A o[M][DP / 16], m[M], l[M];
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        m[i] = ninf;
+        l[i] = 0;
+#pragma unroll
+        for (int e = 0; e < DP / 16; ++e) o[i][e] = 0;
+    }
+    load_tile<T, A, TILE, DP>(Qs, q, a.qs[1], q0, a.Lq, a.D, vec);
+    for (int k0 = 0; k0 < n; k0 += TILE) {
+        __syncthreads();
+        load_tile<T, A, TILE, DP>(Ks, k, a.ks[1], k0, n, a.D, vec);
+        load_tile<T, A, TILE, DP>(Vs, v, a.vs[1], k0, n, a.D, vec);
+        __syncthreads();
+        A s[M][M] = {};
+        mul_rows<A, TILE, DP>(s, Qs, Ks, ty, tx);
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            A mx = ninf;
+#pragma unroll
+            for (int j = 0; j < M; ++j) {
+                s[i][j] = k0 + tx + 16 * j < n ? s[i][j] * c : ninf;
+                mx = s[i][j] > mx ? s[i][j] : mx;
+            }
+            mx = max16(mx);
+            const A mn = mx > m[i] ? mx : m[i];
+            const A base = mn == ninf ? A(0) : mn;       // every score so far is -inf: exp(-inf - 0) = 0
+            const A f = exp_acc(m[i] - base);
+            m[i] = mn;
+            A t = 0;
+#pragma unroll
+            for (int j = 0; j < M; ++j) {
+                const A p = exp_acc(s[i][j] - base);
+                t += p;
+                Ps[(ty * M + i) * LP + tx + 16 * j] = p;
+            }
+            l[i] = l[i] * f + sum16(t);
+#pragma unroll
+            for (int e = 0; e < DP / 16; ++e) o[i][e] *= f;
+        }
+        __syncwarp();                     // a warp reads back only the rows its own threads wrote
+        mul_cols<A, TILE, DP>(o, Ps, Vs, ty, tx);
+    }
+    A f[M];
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        f[i] = n > 0 ? A(1) / l[i] : A(0);
+        const int r = q0 + ty * M + i;
+        if (a.lse && tx == 0 && r < a.Lq)
+            static_cast<A*>(a.lse)[(int64_t(b) * a.Hq + h) * a.Lq + r] = n > 0 ? m[i] / A(LOG2E) + log_acc(l[i]) : ninf;
+    }
+    T* out = static_cast<T*>(const_cast<void*>(a.o)) + b * a.os[0] + h * a.os[2];
+    store_rows<T, A, TILE, DP>(out, a.os[1], q0, a.Lq, a.D, o, f, ty, tx);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+attn_delta_kernel(AttnArgs a) {
+    using A = typename AccOf<T>::type;
+    const int lane = threadIdx.x % 32;
+    const int64_t i = int64_t(blockIdx.x) * 8 + threadIdx.x / 32;      // ((b * Lq) + r) * Hq + h
+    if (i >= int64_t(a.B) * a.Lq * a.Hq) return;
+    const int h = int(i % a.Hq), r = int(i / a.Hq % a.Lq), b = int(i / a.Hq / a.Lq);
+    const T* o = static_cast<const T*>(a.o) + b * a.os[0] + r * a.os[1] + h * a.os[2];
+    const T* d = static_cast<const T*>(a.dout) + b * a.dos[0] + r * a.dos[1] + h * a.dos[2];
+    A s = 0;
+    for (int c = lane; c < a.D; c += 32) s += A(to_acc(o[c])) * A(to_acc(d[c]));
+    for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w, 32);
+    if (lane == 0) static_cast<A*>(a.delta)[(int64_t(b) * a.Hq + h) * a.Lq + r] = s;
+}
+
+// dQ: a block per tile of positions
+template <typename T, int TILE, int DP>
+__global__ void __launch_bounds__(THREADS)
+attn_dq_simt_kernel(AttnArgs a, bool vec) {
+    using A = typename AccOf<T>::type;
+    constexpr int M = TILE / 16, V = VecOf<A>::N, LD = DP + V, LP = TILE + V;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    A* Qs = reinterpret_cast<A*>(smem_raw);
+    A* Gs = Qs + TILE * LD;
+    A* Ks = Gs + TILE * LD;
+    A* Vs = Ks + TILE * LD;
+    A* Ps = Vs + TILE * LD;
+    const int tiles = (a.Lq + TILE - 1) / TILE;
+    const int q0 = int(blockIdx.x % tiles) * TILE;
+    const int h = int(blockIdx.x / tiles % a.Hq), b = int(blockIdx.x / tiles / a.Hq);
+    const int g = h / (a.Hq / a.Hkv);
+    const int n = attn_len(a, b);
+    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+    const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + g * a.ks[2];
+    const T* v = static_cast<const T*>(a.v) + b * a.vs[0] + g * a.vs[2];
+    const A c = A(a.scale * LOG2E);
+    A acc[M][DP / 16], lse[M], dl[M], f[M];
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        const int r = q0 + ty * M + i;
+        const int64_t at = (int64_t(b) * a.Hq + h) * a.Lq + r;
+        lse[i] = r < a.Lq ? static_cast<const A*>(a.lse)[at] * A(LOG2E) : A(0);
+        dl[i] = r < a.Lq ? static_cast<const A*>(a.delta)[at] : A(0);
+        f[i] = A(a.scale);
+#pragma unroll
+        for (int e = 0; e < DP / 16; ++e) acc[i][e] = 0;
+    }
+    load_tile<T, A, TILE, DP>(Qs, static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2], a.qs[1], q0, a.Lq, a.D, vec);
+    load_tile<T, A, TILE, DP>(Gs, static_cast<const T*>(a.dout) + b * a.dos[0] + h * a.dos[2], a.dos[1], q0, a.Lq, a.D, vec);
+    for (int k0 = 0; k0 < n; k0 += TILE) {
+        __syncthreads();
+        load_tile<T, A, TILE, DP>(Ks, k, a.ks[1], k0, n, a.D, vec);
+        load_tile<T, A, TILE, DP>(Vs, v, a.vs[1], k0, n, a.D, vec);
+        __syncthreads();
+        A s[M][M] = {}, dp[M][M] = {};
+        mul_rows<A, TILE, DP>(s, Qs, Ks, ty, tx);
+        mul_rows<A, TILE, DP>(dp, Gs, Vs, ty, tx);
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+#pragma unroll
+            for (int j = 0; j < M; ++j) {
+                const A p = k0 + tx + 16 * j < n ? exp_acc(s[i][j] * c - lse[i]) : A(0);
+                Ps[(ty * M + i) * LP + tx + 16 * j] = p * (dp[i][j] - dl[i]);
+            }
+        __syncwarp();
+        mul_cols<A, TILE, DP>(acc, Ps, Ks, ty, tx);
+    }
+    T* dq = static_cast<T*>(a.dq) + (int64_t(b) * a.Lq * a.Hq + h) * a.D;
+    store_rows<T, A, TILE, DP>(dq, int64_t(a.Hq) * a.D, q0, a.Lq, a.D, acc, f, ty, tx);
+}
+
+// dK, dV: a block per tile of states, over the positions of every query head of its group
+template <typename T, int TILE, int DP>
+__global__ void __launch_bounds__(THREADS)
+attn_dkv_simt_kernel(AttnArgs a, bool vec) {
+    using A = typename AccOf<T>::type;
+    constexpr int M = TILE / 16, V = VecOf<A>::N, LD = DP + V, LP = TILE + V;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    A* Ks = reinterpret_cast<A*>(smem_raw);
+    A* Vs = Ks + TILE * LD;
+    A* Qs = Vs + TILE * LD;
+    A* Gs = Qs + TILE * LD;
+    A* Ps = Gs + TILE * LD;
+    A* Ss = Ps + TILE * LP;
+    const int tiles = (a.Lk + TILE - 1) / TILE;
+    const int k0 = int(blockIdx.x % tiles) * TILE;
+    const int g = int(blockIdx.x / tiles % a.Hkv), b = int(blockIdx.x / tiles / a.Hkv);
+    const int G = a.Hq / a.Hkv;
+    const int n = attn_len(a, b);
+    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+    const A c = A(a.scale * LOG2E);
+    A dk[M][DP / 16], dv[M][DP / 16], fk[M], fv[M];
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        fk[i] = A(a.scale);
+        fv[i] = 1;
+#pragma unroll
+        for (int e = 0; e < DP / 16; ++e) { dk[i][e] = 0; dv[i][e] = 0; }
+    }
+    if (k0 < n) {
+        load_tile<T, A, TILE, DP>(Ks, static_cast<const T*>(a.k) + b * a.ks[0] + g * a.ks[2], a.ks[1], k0, n, a.D, vec);
+        load_tile<T, A, TILE, DP>(Vs, static_cast<const T*>(a.v) + b * a.vs[0] + g * a.vs[2], a.vs[1], k0, n, a.D, vec);
+        for (int h = g * G; h < (g + 1) * G; ++h) {
+            const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2];
+            const T* go = static_cast<const T*>(a.dout) + b * a.dos[0] + h * a.dos[2];
+            for (int q0 = 0; q0 < a.Lq; q0 += TILE) {
+                __syncthreads();
+                load_tile<T, A, TILE, DP>(Qs, q, a.qs[1], q0, a.Lq, a.D, vec);
+                load_tile<T, A, TILE, DP>(Gs, go, a.dos[1], q0, a.Lq, a.D, vec);
+                __syncthreads();
+                A s[M][M] = {}, dp[M][M] = {};
+                mul_rows<A, TILE, DP>(s, Qs, Ks, ty, tx);
+                mul_rows<A, TILE, DP>(dp, Gs, Vs, ty, tx);
+#pragma unroll
+                for (int i = 0; i < M; ++i) {
+                    const int r = q0 + ty * M + i;
+                    const int64_t at = (int64_t(b) * a.Hq + h) * a.Lq + r;
+                    const A lse = r < a.Lq ? static_cast<const A*>(a.lse)[at] * A(LOG2E) : A(0);
+                    const A dl = r < a.Lq ? static_cast<const A*>(a.delta)[at] : A(0);
+#pragma unroll
+                    for (int j = 0; j < M; ++j) {
+                        const A p = r < a.Lq && k0 + tx + 16 * j < n ? exp_acc(s[i][j] * c - lse) : A(0);
+                        Ps[(ty * M + i) * LP + tx + 16 * j] = p;
+                        Ss[(ty * M + i) * LP + tx + 16 * j] = p * (dp[i][j] - dl);
+                    }
+                }
+                __syncthreads();
+                mul_cols_t<A, TILE, DP>(dv, Ps, Gs, ty, tx);
+                mul_cols_t<A, TILE, DP>(dk, Ss, Qs, ty, tx);
+            }
+        }
+    }
+    const int64_t base = (int64_t(b) * a.Lk * a.Hkv + g) * a.D, stride = int64_t(a.Hkv) * a.D;
+    store_rows<T, A, TILE, DP>(static_cast<T*>(a.dk) + base, stride, k0, a.Lk, a.D, dk, fk, ty, tx);
+    store_rows<T, A, TILE, DP>(static_cast<T*>(a.dv) + base, stride, k0, a.Lk, a.D, dv, fv, ty, tx);
+}
+
+// ---------------------------------------------------------------------------
+
+template <typename A>
+constexpr int tile_bytes(int tile, int dp) { return tile * (dp + VecOf<A>::N) * int(sizeof(A)); }
+template <typename A>
+constexpr int score_bytes(int tile) { return tile * (tile + VecOf<A>::N) * int(sizeof(A)); }
+
+constexpr int SMEM_MAX = 227 * 1024;
+// the largest tile of scores whose operands fit the shared memory of an SM
+template <typename A>
+constexpr int fwd_tile(int dp) {
+    for (int t : {64, 32})
+        if (3 * tile_bytes<A>(t, dp) + score_bytes<A>(t) <= SMEM_MAX) return t;
+    return 16;
+}
+template <typename A>
+constexpr int bwd_tile(int dp) {
+    for (int t : {64, 32})
+        if (4 * tile_bytes<A>(t, dp) + 2 * score_bytes<A>(t) <= SMEM_MAX) return t;
+    return 16;
+}
+
+template <typename K>
+int launch(K kernel, int64_t blocks, int smem, cudaStream_t st, const AttnArgs& a, bool vec) {
+    if (blocks <= 0) return NNVB_OK;
+    NNVB_REQUIRE(blocks < (int64_t(1) << 31), "nnvb_cross_attention: too many tiles (%lld) for one launch", (long long)blocks);
+    NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kernel<<<unsigned(blocks), THREADS, smem, st>>>(a, vec);
+    NNVB_CUDA(cudaGetLastError());
+    return NNVB_OK;
+}
+
+bool rows16(const void* p, const int64_t (&s)[3], int64_t esize) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s[0] * esize % 16 == 0 && s[1] * esize % 16 == 0 &&
+           s[2] * esize % 16 == 0;
+}
+
+template <typename T, int DP>
+int forward_t(cudaStream_t st, const AttnArgs& a) {
+    using A = typename AccOf<T>::type;
+    constexpr int TILE = fwd_tile<A>(DP);
+    const bool vec = a.D * sizeof(T) % 16 == 0 && rows16(a.q, a.qs, sizeof(T)) && rows16(a.k, a.ks, sizeof(T)) &&
+                     rows16(a.v, a.vs, sizeof(T));
+    return launch(attn_fwd_simt_kernel<T, TILE, DP>, ceil_div(a.Lq, TILE) * a.Hq * a.B,
+                  3 * tile_bytes<A>(TILE, DP) + score_bytes<A>(TILE), st, a, vec);
+}
+
+template <typename T, int DP>
+int backward_t(cudaStream_t st, const AttnArgs& a) {
+    using A = typename AccOf<T>::type;
+    constexpr int TILE = bwd_tile<A>(DP);
+    const bool vec = a.D * sizeof(T) % 16 == 0 && rows16(a.q, a.qs, sizeof(T)) && rows16(a.k, a.ks, sizeof(T)) &&
+                     rows16(a.v, a.vs, sizeof(T)) && rows16(a.dout, a.dos, sizeof(T));
+    const int smem = 4 * tile_bytes<A>(TILE, DP) + 2 * score_bytes<A>(TILE);
+    NNVB_TRY(launch(attn_dq_simt_kernel<T, TILE, DP>, ceil_div(a.Lq, TILE) * a.Hq * a.B, smem, st, a, vec));
+    return launch(attn_dkv_simt_kernel<T, TILE, DP>, ceil_div(a.Lk, TILE) * a.Hkv * a.B, smem, st, a, vec);
+}
+
+template <typename T>
+int by_head(cudaStream_t st, const AttnArgs& a, bool backward) {
+    if (a.D <= 64) return backward ? backward_t<T, 64>(st, a) : forward_t<T, 64>(st, a);
+    if (a.D <= 128) return backward ? backward_t<T, 128>(st, a) : forward_t<T, 128>(st, a);
+    return backward ? backward_t<T, 256>(st, a) : forward_t<T, 256>(st, a);
+}
+
+int by_type(cudaStream_t st, const AttnArgs& a, bool backward) {
+    switch (a.dtype) {
+        case NNVB_F64: return by_head<double>(st, a, backward);
+        case NNVB_F32: return by_head<float>(st, a, backward);
+        case NNVB_BF16: return by_head<__nv_bfloat16>(st, a, backward);
+        default: return by_head<__half>(st, a, backward);
+    }
+}
+
+}  // namespace
+
+int attn_forward_simt(cudaStream_t st, const AttnArgs& a) { return by_type(st, a, false); }
+int attn_backward_simt(cudaStream_t st, const AttnArgs& a) { return by_type(st, a, true); }
+
+int attn_delta(cudaStream_t st, const AttnArgs& a) {
+    const int64_t rows = int64_t(a.B) * a.Lq * a.Hq;
+    if (rows == 0) return NNVB_OK;
+    const int64_t blocks = ceil_div(rows, 8);
+    NNVB_REQUIRE(blocks < (int64_t(1) << 31), "nnvb_cross_attention_backward: too many rows (%lld)", (long long)rows);
+    switch (a.dtype) {
+        case NNVB_F64: attn_delta_kernel<double><<<unsigned(blocks), 256, 0, st>>>(a); break;
+        case NNVB_F32: attn_delta_kernel<float><<<unsigned(blocks), 256, 0, st>>>(a); break;
+        case NNVB_BF16: attn_delta_kernel<__nv_bfloat16><<<unsigned(blocks), 256, 0, st>>>(a); break;
+        default: attn_delta_kernel<__half><<<unsigned(blocks), 256, 0, st>>>(a); break;
+    }
+    NNVB_CUDA(cudaGetLastError());
+    return NNVB_OK;
+}
+
+}  // namespace nnvb

@@ -36,6 +36,9 @@ void set_error(const char* fmt, ...);
         }                               \
     } while (0)
 
+// Bytes of an element of an nnvb_dtype; 0 for any other value.
+int64_t dtype_bytes(int dtype);
+
 static inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 static inline int64_t ceil_div(int64_t x, int64_t m) { return (x + m - 1) / m; }
 
