@@ -70,7 +70,8 @@ int nnvb_cross_attention_forward(void* stream, const nnvb_attention_desc* d, con
     NNVB_REQUIRE(q && out && (d->kv_len == 0 || (k && v)), "nnvb_cross_attention_forward: NULL pointer");
     AttnArgs a = make_args(d);
     a.q = q; a.k = k; a.v = v; a.o = out; a.lse = lse; a.lengths = lengths;
-    return attn_forward_simt(static_cast<cudaStream_t>(stream), a);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return attn_tc_takes_forward(a) ? attn_forward_tc(st, a) : attn_forward_simt(st, a);
 }
 
 int64_t nnvb_cross_attention_workspace(const nnvb_attention_desc* d) {

@@ -184,6 +184,13 @@ struct Layer {
     double* bn_rden = nullptr;
     double* bn_scale = nullptr;
     double* bn_offset = nullptr;
+    // layer norm, attention: T positions of `cols` entries; bn_scale / bn_offset are the layer norm's weights
+    int64_t cols = 0;
+    double eps = 0.0;
+    double* keys = nullptr;
+    double* values = nullptr;
+    int64_t heads = 0, kv_heads = 0, head_dim = 0, states = 0;
+    double attn_scale = 0.0;
     bool fused_into_prev = false;      // bn applied in the previous conv's epilogue
     int fused_bn = -1;                 // conv: index of the bn layer it applies
 };
@@ -195,6 +202,7 @@ struct nnvb_net {
     int64_t in_shape[3] = {0, 0, 0};
     int64_t out_shape[3] = {0, 0, 0};
     int n_relu = 0;
+    bool evaluate_only = false;        // holds a layer without an approx-star reach
 };
 
 struct nnvb_batch {
@@ -704,6 +712,53 @@ int nnvb_net_create(nnvb_ctx* ctx, const nnvb_layer_desc* layers, int n_layers, 
                 L.Ho = H; L.Wo = W; L.Co = C;
                 net->n_relu += 1;
                 break;
+            case NNVB_LAYER_LAYERNORM: {
+                const int64_t cols = d.cout;
+                if (cols < 1 || !((C == 1 && H == cols) || H * W * C == cols)) {
+                    set_error("layer %d (layernorm): %lld channels of parameters for an input of %lld x %lld x %lld "
+                              "(a sequence [channels, T, 1] or a vector expected)",
+                              li, (long long)cols, (long long)H, (long long)W, (long long)C);
+                    return fail(NNVB_E_ARG);
+                }
+                if (!(std::isfinite(d.bn_eps) && d.bn_eps >= 0)) {
+                    set_error("layer %d (layernorm): Epsilon must be finite and not negative", li);
+                    return fail(NNVB_E_ARG);
+                }
+                int s = NNVB_OK;
+                if (d.bn_scale) s = upload_vec(net.get(), std::vector<double>(d.bn_scale, d.bn_scale + cols), &L.bn_scale);
+                if (!s && d.bn_offset)
+                    s = upload_vec(net.get(), std::vector<double>(d.bn_offset, d.bn_offset + cols), &L.bn_offset);
+                if (s) return fail(s);
+                L.cols = cols;
+                L.eps = d.bn_eps;
+                L.Ho = H; L.Wo = W; L.Co = C;
+                net->evaluate_only = true;
+                break;
+            }
+            case NNVB_LAYER_ATTENTION: {
+                const int64_t E = int64_t(d.kh) * d.cin;
+                if (!(d.W && d.b && d.kh > 0 && d.kw > 0 && d.kh % d.kw == 0 && d.cin > 0 && d.cin <= 256 && d.cout > 0 &&
+                      std::isfinite(d.bn_eps) && d.bn_eps >= 0)) {
+                    set_error("layer %d (attention): bad parameters", li);
+                    return fail(NNVB_E_ARG);
+                }
+                if (!((C == 1 && H == E) || H * W * C == E)) {
+                    set_error("layer %d (attention): %d heads of %d channels for an input of %lld x %lld x %lld "
+                              "(a sequence [heads * channels, T, 1] or a vector expected)",
+                              li, d.kh, d.cin, (long long)H, (long long)W, (long long)C);
+                    return fail(NNVB_E_ARG);
+                }
+                const size_t nkv = size_t(d.cin) * d.kw * d.cout;
+                int s = upload_vec(net.get(), std::vector<double>(d.W, d.W + nkv), &L.keys);
+                if (!s) s = upload_vec(net.get(), std::vector<double>(d.b, d.b + nkv), &L.values);
+                if (s) return fail(s);
+                L.cols = E;
+                L.heads = d.kh; L.kv_heads = d.kw; L.head_dim = d.cin; L.states = d.cout;
+                L.attn_scale = d.bn_eps > 0 ? d.bn_eps : 1.0 / std::sqrt(double(d.cin));
+                L.Ho = H; L.Wo = W; L.Co = C;
+                net->evaluate_only = true;
+                break;
+            }
             default:
                 set_error("layer %d: type %d is outside the approx-star path of this engine", li, d.type);
                 return fail(NNVB_E_UNSUPPORTED);
@@ -766,6 +821,12 @@ int nnvb_net_out_shape(const nnvb_net* net, int64_t shape[3]) {
 int nnvb_batch_create(nnvb_net* net, int n_queries, nnvb_batch** out) {
     NNVB_REQUIRE(net && out, "nnvb_batch_create: NULL argument");
     NNVB_REQUIRE(n_queries > 0, "nnvb_batch_create: need at least one query");
+    *out = nullptr;
+    if (net->evaluate_only) {
+        set_error("nnvb_batch_create: layer normalisation and attention layers have no approx-star reach in this engine "
+                  "(the network can be evaluated)");
+        return NNVB_E_UNSUPPORTED;
+    }
     auto b = new nnvb_batch();
     b->net = net;
     b->nq = n_queries;
@@ -2055,6 +2116,42 @@ int output_ranges(nnvb_batch* b) {
     return NNVB_OK;
 }
 
+// One column of n points holds T positions of L.cols entries each.  When the columns follow one another without
+// padding, or hold one position each, all positions are rows of one call.
+int layer_norm_points(cudaStream_t st, const Layer& L, const double* X, int64_t ld, double* Y, int64_t n, int64_t* launches) {
+    const int64_t T = L.Ho * L.Wo * L.Co / L.cols;
+    auto rows = [&](const double* x, double* y, int64_t count, int64_t stride) {
+        ++*launches;
+        return nnvb_layer_norm_forward(st, NNVB_F64, count, L.cols, x, stride, L.bn_scale, L.bn_offset, L.eps, y, stride,
+                                       nullptr, nullptr);
+    };
+    if (T == 1) return rows(X, Y, n, ld);
+    if (ld == T * L.cols) return rows(X, Y, n * T, L.cols);
+    if (n < T) {
+        for (int64_t i = 0; i < n; ++i) NNVB_TRY(rows(X + i * ld, Y + i * ld, T, L.cols));
+    } else {
+        for (int64_t t = 0; t < T; ++t) NNVB_TRY(rows(X + t * L.cols, Y + t * L.cols, n, ld));
+    }
+    return NNVB_OK;
+}
+
+int attention_points(cudaStream_t st, const Layer& L, const double* X, int64_t ld, double* Y, int64_t n, int64_t* launches) {
+    const int64_t T = L.Ho * L.Wo * L.Co / L.cols;
+    const bool rows = T == 1 || ld == T * L.cols;          // every position reads the same states
+    nnvb_attention_desc d{};
+    d.dtype = NNVB_F64;
+    d.batch = rows ? 1 : n;
+    d.q_len = rows ? n * T : T;
+    d.kv_len = L.states;
+    d.q_heads = L.heads; d.kv_heads = L.kv_heads; d.head_dim = L.head_dim;
+    d.scale = L.attn_scale;
+    d.q_stride[0] = ld; d.q_stride[1] = T == 1 ? ld : L.cols; d.q_stride[2] = L.head_dim;
+    d.k_stride[0] = 0; d.k_stride[1] = L.kv_heads * L.head_dim; d.k_stride[2] = L.head_dim;
+    for (int i = 0; i < 3; ++i) { d.v_stride[i] = d.k_stride[i]; d.out_stride[i] = d.q_stride[i]; }
+    ++*launches;
+    return nnvb_cross_attention_forward(st, &d, X, L.keys, L.values, nullptr, Y, nullptr);
+}
+
 // Run the layers over n points X [ld x n] held in wk.wit[0] (wk.wit[1] is the other buffer).  With a batch
 // (witness pass, one point per halfspace pair) the ReLU layers apply the relaxed ReLU of the pair's query;
 // without one (b == nullptr) they apply max(x, 0): NN.evaluate on n inputs at once.
@@ -2096,6 +2193,12 @@ int forward_points(nnvb_net* net, WorkBufs* wk, nnvb_batch* b, int n, const int3
                 ChanAffine bn{L.bn_mean, L.bn_den, L.bn_rden, L.bn_scale, L.bn_offset};
                 NNVB_TRY(launch_bn_f64(st, bn, L.H * L.W, N, cur, ld, n, n, &ctx->launches));
             }
+        } else if (L.type == NNVB_LAYER_LAYERNORM) {
+            NNVB_TRY(layer_norm_points(st, L, cur, ld, oth, n, &ctx->launches));
+            std::swap(cur, oth);
+        } else if (L.type == NNVB_LAYER_ATTENTION) {
+            NNVB_TRY(attention_points(st, L, cur, ld, oth, n, &ctx->launches));
+            std::swap(cur, oth);
         } else if (L.type == NNVB_LAYER_RELU) {
             if (b != nullptr) {
                 ReluLayerRecord& r = *wk->relu[relu_i++];

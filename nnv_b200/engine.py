@@ -170,6 +170,31 @@ def make_layer_desc(layer, keep):
         d.avgpool_divisor = L.POOL_DIV_INSIDE if div == "inside" else L.POOL_DIV_WINDOW
     elif t == "relu":
         d.type = L.LAYER_RELU
+    elif t == "layernorm":
+        cols = int(layer["channels"])
+        d.type = L.LAYER_LAYERNORM
+        d.cout = cols
+        for key, field in (("scale", "bn_scale"), ("offset", "bn_offset")):
+            if layer.get(key) is not None:
+                a = _f64(layer[key]).ravel()
+                if a.size != cols:
+                    raise ValueError("layernorm %s must have %d entries, got %d" % (key, cols, a.size))
+                keep.append(a)
+                setattr(d, field, _dp(a))
+        d.bn_eps = float(layer.get("eps", 1e-5))
+    elif t == "attention":
+        K, V = _f64(layer["keys"]), _f64(layer["values"])
+        if K.ndim != 3 or K.shape != V.shape:
+            raise ValueError("attention keys and values must be [channels, heads, states] of one shape")
+        scale = float(layer.get("scale") or 0.0)
+        if not (np.isfinite(scale) and scale >= 0):
+            raise ValueError("the factor on the scores must be finite and positive")
+        keep += [K, V]
+        d.type = L.LAYER_ATTENTION
+        d.cin, d.kw, d.cout = K.shape
+        d.kh = int(layer["heads"])
+        d.W, d.b = _dp(K), _dp(V)
+        d.bn_eps = scale
     else:
         raise ValueError("layer type %r is outside the approx-star path of this engine" % (t,))
     return d

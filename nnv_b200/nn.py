@@ -32,7 +32,8 @@ from . import _lib as L
 from .engine import Batch, Context, Network
 
 __all__ = ["NN", "ImageStar", "Star", "HalfSpace", "ImageInputLayer", "FlattenLayer", "Conv2DLayer", "FullyConnectedLayer",
-           "BatchNormalizationLayer", "AveragePooling2DLayer", "ReluLayer", "verify_specification",
+           "BatchNormalizationLayer", "AveragePooling2DLayer", "ReluLayer", "LayerNormalizationLayer", "AttentionLayer",
+           "verify_specification",
            "default_context"]
 
 _ctx = None
@@ -602,6 +603,57 @@ class ReluLayer(_Layer):
 
     def _desc(self):
         return {"type": "relu"}
+
+
+class LayerNormalizationLayer(_Layer):
+    """MATLAB's layerNormalizationLayer on a vector of ``NumChannels`` entries or a sequence [NumChannels, T, 1]: every
+    position is normalised over its channels, (x - mean) / sqrt(var + Epsilon) * Scale + Offset.  For
+    ``NN.evaluate`` and ``NN.falsify``; the layer has no approx-star reach here."""
+
+    def __init__(self, NumChannels, Scale=None, Offset=None, Epsilon=1e-5, Name="layernorm"):
+        self.NumChannels, self.Epsilon, self.Name = int(NumChannels), float(Epsilon), Name
+        if self.NumChannels < 1:
+            raise ValueError("Invalid number of channels")
+        if not (np.isfinite(self.Epsilon) and self.Epsilon >= 0):
+            raise ValueError("Epsilon must be finite and not negative")
+        self.Scale = None if Scale is None else np.asarray(Scale, dtype=np.float64).ravel()
+        self.Offset = None if Offset is None else np.asarray(Offset, dtype=np.float64).ravel()
+        for a in (self.Scale, self.Offset):
+            if a is not None and a.size != self.NumChannels:
+                raise ValueError("Inconsistency between the number of channels and the size of Scale or Offset")
+
+    def _desc(self):
+        return {"type": "layernorm", "channels": self.NumChannels, "scale": self.Scale, "offset": self.Offset,
+                "eps": self.Epsilon}
+
+
+class AttentionLayer(_Layer):
+    """MATLAB's attentionLayer with the keys and values of a fixed encoder output: the input, a sequence
+    [NumHeads * channels, T, 1] or one position as a vector, holds the queries; ``Keys`` and ``Values`` are
+    [channels, state heads, states] (or [channels * state heads, states] with ``NumStateHeads``).  Query head h
+    reads state head h // (NumHeads / state heads); ``Scale`` defaults to 1/sqrt(channels).  For ``NN.evaluate``
+    and ``NN.falsify``; the layer has no approx-star reach here."""
+
+    def __init__(self, NumHeads, Keys, Values, NumStateHeads=None, Scale=None, Name="attention"):
+        K, V = np.asarray(Keys, dtype=np.float64), np.asarray(Values, dtype=np.float64)
+        self.NumHeads, self.Name = int(NumHeads), Name
+        hk = int(NumStateHeads) if NumStateHeads is not None else (K.shape[1] if K.ndim == 3 else self.NumHeads)
+        if K.shape != V.shape or K.ndim not in (2, 3):
+            raise ValueError("Keys and Values must be [channels, heads, states] of one shape")
+        if hk < 1 or self.NumHeads < 1 or self.NumHeads % hk:
+            raise ValueError("%d heads cannot share %d state heads evenly" % (self.NumHeads, hk))
+        if K.ndim == 2:
+            if K.shape[0] % hk:
+                raise ValueError("Inconsistency between the rows of Keys and the number of heads")
+            K, V = (a.reshape(K.shape[0] // hk, hk, -1, order="F") for a in (K, V))
+        if K.shape[1] != hk or K.size == 0 or K.shape[0] > 256:
+            raise ValueError("Keys must have %d heads of 1..256 channels and at least one state" % hk)
+        if Scale is not None and not (np.isfinite(Scale) and Scale > 0):
+            raise ValueError("Scale must be finite and positive")
+        self.Keys, self.Values, self.Scale = K, V, Scale
+
+    def _desc(self):
+        return {"type": "attention", "heads": self.NumHeads, "keys": self.Keys, "values": self.Values, "scale": self.Scale}
 
 
 class ImageInputLayer(_Layer):
