@@ -76,7 +76,8 @@ int nnvb_cross_attention_forward(void* stream, const nnvb_attention_desc* d, con
 
 int64_t nnvb_cross_attention_workspace(const nnvb_attention_desc* d) {
     if (!d || d->batch < 0 || d->q_len < 0 || d->q_heads < 0) return 0;
-    return round_up(d->batch * d->q_len * d->q_heads * (d->dtype == NNVB_F64 ? 8 : 4), 16);
+    // delta, and for the tensor cores the log-sum-exp beside it, in rows padded to a tile
+    return d->batch * d->q_heads * round_up(d->q_len, 64) * 8;
 }
 
 int nnvb_cross_attention_backward(void* stream, const nnvb_attention_desc* d, const void* dout, const void* q,
@@ -106,6 +107,7 @@ int nnvb_cross_attention_backward(void* stream, const nnvb_attention_desc* d, co
     AttnArgs a = make_args(d);
     a.dout = dout; a.q = q; a.k = k; a.v = v; a.o = out; a.lse = const_cast<void*>(lse); a.lengths = lengths;
     a.dq = dq; a.dk = dk; a.dv = dv; a.delta = workspace;
+    if (attn_tc_takes_backward(a)) return attn_backward_tc(st, a);
     NNVB_TRY(attn_delta(st, a));
     return attn_backward_simt(st, a);
 }

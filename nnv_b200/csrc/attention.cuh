@@ -13,7 +13,7 @@ struct AttnArgs {
     void* lse;
     const int32_t* lengths;
     void *dq, *dk, *dv;
-    void* delta;                   // [B, Hq, Lq] sum_d dout * out
+    void* delta;                   // workspace: [B, Hq, Lq] sum_d dout * out (and the log-sum-exp beside it on the tensor cores)
     double scale;
     int B, Lq, Lk, Hq, Hkv, D;
     int dtype;
@@ -39,6 +39,8 @@ int attn_backward_simt(cudaStream_t st, const AttnArgs& a);
 // 16-bit types on the tensor cores; head size a multiple of 8 up to 128, 16-byte aligned rows
 bool attn_tc_takes_forward(const AttnArgs& a);
 int attn_forward_tc(cudaStream_t st, const AttnArgs& a);
+bool attn_tc_takes_backward(const AttnArgs& a);
+int attn_backward_tc(cudaStream_t st, const AttnArgs& a);
 int attn_delta(cudaStream_t st, const AttnArgs& a);
 
 }  // namespace nnvb

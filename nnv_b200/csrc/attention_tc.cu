@@ -295,6 +295,283 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------
+// Backward.  P = exp2(c S - lse'), dS = P (dP - delta) with lse' = lse log2 e.  One kernel serves both passes:
+//   dQ       resident Q and dO (128 positions), streamed K and V:   S = Q K^T,  dP = dO V^T,  dQ += dS K
+//   dK, dV   resident K and V (128 states), streamed Q and dO of every query head of the group:
+//            S^T = K Q^T,  dP^T = V dO^T,  dV += P^T dO,  dK += dS^T Q
+// so each gradient row is summed in tensor memory by one block, in a fixed order.  That costs seven products a pair
+// instead of five with atomic additions to dQ.  Streamed tiles have 64 rows, which lets two of them be in flight in
+// tensor memory beside 128 x 128 accumulators: while one tile is in the softmax arithmetic of a warpgroup the next
+// one's S and dP run.  P and dS are rounded to the tensors' type (operands of 16-bit products); everything else is fp32.
+// Streamed tiles serve as K-major operand of S and dP and as MN-major operand of the gradients.
+
+constexpr int BROWS = 64;                          // rows of a streamed tile
+
+template <int DP>
+struct BwdSmem {
+    static constexpr int ABOX = ROWS * 128, ATILE = ABOX * (DP / 64);
+    static constexpr int BBOX = BROWS * 128, BTILE = BBOX * (DP / 64);
+    static constexpr int STATS = 2 * BROWS * 4;    // lse' and delta of the streamed positions
+    static constexpr int STAGES = 4;
+    static constexpr int BYTES = 2 * ATILE + STAGES * 2 * BTILE + STAGES * STATS + 1024;
+};
+
+struct BwdMaps {
+    CUtensorMap a0, a1, b0, b1;
+};
+
+// stats: [B, Hq, LqP] lse' then the same of delta; LqP = Lq rounded up to 64, the rows behind Lq hold +inf and 0
+template <typename T>
+__global__ void __launch_bounds__(256)
+attn_stats_tc_kernel(AttnArgs a, int LqP) {
+    const int lane = threadIdx.x % 16;
+    const int64_t i = int64_t(blockIdx.x) * 16 + threadIdx.x / 16;     // ((b * LqP) + r) * Hq + h
+    const bool live = i < int64_t(a.B) * LqP * a.Hq;
+    const int h = int(i % a.Hq), r = int(i / a.Hq % LqP), b = int(i / a.Hq / LqP);
+    float s = 0.f;
+    if (live && r < a.Lq && lane * 8 < a.D) {
+        const auto o = *reinterpret_cast<const Pack<T, 8>*>(static_cast<const T*>(a.o) + b * a.os[0] + r * a.os[1] + h * a.os[2] + lane * 8);
+        const auto d = *reinterpret_cast<const Pack<T, 8>*>(static_cast<const T*>(a.dout) + b * a.dos[0] + r * a.dos[1] + h * a.dos[2] + lane * 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += to_acc(o.v[e]) * to_acc(d.v[e]);
+    }
+    for (int w = 8; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w, 32);
+    if (live && lane == 0) {
+        float* st = static_cast<float*>(a.delta);
+        const int64_t at = (int64_t(b) * a.Hq + h) * LqP + r;
+        st[at] = r < a.Lq ? static_cast<const float*>(a.lse)[(int64_t(b) * a.Hq + h) * a.Lq + r] * float(LOG2E) : INFINITY;
+        st[int64_t(a.B) * a.Hq * LqP + at] = s;
+    }
+}
+
+template <typename T, int DP, bool KV>
+__global__ void __launch_bounds__(FWD_THREADS, 1)
+attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
+    using SM = BwdSmem<DP>;
+    constexpr int STAGES = SM::STAGES;
+    extern __shared__ unsigned char raw[];
+    unsigned char* base = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
+    unsigned char* res = base;                             // A0, A1
+    unsigned char* ring = base + 2 * SM::ATILE;            // B0, B1 per stage
+    float* stats = reinterpret_cast<float*>(ring + STAGES * 2 * SM::BTILE);
+    __shared__ uint64_t full[STAGES], empty[STAGES], a_full, s_ready[2], p_ready[2], o_ready, tail, drain;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag;
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int own_len = KV ? a.Lk : a.Lq, own_heads = KV ? a.Hkv : a.Hq;
+    const int tiles = (own_len + ROWS - 1) / ROWS;
+    const int r0 = int(blockIdx.x % tiles) * ROWS;
+    const int oh = int(blockIdx.x / tiles % own_heads), b = int(blockIdx.x / tiles / own_heads);
+    const int G = a.Hq / a.Hkv;
+    const int n = attn_len(a, b);
+    // streamed tiles: positions of all query heads of the group, or valid states
+    const int per_head = KV ? (a.Lq + BROWS - 1) / BROWS : (n + BROWS - 1) / BROWS;
+    const int steps = KV ? (r0 < n ? per_head * G : 0) : per_head;
+
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        mbar_init(&a_full, 1);
+        mbar_init(&o_ready, 1);
+        mbar_init(&tail, 1);
+        mbar_init(&drain, 1);
+        for (int t = 0; t < 2; ++t) { mbar_init(&s_ready[t], 1); mbar_init(&p_ready[t], ROWS); }
+        mbar_init_fence();
+    }
+    if (warp == 8) tmem_alloc(&tmem_slot, 512);
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = tmem_slot;
+    volatile int* abort = &abort_flag;
+    // tensor memory: S and dP of the two tiles in flight, 64 columns each (P and dS go over them as 16-bit values);
+    // the accumulators of dQ / dK at 256 and of dV at 384
+    const float* st_lse = static_cast<const float*>(a.delta);
+    const float* st_delta = st_lse + int64_t(a.B) * a.Hq * LqP;
+
+    if (warp == 9) {
+        // ---- copies -------------------------------------------------------------------------------------------
+        const int64_t *as0 = KV ? a.ks : a.qs, *as1 = KV ? a.vs : a.dos, *bs0 = KV ? a.qs : a.ks, *bs1 = KV ? a.dos : a.vs;
+        if (lane == 0 && steps > 0) {
+            mbar_expect_bytes(&a_full, 2 * SM::ATILE);
+            load_tile(res, &maps.a0, DP / 64, SM::ABOX, r0, as0[2] ? oh : 0, as0[0] ? b : 0, &a_full);
+            load_tile(res + SM::ATILE, &maps.a1, DP / 64, SM::ABOX, r0, as1[2] ? oh : 0, as1[0] ? b : 0, &a_full);
+        }
+        int it = 0;
+        bool ok = true;
+        for (; it < steps; ++it) {
+            const int s = it % STAGES;
+            if (it >= STAGES) ok = mbar_wait_or_abort(&empty[s], (it / STAGES - 1) & 1, abort);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const int sh = KV ? oh * G + it / per_head : oh / G;           // streamed head
+            const int row = it % per_head * BROWS;
+            unsigned char* dst = ring + s * 2 * SM::BTILE;
+            const int rest = KV ? BROWS : n - row;
+            // K rows behind the valid states may hold anything, and 0 * NaN is NaN: they are cleared here.  (V
+            // needs nothing: its rows only make columns of dP that are masked.)
+            const bool clear = rest < BROWS && n < a.Lk;
+            uint64_t* bar = clear ? &tail : &full[s];
+            if (lane == 0) {
+                mbar_expect_bytes(bar, 2 * SM::BTILE + (KV ? SM::STATS : 0));
+                load_tile(dst, &maps.b0, DP / 64, SM::BBOX, row, bs0[2] ? sh : 0, bs0[0] ? b : 0, bar);
+                load_tile(dst + SM::BTILE, &maps.b1, DP / 64, SM::BBOX, row, bs1[2] ? sh : 0, bs1[0] ? b : 0, bar);
+                if (KV) {
+                    const int64_t at = (int64_t(b) * a.Hq + sh) * LqP + row;
+                    bulk_copy_g2s(stats + s * 2 * BROWS, st_lse + at, BROWS * 4, bar);
+                    bulk_copy_g2s(stats + s * 2 * BROWS + BROWS, st_delta + at, BROWS * 4, bar);
+                }
+            }
+            if (clear) {
+                ok = __all_sync(0xffffffffu, mbar_wait_or_abort(&tail, 0, abort));
+                for (int j = lane; j < (BROWS - rest) * 8 * (DP / 64); j += 32) {
+                    const int box = j / ((BROWS - rest) * 8), r = j % ((BROWS - rest) * 8);
+                    *reinterpret_cast<uint4*>(dst + box * SM::BBOX + rest * 128 + r * 16) = make_uint4(0, 0, 0, 0);
+                }
+                async_proxy_fence();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[s]);
+            }
+        }
+        if (!ok && lane == 0) {            // gave up: the copies issued so far still write to this block's memory
+            mbar_wait(&a_full, 0, 1 << 20);
+            for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j) mbar_wait(&full[j % STAGES], (j / STAGES) & 1, 1 << 20);
+        }
+    } else if (warp == 8) {
+        // ---- products -----------------------------------------------------------------------------------------
+        if (lane == 0 && steps > 0) {
+            constexpr uint32_t id_s = mma_idesc(is_bf16<T>, 128, BROWS, false);
+            constexpr uint32_t id_g = mma_idesc(is_bf16<T>, 128, DP, true);
+            const int ksteps = (a.D + 15) / 16;
+            const uint32_t a_addr = smem_u32(res), r_addr = smem_u32(ring);
+            auto scores = [&](int j) {
+                const uint32_t d = tmem + (j & 1) * 128, b_addr = r_addr + (j % STAGES) * 2 * SM::BTILE;
+                for (int w = 0; w < 2; ++w)
+                    for (int k = 0; k < ksteps; ++k)
+                        mma_ss(d + w * 64, desc_k_major(a_addr + w * SM::ATILE + (k / 4) * SM::ABOX + (k % 4) * 32),
+                               desc_k_major(b_addr + w * SM::BTILE + (k / 4) * SM::BBOX + (k % 4) * 32), id_s, k > 0);
+                mma_commit(&s_ready[j & 1]);
+            };
+            bool ok = mbar_wait_or_abort(&a_full, 0, abort) && mbar_wait_or_abort(&full[0], 0, abort);
+            if (ok) scores(0);
+            for (int j = 0; j < steps && ok; ++j) {
+                if (j + 1 < steps) {
+                    ok = mbar_wait_or_abort(&full[(j + 1) % STAGES], ((j + 1) / STAGES) & 1, abort);
+                    // goes over P and dS of tile j - 1, whose products were issued before: they run in order
+                    if (ok) scores(j + 1);
+                }
+                ok = ok && mbar_wait_or_abort(&p_ready[j & 1], (j / 2) & 1, abort);
+                if (!ok) break;
+                tmem_fence_after();
+                const uint32_t d = tmem + (j & 1) * 128, b_addr = r_addr + (j % STAGES) * 2 * SM::BTILE;
+                for (int k = 0; k < BROWS / 16; ++k)
+                    mma_ts(tmem + 256, d + 64 + k * 8, desc_mn_major(b_addr + k * 2048, SM::BBOX), id_g, j > 0 || k > 0);
+                if (KV)
+                    for (int k = 0; k < BROWS / 16; ++k)
+                        mma_ts(tmem + 384, d + k * 8, desc_mn_major(b_addr + SM::BTILE + k * 2048, SM::BBOX), id_g, j > 0 || k > 0);
+                mma_commit(&empty[j % STAGES]);
+            }
+            if (ok) {
+                mma_commit(&o_ready);
+                ok = mbar_wait_or_abort(&o_ready, 0, abort);
+            }
+            if (!ok) {                     // gave up: nothing may still write to the tensor memory that is freed below
+                mma_commit(&drain);
+                mbar_wait(&drain, 0, 1 << 20);
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- P and dS: one row per thread, a warpgroup takes every other tile ---------------------------------------
+        const int t = warp / 4;
+        const uint32_t lanes = tmem + (uint32_t(warp % 4) << 21);
+        const uint32_t s_at = lanes + t * 128;
+        const int row = r0 + (warp % 4) * 32 + lane;
+        const float c = float(a.scale * LOG2E);
+        float my_lse = 0.f, my_delta = 0.f;
+        if (!KV && row < a.Lq) {
+            my_lse = st_lse[(int64_t(b) * a.Hq + oh) * LqP + row];
+            my_delta = st_delta[(int64_t(b) * a.Hq + oh) * LqP + row];
+        }
+        const bool dead = KV ? row >= n : row >= a.Lq;     // rows of states without weight, rows behind the last
+        bool ok = true;
+        for (int j = t; j < steps; j += 2) {
+            ok = mbar_wait_or_abort(&full[j % STAGES], (j / STAGES) & 1, abort) &&
+                 mbar_wait_or_abort(&s_ready[t], (j / 2) & 1, abort);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            tmem_fence_after();
+            const float* sl = stats + (j % STAGES) * 2 * BROWS;
+            const int rest = KV ? BROWS : n - j * BROWS;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t s[32], d[32], p[16], q[16];
+                tmem_load32(s, s_at + half * 32);
+                tmem_load32(d, s_at + 64 + half * 32);
+                tmem_wait_load();
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    float pv[2], dv[2];
+#pragma unroll
+                    for (int f = 0; f < 2; ++f) {
+                        const int col = half * 32 + e + f;
+                        const float lse = KV ? sl[col] : my_lse, dl = KV ? sl[BROWS + col] : my_delta;
+                        const float x = ex2(__uint_as_float(s[e + f]) * c - lse);
+                        const bool off = dead || col >= rest;
+                        pv[f] = off ? 0.f : x;
+                        dv[f] = off ? 0.f : x * (__uint_as_float(d[e + f]) - dl);
+                    }
+                    p[e / 2] = pack2<T>(pv[0], pv[1]);
+                    q[e / 2] = pack2<T>(dv[0], dv[1]);
+                }
+                // P lands on columns of S that this thread has read: the first half goes over columns 0..15
+                if (KV) tmem_store16(s_at + half * 16, p);
+                tmem_store16(s_at + 64 + half * 16, q);
+            }
+            tmem_wait_store();
+            tmem_fence_before();
+            mbar_arrive(&p_ready[t]);
+        }
+        if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait_or_abort(&o_ready, 0, abort));
+        tmem_fence_after();
+        // warpgroup 0 writes dQ's lower columns (dK), warpgroup 1 the upper ones (dV)
+        const bool value = KV && t == 1;
+        const float f = !ok ? NAN : (value ? 1.f : float(a.scale));
+        T* out = static_cast<T*>(KV ? (value ? a.dv : a.dk) : a.dq) +
+                 (int64_t(b) * own_len * own_heads + int64_t(row) * own_heads + oh) * a.D;
+        const uint32_t o_at = lanes + 256 + (value ? 128 : 0);
+        constexpr int NJ = DP / 32;
+#pragma unroll 1
+        for (int j = KV ? 0 : t * (NJ / 2); j < (KV ? NJ : (t + 1) * (NJ / 2)); ++j) {
+            uint32_t o[32];
+            if (steps > 0 && ok) {
+                tmem_load32(o, o_at + j * 32);
+                tmem_wait_load();
+            }
+            const bool zero = ok && (steps == 0 || dead);
+            if (row < own_len) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    if (j * 32 + e < a.D) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = __uint_as_float(o[e + 2 * i]) * f, y = __uint_as_float(o[e + 2 * i + 1]) * f;
+                            w[i] = zero ? 0u : pack2<T>(ok ? x : NAN, ok ? y : NAN);
+                        }
+                        *reinterpret_cast<uint4*>(out + j * 32 + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+        }
+    }
+    tmem_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && abort_flag) atomicAdd(&g_timeouts, 1ull);
+    if (warp == 8) tmem_free(tmem, 512);
+}
+
+// ---------------------------------------------------------------------------
 // host side
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -361,6 +638,36 @@ int forward_t(cudaStream_t st, const AttnArgs& a) {
     return NNVB_OK;
 }
 
+template <typename T, int DP>
+int backward_t(cudaStream_t st, const AttnArgs& a) {
+    using SM = BwdSmem<DP>;
+    const int64_t LqP = round_up(a.Lq, BROWS);
+    const int64_t rows = LqP * a.B * a.Hq;
+    const int64_t bq = ceil_div(a.Lq, ROWS) * a.Hq * a.B, bk = ceil_div(a.Lk, ROWS) * a.Hkv * a.B;
+    NNVB_REQUIRE(ceil_div(rows, 16) < (int64_t(1) << 31) && bq < (int64_t(1) << 31) && bk < (int64_t(1) << 31),
+                 "nnvb_cross_attention_backward: too many tiles for one launch");
+    attn_stats_tc_kernel<T><<<unsigned(ceil_div(rows, 16)), 256, 0, st>>>(a, int(LqP));
+    NNVB_CUDA(cudaGetLastError());
+    BwdMaps mq{}, mk{};
+    NNVB_TRY(make_map(&mq.a0, a.dtype, a.q, a.qs, a.D, a.Lq, a.Hq, a.B, ROWS));
+    NNVB_TRY(make_map(&mq.a1, a.dtype, a.dout, a.dos, a.D, a.Lq, a.Hq, a.B, ROWS));
+    NNVB_TRY(make_map(&mq.b0, a.dtype, a.k, a.ks, a.D, a.Lk, a.Hkv, a.B, BROWS));
+    NNVB_TRY(make_map(&mq.b1, a.dtype, a.v, a.vs, a.D, a.Lk, a.Hkv, a.B, BROWS));
+    NNVB_TRY(make_map(&mk.a0, a.dtype, a.k, a.ks, a.D, a.Lk, a.Hkv, a.B, ROWS));
+    NNVB_TRY(make_map(&mk.a1, a.dtype, a.v, a.vs, a.D, a.Lk, a.Hkv, a.B, ROWS));
+    NNVB_TRY(make_map(&mk.b0, a.dtype, a.q, a.qs, a.D, a.Lq, a.Hq, a.B, BROWS));
+    NNVB_TRY(make_map(&mk.b1, a.dtype, a.dout, a.dos, a.D, a.Lq, a.Hq, a.B, BROWS));
+    auto kq = attn_bwd_tc_kernel<T, DP, false>;
+    auto kk = attn_bwd_tc_kernel<T, DP, true>;
+    NNVB_CUDA(cudaFuncSetAttribute(kq, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::BYTES));
+    NNVB_CUDA(cudaFuncSetAttribute(kk, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::BYTES));
+    kq<<<unsigned(bq), FWD_THREADS, SM::BYTES, st>>>(mq, a, int(LqP));
+    NNVB_CUDA(cudaGetLastError());
+    kk<<<unsigned(bk), FWD_THREADS, SM::BYTES, st>>>(mk, a, int(LqP));
+    NNVB_CUDA(cudaGetLastError());
+    return NNVB_OK;
+}
+
 }  // namespace
 
 bool attn_tc_takes_forward(const AttnArgs& a) {
@@ -375,6 +682,16 @@ bool attn_tc_takes_forward(const AttnArgs& a) {
 int attn_forward_tc(cudaStream_t st, const AttnArgs& a) {
     if (a.dtype == NNVB_BF16) return a.D <= 64 ? forward_t<__nv_bfloat16, 64>(st, a) : forward_t<__nv_bfloat16, 128>(st, a);
     return a.D <= 64 ? forward_t<__half, 64>(st, a) : forward_t<__half, 128>(st, a);
+}
+
+bool attn_tc_takes_backward(const AttnArgs& a) {
+    auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    return attn_tc_takes_forward(a) && tma_rows(a.dout, a.dos, a.Lq) && aligned(a.dq) && aligned(a.dk) && aligned(a.dv);
+}
+
+int attn_backward_tc(cudaStream_t st, const AttnArgs& a) {
+    if (a.dtype == NNVB_BF16) return a.D <= 64 ? backward_t<__nv_bfloat16, 64>(st, a) : backward_t<__nv_bfloat16, 128>(st, a);
+    return a.D <= 64 ? backward_t<__half, 64>(st, a) : backward_t<__half, 128>(st, a);
 }
 
 }  // namespace nnvb
