@@ -144,16 +144,17 @@ SIGNATURES = {
     # device pointers travel as integers (c_void_p)
     "nnvb_estimate_ranges_noalloc": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
                                                C.c_void_p, C.c_void_p, C.c_void_p]),
+    # an nnvb_attention_desc travels as an address too: AttentionDesc by reference or its packed bytes
     "nnvb_layer_norm_forward": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
                                           C.c_void_p, C.c_double, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
     "nnvb_layer_norm_workspace": (C.c_int64, [C.c_int, C.c_int64, C.c_int64]),
     "nnvb_layer_norm_backward": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
                                            C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
                                            C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64]),
-    "nnvb_cross_attention_forward": (C.c_int, [C.c_void_p, C.POINTER(AttentionDesc), C.c_void_p, C.c_void_p, C.c_void_p,
+    "nnvb_cross_attention_forward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                                C.c_void_p, C.c_void_p, C.c_void_p]),
-    "nnvb_cross_attention_workspace": (C.c_int64, [C.POINTER(AttentionDesc)]),
-    "nnvb_cross_attention_backward": (C.c_int, [C.c_void_p, C.POINTER(AttentionDesc), C.c_void_p, C.c_void_p, C.c_void_p,
+    "nnvb_cross_attention_workspace": (C.c_int64, [C.c_void_p]),
+    "nnvb_cross_attention_backward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                                 C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                                 C.c_void_p, C.c_void_p, C.c_int64]),
 }

@@ -20,6 +20,10 @@ def _desc(**kw):
 def test_descriptor_layout():
     assert C.sizeof(_lib.AttentionDesc) == 8 + 6 * 8 + 8 + 5 * 24
     assert _lib.AttentionDesc.scale.offset == 56 and _lib.AttentionDesc.q_stride.offset == 64
+    d = _desc()
+    packed = ops._DESC.pack(_lib.BF16, 0, 2, 3, 4, 8, 2, 16, 0.25, *d.q_stride, *d.k_stride, *d.v_stride, *d.out_stride,
+                            *d.dout_stride)
+    assert packed == bytes(d)
 
 
 @pytest.mark.parametrize("change,word", [
