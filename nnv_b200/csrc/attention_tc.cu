@@ -39,6 +39,14 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi
     return *reinterpret_cast<uint32_t*>(&x);
 }
 
+// the halves of a packed register as floats
+template <typename T> __device__ __forceinline__ float unpack_lo(uint32_t x);
+template <typename T> __device__ __forceinline__ float unpack_hi(uint32_t x);
+template <> __device__ __forceinline__ float unpack_lo<__nv_bfloat16>(uint32_t x) { return __uint_as_float(x << 16); }
+template <> __device__ __forceinline__ float unpack_hi<__nv_bfloat16>(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+template <> __device__ __forceinline__ float unpack_lo<__half>(uint32_t x) { return __half2float(__ushort_as_half(x & 0xffff)); }
+template <> __device__ __forceinline__ float unpack_hi<__half>(uint32_t x) { return __half2float(__ushort_as_half(x >> 16)); }
+
 // 2^x to about 2 units in the last place, 0 below 2^-126: the weights' own rounding is 2^15 times coarser
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -115,7 +123,7 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
         for (int i = 0; i < steps && ok; ++i) {
             for (int kv = 0; kv < 2; ++kv, ++it) {
                 const int s = it % STAGES;
-                if (it >= STAGES) ok = mbar_wait_or_abort(&empty[s], (it / STAGES - 1) & 1, abort);
+                if (it >= STAGES) ok = mbar_wait_fast(&empty[s], (it / STAGES - 1) & 1, abort);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 unsigned char* dst = ring + s * SM::TILE;
@@ -127,7 +135,7 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
                         mbar_expect_bytes(&tail, SM::TILE);
                         load_tile(dst, &maps.v, DP / 64, SM::BOX, i * ROWS, vh, vb, &tail);
                     }
-                    ok = __all_sync(0xffffffffu, mbar_wait_or_abort(&tail, 0, abort));
+                    ok = __all_sync(0xffffffffu, mbar_wait_fast(&tail, 0, abort));
                     for (int j = lane; j < (ROWS - rest) * 8 * (DP / 64); j += 32) {
                         const int box = j / ((ROWS - rest) * 8), r = j % ((ROWS - rest) * 8);
                         *reinterpret_cast<uint4*>(dst + box * SM::BOX + rest * 128 + r * 16) = make_uint4(0, 0, 0, 0);
@@ -153,13 +161,15 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
             const int ksteps = (a.D + 15) / 16;
             const uint32_t q_addr = smem_u32(sq), r_addr = smem_u32(ring);
             auto scores = [&](int t, int s) {
-                for (int k = 0; k < ksteps; ++k) {
-                    const uint32_t off = (k / 4) * SM::BOX + (k % 4) * 32;
-                    mma_ss(tmem + t * 128, desc_k_major(q_addr + t * SM::TILE + off), desc_k_major(r_addr + s * SM::TILE + off), id_s, k > 0);
+                const uint32_t qd = desc_k_major(q_addr + t * SM::TILE), kd = desc_k_major(r_addr + s * SM::TILE);
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) {
+                    const uint32_t off = ((k / 4) * SM::BOX + (k % 4) * 32) >> 4;
+                    if (k < ksteps) mma_ss(tmem + t * 128, qd + off, kd + off, id_s, k > 0);
                 }
                 mma_commit(&s_ready[t]);
             };
-            bool ok = mbar_wait_or_abort(&q_full, 0, abort) && mbar_wait_or_abort(&full[0], 0, abort);
+            bool ok = mbar_wait_fast(&q_full, 0, abort) && mbar_wait_fast(&full[0], 0, abort);
             if (ok) {
                 for (int t = 0; t < live; ++t) scores(t, 0);
                 mma_commit(&empty[0]);
@@ -167,15 +177,16 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
             for (int i = 0; i < steps && ok; ++i) {
                 const int vi = 2 * i + 1, ki = 2 * i + 2;
                 const bool next = i + 1 < steps;
-                ok = mbar_wait_or_abort(&full[vi % STAGES], (vi / STAGES) & 1, abort);
-                if (ok && next) ok = mbar_wait_or_abort(&full[ki % STAGES], (ki / STAGES) & 1, abort);
+                ok = mbar_wait_fast(&full[vi % STAGES], (vi / STAGES) & 1, abort);
+                if (ok && next) ok = mbar_wait_fast(&full[ki % STAGES], (ki / STAGES) & 1, abort);
                 for (int t = 0; t < live && ok; ++t) {
-                    ok = mbar_wait_or_abort(&p_ready[t], i & 1, abort);
+                    ok = mbar_wait_fast(&p_ready[t], i & 1, abort);
                     if (!ok) break;
                     tmem_fence_after();
+                    const uint32_t vd = desc_mn_major(r_addr + (vi % STAGES) * SM::TILE, SM::BOX);
+#pragma unroll
                     for (int k = 0; k < ROWS / 16; ++k)
-                        mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8,
-                               desc_mn_major(r_addr + (vi % STAGES) * SM::TILE + k * 2048, SM::BOX), id_o, i > 0 || k > 0);
+                        mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, vd + k * (2048 >> 4), id_o, i > 0 || k > 0);
                     // S of the next states goes over P of these: products issued by one thread run in order
                     if (next) scores(t, ki % STAGES);
                     else mma_commit(&o_ready[t]);
@@ -186,7 +197,7 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
                 }
             }
             // the last commit has arrived: nothing touches this block's barriers after it has left
-            if (ok) ok = mbar_wait_or_abort(&empty[(2 * steps - 1) % STAGES], ((2 * steps - 1) / STAGES) & 1, abort);
+            if (ok) ok = mbar_wait_fast(&empty[(2 * steps - 1) % STAGES], ((2 * steps - 1) / STAGES) & 1, abort);
             if (!ok) {                     // gave up: nothing may still write to the tensor memory that is freed below
                 mma_commit(&drain);
                 mbar_wait(&drain, 0, 1 << 20);
@@ -203,7 +214,7 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
         float m = -INFINITY, l = 0.f;      // m: the maximum in use, of the scores without the factor
         bool ok = true;
         for (int i = 0; i < steps; ++i) {
-            ok = mbar_wait_or_abort(&s_ready[t], i & 1, abort);
+            ok = mbar_wait_fast(&s_ready[t], i & 1, abort);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tmem_fence_after();
             uint32_t s[4][32];
@@ -256,7 +267,7 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
             tmem_fence_before();
             mbar_arrive(&p_ready[t]);
         }
-        if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait_or_abort(&o_ready[t], 0, abort));
+        if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait_fast(&o_ready[t], 0, abort));
         tmem_fence_after();
         const float f = !ok ? NAN : (n > 0 ? 1.f / l : 0.f);
         T* out = static_cast<T*>(const_cast<void*>(a.o)) + int64_t(b) * a.os[0] + int64_t(row) * a.os[1] + int64_t(h) * a.os[2];
@@ -299,13 +310,23 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
 //   dQ       resident Q and dO (128 positions), streamed K and V:   S = Q K^T,  dP = dO V^T,  dQ += dS K
 //   dK, dV   resident K and V (128 states), streamed Q and dO of every query head of the group:
 //            S^T = K Q^T,  dP^T = V dO^T,  dV += P^T dO,  dK += dS^T Q
-// so each gradient row is summed in tensor memory by one block, in a fixed order.  That costs seven products a pair
-// instead of five with atomic additions to dQ.  Streamed tiles have 64 rows, which lets two of them be in flight in
-// tensor memory beside 128 x 128 accumulators: while one tile is in the softmax arithmetic of a warpgroup the next
-// one's S and dP run.  P and dS are rounded to the tensors' type (operands of 16-bit products); everything else is fp32.
-// Streamed tiles serve as K-major operand of S and dP and as MN-major operand of the gradients.
+// so each gradient row is summed in tensor memory by one block, in a fixed order.  Separate passes compute S and dP
+// twice: seven products a pair instead of the five of one pass that would add to dQ atomically.
+//
+// Streamed tiles have 64 rows, which lets two of them be in flight in tensor memory beside 128 x 128 accumulators;
+// they serve as K-major operand of S and dP and as MN-major operand of the gradients.  Sixteen warps do the softmax
+// arithmetic: two warpgroups per tile in flight, one row and half of its 64 columns per thread (with one warpgroup per
+// tile the products waited for it: a quarter of the tensor pipe's cycles were used).
+//
+// Roundings: P is rounded to the tensors' type, as in the forward pass.  dS enters its product as the sum of two
+// 16-bit values (its rounding and the rounding of what is left), an eighth and a ninth product: its rounding error
+// would be as large as that of storing dQ and dK, and the terms of dS cancel in their row sums.  delta comes from the
+// stored output, whose rounding weighs little once a row attends to many states; entries of up to 128 states, where
+// the pass over dQ holds whole rows of P and dP in tensor memory, take the exact sum of P dP instead.
 
 constexpr int BROWS = 64;                          // rows of a streamed tile
+constexpr int BWD_SOFT = 512;                      // threads of the softmax arithmetic
+constexpr int BWD_THREADS = BWD_SOFT + 64;
 
 template <int DP>
 struct BwdSmem {
@@ -345,7 +366,7 @@ attn_stats_tc_kernel(AttnArgs a, int LqP) {
 }
 
 template <typename T, int DP, bool KV>
-__global__ void __launch_bounds__(FWD_THREADS, 1)
+__global__ void __launch_bounds__(BWD_THREADS, 1)
 attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
     using SM = BwdSmem<DP>;
     constexpr int STAGES = SM::STAGES;
@@ -354,9 +375,10 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
     unsigned char* res = base;                             // A0, A1
     unsigned char* ring = base + 2 * SM::ATILE;            // B0, B1 per stage
     float* stats = reinterpret_cast<float*>(ring + STAGES * 2 * SM::BTILE);
-    __shared__ uint64_t full[STAGES], empty[STAGES], a_full, s_ready[2], p_ready[2], o_ready, tail, drain;
+    __shared__ uint64_t full[STAGES], empty[STAGES], a_full, s_ready[2], p_ready[2], o_ready, x_ready, tail, drain;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
+    __shared__ float row_sum[4][ROWS];
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int own_len = KV ? a.Lk : a.Lq, own_heads = KV ? a.Hkv : a.Hq;
@@ -373,24 +395,26 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
         abort_flag = 0;
         for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         mbar_init(&a_full, 1);
+        mbar_init(&x_ready, steps > 1 ? 4 * ROWS : 2 * ROWS);
         mbar_init(&o_ready, 1);
         mbar_init(&tail, 1);
         mbar_init(&drain, 1);
-        for (int t = 0; t < 2; ++t) { mbar_init(&s_ready[t], 1); mbar_init(&p_ready[t], ROWS); }
+        for (int t = 0; t < 2; ++t) { mbar_init(&s_ready[t], 1); mbar_init(&p_ready[t], 2 * ROWS); }
         mbar_init_fence();
     }
-    if (warp == 8) tmem_alloc(&tmem_slot, 512);
+    if (warp == 16) tmem_alloc(&tmem_slot, 512);
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
     const uint32_t tmem = tmem_slot;
     volatile int* abort = &abort_flag;
-    // tensor memory: S and dP of the two tiles in flight, 64 columns each (P and dS go over them as 16-bit values);
-    // the accumulators of dQ / dK at 256 and of dV at 384
+    // Tensor memory, columns: tile in flight t at 128 t: S 0..63, dP 64..127; the accumulators of dQ / dK at 256 and of
+    // dV at 384.  The two warpgroups of a tile own 32 columns of S and of dP each and put their 16-bit operands there:
+    // P over the lower half of their columns of S, the rest of dS over the upper half, dS over the lower half of dP.
     const float* st_lse = static_cast<const float*>(a.delta);
-    const float* st_delta = st_lse + int64_t(a.B) * a.Hq * LqP;
+    float* st_delta = static_cast<float*>(a.delta) + int64_t(a.B) * a.Hq * LqP;
 
-    if (warp == 9) {
+    if (warp == 17) {
         // ---- copies -------------------------------------------------------------------------------------------
         const int64_t *as0 = KV ? a.ks : a.qs, *as1 = KV ? a.vs : a.dos, *bs0 = KV ? a.qs : a.ks, *bs1 = KV ? a.dos : a.vs;
         if (lane == 0 && steps > 0) {
@@ -402,7 +426,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
         bool ok = true;
         for (; it < steps; ++it) {
             const int s = it % STAGES;
-            if (it >= STAGES) ok = mbar_wait_or_abort(&empty[s], (it / STAGES - 1) & 1, abort);
+            if (it >= STAGES) ok = mbar_wait_fast(&empty[s], (it / STAGES - 1) & 1, abort);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const int sh = KV ? oh * G + it / per_head : oh / G;           // streamed head
@@ -424,7 +448,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
                 }
             }
             if (clear) {
-                ok = __all_sync(0xffffffffu, mbar_wait_or_abort(&tail, 0, abort));
+                ok = __all_sync(0xffffffffu, mbar_wait_fast(&tail, 0, abort));
                 for (int j = lane; j < (BROWS - rest) * 8 * (DP / 64); j += 32) {
                     const int box = j / ((BROWS - rest) * 8), r = j % ((BROWS - rest) * 8);
                     *reinterpret_cast<uint4*>(dst + box * SM::BBOX + rest * 128 + r * 16) = make_uint4(0, 0, 0, 0);
@@ -438,7 +462,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
             mbar_wait(&a_full, 0, 1 << 20);
             for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j) mbar_wait(&full[j % STAGES], (j / STAGES) & 1, 1 << 20);
         }
-    } else if (warp == 8) {
+    } else if (warp == 16) {
         // ---- products -----------------------------------------------------------------------------------------
         if (lane == 0 && steps > 0) {
             constexpr uint32_t id_s = mma_idesc(is_bf16<T>, 128, BROWS, false);
@@ -447,34 +471,42 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
             const uint32_t a_addr = smem_u32(res), r_addr = smem_u32(ring);
             auto scores = [&](int j) {
                 const uint32_t d = tmem + (j & 1) * 128, b_addr = r_addr + (j % STAGES) * 2 * SM::BTILE;
-                for (int w = 0; w < 2; ++w)
-                    for (int k = 0; k < ksteps; ++k)
-                        mma_ss(d + w * 64, desc_k_major(a_addr + w * SM::ATILE + (k / 4) * SM::ABOX + (k % 4) * 32),
-                               desc_k_major(b_addr + w * SM::BTILE + (k / 4) * SM::BBOX + (k % 4) * 32), id_s, k > 0);
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const uint32_t ad = desc_k_major(a_addr + w * SM::ATILE), bd = desc_k_major(b_addr + w * SM::BTILE);
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k)
+                        if (k < ksteps)
+                            mma_ss(d + w * 64, ad + (((k / 4) * SM::ABOX + (k % 4) * 32) >> 4), bd + (((k / 4) * SM::BBOX + (k % 4) * 32) >> 4),
+                                   id_s, k > 0);
+                }
                 mma_commit(&s_ready[j & 1]);
             };
-            bool ok = mbar_wait_or_abort(&a_full, 0, abort) && mbar_wait_or_abort(&full[0], 0, abort);
+            bool ok = mbar_wait_fast(&a_full, 0, abort) && mbar_wait_fast(&full[0], 0, abort);
             if (ok) scores(0);
             for (int j = 0; j < steps && ok; ++j) {
                 if (j + 1 < steps) {
-                    ok = mbar_wait_or_abort(&full[(j + 1) % STAGES], ((j + 1) / STAGES) & 1, abort);
+                    ok = mbar_wait_fast(&full[(j + 1) % STAGES], ((j + 1) / STAGES) & 1, abort);
                     // goes over P and dS of tile j - 1, whose products were issued before: they run in order
                     if (ok) scores(j + 1);
                 }
-                ok = ok && mbar_wait_or_abort(&p_ready[j & 1], (j / 2) & 1, abort);
+                ok = ok && mbar_wait_fast(&p_ready[j & 1], (j / 2) & 1, abort);
                 if (!ok) break;
                 tmem_fence_after();
                 const uint32_t d = tmem + (j & 1) * 128, b_addr = r_addr + (j % STAGES) * 2 * SM::BTILE;
-                for (int k = 0; k < BROWS / 16; ++k)
-                    mma_ts(tmem + 256, d + 64 + k * 8, desc_mn_major(b_addr + k * 2048, SM::BBOX), id_g, j > 0 || k > 0);
-                if (KV)
-                    for (int k = 0; k < BROWS / 16; ++k)
-                        mma_ts(tmem + 384, d + k * 8, desc_mn_major(b_addr + SM::BTILE + k * 2048, SM::BBOX), id_g, j > 0 || k > 0);
+                const uint32_t b0 = desc_mn_major(b_addr, SM::BBOX), b1 = desc_mn_major(b_addr + SM::BTILE, SM::BBOX);
+#pragma unroll
+                for (int k = 0; k < BROWS / 16; ++k) {
+                    const uint32_t at = d + (k / 2) * 32 + (k % 2) * 8;
+                    mma_ts(tmem + 256, at + 64, b0 + k * (2048 >> 4), id_g, j > 0 || k > 0);
+                    mma_ts(tmem + 256, at + 16, b0 + k * (2048 >> 4), id_g, true);
+                    if (KV) mma_ts(tmem + 384, at, b1 + k * (2048 >> 4), id_g, j > 0 || k > 0);
+                }
                 mma_commit(&empty[j % STAGES]);
             }
             if (ok) {
                 mma_commit(&o_ready);
-                ok = mbar_wait_or_abort(&o_ready, 0, abort);
+                ok = mbar_wait_fast(&o_ready, 0, abort);
             }
             if (!ok) {                     // gave up: nothing may still write to the tensor memory that is freed below
                 mma_commit(&drain);
@@ -483,66 +515,91 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
         }
         __syncwarp();
     } else {
-        // ---- P and dS: one row per thread, a warpgroup takes every other tile ---------------------------------------
-        const int t = warp / 4;
+        // ---- P and dS ---------------------------------------------------------------------------------------------
+        const int wg = warp / 4, t = wg / 2, half = wg % 2;
         const uint32_t lanes = tmem + (uint32_t(warp % 4) << 21);
-        const uint32_t s_at = lanes + t * 128;
-        const int row = r0 + (warp % 4) * 32 + lane;
+        const uint32_t s_at = lanes + t * 128 + half * 32, d_at = s_at + 64;
+        const int local = (warp % 4) * 32 + lane, row = r0 + local;
         const float c = float(a.scale * LOG2E);
         float my_lse = 0.f, my_delta = 0.f;
         if (!KV && row < a.Lq) {
             my_lse = st_lse[(int64_t(b) * a.Hq + oh) * LqP + row];
             my_delta = st_delta[(int64_t(b) * a.Hq + oh) * LqP + row];
         }
-        const bool dead = KV ? row >= n : row >= a.Lq;     // rows of states without weight, rows behind the last
         bool ok = true;
         for (int j = t; j < steps; j += 2) {
-            ok = mbar_wait_or_abort(&full[j % STAGES], (j / STAGES) & 1, abort) &&
-                 mbar_wait_or_abort(&s_ready[t], (j / 2) & 1, abort);
+            ok = mbar_wait_fast(&full[j % STAGES], (j / STAGES) & 1, abort) &&
+                 mbar_wait_fast(&s_ready[t], (j / 2) & 1, abort);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tmem_fence_after();
-            const float* sl = stats + (j % STAGES) * 2 * BROWS;
-            const int rest = KV ? BROWS : n - j * BROWS;
+            const float* sl = stats + (j % STAGES) * 2 * BROWS + half * 32;
+            const int rest = KV ? 32 : n - j * BROWS - half * 32;          // columns with weight
+            uint32_t s[32];
+            tmem_load32(s, s_at);
+            tmem_wait_load();
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t s[32], d[32], p[16], q[16];
-                tmem_load32(s, s_at + half * 32);
-                tmem_load32(d, s_at + 64 + half * 32);
+            for (int e = 0; e < 32; ++e) {
+                const float x = ex2(__uint_as_float(s[e]) * c - (KV ? sl[e] : my_lse));
+                s[e] = __float_as_uint(!KV && e >= rest ? 0.f : x);
+            }
+            if (!KV && steps <= 2) {
+                float sum = 0.f;
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    uint32_t d[16];
+                    tmem_load16(d, d_at + g * 16);
+                    tmem_wait_load();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (g * 16 + e < rest) sum += __uint_as_float(s[g * 16 + e]) * __uint_as_float(d[e]);
+                }
+                row_sum[wg][local] = sum;
+                mbar_arrive(&x_ready);
+                ok = __all_sync(0xffffffffu, mbar_wait_fast(&x_ready, 0, abort));
+                if (!ok) break;
+                my_delta = row_sum[0][local] + row_sum[1][local];
+                if (steps == 2) my_delta += row_sum[2][local] + row_sum[3][local];
+                if (wg == 0 && row < a.Lq) st_delta[(int64_t(b) * a.Hq + oh) * LqP + row] = my_delta;     // for the pass over dK, dV
+            }
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                uint32_t d[16], p[8], hi[8], lo[8];
+                tmem_load16(d, d_at + g * 16);
                 tmem_wait_load();
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    float pv[2], dv[2];
+                for (int e = 0; e < 16; e += 2) {
+                    float ds[2];
 #pragma unroll
                     for (int f = 0; f < 2; ++f) {
-                        const int col = half * 32 + e + f;
-                        const float lse = KV ? sl[col] : my_lse, dl = KV ? sl[BROWS + col] : my_delta;
-                        const float x = ex2(__uint_as_float(s[e + f]) * c - lse);
-                        const bool off = dead || col >= rest;
-                        pv[f] = off ? 0.f : x;
-                        dv[f] = off ? 0.f : x * (__uint_as_float(d[e + f]) - dl);
+                        const int col = g * 16 + e + f;
+                        ds[f] = __uint_as_float(s[col]) * (__uint_as_float(d[e + f]) - (KV ? sl[BROWS + col] : my_delta));
+                        if (!KV && col >= rest) ds[f] = 0.f;               // dP there may be 0 * NaN
                     }
-                    p[e / 2] = pack2<T>(pv[0], pv[1]);
-                    q[e / 2] = pack2<T>(dv[0], dv[1]);
+                    if (KV) p[e / 2] = pack2<T>(__uint_as_float(s[g * 16 + e]), __uint_as_float(s[g * 16 + e + 1]));
+                    hi[e / 2] = pack2<T>(ds[0], ds[1]);
+                    lo[e / 2] = pack2<T>(ds[0] - unpack_lo<T>(hi[e / 2]), ds[1] - unpack_hi<T>(hi[e / 2]));
                 }
-                // P lands on columns of S that this thread has read: the first half goes over columns 0..15
-                if (KV) tmem_store16(s_at + half * 16, p);
-                tmem_store16(s_at + 64 + half * 16, q);
+                if (KV) tmem_store8(s_at + g * 8, p);
+                tmem_store8(s_at + 16 + g * 8, lo);
+                tmem_store8(d_at + g * 8, hi);
             }
             tmem_wait_store();
             tmem_fence_before();
             mbar_arrive(&p_ready[t]);
         }
-        if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait_or_abort(&o_ready, 0, abort));
+        if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait_fast(&o_ready, 0, abort));
         tmem_fence_after();
-        // warpgroup 0 writes dQ's lower columns (dK), warpgroup 1 the upper ones (dV)
+        // dK: warpgroups 0 and 1, dV: 2 and 3, half of the columns each; dQ: every warpgroup a chunk of 32
         const bool value = KV && t == 1;
+        const bool dead = KV && row >= n;                  // states without weight: their rows of S may hold anything
         const float f = !ok ? NAN : (value ? 1.f : float(a.scale));
         T* out = static_cast<T*>(KV ? (value ? a.dv : a.dk) : a.dq) +
                  (int64_t(b) * own_len * own_heads + int64_t(row) * own_heads + oh) * a.D;
         const uint32_t o_at = lanes + 256 + (value ? 128 : 0);
         constexpr int NJ = DP / 32;
+        const int j0 = KV ? half * (NJ / 2) : wg, j1 = KV ? j0 + NJ / 2 : (wg < NJ ? wg + 1 : wg);
 #pragma unroll 1
-        for (int j = KV ? 0 : t * (NJ / 2); j < (KV ? NJ : (t + 1) * (NJ / 2)); ++j) {
+        for (int j = j0; j < j1; ++j) {
             uint32_t o[32];
             if (steps > 0 && ok) {
                 tmem_load32(o, o_at + j * 32);
@@ -568,7 +625,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
     tmem_fence_before();
     __syncthreads();
     if (threadIdx.x == 0 && abort_flag) atomicAdd(&g_timeouts, 1ull);
-    if (warp == 8) tmem_free(tmem, 512);
+    if (warp == 16) tmem_free(tmem, 512);
 }
 
 // ---------------------------------------------------------------------------
@@ -661,9 +718,9 @@ int backward_t(cudaStream_t st, const AttnArgs& a) {
     auto kk = attn_bwd_tc_kernel<T, DP, true>;
     NNVB_CUDA(cudaFuncSetAttribute(kq, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::BYTES));
     NNVB_CUDA(cudaFuncSetAttribute(kk, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::BYTES));
-    kq<<<unsigned(bq), FWD_THREADS, SM::BYTES, st>>>(mq, a, int(LqP));
+    kq<<<unsigned(bq), BWD_THREADS, SM::BYTES, st>>>(mq, a, int(LqP));
     NNVB_CUDA(cudaGetLastError());
-    kk<<<unsigned(bk), FWD_THREADS, SM::BYTES, st>>>(mk, a, int(LqP));
+    kk<<<unsigned(bk), BWD_THREADS, SM::BYTES, st>>>(mk, a, int(LqP));
     NNVB_CUDA(cudaGetLastError());
     return NNVB_OK;
 }

@@ -18,12 +18,12 @@ namespace nnvb {
 
 // ---- descriptors ---------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t leading_bytes, uint32_t stride_bytes) {
-    return uint64_t((addr & 0x3ffff) >> 4) | uint64_t(leading_bytes >> 4) << 16 | uint64_t(stride_bytes >> 4) << 32 |
-           uint64_t(1) << 46 | uint64_t(2) << 61;         // descriptor version 1, 128-byte swizzle
-}
-__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) { return smem_desc(addr, 16, 1024); }
-__device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr, uint32_t tile_bytes) { return smem_desc(addr, tile_bytes, 1024); }
+// The low word holds the address and the leading stride, the high word (stride of eight rows, version 1, 128-byte
+// swizzle) is the same for all: a step moves the low word by its bytes / 16.  One thread issues every product of a block,
+// so what it computes per product counts.
+constexpr uint32_t DESC_HIGH = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_k_major(uint32_t addr) { return (addr >> 4) | 1u << 16; }
+__device__ __forceinline__ uint32_t desc_mn_major(uint32_t addr, uint32_t tile_bytes) { return (addr >> 4) | (tile_bytes >> 4) << 16; }
 
 // 16-bit operands, fp32 accumulator; b_mn: B is MN-major
 __host__ __device__ constexpr uint32_t mma_idesc(bool bf16, int M, int N, bool b_mn) {
@@ -55,6 +55,18 @@ __device__ __forceinline__ void tmem_load32(uint32_t (&r)[32], uint32_t addr) {
           "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
 }
+__device__ __forceinline__ void tmem_load16(uint32_t (&r)[16], uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
@@ -77,23 +89,33 @@ __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::
 
 // ---- matrix products (one thread issues) -----------------------------------------------------------------------------
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-        "r"(uint32_t(accumulate))
+        "{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.u32 p, %4, 0;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %5};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+        "r"(uint32_t(accumulate)), "r"(DESC_HIGH)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
-        "r"(uint32_t(accumulate))
+        "{\n .reg .pred p;\n .reg .b64 y;\n setp.ne.u32 p, %4, 0;\n mov.b64 y, {%2, %5};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+        "r"(uint32_t(accumulate)), "r"(DESC_HIGH)
         : "memory");
 }
 // one arrival on the barrier once every product this thread has issued is done
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// mbar_wait_or_abort whose first look costs no clock read: most waits on the path of the products find their barrier done
+__device__ __forceinline__ bool mbar_wait_fast(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok)
+                 : "r"(smem_u32(bar)), "r"(parity)
+                 : "memory");
+    return ok || mbar_wait_or_abort(bar, parity, abort_flag);
 }
 
 // ---- tensor copies -----------------------------------------------------------------------------------------------------
