@@ -100,14 +100,14 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
         mbar_init(&q_full, 1);
         mbar_init(&tail, 1);
         mbar_init(&drain, 1);
-        for (int t = 0; t < 2; ++t) { mbar_init(&s_ready[t], 1); mbar_init(&p_ready[t], ROWS); mbar_init(&o_ready[t], 1); }
+        for (int t = 0; t < 2; ++t) { mbar_init(&s_ready[t], 1); mbar_init(&p_ready[t], 4); mbar_init(&o_ready[t], 1); }
         mbar_init_fence();
     }
     if (warp == 8) tmem_alloc(&tmem_slot, 512);
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    const uint32_t tmem = tmem_slot;
+    constexpr uint32_t tmem = 0;           // all 512 columns are this block's, so they start at column 0
     volatile int* abort = &abort_flag;
 
     if (warp == 9) {
@@ -155,7 +155,8 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
         }
     } else if (warp == 8) {
         // ---- products -----------------------------------------------------------------------------------------
-        if (lane == 0 && n > 0) {
+        const uint32_t leader = elect_lane();
+        if (n > 0) {
             constexpr uint32_t id_s = mma_idesc(is_bf16<T>, 128, ROWS, false);
             constexpr uint32_t id_o = mma_idesc(is_bf16<T>, 128, DP, true);
             const int ksteps = (a.D + 15) / 16;
@@ -165,41 +166,41 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k) {
                     const uint32_t off = ((k / 4) * SM::BOX + (k % 4) * 32) >> 4;
-                    if (k < ksteps) mma_ss(tmem + t * 128, qd + off, kd + off, id_s, k > 0);
+                    if (k < ksteps) mma_ss(leader, tmem + t * 128, qd + off, kd + off, id_s, k > 0);
                 }
-                mma_commit(&s_ready[t]);
+                mma_commit(leader, &s_ready[t]);
             };
-            bool ok = mbar_wait_fast(&q_full, 0, abort) && mbar_wait_fast(&full[0], 0, abort);
+            bool ok = warp_wait(&q_full, 0, abort) && warp_wait(&full[0], 0, abort);
             if (ok) {
                 for (int t = 0; t < live; ++t) scores(t, 0);
-                mma_commit(&empty[0]);
+                mma_commit(leader, &empty[0]);
             }
             for (int i = 0; i < steps && ok; ++i) {
                 const int vi = 2 * i + 1, ki = 2 * i + 2;
                 const bool next = i + 1 < steps;
-                ok = mbar_wait_fast(&full[vi % STAGES], (vi / STAGES) & 1, abort);
-                if (ok && next) ok = mbar_wait_fast(&full[ki % STAGES], (ki / STAGES) & 1, abort);
+                ok = warp_wait(&full[vi % STAGES], (vi / STAGES) & 1, abort);
+                if (ok && next) ok = warp_wait(&full[ki % STAGES], (ki / STAGES) & 1, abort);
                 for (int t = 0; t < live && ok; ++t) {
-                    ok = mbar_wait_fast(&p_ready[t], i & 1, abort);
+                    ok = warp_wait(&p_ready[t], i & 1, abort);
                     if (!ok) break;
                     tmem_fence_after();
                     const uint32_t vd = desc_mn_major(r_addr + (vi % STAGES) * SM::TILE, SM::BOX);
 #pragma unroll
                     for (int k = 0; k < ROWS / 16; ++k)
-                        mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, vd + k * (2048 >> 4), id_o, i > 0 || k > 0);
+                        mma_ts(leader, tmem + 256 + t * 128, tmem + t * 128 + k * 8, vd + k * (2048 >> 4), id_o, i > 0 || k > 0);
                     // S of the next states goes over P of these: products issued by one thread run in order
                     if (next) scores(t, ki % STAGES);
-                    else mma_commit(&o_ready[t]);
+                    else mma_commit(leader, &o_ready[t]);
                 }
                 if (ok) {
-                    mma_commit(&empty[vi % STAGES]);
-                    if (next) mma_commit(&empty[ki % STAGES]);
+                    mma_commit(leader, &empty[vi % STAGES]);
+                    if (next) mma_commit(leader, &empty[ki % STAGES]);
                 }
             }
             // the last commit has arrived: nothing touches this block's barriers after it has left
-            if (ok) ok = mbar_wait_fast(&empty[(2 * steps - 1) % STAGES], ((2 * steps - 1) / STAGES) & 1, abort);
+            if (ok) ok = warp_wait(&empty[(2 * steps - 1) % STAGES], ((2 * steps - 1) / STAGES) & 1, abort);
             if (!ok) {                     // gave up: nothing may still write to the tensor memory that is freed below
-                mma_commit(&drain);
+                mma_commit(leader, &drain);
                 mbar_wait(&drain, 0, 1 << 20);
             }
         }
@@ -265,7 +266,8 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tmem_wait_store();
             tmem_fence_before();
-            mbar_arrive(&p_ready[t]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_ready[t]);           // one arrival a warp: arrivals on a barrier are served one by one
         }
         if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait_fast(&o_ready[t], 0, abort));
         tmem_fence_after();
@@ -395,18 +397,18 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
         abort_flag = 0;
         for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         mbar_init(&a_full, 1);
-        mbar_init(&x_ready, steps > 1 ? 4 * ROWS : 2 * ROWS);
+        mbar_init(&x_ready, steps > 1 ? 16 : 8);
         mbar_init(&o_ready, 1);
         mbar_init(&tail, 1);
         mbar_init(&drain, 1);
-        for (int t = 0; t < 2; ++t) { mbar_init(&s_ready[t], 1); mbar_init(&p_ready[t], 2 * ROWS); }
+        for (int t = 0; t < 2; ++t) { mbar_init(&s_ready[t], 1); mbar_init(&p_ready[t], 8); }
         mbar_init_fence();
     }
     if (warp == 16) tmem_alloc(&tmem_slot, 512);
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    const uint32_t tmem = tmem_slot;
+    constexpr uint32_t tmem = 0;           // all 512 columns are this block's, so they start at column 0
     volatile int* abort = &abort_flag;
     // Tensor memory, columns: tile in flight t at 128 t: S 0..63, dP 64..127; the accumulators of dQ / dK at 256 and of
     // dV at 384.  The two warpgroups of a tile own 32 columns of S and of dP each and put their 16-bit operands there:
@@ -464,7 +466,8 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
         }
     } else if (warp == 16) {
         // ---- products -----------------------------------------------------------------------------------------
-        if (lane == 0 && steps > 0) {
+        const uint32_t leader = elect_lane();
+        if (steps > 0) {
             constexpr uint32_t id_s = mma_idesc(is_bf16<T>, 128, BROWS, false);
             constexpr uint32_t id_g = mma_idesc(is_bf16<T>, 128, DP, true);
             const int ksteps = (a.D + 15) / 16;
@@ -477,20 +480,20 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
 #pragma unroll
                     for (int k = 0; k < DP / 16; ++k)
                         if (k < ksteps)
-                            mma_ss(d + w * 64, ad + (((k / 4) * SM::ABOX + (k % 4) * 32) >> 4), bd + (((k / 4) * SM::BBOX + (k % 4) * 32) >> 4),
+                            mma_ss(leader, d + w * 64, ad + (((k / 4) * SM::ABOX + (k % 4) * 32) >> 4), bd + (((k / 4) * SM::BBOX + (k % 4) * 32) >> 4),
                                    id_s, k > 0);
                 }
-                mma_commit(&s_ready[j & 1]);
+                mma_commit(leader, &s_ready[j & 1]);
             };
-            bool ok = mbar_wait_fast(&a_full, 0, abort) && mbar_wait_fast(&full[0], 0, abort);
+            bool ok = warp_wait(&a_full, 0, abort) && warp_wait(&full[0], 0, abort);
             if (ok) scores(0);
             for (int j = 0; j < steps && ok; ++j) {
                 if (j + 1 < steps) {
-                    ok = mbar_wait_fast(&full[(j + 1) % STAGES], ((j + 1) / STAGES) & 1, abort);
+                    ok = warp_wait(&full[(j + 1) % STAGES], ((j + 1) / STAGES) & 1, abort);
                     // goes over P and dS of tile j - 1, whose products were issued before: they run in order
                     if (ok) scores(j + 1);
                 }
-                ok = ok && mbar_wait_fast(&p_ready[j & 1], (j / 2) & 1, abort);
+                ok = ok && warp_wait(&p_ready[j & 1], (j / 2) & 1, abort);
                 if (!ok) break;
                 tmem_fence_after();
                 const uint32_t d = tmem + (j & 1) * 128, b_addr = r_addr + (j % STAGES) * 2 * SM::BTILE;
@@ -498,18 +501,18 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
 #pragma unroll
                 for (int k = 0; k < BROWS / 16; ++k) {
                     const uint32_t at = d + (k / 2) * 32 + (k % 2) * 8;
-                    mma_ts(tmem + 256, at + 64, b0 + k * (2048 >> 4), id_g, j > 0 || k > 0);
-                    mma_ts(tmem + 256, at + 16, b0 + k * (2048 >> 4), id_g, true);
-                    if (KV) mma_ts(tmem + 384, at, b1 + k * (2048 >> 4), id_g, j > 0 || k > 0);
+                    mma_ts(leader, tmem + 256, at + 64, b0 + k * (2048 >> 4), id_g, j > 0 || k > 0);
+                    mma_ts(leader, tmem + 256, at + 16, b0 + k * (2048 >> 4), id_g, true);
+                    if (KV) mma_ts(leader, tmem + 384, at, b1 + k * (2048 >> 4), id_g, j > 0 || k > 0);
                 }
-                mma_commit(&empty[j % STAGES]);
+                mma_commit(leader, &empty[j % STAGES]);
             }
             if (ok) {
-                mma_commit(&o_ready);
-                ok = mbar_wait_fast(&o_ready, 0, abort);
+                mma_commit(leader, &o_ready);
+                ok = warp_wait(&o_ready, 0, abort);
             }
             if (!ok) {                     // gave up: nothing may still write to the tensor memory that is freed below
-                mma_commit(&drain);
+                mma_commit(leader, &drain);
                 mbar_wait(&drain, 0, 1 << 20);
             }
         }
@@ -554,7 +557,8 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
                         if (g * 16 + e < rest) sum += __uint_as_float(s[g * 16 + e]) * __uint_as_float(d[e]);
                 }
                 row_sum[wg][local] = sum;
-                mbar_arrive(&x_ready);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&x_ready);
                 ok = __all_sync(0xffffffffu, mbar_wait_fast(&x_ready, 0, abort));
                 if (!ok) break;
                 my_delta = row_sum[0][local] + row_sum[1][local];
@@ -585,7 +589,8 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
             }
             tmem_wait_store();
             tmem_fence_before();
-            mbar_arrive(&p_ready[t]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_ready[t]);           // one arrival a warp: arrivals on a barrier are served one by one
         }
         if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait_fast(&o_ready, 0, abort));
         tmem_fence_after();

@@ -87,25 +87,36 @@ __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* r) {
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 
-// ---- matrix products (one thread issues) -----------------------------------------------------------------------------
+// ---- matrix products -------------------------------------------------------------------------------------------------
+// A whole warp runs the code around the products, so that descriptors and addresses are warp-uniform values (the
+// instruction takes them from uniform registers; from a branch of one lane each product pays for moving them there);
+// `leader` is true in the one lane that issues.
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t e;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
+    return e;
+}
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.u32 p, %4, 0;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %5};\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
-        "r"(uint32_t(accumulate)), "r"(DESC_HIGH)
+        "{\n .reg .pred p, e;\n .reg .b64 x, y;\n setp.ne.u32 e, %6, 0;\n setp.ne.u32 p, %4, 0;\n mov.b64 x, {%1, %5};\n"
+        " mov.b64 y, {%2, %5};\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b),
+        "r"(idesc), "r"(accumulate), "r"(DESC_HIGH), "r"(leader)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n .reg .pred p;\n .reg .b64 y;\n setp.ne.u32 p, %4, 0;\n mov.b64 y, {%2, %5};\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
-        "r"(uint32_t(accumulate)), "r"(DESC_HIGH)
+        "{\n .reg .pred p, e;\n .reg .b64 y;\n setp.ne.u32 e, %6, 0;\n setp.ne.u32 p, %4, 0;\n mov.b64 y, {%2, %5};\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+        "r"(accumulate), "r"(DESC_HIGH), "r"(leader)
         : "memory");
 }
-// one arrival on the barrier once every product this thread has issued is done
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar)) : "memory");
+// one arrival on the barrier once every product the leader has issued is done
+__device__ __forceinline__ void mma_commit(uint32_t leader, uint64_t* bar) {
+    asm volatile(
+        "{\n .reg .pred e;\n setp.ne.u32 e, %1, 0;\n"
+        " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)), "r"(leader)
+        : "memory");
 }
 
 // mbar_wait_or_abort whose first look costs no clock read: most waits on the path of the products find their barrier done
@@ -116,6 +127,10 @@ __device__ __forceinline__ bool mbar_wait_fast(uint64_t* bar, uint32_t parity, v
                  : "r"(smem_u32(bar)), "r"(parity)
                  : "memory");
     return ok || mbar_wait_or_abort(bar, parity, abort_flag);
+}
+
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    return __all_sync(0xffffffffu, mbar_wait_fast(bar, parity, abort_flag));
 }
 
 // ---- tensor copies -----------------------------------------------------------------------------------------------------
