@@ -4,143 +4,339 @@
 //   backward  g = dy * scale,   dx = r (g - mean_j g - z mean_j(g z)),
 //             dscale = sum_rows dy z,   doffset = sum_rows dy
 //
-// Both directions are bound by memory: forward reads x and writes y, backward reads x and dy and writes dx.  A row
-// is read once into the registers of a group of TPR threads (a part of a warp, a warp, or a whole block for wide
-// rows), so the mean, the squared deviations and the result all come from one read; the deviations are summed in a
-// second pass over registers, because E[x^2] - mean^2 loses the variance of rows with a large mean.  Sums are held
-// in float (double for double).
+// Both directions are bound by memory: forward reads x and writes y, backward reads x and dy and writes dx.  So the rows
+// pass through shared memory: blocks stay on the SMs and walk over tiles of rows, and the copy engine (cp.async.bulk)
+// keeps the tiles ahead on their way while a tile is worked on, whatever the arithmetic waits for.  A tile of dense rows
+// is one copy, so rows of any width move at full speed; rows that are not whole 16-byte pieces are only read element by
+// element from shared memory.
 //
-// The weights' gradients are sums over the rows.  The backward kernel keeps one CTA (or a few) on every SM that walks
-// over rows; a thread holds the same columns for all its rows and sums them in registers, the block adds its
-// groups in shared memory and writes one partial row, and a second kernel adds the partial rows in a fixed order:
-// no atomics, the same bits every time.
+// A group of TPR threads (part of a warp up to the block) takes a row, N accesses of VEC elements per thread, and works
+// on it in registers: forward the mean and then the squared deviations from it (E[x^2] - mean^2 would lose the
+// variance of rows with a large mean), backward the sums of g and g (x - mu).  Groups share nothing but the tiles, so
+// a group's barriers stop no other group.  About 16 elements per thread spread what a row costs besides its elements;
+// with fewer the instruction issue is the bound, not memory.  A thread keeps its columns for all rows, so the weights,
+// and the sums over rows for their gradients, stay in registers; they leave a block as one partial row, and a second
+// kernel adds the partial rows in a fixed order: no atomics, the same bits every time.
+// Sums are held in float (double for double).
 #include <algorithm>
 #include <initializer_list>
 
 #include "common.cuh"
+#include "mma_f64.cuh"
 #include "tensor_types.cuh"
 
 namespace nnvb {
 namespace {
 
-constexpr int LN_BLOCK = 256;           // threads of a block whose rows fit a warp or less
-
 template <typename A>
-__device__ __forceinline__ A warp_sum(A x, int width) {
-    for (int o = width / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o, 32);
+__device__ __forceinline__ A warp_sum(A x) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o, 32);
     return x;
 }
 
-// Sum of x over the TPR threads of a row, the same bits in each of them.  `red` holds one value per warp of a group;
-// two alternating halves let one barrier per call suffice.
+// Sums of x and y over the TPR threads of a group, the same bits in each of them.  `red` holds a pair per warp, in two
+// halves that take turns, so that one barrier among the group's warps per call suffices.
 template <int TPR, typename A>
-__device__ __forceinline__ A group_sum(A x, A* red, int& flip) {
-    if constexpr (TPR <= 32) {
-        return warp_sum(x, TPR);
-    } else {
-        constexpr int W = TPR / 32;
-        x = warp_sum(x, 32);
-        const int warp = threadIdx.x / 32;
-        A* r = red + (flip ? 32 : 0);
-        flip ^= 1;
-        if (threadIdx.x % 32 == 0) r[warp] = x;
-        __syncthreads();
-        const int w0 = warp / W * W;
-        A s = 0;
+__device__ __forceinline__ void group_sum(A& x, A& y, A (*red)[2], int& flip) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) s += r[w0 + i];
-        return s;
+    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) {
+        x += __shfl_xor_sync(0xffffffffu, x, o, 32);
+        y += __shfl_xor_sync(0xffffffffu, y, o, 32);
+    }
+    if constexpr (TPR > 32) {
+        constexpr int W = TPR / 32;
+        const int warp = threadIdx.x / 32, w0 = warp / W * W;
+        A(*r)[2] = red + flip;
+        flip ^= 32;
+        if (threadIdx.x % 32 == 0) { r[warp][0] = x; r[warp][1] = y; }
+        named_bar_sync(1 + warp / W, TPR);
+        x = y = 0;
+#pragma unroll
+        for (int i = 0; i < W; ++i) { x += r[w0 + i][0]; y += r[w0 + i][1]; }
+    }
+}
+template <int TPR, typename A>
+__device__ __forceinline__ A group_sum1(A x, A (*red)[2], int& flip) {
+    A y = 0;
+    group_sum<TPR>(x, y, red, flip);
+    return x;
+}
+
+// Makes the compiler forget what it has derived from 16-bit elements: converting them again is one instruction each,
+// keeping the converted values as well costs three times the registers.
+template <typename T, int VEC>
+__device__ __forceinline__ void ln_forget(Pack<T, VEC>& p) {
+    if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&p);
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) asm volatile("" : "+r"(w[i]));
     }
 }
 
-template <typename A>
-struct Two { A a, b; };
+constexpr int LN_THREADS = 512;
+constexpr int LN_STAGES = 3;
 
-template <int TPR, typename A>
-__device__ __forceinline__ Two<A> group_sum2(A x, A y, Two<A>* red, int& flip) {
-    if constexpr (TPR <= 32) {
-        return {warp_sum(x, TPR), warp_sum(y, TPR)};
-    } else {
-        constexpr int W = TPR / 32;
-        x = warp_sum(x, 32);
-        y = warp_sum(y, 32);
-        const int warp = threadIdx.x / 32;
-        Two<A>* r = red + (flip ? 32 : 0);
-        flip ^= 1;
-        if (threadIdx.x % 32 == 0) r[warp] = {x, y};
-        __syncthreads();
-        const int w0 = warp / W * W;
-        Two<A> s{0, 0};
-#pragma unroll
-        for (int i = 0; i < W; ++i) { s.a += r[w0 + i].a; s.b += r[w0 + i].b; }
-        return s;
-    }
-}
+// How the rows of a tile reach shared memory: as one copy (dense rows), one copy a row (rows of whole 16-byte pieces that
+// lie apart), or by plain loads (anything else).
+enum { LN_RANGE = 0, LN_BY_ROW = 1, LN_PLAIN = 2 };
 
-// TPR threads per row, NV accesses of VEC elements per thread; TPR * NV * VEC >= cols.
-template <typename T, int VEC, int TPR, int NV>
-__global__ void __launch_bounds__(TPR > LN_BLOCK ? TPR : LN_BLOCK)
-ln_forward_kernel(int64_t rows, int cols, const T* __restrict__ x, int64_t ldx, const T* __restrict__ scale,
-                  const T* __restrict__ offset, typename AccOf<T>::type eps, T* __restrict__ y, int64_t ldy,
-                  typename AccOf<T>::type* __restrict__ mean_out, typename AccOf<T>::type* __restrict__ rstd_out) {
+struct LnTile {
+    int64_t rows, n_tiles;
+    int64_t ldx, lddy, ldo;
+    const void *x, *dy, *scale, *offset;
+    void *out, *mean, *rstd, *partial;
+    double eps;
+    int cols;
+    int R, tensor_bytes;                         // rows of a tile; bytes of one tensor's rows in a stage
+    int mode;
+};
+
+template <typename T, int VEC, int TPR, int N, bool BWD, int MINB>
+__global__ void __launch_bounds__(LN_THREADS, MINB)
+ln_tile_kernel(const __grid_constant__ LnTile p) {
     using A = typename AccOf<T>::type;
     using P = Pack<T, VEC>;
-    constexpr int BLOCK = TPR > LN_BLOCK ? TPR : LN_BLOCK;
-    constexpr int RPB = BLOCK / TPR;
-    __shared__ A red[64];
-    int flip = 0;
-    const int t = threadIdx.x % TPR;
-    const int64_t row = int64_t(blockIdx.x) * RPB + threadIdx.x / TPR;
-    const bool live = row < rows;
-    const T* xr = x + (live ? row : 0) * ldx;
-    P buf[NV];
-    const int c0 = t * VEC;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = c0 + i * TPR * VEC;
-        if (c < cols && live) buf[i] = *reinterpret_cast<const P*>(xr + c);
-    }
-    A s = 0;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (c0 + i * TPR * VEC < cols && live) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) s += to_acc(buf[i].v[e]);
+    constexpr int GROUPS = LN_THREADS / TPR;
+    constexpr bool AGAIN = N * VEC * sizeof(A) > 64;       // wide rows: 16-bit values are converted again, not kept
+    extern __shared__ __align__(128) unsigned char ring[];
+    __shared__ uint64_t full[LN_STAGES], empty[LN_STAGES];
+    __shared__ int abort_flag;
+    __shared__ A red[64][2];
+    const int tid = threadIdx.x;
+    const int cols = p.cols, R = p.R;
+    const int stage_bytes = p.tensor_bytes * (BWD ? 2 : 1);
+    const T *x = static_cast<const T*>(p.x), *dy = static_cast<const T*>(p.dy);
+    const int64_t pitch = int64_t(cols) * sizeof(T);
+
+    auto rows_of = [&](int64_t tile) { return int(p.rows - tile * R < R ? p.rows - tile * R : R); };
+    // bytes before the first row of a tile in its stage
+    auto lead = [&](int64_t tile) { return p.mode == LN_RANGE ? int(tile * R * pitch % 16) : 0; };
+    // Bytes that one tensor's copy of a tile moves.  A range runs from the boundary before its first row to the one behind
+    // its last, but not past the last boundary inside the tensor: what lies behind that is loaded apart.
+    auto bytes_of = [&](int64_t tile) {
+        if (p.mode != LN_RANGE) return uint32_t(rows_of(tile) * pitch);
+        const int64_t from = tile * R * pitch / 16 * 16, to = (tile * R + rows_of(tile)) * pitch, last = p.rows * pitch / 16 * 16;
+        const int64_t end = (to + 15) / 16 * 16 < last ? (to + 15) / 16 * 16 : last;
+        return uint32_t(end > from ? end - from : 0);
+    };
+    auto copy = [&](const T* src, int64_t ld, int64_t tile, unsigned char* dst, uint64_t* bar) {
+        if (p.mode == LN_RANGE) {
+            const uint32_t bytes = bytes_of(tile);
+            if (bytes) bulk_copy_g2s(dst, reinterpret_cast<const char*>(src) + tile * R * pitch / 16 * 16, bytes, bar);
+        } else {
+            for (int r = 0; r < rows_of(tile); ++r) bulk_copy_g2s(dst + r * pitch, src + (tile * R + r) * ld, uint32_t(pitch), bar);
         }
-    const A inv_n = A(1) / A(cols);
-    const A mean = group_sum<TPR>(s, red, flip) * inv_n;
-    A q = 0;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (c0 + i * TPR * VEC < cols && live) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const A d = to_acc(buf[i].v[e]) - mean;
-                q += d * d;
-            }
-        }
-    const A rstd = rsqrt_acc(group_sum<TPR>(q, red, flip) * inv_n + eps);
-    if (!live) return;
-    if (t == 0) {
-        if (mean_out) mean_out[row] = mean;
-        if (rstd_out) rstd_out[row] = rstd;
+    };
+    auto request = [&](int64_t tile, int s) {              // one thread
+        unsigned char* dst = ring + s * stage_bytes;
+        mbar_expect_bytes(&full[s], bytes_of(tile) * (BWD ? 2 : 1));
+        copy(x, p.ldx, tile, dst, &full[s]);
+        if (BWD) copy(dy, p.lddy, tile, dst + p.tensor_bytes, &full[s]);
+    };
+
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < LN_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], LN_THREADS / 32); }
+        mbar_init_fence();
+        if (p.mode != LN_PLAIN)
+            for (int s = 0; s < LN_STAGES; ++s)
+                if (blockIdx.x + int64_t(s) * gridDim.x < p.n_tiles) request(blockIdx.x + int64_t(s) * gridDim.x, s);
     }
-    T* yr = y + row * ldy;
+
+    const int t = tid % TPR, grp = tid / TPR;
+    P sc[N], of[BWD ? 1 : N];
+    A acc_s[BWD ? N : 1][VEC], acc_o[BWD ? N : 1][VEC];
+    const bool has_s = p.scale != nullptr, has_o = !BWD && p.offset != nullptr;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = c0 + i * TPR * VEC;
+    for (int i = 0; i < N; ++i) {
+        const int c = (t + i * TPR) * VEC;
         if (c < cols) {
-            P sc, of, o;
-            if (scale) sc = *reinterpret_cast<const P*>(scale + c);
-            if (offset) of = *reinterpret_cast<const P*>(offset + c);
+            if (has_s) sc[i] = *reinterpret_cast<const P*>(static_cast<const T*>(p.scale) + c);
+            if constexpr (!BWD)
+                if (has_o) of[i] = *reinterpret_cast<const P*>(static_cast<const T*>(p.offset) + c);
+        }
+        if constexpr (BWD)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                A z = (to_acc(buf[i].v[e]) - mean) * rstd;
-                if (scale) z *= to_acc(sc.v[e]);
-                if (offset) z += to_acc(of.v[e]);
-                o.v[e] = from_acc<T, A>(z);
+            for (int e = 0; e < VEC; ++e) { acc_s[i][e] = 0; acc_o[i][e] = 0; }
+    }
+    __syncthreads();
+
+    const A inv_n = A(1) / A(cols), eps = A(p.eps);
+    int flip = 0, s = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    // A failed wait changes no control flow: the groups' barriers need every thread.  The results become NaN.
+    for (int64_t tile = blockIdx.x; tile < p.n_tiles; tile += gridDim.x) {
+        unsigned char* st = ring + s * stage_bytes;
+        const int n = rows_of(tile);
+        const int64_t row0 = tile * R;
+        if (p.mode == LN_PLAIN) {
+            __syncthreads();
+            for (int i = tid; i < n * cols; i += LN_THREADS) {
+                const int r = i / cols, c = i % cols;
+                reinterpret_cast<T*>(st)[i] = x[(row0 + r) * p.ldx + c];
+                if (BWD) reinterpret_cast<T*>(st + p.tensor_bytes)[i] = dy[(row0 + r) * p.lddy + c];
             }
-            *reinterpret_cast<P*>(yr + c) = o;
+            __syncthreads();
+        } else {
+            ok = ok && mbar_wait_or_abort(&full[s], phase, &abort_flag);
+            if (p.mode == LN_RANGE && tile + 8 >= p.n_tiles) {       // under 16 bytes: at most 7 tiles of one element
+                const int64_t all = n * pitch, got = int64_t(bytes_of(tile)) - lead(tile);
+                const int left = int((all - (got > 0 ? (got < all ? got : all) : 0)) / int(sizeof(T)));
+                if (left > 0) {                 // the tensor's last elements
+                    if (tid < left) {
+                        const int64_t at = int64_t(n) * cols - left + tid;
+                        reinterpret_cast<T*>(st + lead(tile))[at] = x[row0 * cols + at];
+                        if (BWD) reinterpret_cast<T*>(st + p.tensor_bytes + lead(tile))[at] = dy[row0 * cols + at];
+                    }
+                    __syncthreads();
+                }
+            }
+        }
+        const T* sx = reinterpret_cast<const T*>(st + lead(tile)) + grp * cols;
+        const T* sg = reinterpret_cast<const T*>(st + p.tensor_bytes + lead(tile)) + grp * cols;
+        T* out = static_cast<T*>(p.out) + (row0 + grp) * p.ldo;
+        for (int base = 0; base < n; base += GROUPS, sx += GROUPS * cols, sg += GROUPS * cols, out += GROUPS * p.ldo) {
+            const int64_t row = row0 + base + grp;
+            const bool live = base + grp < n;
+            if (TPR >= 32 && !live) break;      // groups of whole warps go on to the next tile
+            P px[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = (t + i * TPR) * VEC;
+                if (live && c < cols) px[i] = *reinterpret_cast<const P*>(sx + c);
+            }
+            if constexpr (!BWD) {
+                A sum = 0;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (live && (t + i * TPR) * VEC < cols)
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) sum += to_acc(px[i].v[e]);
+                const A mean = group_sum1<TPR>(sum, red, flip) * inv_n;
+                A dev = 0;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (live && (t + i * TPR) * VEC < cols) {
+                        if (AGAIN) ln_forget(px[i]);
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) {
+                            const A d = to_acc(px[i].v[e]) - mean;
+                            dev += d * d;
+                        }
+                    }
+                A rstd = rsqrt_acc(group_sum1<TPR>(dev, red, flip) * inv_n + eps);
+                if (live && t == 0) {
+                    if (p.mean) static_cast<A*>(p.mean)[row] = mean;
+                    if (p.rstd) static_cast<A*>(p.rstd)[row] = rstd;
+                }
+                if (!ok) rstd = A(NAN);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int c = (t + i * TPR) * VEC;
+                    if (live && c < cols) {
+                        P o;
+                        if (AGAIN) ln_forget(px[i]);
+                        if (has_s) ln_forget(sc[i]);
+                        if (has_o) ln_forget(of[i]);
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) {
+                            A z = (to_acc(px[i].v[e]) - mean) * rstd;
+                            if (has_s) z *= to_acc(sc[i].v[e]);
+                            if (has_o) z += to_acc(of[i].v[e]);
+                            o.v[e] = from_acc<T, A>(z);
+                        }
+                        *reinterpret_cast<P*>(out + c) = o;
+                    }
+                }
+            } else {
+                P pg[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int c = (t + i * TPR) * VEC;
+                    if (live && c < cols) pg[i] = *reinterpret_cast<const P*>(sg + c);
+                }
+                const A mu = live ? __ldg(static_cast<const A*>(p.mean) + row) : A(0);
+                const A rs = live ? __ldg(static_cast<const A*>(p.rstd) + row) : A(0);
+                A s1 = 0, s2 = 0;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (live && (t + i * TPR) * VEC < cols) {
+                        if (has_s) ln_forget(sc[i]);
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) {
+                            const A d = to_acc(pg[i].v[e]), g = has_s ? d * to_acc(sc[i].v[e]) : d;
+                            s1 += g;
+                            s2 += g * (to_acc(px[i].v[e]) - mu);
+                        }
+                    }
+                group_sum<TPR>(s1, s2, red, flip);
+                const A k1 = s1 * inv_n * rs, k2 = s2 * inv_n * rs * rs * rs;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int c = (t + i * TPR) * VEC;
+                    if (live && c < cols) {
+                        P o;
+                        if (AGAIN) {
+                            ln_forget(px[i]);
+                            ln_forget(pg[i]);
+                            if (has_s) ln_forget(sc[i]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) {
+                            const A xc = to_acc(px[i].v[e]) - mu, d = to_acc(pg[i].v[e]), dr = d * rs;
+                            acc_s[i][e] += dr * xc;
+                            acc_o[i][e] += d;
+                            const A g = has_s ? dr * to_acc(sc[i].v[e]) : dr;
+                            o.v[e] = from_acc<T, A>(g - (k1 + xc * k2));
+                        }
+                        *reinterpret_cast<P*>(out + c) = o;
+                    }
+                }
+            }
+        }
+        if (p.mode != LN_PLAIN) {
+            __syncwarp();
+            if (tid % 32 == 0) mbar_arrive(&empty[s]);
+            // The stage of the tile before is requested again now: by this time the other warps are through with it, so
+            // the thread that asks hardly waits.
+            if (tid == 0 && tile != int64_t(blockIdx.x)) {
+                const int64_t next = tile + int64_t(LN_STAGES - 1) * gridDim.x;
+                const int sp = s ? s - 1 : LN_STAGES - 1;
+                if (next < p.n_tiles && ok) {
+                    ok = mbar_wait_or_abort(&empty[sp], s ? phase : phase ^ 1, &abort_flag);
+                    async_proxy_fence();
+                    if (ok) request(next, sp);
+                }
+            }
+        }
+        if (++s == LN_STAGES) { s = 0; phase ^= 1; }
+    }
+    if (!ok && tid == 0)                        // gave up: copies may still be on their way into this block's memory
+        for (int i = 0; i < LN_STAGES; ++i) mbar_wait(&full[i], phase, 1 << 20);
+
+    if constexpr (BWD) {
+        if (!p.partial) return;
+        // the groups' sums, added in group order, one access of columns at a time through the ring
+        A* buf = reinterpret_cast<A*>(ring);
+        A* ps = static_cast<A*>(p.partial) + int64_t(blockIdx.x) * 2 * cols;
+        const A bad = ok ? A(0) : A(NAN);
+#pragma unroll
+        for (int k = 0; k < 2 * N; ++k) {
+            const int i = k >> 1;
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) buf[tid * VEC + e] = ((k & 1) ? acc_o[i][e] : acc_s[i][e]) + bad;
+            __syncthreads();
+            for (int j = tid; j < TPR * VEC; j += LN_THREADS) {
+                const int c = i * TPR * VEC + j;
+                if (c < cols) {
+                    A sum = 0;
+                    for (int g = 0; g < GROUPS; ++g) sum += buf[g * TPR * VEC + j];
+                    ps[(k & 1) * int64_t(cols) + c] = sum;
+                }
+            }
         }
     }
 }
@@ -152,20 +348,20 @@ ln_forward_wide_kernel(int64_t cols, const T* __restrict__ x, int64_t ldx, const
                        const T* __restrict__ offset, typename AccOf<T>::type eps, T* __restrict__ y, int64_t ldy,
                        typename AccOf<T>::type* __restrict__ mean_out, typename AccOf<T>::type* __restrict__ rstd_out) {
     using A = typename AccOf<T>::type;
-    __shared__ A red[64];
+    __shared__ A red[64][2];
     int flip = 0;
     const int64_t row = blockIdx.x;
     const T* xr = x + row * ldx;
     A s = 0;
     for (int64_t c = threadIdx.x; c < cols; c += 1024) s += to_acc(xr[c]);
     const A inv_n = A(1) / A(cols);
-    const A mean = group_sum<1024>(s, red, flip) * inv_n;
+    const A mean = group_sum1<1024>(s, red, flip) * inv_n;
     A q = 0;
     for (int64_t c = threadIdx.x; c < cols; c += 1024) {
         const A d = to_acc(xr[c]) - mean;
         q += d * d;
     }
-    const A rstd = rsqrt_acc(group_sum<1024>(q, red, flip) * inv_n + eps);
+    const A rstd = rsqrt_acc(group_sum1<1024>(q, red, flip) * inv_n + eps);
     if (threadIdx.x == 0) {
         if (mean_out) mean_out[row] = mean;
         if (rstd_out) rstd_out[row] = rstd;
@@ -179,143 +375,27 @@ ln_forward_wide_kernel(int64_t cols, const T* __restrict__ x, int64_t ldx, const
     }
 }
 
-// Walks rows blockIdx.x * RPB + group, + gridDim.x * RPB, ...; partial[blockIdx.x] = {sums of dy z, sums of dy}.
-template <typename T, int VEC, int TPR, int NV>
-__global__ void __launch_bounds__(TPR > LN_BLOCK ? TPR : LN_BLOCK)
-ln_backward_kernel(int64_t rows, int cols, const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx,
-                   const T* __restrict__ scale, const typename AccOf<T>::type* __restrict__ mean,
-                   const typename AccOf<T>::type* __restrict__ rstd, T* __restrict__ dx, int64_t lddx,
-                   typename AccOf<T>::type* __restrict__ partial) {
-    using A = typename AccOf<T>::type;
-    using P = Pack<T, VEC>;
-    constexpr int BLOCK = TPR > LN_BLOCK ? TPR : LN_BLOCK;
-    constexpr int RPB = BLOCK / TPR;
-    __shared__ Two<A> red[64];
-    int flip = 0;
-    const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
-    const int c0 = t * VEC;
-    P sc[NV];
-    A acc_s[NV][VEC], acc_o[NV][VEC];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = c0 + i * TPR * VEC;
-        if (scale && c < cols) sc[i] = *reinterpret_cast<const P*>(scale + c);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) { acc_s[i][e] = 0; acc_o[i][e] = 0; }
-    }
-    const A inv_n = A(1) / A(cols);
-    const int64_t step = int64_t(gridDim.x) * RPB;
-    P bx[NV], bg[NV];
-    A mu = 0, r = 0;
-    auto fetch = [&](int64_t row) {
-        if (row >= rows) return;
-        mu = mean[row];
-        r = rstd[row];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = c0 + i * TPR * VEC;
-            if (c < cols) {
-                bx[i] = *reinterpret_cast<const P*>(x + row * ldx + c);
-                bg[i] = *reinterpret_cast<const P*>(dy + row * lddy + c);
-            }
-        }
-    };
-    fetch(int64_t(blockIdx.x) * RPB + grp);
-    // every group of the block makes the same number of turns: the sums of wide rows meet at barriers
-    for (int64_t base = int64_t(blockIdx.x) * RPB; base < rows; base += step) {
-        const int64_t row = base + grp;
-        const bool live = row < rows;
-        P cx[NV], cg[NV];
-        const A cmu = mu, cr = r;
-        A s1 = 0, s2 = 0;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) { cx[i] = bx[i]; cg[i] = bg[i]; }
-        fetch(row + step);                // the next row is on its way while this one is summed
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (c0 + i * TPR * VEC < cols && live) {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const A z = (to_acc(cx[i].v[e]) - cmu) * cr, d = to_acc(cg[i].v[e]);
-                    acc_s[i][e] += d * z;
-                    acc_o[i][e] += d;
-                    const A g = scale ? d * to_acc(sc[i].v[e]) : d;
-                    s1 += g;
-                    s2 += g * z;
-                }
-            }
-        const Two<A> m = group_sum2<TPR>(s1, s2, red, flip);
-        const A m1 = m.a * inv_n, m2 = m.b * inv_n;
-        if (live) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int c = c0 + i * TPR * VEC;
-                if (c < cols) {
-                    P o;
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const A z = (to_acc(cx[i].v[e]) - cmu) * cr, d = to_acc(cg[i].v[e]);
-                        const A g = scale ? d * to_acc(sc[i].v[e]) : d;
-                        o.v[e] = from_acc<T, A>(cr * (g - m1 - z * m2));
-                    }
-                    *reinterpret_cast<P*>(dx + row * lddx + c) = o;
-                }
-            }
-        }
-    }
-    if (!partial) return;
-    A* ps = partial + int64_t(blockIdx.x) * 2 * cols;
-    if constexpr (RPB == 1) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = c0 + i * TPR * VEC;
-            if (c < cols) {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) { ps[c + e] = acc_s[i][e]; ps[cols + c + e] = acc_o[i][e]; }
-            }
-        }
-    } else {
-        // the groups' sums, added in group order; a slice of columns at a time keeps the buffer small
-        __shared__ A buf[RPB][TPR * VEC];
-#pragma unroll
-        for (int k = 0; k < 2 * NV; ++k) {
-            const int i = k >> 1;
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) buf[grp][c0 + e] = (k & 1) ? acc_o[i][e] : acc_s[i][e];
-            __syncthreads();
-            for (int j = threadIdx.x; j < TPR * VEC; j += BLOCK) {
-                const int c = j + i * TPR * VEC;
-                if (c < cols) {
-                    A s = 0;
-                    for (int g = 0; g < RPB; ++g) s += buf[g][j];
-                    ps[(k & 1) * int64_t(cols) + c] = s;
-                }
-            }
-        }
-    }
-}
-
-// dscale / doffset: partial rows added in order, 32 columns per block, the rows over 8 warps.
+// dscale / doffset: partial rows added in order, 32 columns per block, the rows over 32 warps
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 ln_reduce_kernel(int n_parts, int64_t cols, const typename AccOf<T>::type* __restrict__ partial, T* __restrict__ dscale,
                  T* __restrict__ doffset) {
     using A = typename AccOf<T>::type;
-    __shared__ A buf[8][33];
+    __shared__ A buf[32][33];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const int64_t c = int64_t(blockIdx.x) * 32 + lane;      // 0 .. 2 * cols
     A s = 0;
     if (c < 2 * cols)
-#pragma unroll 4
-        for (int p = warp; p < n_parts; p += 8) s += partial[int64_t(p) * 2 * cols + c];
+#pragma unroll 8
+        for (int p = warp; p < n_parts; p += 32) s += partial[int64_t(p) * 2 * cols + c];
     buf[warp][lane] = s;
     __syncthreads();
-    if (warp == 0 && c < 2 * cols) {
-#pragma unroll
-        for (int w = 1; w < 8; ++w) s += buf[w][lane];
-        T* out = c < cols ? dscale : doffset;
-        if (out) out[c < cols ? c : c - cols] = from_acc<T, A>(s);
+    // warp w adds column w over the 32 warps, in the order of the shuffles
+    s = warp_sum(buf[lane][warp]);
+    const int64_t cw = int64_t(blockIdx.x) * 32 + warp;
+    if (lane == 0 && cw < 2 * cols) {
+        T* out = cw < cols ? dscale : doffset;
+        if (out) out[cw < cols ? cw : cw - cols] = from_acc<T, A>(s);
     }
 }
 
@@ -326,7 +406,7 @@ ln_backward_wide_kernel(int64_t cols, const T* __restrict__ dy, int64_t lddy, co
                         const T* __restrict__ scale, const typename AccOf<T>::type* __restrict__ mean,
                         const typename AccOf<T>::type* __restrict__ rstd, T* __restrict__ dx, int64_t lddx) {
     using A = typename AccOf<T>::type;
-    __shared__ Two<A> red[64];
+    __shared__ A red[64][2];
     int flip = 0;
     const int64_t row = blockIdx.x;
     const T *xr = x + row * ldx, *gr = dy + row * lddy;
@@ -338,8 +418,8 @@ ln_backward_wide_kernel(int64_t cols, const T* __restrict__ dy, int64_t lddy, co
         s1 += g;
         s2 += g * z;
     }
-    const Two<A> m = group_sum2<1024>(s1, s2, red, flip);
-    const A m1 = m.a / A(cols), m2 = m.b / A(cols);
+    group_sum<1024>(s1, s2, red, flip);
+    const A m1 = s1 / A(cols), m2 = s2 / A(cols);
     for (int64_t c = threadIdx.x; c < cols; c += 1024) {
         const A z = (to_acc(xr[c]) - mu) * r;
         const A g = scale ? to_acc(gr[c]) * to_acc(scale[c]) : to_acc(gr[c]);
@@ -368,10 +448,6 @@ ln_weights_wide_kernel(int64_t rows, int64_t cols, const T* __restrict__ dy, int
 // ---------------------------------------------------------------------------
 // host side
 
-// The group of threads a row is given: the smallest that holds it.  Wider groups than needed leave lanes idle on
-// narrow rows; more elements per thread than these cost the registers that keep rows in flight.
-//   16-byte accesses: up to 4 per thread.  Rows whose width or alignment rules them out are read element by element,
-//   up to 8 per thread in groups of a warp or less and 16 in larger ones.
 struct LnArgs {
     cudaStream_t st;
     int64_t rows, cols;
@@ -395,105 +471,114 @@ int sm_count() {
     return n[dev];
 }
 
-template <typename T, int VEC, int TPR, int NV>
-void run_forward(const LnArgs& a) {
+constexpr int LN_MAX_PARTS = 2 * 148;        // partial rows of the weights' gradients: blocks that fit at once
+
+template <typename T, int VEC, int TPR, int N, bool BWD, int MINB>
+int ln_tile(LnArgs& a, int mode) {
+    constexpr int GROUPS = LN_THREADS / TPR, TENSORS = BWD ? 2 : 1;
+    const int64_t slots = std::min(sm_count(), 148) * MINB;
+    const int64_t pitch = a.cols * int64_t(sizeof(T));
+    LnTile p{};
+    p.rows = a.rows; p.cols = int(a.cols);
+    p.ldx = a.ldx; p.lddy = a.lddy; p.ldo = a.ldo;
+    p.x = a.x; p.dy = a.dy; p.scale = a.scale; p.offset = a.offset;
+    p.out = a.out; p.mean = a.mean; p.rstd = a.rstd; p.partial = a.partial;
+    p.eps = a.eps;
+    p.mode = mode;
+    // as many rounds of all groups as a stage holds, but no more rows than spread over all blocks
+    const int64_t budget = (MINB == 2 ? 100 : 200) * 1024 / LN_STAGES;
+    int64_t R = (budget - 32 * TENSORS - 256) / (TENSORS * pitch);
+    R = std::min<int64_t>(R, ceil_div(a.rows, slots));
+    R = R >= GROUPS ? R / GROUPS * GROUPS : std::max<int64_t>(R, 1);
+    p.R = int(R);
+    p.n_tiles = ceil_div(a.rows, R);
+    p.tensor_bytes = int(round_up(R * pitch + 32, 128));
     using A = typename AccOf<T>::type;
-    constexpr int BLOCK = TPR > LN_BLOCK ? TPR : LN_BLOCK;
-    constexpr int RPB = BLOCK / TPR;
-    ln_forward_kernel<T, VEC, TPR, NV><<<unsigned(ceil_div(a.rows, RPB)), BLOCK, 0, a.st>>>(
-        a.rows, int(a.cols), static_cast<const T*>(a.x), a.ldx, static_cast<const T*>(a.scale),
-        static_cast<const T*>(a.offset), A(a.eps), static_cast<T*>(a.out), a.ldo, static_cast<A*>(a.mean),
-        static_cast<A*>(a.rstd));
-}
-
-template <typename T, int VEC, int TPR, int NV>
-void run_backward(const LnArgs& a) {
-    using A = typename AccOf<T>::type;
-    constexpr int BLOCK = TPR > LN_BLOCK ? TPR : LN_BLOCK;
-    ln_backward_kernel<T, VEC, TPR, NV><<<unsigned(a.grid), BLOCK, 0, a.st>>>(
-        a.rows, int(a.cols), static_cast<const T*>(a.dy), a.lddy, static_cast<const T*>(a.x), a.ldx,
-        static_cast<const T*>(a.scale), static_cast<const A*>(a.mean), static_cast<const A*>(a.rstd),
-        static_cast<T*>(a.out), a.ldo, static_cast<A*>(a.partial));
-}
-
-template <int VEC_, int TPR_, int NV_>
-struct LnVariant {
-    static constexpr int VEC = VEC_, TPR = TPR_, NV = NV_;
-};
-
-// Calls f(LnVariant<VEC, TPR, NV>{}) for the variant of `cols`; false for rows wider than a block holds.
-template <typename T, typename F>
-bool ln_variant(int64_t cols, bool vec, F&& f) {
-    constexpr int V = 16 / sizeof(T);
-    if (vec) {
-        if (cols <= 8 * 4 * V) f(LnVariant<V, 8, 4>{});
-        else if (cols <= 32 * 4 * V) f(LnVariant<V, 32, 4>{});
-        else if (cols <= 128 * 4 * V) f(LnVariant<V, 128, 4>{});
-        else if (cols <= 512 * 4 * V) f(LnVariant<V, 512, 4>{});
-        else return false;
-    } else {
-        if (cols <= 8 * 8) f(LnVariant<1, 8, 8>{});
-        else if (cols <= 32 * 8) f(LnVariant<1, 32, 8>{});
-        else if (cols <= 128 * 16) f(LnVariant<1, 128, 16>{});
-        else if (cols <= 512 * 16) f(LnVariant<1, 512, 16>{});
-        else return false;
-    }
-    return true;
-}
-
-template <typename T>
-bool aligned_rows(int64_t cols, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> lds) {
-    constexpr int64_t V = 16 / sizeof(T);
-    if (cols % V) return false;
-    for (const void* p : ptrs)
-        if (reinterpret_cast<uintptr_t>(p) % 16) return false;
-    for (int64_t l : lds)
-        if (l % V) return false;
-    return true;
-}
-
-template <typename T>
-int ln_forward_t(const LnArgs& a) {
-    using A = typename AccOf<T>::type;
-    const bool vec = aligned_rows<T>(a.cols, {a.x, a.scale, a.offset, a.out}, {a.ldx, a.ldo});
-    const bool done = ln_variant<T>(a.cols, vec, [&](auto v) { run_forward<T, decltype(v)::VEC, decltype(v)::TPR, decltype(v)::NV>(a); });
-    if (!done)
-        ln_forward_wide_kernel<T><<<unsigned(a.rows), 1024, 0, a.st>>>(
-            a.cols, static_cast<const T*>(a.x), a.ldx, static_cast<const T*>(a.scale), static_cast<const T*>(a.offset),
-            A(a.eps), static_cast<T*>(a.out), a.ldo, static_cast<A*>(a.mean), static_cast<A*>(a.rstd));
+    const int smem = std::max<int>(LN_STAGES * p.tensor_bytes * TENSORS, BWD ? LN_THREADS * VEC * int(sizeof(A)) : 0);
+    a.grid = int(std::min<int64_t>(p.n_tiles, slots));
+    auto kernel = ln_tile_kernel<T, VEC, TPR, N, BWD, MINB>;
+    NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kernel<<<unsigned(a.grid), LN_THREADS, smem, a.st>>>(p);
     NNVB_CUDA(cudaGetLastError());
     return NNVB_OK;
 }
 
-constexpr int LN_MAX_PARTS = 1024;
+// The narrowest group that holds the columns with about 16 elements (8 doubles) per thread.
+template <typename T, int VEC, bool BWD>
+int ln_by_width(LnArgs& a, int mode, bool* done) {
+    constexpr int E = sizeof(T) == 8 ? 8 : 16, N = E / VEC;
+    constexpr int M = 1;
+    const int64_t c = a.cols;
+    *done = true;
+    if (c <= 8 * E / 2) return ln_tile<T, VEC, 8, N / 2, BWD, M>(a, mode);
+    if (c <= 8 * E) return ln_tile<T, VEC, 8, N, BWD, M>(a, mode);
+    if (c <= 32 * E / 2) return ln_tile<T, VEC, 32, N / 2, BWD, M>(a, mode);
+    if (c <= 32 * E) return ln_tile<T, VEC, 32, N, BWD, M>(a, mode);
+    if (c <= 64 * E) return ln_tile<T, VEC, 64, N, BWD, M>(a, mode);
+    if (c <= 128 * E) return ln_tile<T, VEC, 128, N, BWD, M>(a, mode);
+    if (c <= 256 * E) return ln_tile<T, VEC, 256, N, BWD, M>(a, mode);
+    if (c <= 512 * E) return ln_tile<T, VEC, 512, N, BWD, M>(a, mode);
+    // the ring holds a row per stage at least
+    const int64_t row = round_up(c * int64_t(sizeof(T)) + 32, 128) * (BWD ? 2 : 1);
+    if (c <= 512 * 2 * E && row * LN_STAGES <= 200 * 1024) return ln_tile<T, VEC, 512, 2 * N, BWD, M>(a, mode);
+    *done = false;
+    return NNVB_OK;
+}
+
+// Whether all rows are whole 16-byte pieces on 16-byte boundaries, and how tiles of them are copied.
+template <typename T>
+void ln_access(const LnArgs& a, bool bwd, bool* vec, int* mode) {
+    constexpr int64_t V = 16 / sizeof(T);
+    auto on16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    const bool base = on16(a.x) && (!bwd || on16(a.dy));
+    const bool pieces = base && a.cols % V == 0 && a.ldx % V == 0 && (!bwd || a.lddy % V == 0);
+    *vec = pieces && on16(a.scale) && on16(a.offset) && on16(a.out) && a.ldo % V == 0;
+    if (base && a.ldx == a.cols && (!bwd || a.lddy == a.cols)) *mode = LN_RANGE;
+    else *mode = pieces ? LN_BY_ROW : LN_PLAIN;
+}
+
+template <typename T, bool BWD>
+int ln_run(LnArgs& a, bool* done) {
+    bool vec;
+    int mode;
+    ln_access<T>(a, BWD, &vec, &mode);
+    return vec ? ln_by_width<T, 16 / sizeof(T), BWD>(a, mode, done) : ln_by_width<T, 1, BWD>(a, mode, done);
+}
+
+template <typename T>
+int ln_forward_t(LnArgs a) {
+    using A = typename AccOf<T>::type;
+    bool done;
+    NNVB_TRY((ln_run<T, false>(a, &done)));
+    if (done) return NNVB_OK;
+    ln_forward_wide_kernel<T><<<unsigned(a.rows), 1024, 0, a.st>>>(
+        a.cols, static_cast<const T*>(a.x), a.ldx, static_cast<const T*>(a.scale), static_cast<const T*>(a.offset),
+        A(a.eps), static_cast<T*>(a.out), a.ldo, static_cast<A*>(a.mean), static_cast<A*>(a.rstd));
+    NNVB_CUDA(cudaGetLastError());
+    return NNVB_OK;
+}
 
 template <typename T>
 int ln_backward_t(LnArgs a, void* dscale, void* doffset) {
     using A = typename AccOf<T>::type;
-    const bool vec = aligned_rows<T>(a.cols, {a.dy, a.x, a.scale, a.out}, {a.lddy, a.ldx, a.ldo});
-    const int sms = sm_count();
-    const bool done = ln_variant<T>(a.cols, vec, [&](auto v) {
-        constexpr int TPR = decltype(v)::TPR, BLOCK = TPR > LN_BLOCK ? TPR : LN_BLOCK;
-        const int64_t per_sm = BLOCK > 256 ? 2 : 4;
-        a.grid = int(std::min<int64_t>({ceil_div(a.rows, BLOCK / TPR), sms * per_sm, LN_MAX_PARTS}));
-        run_backward<T, decltype(v)::VEC, decltype(v)::TPR, decltype(v)::NV>(a);
-    });
+    bool done;
+    NNVB_TRY((ln_run<T, true>(a, &done)));
     if (!done) {
         ln_backward_wide_kernel<T><<<unsigned(a.rows), 1024, 0, a.st>>>(
             a.cols, static_cast<const T*>(a.dy), a.lddy, static_cast<const T*>(a.x), a.ldx, static_cast<const T*>(a.scale),
             static_cast<const A*>(a.mean), static_cast<const A*>(a.rstd), static_cast<T*>(a.out), a.ldo);
+        NNVB_CUDA(cudaGetLastError());
         if (a.partial) {
-            NNVB_CUDA(cudaGetLastError());
             const int64_t cb = ceil_div(a.cols, 256);
-            a.grid = int(std::max<int64_t>(1, std::min<int64_t>({a.rows, LN_MAX_PARTS, ceil_div(int64_t(sms) * 8, cb)})));
+            a.grid = int(std::max<int64_t>(1, std::min<int64_t>({a.rows, LN_MAX_PARTS, ceil_div(int64_t(sm_count()) * 8, cb)})));
             ln_weights_wide_kernel<T><<<dim3(unsigned(cb), unsigned(a.grid)), 256, 0, a.st>>>(
                 a.rows, a.cols, static_cast<const T*>(a.dy), a.lddy, static_cast<const T*>(a.x), a.ldx,
                 static_cast<const A*>(a.mean), static_cast<const A*>(a.rstd), static_cast<A*>(a.partial));
+            NNVB_CUDA(cudaGetLastError());
         }
     }
-    NNVB_CUDA(cudaGetLastError());
     if (a.partial) {
-        ln_reduce_kernel<T><<<unsigned(ceil_div(2 * a.cols, 32)), 256, 0, a.st>>>(
+        ln_reduce_kernel<T><<<unsigned(ceil_div(2 * a.cols, 32)), 1024, 0, a.st>>>(
             a.grid, a.cols, static_cast<const A*>(a.partial), static_cast<T*>(dscale), static_cast<T*>(doffset));
         NNVB_CUDA(cudaGetLastError());
     }
