@@ -20,6 +20,7 @@
 // Sums are held in float (double for double).
 #include <algorithm>
 #include <initializer_list>
+#include <type_traits>
 
 #include "common.cuh"
 #include "mma_f64.cuh"
@@ -35,32 +36,40 @@ __device__ __forceinline__ A warp_sum(A x) {
     return x;
 }
 
-// Sums of x and y over the TPR threads of a group, the same bits in each of them.  `red` holds a pair per warp, in two
-// halves that take turns, so that one barrier among the group's warps per call suffices.
-template <int TPR, typename A>
-__device__ __forceinline__ void group_sum(A& x, A& y, A (*red)[2], int& flip) {
+// Sums of K values over the TPR threads of a group, the same bits in each of them.  `red` holds a value per warp and
+// sum, in two halves that take turns, so that one barrier among the group's warps per call suffices.
+template <int TPR, int K, typename A>
+__device__ __forceinline__ void group_sum(A (&v)[K], A (*red)[32], int& flip) {
 #pragma unroll
-    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) {
-        x += __shfl_xor_sync(0xffffffffu, x, o, 32);
-        y += __shfl_xor_sync(0xffffffffu, y, o, 32);
-    }
+    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o, 32);
     if constexpr (TPR > 32) {
-        constexpr int W = TPR / 32;
+        constexpr int W = TPR / 32, V = W * sizeof(A) < 16 ? W : 16 / sizeof(A);
         const int warp = threadIdx.x / 32, w0 = warp / W * W;
-        A(*r)[2] = red + flip;
-        flip ^= 32;
-        if (threadIdx.x % 32 == 0) { r[warp][0] = x; r[warp][1] = y; }
-        named_bar_sync(1 + warp / W, TPR);
-        x = y = 0;
+        A(*r)[32] = red + flip;
+        flip ^= 2;
+        if (threadIdx.x % 32 == 0)
 #pragma unroll
-        for (int i = 0; i < W; ++i) { x += r[w0 + i][0]; y += r[w0 + i][1]; }
+            for (int k = 0; k < K; ++k) r[k][warp] = v[k];
+        named_bar_sync(1 + warp / W, TPR);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            v[k] = 0;
+#pragma unroll
+            for (int i = 0; i < W; i += V) {
+                const auto q = *reinterpret_cast<const Pack<A, V>*>(&r[k][w0 + i]);
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[k] += q.v[e];
+            }
+        }
     }
 }
 template <int TPR, typename A>
-__device__ __forceinline__ A group_sum1(A x, A (*red)[2], int& flip) {
-    A y = 0;
-    group_sum<TPR>(x, y, red, flip);
-    return x;
+__device__ __forceinline__ A group_sum1(A x, A (*red)[32], int& flip) {
+    A v[1] = {x};
+    group_sum<TPR>(v, red, flip);
+    return v[0];
 }
 
 // Makes the compiler forget what it has derived from 16-bit elements: converting them again is one instruction each,
@@ -102,7 +111,7 @@ ln_tile_kernel(const __grid_constant__ LnTile p) {
     extern __shared__ __align__(128) unsigned char ring[];
     __shared__ uint64_t full[LN_STAGES], empty[LN_STAGES];
     __shared__ int abort_flag;
-    __shared__ A red[64][2];
+    __shared__ __align__(16) A red[4][32];
     const int tid = threadIdx.x;
     const int cols = p.cols, R = p.R;
     const int stage_bytes = p.tensor_bytes * (BWD ? 2 : 1);
@@ -145,8 +154,23 @@ ln_tile_kernel(const __grid_constant__ LnTile p) {
     }
 
     const int t = tid % TPR, grp = tid / TPR;
-    P sc[N], of[BWD ? 1 : N];
-    A acc_s[BWD ? N : 1][VEC], acc_o[BWD ? N : 1][VEC];
+    P sc[N], of[N];
+    // elements are worked on in pairs (one instruction for two floats) where an access holds pairs
+    constexpr int UN = VEC > 1 ? 2 : 1, H = VEC / UN;
+    using U = typename std::conditional<VEC == 1, A, Pair<A>>::type;
+    auto one = [](A x) { if constexpr (VEC == 1) return x; else return Pair<A>{x, x}; };
+    auto unit = [](const P& v, int e) {
+        if constexpr (VEC == 1) return A(to_acc(v.v[0]));
+        else return Pair<A>{A(to_acc(v.v[e])), A(to_acc(v.v[e + 1]))};
+    };
+    auto put = [](P& o, int e, U z) {
+        if constexpr (VEC == 1) o.v[0] = from_acc<T, A>(z);
+        else {
+            o.v[e] = from_acc<T, A>(z.x);
+            o.v[e + 1] = from_acc<T, A>(z.y);
+        }
+    };
+    U acc_s[BWD ? N * H : 1], acc_o[BWD ? N * H : 1];
     const bool has_s = p.scale != nullptr, has_o = !BWD && p.offset != nullptr;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -156,10 +180,9 @@ ln_tile_kernel(const __grid_constant__ LnTile p) {
             if constexpr (!BWD)
                 if (has_o) of[i] = *reinterpret_cast<const P*>(static_cast<const T*>(p.offset) + c);
         }
-        if constexpr (BWD)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) { acc_s[i][e] = 0; acc_o[i][e] = 0; }
     }
+#pragma unroll
+    for (int f = 0; f < (BWD ? N * H : 1); ++f) acc_s[f] = acc_o[f] = one(0);
     __syncthreads();
 
     const A inv_n = A(1) / A(cols), eps = A(p.eps);
@@ -202,81 +225,78 @@ ln_tile_kernel(const __grid_constant__ LnTile p) {
             const bool live = base + grp < n;
             if (TPR >= 32 && !live) break;      // groups of whole warps go on to the next tile
             P px[N];
+            auto has = [&](int i) { return live && (t + i * TPR) * VEC < cols; };
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int c = (t + i * TPR) * VEC;
-                if (live && c < cols) px[i] = *reinterpret_cast<const P*>(sx + c);
-            }
+            for (int i = 0; i < N; ++i)
+                if (has(i)) px[i] = *reinterpret_cast<const P*>(sx + (t + i * TPR) * VEC);
             if constexpr (!BWD) {
-                A sum = 0;
+                U sum = one(0);
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (live && (t + i * TPR) * VEC < cols)
+                    if (has(i))
 #pragma unroll
-                        for (int e = 0; e < VEC; ++e) sum += to_acc(px[i].v[e]);
-                const A mean = group_sum1<TPR>(sum, red, flip) * inv_n;
-                A dev = 0;
+                        for (int e = 0; e < VEC; e += UN) sum = add2(sum, unit(px[i], e));
+                const A mean = group_sum1<TPR>(across(sum), red, flip) * inv_n;
+                U dev = one(0);
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (live && (t + i * TPR) * VEC < cols) {
+                    if (has(i)) {
                         if (AGAIN) ln_forget(px[i]);
 #pragma unroll
-                        for (int e = 0; e < VEC; ++e) {
-                            const A d = to_acc(px[i].v[e]) - mean;
-                            dev += d * d;
+                        for (int e = 0; e < VEC; e += UN) {
+                            const U d = add2(unit(px[i], e), one(-mean));
+                            dev = fma2(d, d, dev);
                         }
                     }
-                A rstd = rsqrt_acc(group_sum1<TPR>(dev, red, flip) * inv_n + eps);
+                A rstd = rsqrt_acc(group_sum1<TPR>(across(dev), red, flip) * inv_n + eps);
                 if (live && t == 0) {
                     if (p.mean) static_cast<A*>(p.mean)[row] = mean;
                     if (p.rstd) static_cast<A*>(p.rstd)[row] = rstd;
                 }
                 if (!ok) rstd = A(NAN);
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const int c = (t + i * TPR) * VEC;
-                    if (live && c < cols) {
+                for (int i = 0; i < N; ++i)
+                    if (has(i)) {
                         P o;
-                        if (AGAIN) ln_forget(px[i]);
-                        if (has_s) ln_forget(sc[i]);
-                        if (has_o) ln_forget(of[i]);
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e) {
-                            A z = (to_acc(px[i].v[e]) - mean) * rstd;
-                            if (has_s) z *= to_acc(sc[i].v[e]);
-                            if (has_o) z += to_acc(of[i].v[e]);
-                            o.v[e] = from_acc<T, A>(z);
+                        if (AGAIN) {
+                            ln_forget(px[i]);
+                            if (has_s) ln_forget(sc[i]);
+                            if (has_o) ln_forget(of[i]);
                         }
-                        *reinterpret_cast<P*>(out + c) = o;
+#pragma unroll
+                        for (int e = 0; e < VEC; e += UN) {
+                            U z = mul2(add2(unit(px[i], e), one(-mean)), one(rstd));
+                            if (has_s) z = has_o ? fma2(z, unit(sc[i], e), unit(of[i], e)) : mul2(z, unit(sc[i], e));
+                            else if (has_o) z = add2(z, unit(of[i], e));
+                            put(o, e, z);
+                        }
+                        *reinterpret_cast<P*>(out + (t + i * TPR) * VEC) = o;
                     }
-                }
             } else {
                 P pg[N];
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const int c = (t + i * TPR) * VEC;
-                    if (live && c < cols) pg[i] = *reinterpret_cast<const P*>(sg + c);
-                }
+                for (int i = 0; i < N; ++i)
+                    if (has(i)) pg[i] = *reinterpret_cast<const P*>(sg + (t + i * TPR) * VEC);
                 const A mu = live ? __ldg(static_cast<const A*>(p.mean) + row) : A(0);
                 const A rs = live ? __ldg(static_cast<const A*>(p.rstd) + row) : A(0);
-                A s1 = 0, s2 = 0;
+                U s1 = one(0), s2 = one(0);
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (live && (t + i * TPR) * VEC < cols) {
-                        if (has_s) ln_forget(sc[i]);
+                    if (has(i)) {
+                        if (AGAIN && has_s) ln_forget(sc[i]);
 #pragma unroll
-                        for (int e = 0; e < VEC; ++e) {
-                            const A d = to_acc(pg[i].v[e]), g = has_s ? d * to_acc(sc[i].v[e]) : d;
-                            s1 += g;
-                            s2 += g * (to_acc(px[i].v[e]) - mu);
+                        for (int e = 0; e < VEC; e += UN) {
+                            const U d = unit(pg[i], e), g = has_s ? mul2(d, unit(sc[i], e)) : d;
+                            s1 = add2(s1, g);
+                            s2 = fma2(g, add2(unit(px[i], e), one(-mu)), s2);
                         }
                     }
-                group_sum<TPR>(s1, s2, red, flip);
-                const A k1 = s1 * inv_n * rs, k2 = s2 * inv_n * rs * rs * rs;
+                A sums[2] = {across(s1), across(s2)};
+                group_sum<TPR>(sums, red, flip);
+                const A k1 = -sums[0] * inv_n * rs, k2 = -sums[1] * inv_n * rs * rs * rs;
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const int c = (t + i * TPR) * VEC;
-                    if (live && c < cols) {
+                for (int i = 0; i < N; ++i)
+                    if (has(i)) {
                         P o;
                         if (AGAIN) {
                             ln_forget(px[i]);
@@ -284,16 +304,16 @@ ln_tile_kernel(const __grid_constant__ LnTile p) {
                             if (has_s) ln_forget(sc[i]);
                         }
 #pragma unroll
-                        for (int e = 0; e < VEC; ++e) {
-                            const A xc = to_acc(px[i].v[e]) - mu, d = to_acc(pg[i].v[e]), dr = d * rs;
-                            acc_s[i][e] += dr * xc;
-                            acc_o[i][e] += d;
-                            const A g = has_s ? dr * to_acc(sc[i].v[e]) : dr;
-                            o.v[e] = from_acc<T, A>(g - (k1 + xc * k2));
+                        for (int e = 0; e < VEC; e += UN) {
+                            const U xc = add2(unit(px[i], e), one(-mu)), d = unit(pg[i], e), dr = mul2(d, one(rs));
+                            U &as = acc_s[i * H + e / UN], &ao = acc_o[i * H + e / UN];
+                            as = fma2(dr, xc, as);
+                            ao = add2(ao, d);
+                            const U k = fma2(xc, one(k2), one(k1));
+                            put(o, e, has_s ? fma2(dr, unit(sc[i], e), k) : add2(dr, k));
                         }
-                        *reinterpret_cast<P*>(out + c) = o;
+                        *reinterpret_cast<P*>(out + (t + i * TPR) * VEC) = o;
                     }
-                }
             }
         }
         if (p.mode != LN_PLAIN) {
@@ -327,7 +347,11 @@ ln_tile_kernel(const __grid_constant__ LnTile p) {
             const int i = k >> 1;
             __syncthreads();
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) buf[tid * VEC + e] = ((k & 1) ? acc_o[i][e] : acc_s[i][e]) + bad;
+            for (int e = 0; e < VEC; ++e) {
+                const U a = (k & 1) ? acc_o[i * H + e / UN] : acc_s[i * H + e / UN];
+                if constexpr (VEC == 1) buf[tid] = a + bad;
+                else buf[tid * VEC + e] = (e % 2 ? a.y : a.x) + bad;
+            }
             __syncthreads();
             for (int j = tid; j < TPR * VEC; j += LN_THREADS) {
                 const int c = i * TPR * VEC + j;
@@ -348,7 +372,7 @@ ln_forward_wide_kernel(int64_t cols, const T* __restrict__ x, int64_t ldx, const
                        const T* __restrict__ offset, typename AccOf<T>::type eps, T* __restrict__ y, int64_t ldy,
                        typename AccOf<T>::type* __restrict__ mean_out, typename AccOf<T>::type* __restrict__ rstd_out) {
     using A = typename AccOf<T>::type;
-    __shared__ A red[64][2];
+    __shared__ __align__(16) A red[4][32];
     int flip = 0;
     const int64_t row = blockIdx.x;
     const T* xr = x + row * ldx;
@@ -406,7 +430,7 @@ ln_backward_wide_kernel(int64_t cols, const T* __restrict__ dy, int64_t lddy, co
                         const T* __restrict__ scale, const typename AccOf<T>::type* __restrict__ mean,
                         const typename AccOf<T>::type* __restrict__ rstd, T* __restrict__ dx, int64_t lddx) {
     using A = typename AccOf<T>::type;
-    __shared__ A red[64][2];
+    __shared__ __align__(16) A red[4][32];
     int flip = 0;
     const int64_t row = blockIdx.x;
     const T *xr = x + row * ldx, *gr = dy + row * lddy;
@@ -418,8 +442,9 @@ ln_backward_wide_kernel(int64_t cols, const T* __restrict__ dy, int64_t lddy, co
         s1 += g;
         s2 += g * z;
     }
-    group_sum<1024>(s1, s2, red, flip);
-    const A m1 = s1 / A(cols), m2 = s2 / A(cols);
+    A sums[2] = {s1, s2};
+    group_sum<1024>(sums, red, flip);
+    const A m1 = sums[0] / A(cols), m2 = sums[1] / A(cols);
     for (int64_t c = threadIdx.x; c < cols; c += 1024) {
         const A z = (to_acc(xr[c]) - mu) * r;
         const A g = scale ? to_acc(gr[c]) * to_acc(scale[c]) : to_acc(gr[c]);

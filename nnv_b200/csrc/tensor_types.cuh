@@ -29,6 +29,49 @@ struct alignas(sizeof(T) * N) Pack {
     T v[N];
 };
 
+// Pairs of sums: two float operations are one instruction (f32x2), two doubles are two.
+template <typename A> struct Pair { A x, y; };
+__device__ __forceinline__ uint64_t pair_bits(Pair<float> a) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+    return r;
+}
+__device__ __forceinline__ Pair<float> pair_of(uint64_t b) {
+    Pair<float> a;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(b));
+    return a;
+}
+__device__ __forceinline__ Pair<float> add2(Pair<float> a, Pair<float> b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+    return pair_of(r);
+}
+__device__ __forceinline__ Pair<float> mul2(Pair<float> a, Pair<float> b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+    return pair_of(r);
+}
+__device__ __forceinline__ Pair<float> fma2(Pair<float> a, Pair<float> b, Pair<float> c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)), "l"(pair_bits(c)));
+    return pair_of(r);
+}
+__device__ __forceinline__ Pair<double> add2(Pair<double> a, Pair<double> b) { return {a.x + b.x, a.y + b.y}; }
+__device__ __forceinline__ Pair<double> mul2(Pair<double> a, Pair<double> b) { return {a.x * b.x, a.y * b.y}; }
+__device__ __forceinline__ Pair<double> fma2(Pair<double> a, Pair<double> b, Pair<double> c) {
+    return {fma(a.x, b.x, c.x), fma(a.y, b.y, c.y)};
+}
+// a single sum, for elements that do not come in pairs
+__device__ __forceinline__ float add2(float a, float b) { return a + b; }
+__device__ __forceinline__ float mul2(float a, float b) { return a * b; }
+__device__ __forceinline__ float fma2(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ double add2(double a, double b) { return a + b; }
+__device__ __forceinline__ double mul2(double a, double b) { return a * b; }
+__device__ __forceinline__ double fma2(double a, double b, double c) { return fma(a, b, c); }
+template <typename A> __device__ __forceinline__ A across(Pair<A> a) { return a.x + a.y; }
+__device__ __forceinline__ float across(float a) { return a; }
+__device__ __forceinline__ double across(double a) { return a; }
+
 __device__ __forceinline__ float rsqrt_acc(float x) { return 1.0f / sqrtf(x); }
 __device__ __forceinline__ double rsqrt_acc(double x) { return 1.0 / sqrt(x); }
 
