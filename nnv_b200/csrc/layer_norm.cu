@@ -120,11 +120,11 @@ ln_tile_kernel(const __grid_constant__ LnTile p) {
 
     auto rows_of = [&](int64_t tile) { return int(p.rows - tile * R < R ? p.rows - tile * R : R); };
     // bytes before the first row of a tile in its stage
-    auto lead = [&](int64_t tile) { return p.mode == LN_RANGE ? int(tile * R * pitch % 16) : 0; };
+    auto lead = [&](int64_t tile) { return VEC == 1 && p.mode == LN_RANGE ? int(uint32_t(tile * R * pitch) % 16) : 0; };
     // Bytes that one tensor's copy of a tile moves.  A range runs from the boundary before its first row to the one behind
     // its last, but not past the last boundary inside the tensor: what lies behind that is loaded apart.
     auto bytes_of = [&](int64_t tile) {
-        if (p.mode != LN_RANGE) return uint32_t(rows_of(tile) * pitch);
+        if (VEC > 1 || p.mode != LN_RANGE) return uint32_t(rows_of(tile) * pitch);
         const int64_t from = tile * R * pitch / 16 * 16, to = (tile * R + rows_of(tile)) * pitch, last = p.rows * pitch / 16 * 16;
         const int64_t end = (to + 15) / 16 * 16 < last ? (to + 15) / 16 * 16 : last;
         return uint32_t(end > from ? end - from : 0);
@@ -204,7 +204,7 @@ ln_tile_kernel(const __grid_constant__ LnTile p) {
             __syncthreads();
         } else {
             ok = ok && mbar_wait_or_abort(&full[s], phase, &abort_flag);
-            if (p.mode == LN_RANGE && tile + 8 >= p.n_tiles) {       // under 16 bytes: at most 7 tiles of one element
+            if (VEC == 1 && p.mode == LN_RANGE && tile + 8 >= p.n_tiles) {       // under 16 bytes: at most 7 tiles of one element
                 const int64_t all = n * pitch, got = int64_t(bytes_of(tile)) - lead(tile);
                 const int left = int((all - (got > 0 ? (got < all ? got : all) : 0)) / int(sizeof(T)));
                 if (left > 0) {                 // the tensor's last elements

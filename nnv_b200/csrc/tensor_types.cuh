@@ -72,7 +72,7 @@ template <typename A> __device__ __forceinline__ A across(Pair<A> a) { return a.
 __device__ __forceinline__ float across(float a) { return a; }
 __device__ __forceinline__ double across(double a) { return a; }
 
-__device__ __forceinline__ float rsqrt_acc(float x) { return 1.0f / sqrtf(x); }
-__device__ __forceinline__ double rsqrt_acc(double x) { return 1.0 / sqrt(x); }
+__device__ __forceinline__ float rsqrt_acc(float x) { return rsqrtf(x); }
+__device__ __forceinline__ double rsqrt_acc(double x) { return rsqrt(x); }
 
 }  // namespace nnvb
