@@ -61,6 +61,7 @@ __device__ __forceinline__ Pair<double> mul2(Pair<double> a, Pair<double> b) { r
 __device__ __forceinline__ Pair<double> fma2(Pair<double> a, Pair<double> b, Pair<double> c) {
     return {fma(a.x, b.x, c.x), fma(a.y, b.y, c.y)};
 }
+template <typename A> __device__ __forceinline__ Pair<A> both(A x) { return {x, x}; }
 // a single sum, for elements that do not come in pairs
 __device__ __forceinline__ float add2(float a, float b) { return a + b; }
 __device__ __forceinline__ float mul2(float a, float b) { return a * b; }
