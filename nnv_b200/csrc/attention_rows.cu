@@ -317,14 +317,16 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
                  : "memory");
 }
 
-constexpr int RING = 4;                                            // blocks of states of a warp's ring
+
+// blocks of states of a warp's ring: as many as let several blocks share an SM
+template <int DP> constexpr int ROWS_RING = DP == 64 ? 4 : 3;
 
 // WIDE: 9 to 16 rows; else up to 8
 template <typename T, int DP, bool WIDE>
 __global__ void __launch_bounds__(ROWS_THREADS)
 attn_rows_mma_kernel(AttnArgs a) {
     constexpr int KEYS = 16, ROW = DP * 2, BLOCK = KEYS * ROW;     // bytes of a state, of a block of states of K or V
-    constexpr int PIECES = DP / 8, NR = WIDE ? 16 : 8, NT = DP / 8, KS = DP / 16;
+    constexpr int PIECES = DP / 8, NR = WIDE ? 16 : 8, NT = DP / 8, KS = DP / 16, RING = ROWS_RING<DP>;
     extern __shared__ __align__(128) unsigned char rings[];
     __shared__ float part_m[WARPS][NR], part_l[WARPS][NR], all_m[NR], all_l[NR];
     __shared__ __align__(16) float all_o[NR][DP];
@@ -553,9 +555,9 @@ template <typename T, int DP>
 int rows_by_count(cudaStream_t st, const AttnArgs& a) {
     const int64_t rows = int64_t(a.Hq / a.Hkv) * a.Lq;
     if constexpr (sizeof(T) == 2) {
-        constexpr int SMEM = WARPS * RING * 2 * 16 * DP * 2;
-        return rows <= 8 ? launch_rows(attn_rows_mma_kernel<T, DP, false>, st, a, 16, DP == 64 ? 3 : 2, SMEM)
-                         : launch_rows(attn_rows_mma_kernel<T, DP, true>, st, a, 16, DP == 64 ? 3 : 2, SMEM);
+        constexpr int SMEM = WARPS * ROWS_RING<DP> * 2 * 16 * DP * 2;
+        return rows <= 8 ? launch_rows(attn_rows_mma_kernel<T, DP, false>, st, a, 16, 2, SMEM)
+                         : launch_rows(attn_rows_mma_kernel<T, DP, true>, st, a, 16, 2, SMEM);
     } else {
         constexpr int KEYS = RowsShape<T, 1, DP>::KEYS;
         if (rows <= 1) return launch_rows(attn_rows_kernel<T, 1, DP>, st, a, KEYS, 3, 0);

@@ -24,6 +24,8 @@ __device__ unsigned long long g_timeouts;         // waits given up (a broken ha
 
 constexpr int ROWS = 128;                          // rows of a tile of positions, states of a tile
 constexpr int FWD_THREADS = 320;
+constexpr int EMULATED = 4;                        // of 16 exponentials run on the FMA pipe (0: 460 us, 4: 459, 6: 474 at
+                                                   // 8 x 2048 x 4096 x 16 x 128; 416, 387, 407 with 64 channels)
 
 template <typename T> constexpr bool is_bf16 = false;
 template <> constexpr bool is_bf16<__nv_bfloat16> = true;
@@ -52,6 +54,31 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
+// 2^x on the FMA pipe, for a share of the weights: the exponential unit takes 16 a cycle, half of what the tensor pipe
+// needs of them.  x = i + f with f in [-1/2, 1/2]; 2^f by the polynomial of degree 4 that interpolates it at the
+// Chebyshev points (relative error below 5e-6, a 500th of P's rounding), times 2^i.  x <= 8 here; below
+// -125 the result is about 2^-125 instead of less.
+__device__ __forceinline__ Pair<float> ex2_poly(Pair<float> x) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-125.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-125.f));
+    const float magic = 12582912.f;                    // 1.5 * 2^23: adding it rounds to an integer in the low bits
+    const Pair<float> r = add2(x, both(magic));
+    const Pair<float> f = add2(x, mul2(add2(r, both(-magic)), both(-1.f)));
+    Pair<float> y = both(9.666368515e-03f);
+    y = fma2(y, f, both(5.592197584e-02f));
+    y = fma2(y, f, both(2.402234904e-01f));
+    y = fma2(y, f, both(6.931210452e-01f));
+    y = fma2(y, f, both(1.000000000e+00f));
+    // as a product, not as a sum of bits: NaN stays NaN
+    return mul2(y, {__int_as_float((__float_as_int(r.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(r.y) << 23) + 0x3f800000)});
 }
 
 struct TcMaps {
@@ -230,8 +257,11 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
             }
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int j = 0; j < 128; ++j) mx[j % 4] = fmaxf(mx[j % 4], __uint_as_float(s[j / 32][j % 32]));
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            for (int j = 0; j < 128; j += 8)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    mx[e] = max3(mx[e], __uint_as_float(s[(j + 2 * e) / 32][(j + 2 * e) % 32]), __uint_as_float(s[(j + 2 * e) / 32][(j + 2 * e) % 32 + 1]));
+            const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
             const bool raise = m == -INFINITY ? top > m : (top - m) * c > 8.f;
             if (i == 0) {
                 m = top;
@@ -250,20 +280,20 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
                 }
             }
             const float mc = m == -INFINITY ? 0.f : m * c;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            Pair<float> sum[2] = {both(0.f), both(0.f)};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint32_t p[16];
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
-                    const float x = ex2(__uint_as_float(s[j][e]) * c - mc), y = ex2(__uint_as_float(s[j][e + 1]) * c - mc);
-                    sum[e / 2 % 4] += x;
-                    sum[e / 2 % 4] += y;
-                    p[e / 2] = pack2<T>(x, y);
+                    Pair<float> x = fma2({__uint_as_float(s[j][e]), __uint_as_float(s[j][e + 1])}, both(c), both(-mc));
+                    x = e % 16 < EMULATED ? ex2_poly(x) : Pair<float>{ex2(x.x), ex2(x.y)};
+                    sum[e / 2 % 2] = add2(sum[e / 2 % 2], x);
+                    p[e / 2] = pack2<T>(x.x, x.y);
                 }
                 tmem_store16(s_at + j * 16, p);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             tmem_wait_store();
             tmem_fence_before();
             __syncwarp();
@@ -437,7 +467,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
             const int rest = KV ? BROWS : n - row;
             // K rows behind the valid states may hold anything, and 0 * NaN is NaN: they are cleared here.  (V
             // needs nothing: its rows only make columns of dP that are masked.)
-            const bool clear = rest < BROWS && n < a.Lk;
+            const bool clear = !KV && rest < BROWS && n < a.Lk;
             uint64_t* bar = clear ? &tail : &full[s];
             if (lane == 0) {
                 mbar_expect_bytes(bar, 2 * SM::BTILE + (KV ? SM::STATS : 0));
@@ -451,8 +481,9 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
             }
             if (clear) {
                 ok = __all_sync(0xffffffffu, mbar_wait_fast(&tail, 0, abort));
-                for (int j = lane; j < (BROWS - rest) * 8 * (DP / 64); j += 32) {
-                    const int box = j / ((BROWS - rest) * 8), r = j % ((BROWS - rest) * 8);
+                const int pieces = KV ? 8 : (BROWS - rest) * 8;
+                for (int j = lane; j < pieces * (DP / 64); j += 32) {
+                    const int box = j / pieces, r = j % pieces;
                     *reinterpret_cast<uint4*>(dst + box * SM::BBOX + rest * 128 + r * 16) = make_uint4(0, 0, 0, 0);
                 }
                 async_proxy_fence();
@@ -541,9 +572,11 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
             tmem_load32(s, s_at);
             tmem_wait_load();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-                const float x = ex2(__uint_as_float(s[e]) * c - (KV ? sl[e] : my_lse));
-                s[e] = __float_as_uint(!KV && e >= rest ? 0.f : x);
+            for (int e = 0; e < 32; e += 2) {
+                const Pair<float> lse = KV ? *reinterpret_cast<const Pair<float>*>(sl + e) : both(my_lse);
+                const Pair<float> x = fma2({__uint_as_float(s[e]), __uint_as_float(s[e + 1])}, both(c), {-lse.x, -lse.y});
+                s[e] = __float_as_uint(!KV && e >= rest ? 0.f : ex2(x.x));
+                s[e + 1] = __float_as_uint(!KV && e + 1 >= rest ? 0.f : ex2(x.y));
             }
             if (!KV && steps <= 2) {
                 float sum = 0.f;
@@ -572,16 +605,16 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
                 tmem_wait_load();
 #pragma unroll
                 for (int e = 0; e < 16; e += 2) {
-                    float ds[2];
-#pragma unroll
-                    for (int f = 0; f < 2; ++f) {
-                        const int col = g * 16 + e + f;
-                        ds[f] = __uint_as_float(s[col]) * (__uint_as_float(d[e + f]) - (KV ? sl[BROWS + col] : my_delta));
-                        if (!KV && col >= rest) ds[f] = 0.f;               // dP there may be 0 * NaN
-                    }
-                    if (KV) p[e / 2] = pack2<T>(__uint_as_float(s[g * 16 + e]), __uint_as_float(s[g * 16 + e + 1]));
-                    hi[e / 2] = pack2<T>(ds[0], ds[1]);
-                    lo[e / 2] = pack2<T>(ds[0] - unpack_lo<T>(hi[e / 2]), ds[1] - unpack_hi<T>(hi[e / 2]));
+                    const int col = g * 16 + e;
+                    const Pair<float> dl = KV ? *reinterpret_cast<const Pair<float>*>(sl + BROWS + col) : both(my_delta);
+                    const Pair<float> pv{__uint_as_float(s[col]), __uint_as_float(s[col + 1])};
+                    Pair<float> ds = mul2(pv, add2(Pair<float>{__uint_as_float(d[e]), __uint_as_float(d[e + 1])}, Pair<float>{-dl.x, -dl.y}));
+                    if (!KV && col >= rest) ds.x = 0.f;                    // dP there may be 0 * NaN
+                    if (!KV && col + 1 >= rest) ds.y = 0.f;
+                    if (KV) p[e / 2] = pack2<T>(pv.x, pv.y);
+                    hi[e / 2] = pack2<T>(ds.x, ds.y);
+                    ds = add2(ds, Pair<float>{-unpack_lo<T>(hi[e / 2]), -unpack_hi<T>(hi[e / 2])});
+                    lo[e / 2] = pack2<T>(ds.x, ds.y);
                 }
                 if (KV) tmem_store8(s_at + g * 8, p);
                 tmem_store8(s_at + 16 + g * 8, lo);
