@@ -72,6 +72,7 @@ int nnvb_cross_attention_forward(void* stream, const nnvb_attention_desc* d, con
     a.q = q; a.k = k; a.v = v; a.o = out; a.lse = lse; a.lengths = lengths;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (attn_rows_takes(a)) return attn_forward_rows(st, a);
+    if ((d->dtype == NNVB_F64 || d->dtype == NNVB_F32) && d->head_dim <= 128) return attn_forward_wide(st, a);
     return attn_tc_takes_forward(a) ? attn_forward_tc(st, a) : attn_forward_simt(st, a);
 }
 

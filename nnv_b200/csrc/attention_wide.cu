@@ -1,0 +1,396 @@
+// Attention over an encoder's states, forward, for float and double tensors with head sizes up to 128.
+//
+// A block of four warps takes 64 positions of one head and walks over tiles of states with the running maximum and sum of
+// each row's softmax.  K and V tiles arrive by cp.async in a buffer each: V while the scores are computed, the next K
+// while the weights meet V.
+//   double  tensor cores (mma.sync f64 m16n8k8): a warp has 16 rows.  The order of the contraction is free, so channels
+//           (and states) 2t, 2t+1 take the places t, t+4 of a lane: operands are loaded 16 bytes at a time, and scores
+//           become weights in the registers they are in.  Bound by the FP64 pipe.
+//   float   FMA pipe, two terms an instruction: 8 x 16 threads with 8 x 4 scores each; 12 16-byte loads feed 128 FMAs, half
+//           of the cycles the FMAs take.  Bound by the FMA pipe.
+// Where 64-row tiles give the GPU too few blocks, a cluster of up to 16 blocks shares the states of a tile; their results
+// meet in distributed shared memory in a fixed order.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "attention.cuh"
+#include "mma_f64.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace nnvb {
+namespace {
+
+constexpr int BQ = 64, THREADS = 128;
+
+// Row strides (elements) that spread the loads of a warp over all banks.
+template <typename T, int DP>
+struct WideShape {
+    static constexpr bool F64 = sizeof(T) == 8;
+    static constexpr int BK = F64 && DP == 128 ? 32 : 64;          // states of a tile
+    static constexpr int LDQ = F64 ? DP + 8 : DP + 4, LDK = LDQ, LDV = F64 ? DP + 2 : DP + 4, LDP = BK + 4;
+    static constexpr int NQ = BQ * LDQ, NK = BK * LDK, NV = BK * LDV, NP = F64 ? 0 : BQ * LDP;
+    static constexpr int BYTES = (NQ + NK + NV + NP) * int(sizeof(T));
+};
+
+// rows r0 .. r0 + ROWS of a [token] x D slab; rows from n_rows on and columns from D on become 0.  vec: asynchronous
+template <typename T, int ROWS, int DP, int LD>
+__device__ __forceinline__ void load_rows(T* s, const T* g, int64_t stride, int r0, int n_rows, int D, bool vec) {
+    constexpr int V = 16 / sizeof(T), P = DP / V;
+    if (vec) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < ROWS * P; i += THREADS) {
+            const int r = i / P, c = i % P * V;
+            const bool in = r0 + r < n_rows && c < D;              // D is a multiple of V
+            cp_async16(s + r * LD + c, g + (in ? int64_t(r0 + r) * stride + c : 0), in ? 16 : 0);
+        }
+    } else {
+        for (int i = threadIdx.x; i < ROWS * DP; i += THREADS) {
+            const int r = i / DP, c = i % DP;
+            s[r * LD + c] = r0 + r < n_rows && c < D ? g[int64_t(r0 + r) * stride + c] : T(0);
+        }
+    }
+    cp_async_commit();
+}
+
+// A warp's or thread's part of the tile: scores and output of its rows.  Row of index i, and the type's products.
+template <typename T, int DP> struct Work;
+
+template <int DP>
+struct Work<double, DP> {
+    using S = WideShape<double, DP>;
+    static constexpr int NR = 2, NT = S::BK / 8;                   // rows of a lane; 8-state tiles
+    double s[NT][4], o[DP / 8][4];
+    int warp, g, t;
+    __device__ __forceinline__ Work() : warp(threadIdx.x / 32), g(threadIdx.x % 32 / 4), t(threadIdx.x % 4) {
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] = 0;
+    }
+    __device__ __forceinline__ int row(int i) const { return warp * 16 + g + i * 8; }
+    __device__ __forceinline__ void scores(const double* Q, const double* K) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[j][e] = 0;
+        const double* q = Q + row(0) * S::LDQ + 2 * t;
+        const double* k = K + g * S::LDK + 2 * t;
+#pragma unroll 4
+        for (int d = 0; d < DP; d += 8) {
+            const double2 x = *reinterpret_cast<const double2*>(q + d), y = *reinterpret_cast<const double2*>(q + 8 * S::LDQ + d);
+            const double a[4] = {x.x, y.x, x.y, y.y};
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const double2 z = *reinterpret_cast<const double2*>(k + j * 8 * S::LDK + d);
+                const double b[2] = {z.x, z.y};
+                dmma_16x8x8(s[j], a, b);
+            }
+        }
+    }
+    // f(row index, state of the tile, value)
+    template <typename F>
+    __device__ __forceinline__ void each(F&& f) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f(e / 2, j * 8 + 2 * t + e % 2, s[j][e]);
+    }
+    static constexpr int LANES = 4;                                // neighbouring lanes that share a row
+    __device__ __forceinline__ void scale_out(const double (&f)[NR]) {
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] *= f[e / 2];
+    }
+    __device__ __forceinline__ void hand_over(double*) {}          // the weights stay in their registers
+    __device__ __forceinline__ void weigh(const double*, const double* V) {
+        const double* v = V + 2 * t * S::LDV + 2 * g;
+#pragma unroll
+        for (int k = 0; k < NT; ++k) {
+            const double a[4] = {s[k][0], s[k][2], s[k][1], s[k][3]};
+#pragma unroll
+            for (int j = 0; j < DP / 16; ++j) {
+                const double2 x = *reinterpret_cast<const double2*>(v + k * 8 * S::LDV + j * 16);
+                const double2 y = *reinterpret_cast<const double2*>(v + (k * 8 + 1) * S::LDV + j * 16);
+                const double b0[2] = {x.x, y.x}, b1[2] = {x.y, y.y};
+                dmma_16x8x8(o[2 * j], a, b0);
+                dmma_16x8x8(o[2 * j + 1], a, b1);
+            }
+        }
+    }
+    // f(row index, channel, value)
+    template <typename F>
+    __device__ __forceinline__ void each_out(F&& f) const {
+#pragma unroll
+        for (int j = 0; j < DP / 16; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f(i, j * 16 + 4 * t + e, o[2 * j + e % 2][i * 2 + e / 2]);
+    }
+};
+
+template <int DP>
+struct Work<float, DP> {
+    using S = WideShape<float, DP>;
+    static constexpr int NR = 8;
+    float s[NR][4];
+    Pair<float> o[NR][DP / 32];
+    int ty, tx;
+    __device__ __forceinline__ Work() : ty(threadIdx.x / 16), tx(threadIdx.x % 16) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+            for (int e = 0; e < DP / 32; ++e) o[i][e] = both(0.f);
+    }
+    __device__ __forceinline__ int row(int i) const { return ty * NR + i; }
+    __device__ __forceinline__ void scores(const float* Q, const float* K) {
+        Pair<float> acc[NR][4];
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = both(0.f);
+        const float *q = Q + ty * NR * S::LDQ, *k = K + tx * S::LDK;
+#pragma unroll 2
+        for (int d = 0; d < DP; d += 4) {
+            float4 y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(k + 16 * j * S::LDK + d);
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                const float4 x = *reinterpret_cast<const float4*>(q + i * S::LDQ + d);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    acc[i][j] = fma2(Pair<float>{x.x, x.y}, Pair<float>{y[j].x, y[j].y}, acc[i][j]);
+                    acc[i][j] = fma2(Pair<float>{x.z, x.w}, Pair<float>{y[j].z, y[j].w}, acc[i][j]);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[i][j] = across(acc[i][j]);
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F&& f) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f(i, tx + 16 * j, s[i][j]);
+    }
+    static constexpr int LANES = 16;
+    __device__ __forceinline__ void scale_out(const float (&f)[NR]) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+            for (int e = 0; e < DP / 32; ++e) o[i][e] = mul2(o[i][e], both(f[i]));
+    }
+    __device__ __forceinline__ void hand_over(float* P) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) P[row(i) * S::LDP + tx + 16 * j] = s[i][j];
+        __syncwarp();                      // a row's weights are read by the warp that wrote them
+    }
+    __device__ __forceinline__ void weigh(const float* P, const float* V) {
+        const float *p = P + ty * NR * S::LDP, *v = V + tx * 4;
+#pragma unroll 1
+        for (int k = 0; k < S::BK; k += 4) {
+            float4 x[NR];
+#pragma unroll
+            for (int i = 0; i < NR; ++i) x[i] = *reinterpret_cast<const float4*>(p + i * S::LDP + k);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int c = 0; c < DP / 64; ++c) {
+                    const float4 y = *reinterpret_cast<const float4*>(v + (k + e) * S::LDV + 64 * c);
+#pragma unroll
+                    for (int i = 0; i < NR; ++i) {
+                        const float w = e == 0 ? x[i].x : (e == 1 ? x[i].y : (e == 2 ? x[i].z : x[i].w));
+                        o[i][2 * c] = fma2(both(w), Pair<float>{y.x, y.y}, o[i][2 * c]);
+                        o[i][2 * c + 1] = fma2(both(w), Pair<float>{y.z, y.w}, o[i][2 * c + 1]);
+                    }
+                }
+        }
+    }
+    template <typename F>
+    __device__ __forceinline__ void each_out(F&& f) const {
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+            for (int c = 0; c < DP / 64; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f(i, 64 * c + tx * 4 + e, e % 2 ? o[i][2 * c + e / 2].y : o[i][2 * c + e / 2].x);
+    }
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(THREADS)
+attn_fwd_wide_kernel(AttnArgs a, bool vec) {
+    using S = WideShape<T, DP>;
+    using W = Work<T, DP>;
+    constexpr int NR = W::NR;
+    extern __shared__ __align__(128) unsigned char raw[];
+    T* Qs = reinterpret_cast<T*>(raw);
+    T *Ks = Qs + S::NQ, *Vs = Ks + S::NK, *Ps = Vs + S::NV;
+    __shared__ T all_m[BQ], all_l[BQ];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = int(cluster.block_rank()), world = int(cluster.num_blocks());
+    const int tiles = (a.Lq + BQ - 1) / BQ;
+    const int64_t unit = blockIdx.x / world;
+    const int q0 = int(unit % tiles) * BQ;
+    const int h = int(unit / tiles % a.Hq), b = int(unit / tiles / a.Hq);
+    const int g = h / (a.Hq / a.Hkv);
+    const int n = attn_len(a, b);
+    const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + g * a.ks[2];
+    const T* v = static_cast<const T*>(a.v) + b * a.vs[0] + g * a.vs[2];
+    const T c = T(a.scale * LOG2E), ninf = -INFINITY;
+    const int steps = (n + S::BK - 1) / S::BK;
+    W w;
+    T m[NR], l[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) { m[i] = ninf; l[i] = 0; }
+    if (rank < steps) {
+        load_rows<T, BQ, DP, S::LDQ>(Qs, static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2], a.qs[1], q0, a.Lq, a.D, vec);
+        load_rows<T, S::BK, DP, S::LDK>(Ks, k, a.ks[1], rank * S::BK, n, a.D, vec);
+    }
+    for (int it = rank; it < steps; it += world) {
+        const int k0 = it * S::BK;
+        load_rows<T, S::BK, DP, S::LDV>(Vs, v, a.vs[1], k0, n, a.D, vec);
+        cp_async_wait<1>();
+        __syncthreads();
+        w.scores(Qs, Ks);
+        __syncthreads();
+        if (it + world < steps) load_rows<T, S::BK, DP, S::LDK>(Ks, k, a.ks[1], (it + world) * S::BK, n, a.D, vec);
+        else cp_async_commit();
+        T top[NR], f[NR], base[NR];
+#pragma unroll
+        for (int i = 0; i < NR; ++i) top[i] = ninf;
+        const int rest = n - k0;
+        w.each([&](int i, int j, T& x) {
+            x = j < rest ? x * c : ninf;
+            top[i] = x > top[i] ? x : top[i];
+        });
+        bool moved = false;
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+#pragma unroll
+            for (int o = W::LANES / 2; o > 0; o >>= 1) {
+                const T y = __shfl_xor_sync(0xffffffffu, top[i], o, 32);
+                top[i] = y > top[i] ? y : top[i];
+            }
+            const T mn = top[i] > m[i] ? top[i] : m[i];
+            base[i] = mn == ninf ? T(0) : mn;
+            moved = moved || mn != m[i];
+            f[i] = mn != m[i] ? exp_acc(m[i] - base[i]) : T(1);
+            m[i] = mn;
+            l[i] *= f[i];
+        }
+        if (__any_sync(0xffffffffu, moved)) w.scale_out(f);
+        w.each([&](int i, int j, T& x) {
+            x = j < rest ? exp_acc(x - base[i]) : T(0);
+            l[i] += x;
+        });
+        w.hand_over(Ps);
+        cp_async_wait<1>();
+        __syncthreads();
+        w.weigh(Ps, Vs);
+        __syncthreads();
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+        for (int o = W::LANES / 2; o > 0; o >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o, 32);
+    const int64_t lse0 = (int64_t(b) * a.Hq + h) * a.Lq + q0;
+    T* out = static_cast<T*>(const_cast<void*>(a.o)) + b * a.os[0] + int64_t(q0) * a.os[1] + h * a.os[2];
+    const bool first = threadIdx.x % W::LANES == 0;
+    if (world == 1) {
+        T f[NR];
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            f[i] = n > 0 ? T(1) / l[i] : T(0);
+            const int r = w.row(i);
+            if (a.lse && first && q0 + r < a.Lq)
+                static_cast<T*>(a.lse)[lse0 + r] = n > 0 ? m[i] / T(LOG2E) + log_acc(l[i]) : ninf;
+        }
+        w.each_out([&](int i, int d, T x) {
+            const int r = w.row(i);
+            if (q0 + r < a.Lq && d < a.D) out[int64_t(r) * a.os[1] + d] = x * f[i];
+        });
+        return;
+    }
+    // the blocks of a cluster: each leaves its rows over its tiles, then writes a share of the rows
+    __syncthreads();
+    T* mine = Qs;                                                  // [BQ][DP]
+    static_assert(BQ * DP <= S::NQ, "");
+    w.each_out([&](int i, int d, T x) { mine[w.row(i) * DP + d] = x; });
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+        if (first) { all_m[w.row(i)] = m[i]; all_l[w.row(i)] = l[i]; }
+    cluster.sync();
+    for (int i = rank * THREADS + threadIdx.x; i < BQ * DP; i += world * THREADS) {
+        const int r = i / DP, d = i % DP;
+        if (q0 + r >= a.Lq) continue;
+        T top = ninf, sum = 0, x = 0;
+        for (int p = 0; p < world; ++p) {
+            const T y = *cluster.map_shared_rank(&all_m[r], p);
+            top = y > top ? y : top;
+        }
+        const T base = top == ninf ? T(0) : top;
+        for (int p = 0; p < world; ++p) {
+            const T f = exp_acc(*cluster.map_shared_rank(&all_m[r], p) - base);
+            sum += *cluster.map_shared_rank(&all_l[r], p) * f;
+            x += *cluster.map_shared_rank(&mine[i], p) * f;
+        }
+        if (d < a.D) out[int64_t(r) * a.os[1] + d] = n > 0 ? x / sum : T(0);
+        if (d == 0 && a.lse) static_cast<T*>(a.lse)[lse0 + r] = n > 0 ? top / T(LOG2E) + log_acc(sum) : ninf;
+    }
+    cluster.sync();                        // nobody leaves while its shared memory is read
+}
+
+template <typename T, int DP>
+int wide_t(cudaStream_t st, const AttnArgs& a) {
+    using S = WideShape<T, DP>;
+    const int64_t e = sizeof(T);
+    bool vec = a.D * e % 16 == 0;
+    for (auto* s : {a.qs, a.ks, a.vs})
+        for (int i = 0; i < 3; ++i) vec = vec && s[i] * e % 16 == 0;
+    for (const void* p : {a.q, a.k, a.v}) vec = vec && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+    const int64_t units = ceil_div(a.Lq, BQ) * a.Hq * a.B, steps = ceil_div(a.Lk, S::BK);
+    int dev = 0, sms = 148;
+    NNVB_CUDA(cudaGetDevice(&dev));
+    NNVB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    // a cluster's blocks each take two tiles of states at least
+    int world = 1;
+    while (world < 16 && units * world * 2 <= int64_t(sms) * 2 && world * 4 <= steps) world *= 2;
+    NNVB_REQUIRE(units * world < (int64_t(1) << 31), "nnvb_cross_attention_forward: too many tiles (%lld) for one launch",
+                 (long long)units);
+    auto kernel = attn_fwd_wide_kernel<T, DP>;
+    NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
+    if (world > 8) NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(units * world));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = S::BYTES;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = unsigned(world);
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    NNVB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, vec));
+    return NNVB_OK;
+}
+
+}  // namespace
+
+int attn_forward_wide(cudaStream_t st, const AttnArgs& a) {
+    if (a.dtype == NNVB_F64) return a.D <= 64 ? wide_t<double, 64>(st, a) : wide_t<double, 128>(st, a);
+    return a.D <= 64 ? wide_t<float, 64>(st, a) : wide_t<float, 128>(st, a);
+}
+
+}  // namespace nnvb
