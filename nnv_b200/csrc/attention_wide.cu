@@ -227,7 +227,7 @@ struct Work<float, DP> {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 4 && DP == 64 ? 3 : 1)
 attn_fwd_wide_kernel(AttnArgs a, bool vec) {
     using S = WideShape<T, DP>;
     using W = Work<T, DP>;
