@@ -10,9 +10,13 @@
 // A block of 256 threads holds TILE x TILE scores, 16 x 16 threads with (TILE/16)^2 scores each, operands in shared
 // memory in the type sums are held in, rows padded by 16 bytes so that the 16-byte loads of neighbouring rows
 // fall on different banks.  Bound by the FMA pipe: a 4 x 4 register tile needs 8 16-byte loads for 64 FMAs.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "attention.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace nnvb {
 namespace {
@@ -128,6 +132,30 @@ __device__ __forceinline__ void store_rows(T* g, int64_t stride, int r0, int n_r
                     if (d < D) g[int64_t(r) * stride + d] = from_acc<T, A>(acc[i][c * V + e] * f[i]);
                 }
     }
+}
+
+// The blocks of a cluster have summed shares of the same rows: each leaves its sums in `mine`, [TILE][DP], and writes a
+// share of the total, added in block order.
+template <typename T, typename A, int TILE, int DP>
+__device__ void store_shared(cg::cluster_group& cluster, T* g, int64_t stride, int r0, int n_rows, int D, const A* mine, A f) {
+    const int rank = int(cluster.block_rank()), world = int(cluster.num_blocks());
+    for (int i = rank * THREADS + threadIdx.x; i < TILE * DP; i += world * THREADS) {
+        const int r = r0 + i / DP, d = i % DP;
+        if (r >= n_rows || d >= D) continue;
+        A x = 0;
+        for (int p = 0; p < world; ++p) x += *cluster.map_shared_rank(mine + i, p);
+        g[int64_t(r) * stride + d] = from_acc<T, A>(x * f);
+    }
+}
+template <typename A, int TILE, int DP>
+__device__ void leave_rows(A* mine, const A (&acc)[TILE / 16][DP / 16], int ty, int tx) {
+    constexpr int M = TILE / 16, V = VecOf<A>::N, NC = DP / (16 * V);
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int e = 0; e < V; ++e) mine[(ty * M + i) * DP + tx * V + 16 * V * c + e] = acc[i][c * V + e];
 }
 
 template <typename A>
@@ -248,8 +276,11 @@ attn_dq_simt_kernel(AttnArgs a, bool vec) {
     A* Vs = Ks + TILE * LD;
     A* Ps = Vs + TILE * LD;
     const int tiles = (a.Lq + TILE - 1) / TILE;
-    const int q0 = int(blockIdx.x % tiles) * TILE;
-    const int h = int(blockIdx.x / tiles % a.Hq), b = int(blockIdx.x / tiles / a.Hq);
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = int(cluster.block_rank()), world = int(cluster.num_blocks());
+    const int64_t unit = blockIdx.x / world;
+    const int q0 = int(unit % tiles) * TILE;
+    const int h = int(unit / tiles % a.Hq), b = int(unit / tiles / a.Hq);
     const int g = h / (a.Hq / a.Hkv);
     const int n = attn_len(a, b);
     const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
@@ -269,7 +300,7 @@ attn_dq_simt_kernel(AttnArgs a, bool vec) {
     }
     load_tile<T, A, TILE, DP>(Qs, static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2], a.qs[1], q0, a.Lq, a.D, vec);
     load_tile<T, A, TILE, DP>(Gs, static_cast<const T*>(a.dout) + b * a.dos[0] + h * a.dos[2], a.dos[1], q0, a.Lq, a.D, vec);
-    for (int k0 = 0; k0 < n; k0 += TILE) {
+    for (int k0 = rank * TILE; k0 < n; k0 += world * TILE) {
         __syncthreads();
         load_tile<T, A, TILE, DP>(Ks, k, a.ks[1], k0, n, a.D, vec);
         load_tile<T, A, TILE, DP>(Vs, v, a.vs[1], k0, n, a.D, vec);
@@ -288,7 +319,15 @@ attn_dq_simt_kernel(AttnArgs a, bool vec) {
         mul_cols<A, TILE, DP>(acc, Ps, Ks, ty, tx);
     }
     T* dq = static_cast<T*>(a.dq) + (int64_t(b) * a.Lq * a.Hq + h) * a.D;
-    store_rows<T, A, TILE, DP>(dq, int64_t(a.Hq) * a.D, q0, a.Lq, a.D, acc, f, ty, tx);
+    if (world == 1) {
+        store_rows<T, A, TILE, DP>(dq, int64_t(a.Hq) * a.D, q0, a.Lq, a.D, acc, f, ty, tx);
+        return;
+    }
+    __syncthreads();
+    leave_rows<A, TILE, DP>(Qs, acc, ty, tx);
+    cluster.sync();
+    store_shared<T, A, TILE, DP>(cluster, dq, int64_t(a.Hq) * a.D, q0, a.Lq, a.D, Qs, A(a.scale));
+    cluster.sync();                        // nobody leaves while its shared memory is read
 }
 
 // dK, dV: a block per tile of states, over the positions of every query head of its group
@@ -305,8 +344,11 @@ attn_dkv_simt_kernel(AttnArgs a, bool vec) {
     A* Ps = Gs + TILE * LD;
     A* Ss = Ps + TILE * LP;
     const int tiles = (a.Lk + TILE - 1) / TILE;
-    const int k0 = int(blockIdx.x % tiles) * TILE;
-    const int g = int(blockIdx.x / tiles % a.Hkv), b = int(blockIdx.x / tiles / a.Hkv);
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = int(cluster.block_rank()), world = int(cluster.num_blocks());
+    const int64_t unit = blockIdx.x / world;
+    const int k0 = int(unit % tiles) * TILE;
+    const int g = int(unit / tiles % a.Hkv), b = int(unit / tiles / a.Hkv);
     const int G = a.Hq / a.Hkv;
     const int n = attn_len(a, b);
     const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
@@ -322,39 +364,49 @@ attn_dkv_simt_kernel(AttnArgs a, bool vec) {
     if (k0 < n) {
         load_tile<T, A, TILE, DP>(Ks, static_cast<const T*>(a.k) + b * a.ks[0] + g * a.ks[2], a.ks[1], k0, n, a.D, vec);
         load_tile<T, A, TILE, DP>(Vs, static_cast<const T*>(a.v) + b * a.vs[0] + g * a.vs[2], a.vs[1], k0, n, a.D, vec);
-        for (int h = g * G; h < (g + 1) * G; ++h) {
+        const int per_head = (a.Lq + TILE - 1) / TILE;
+        for (int step = rank; step < per_head * G; step += world) {
+            const int h = g * G + step / per_head, q0 = step % per_head * TILE;
             const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2];
             const T* go = static_cast<const T*>(a.dout) + b * a.dos[0] + h * a.dos[2];
-            for (int q0 = 0; q0 < a.Lq; q0 += TILE) {
-                __syncthreads();
-                load_tile<T, A, TILE, DP>(Qs, q, a.qs[1], q0, a.Lq, a.D, vec);
-                load_tile<T, A, TILE, DP>(Gs, go, a.dos[1], q0, a.Lq, a.D, vec);
-                __syncthreads();
-                A s[M][M] = {}, dp[M][M] = {};
-                mul_rows<A, TILE, DP>(s, Qs, Ks, ty, tx);
-                mul_rows<A, TILE, DP>(dp, Gs, Vs, ty, tx);
+            __syncthreads();
+            load_tile<T, A, TILE, DP>(Qs, q, a.qs[1], q0, a.Lq, a.D, vec);
+            load_tile<T, A, TILE, DP>(Gs, go, a.dos[1], q0, a.Lq, a.D, vec);
+            __syncthreads();
+            A s[M][M] = {}, dp[M][M] = {};
+            mul_rows<A, TILE, DP>(s, Qs, Ks, ty, tx);
+            mul_rows<A, TILE, DP>(dp, Gs, Vs, ty, tx);
 #pragma unroll
-                for (int i = 0; i < M; ++i) {
-                    const int r = q0 + ty * M + i;
-                    const int64_t at = (int64_t(b) * a.Hq + h) * a.Lq + r;
-                    const A lse = r < a.Lq ? static_cast<const A*>(a.lse)[at] * A(LOG2E) : A(0);
-                    const A dl = r < a.Lq ? static_cast<const A*>(a.delta)[at] : A(0);
+            for (int i = 0; i < M; ++i) {
+                const int r = q0 + ty * M + i;
+                const int64_t at = (int64_t(b) * a.Hq + h) * a.Lq + r;
+                const A lse = r < a.Lq ? static_cast<const A*>(a.lse)[at] * A(LOG2E) : A(0);
+                const A dl = r < a.Lq ? static_cast<const A*>(a.delta)[at] : A(0);
 #pragma unroll
-                    for (int j = 0; j < M; ++j) {
-                        const A p = r < a.Lq && k0 + tx + 16 * j < n ? exp_acc(s[i][j] * c - lse) : A(0);
-                        Ps[(ty * M + i) * LP + tx + 16 * j] = p;
-                        Ss[(ty * M + i) * LP + tx + 16 * j] = p * (dp[i][j] - dl);
-                    }
+                for (int j = 0; j < M; ++j) {
+                    const A p = r < a.Lq && k0 + tx + 16 * j < n ? exp_acc(s[i][j] * c - lse) : A(0);
+                    Ps[(ty * M + i) * LP + tx + 16 * j] = p;
+                    Ss[(ty * M + i) * LP + tx + 16 * j] = p * (dp[i][j] - dl);
                 }
-                __syncthreads();
-                mul_cols_t<A, TILE, DP>(dv, Ps, Gs, ty, tx);
-                mul_cols_t<A, TILE, DP>(dk, Ss, Qs, ty, tx);
             }
+            __syncthreads();
+            mul_cols_t<A, TILE, DP>(dv, Ps, Gs, ty, tx);
+            mul_cols_t<A, TILE, DP>(dk, Ss, Qs, ty, tx);
         }
     }
     const int64_t base = (int64_t(b) * a.Lk * a.Hkv + g) * a.D, stride = int64_t(a.Hkv) * a.D;
-    store_rows<T, A, TILE, DP>(static_cast<T*>(a.dk) + base, stride, k0, a.Lk, a.D, dk, fk, ty, tx);
-    store_rows<T, A, TILE, DP>(static_cast<T*>(a.dv) + base, stride, k0, a.Lk, a.D, dv, fv, ty, tx);
+    if (world == 1) {
+        store_rows<T, A, TILE, DP>(static_cast<T*>(a.dk) + base, stride, k0, a.Lk, a.D, dk, fk, ty, tx);
+        store_rows<T, A, TILE, DP>(static_cast<T*>(a.dv) + base, stride, k0, a.Lk, a.D, dv, fv, ty, tx);
+        return;
+    }
+    __syncthreads();
+    leave_rows<A, TILE, DP>(Qs, dk, ty, tx);
+    leave_rows<A, TILE, DP>(Gs, dv, ty, tx);
+    cluster.sync();
+    store_shared<T, A, TILE, DP>(cluster, static_cast<T*>(a.dk) + base, stride, k0, a.Lk, a.D, Qs, A(a.scale));
+    store_shared<T, A, TILE, DP>(cluster, static_cast<T*>(a.dv) + base, stride, k0, a.Lk, a.D, Gs, A(1));
+    cluster.sync();                        // nobody leaves while its shared memory is read
 }
 
 // ---------------------------------------------------------------------------
@@ -379,13 +431,30 @@ constexpr int bwd_tile(int dp) {
     return 16;
 }
 
+// `steps`: tiles a block walks over; where there are few blocks a cluster of up to 16 shares them, two each at least
 template <typename K>
-int launch(K kernel, int64_t blocks, int smem, cudaStream_t st, const AttnArgs& a, bool vec) {
-    if (blocks <= 0) return NNVB_OK;
-    NNVB_REQUIRE(blocks < (int64_t(1) << 31), "nnvb_cross_attention: too many tiles (%lld) for one launch", (long long)blocks);
+int launch(K kernel, int64_t units, int64_t steps, int smem, cudaStream_t st, const AttnArgs& a, bool vec) {
+    if (units <= 0) return NNVB_OK;
+    int dev = 0, sms = 148;
+    NNVB_CUDA(cudaGetDevice(&dev));
+    NNVB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    int world = 1;
+    while (world < 16 && units * world * 2 <= sms && world * 4 <= steps) world *= 2;
+    NNVB_REQUIRE(units * world < (int64_t(1) << 31), "nnvb_cross_attention: too many tiles (%lld) for one launch", (long long)units);
     NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    kernel<<<unsigned(blocks), THREADS, smem, st>>>(a, vec);
-    NNVB_CUDA(cudaGetLastError());
+    if (world > 8) NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(units * world));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = size_t(smem);
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = unsigned(world);
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    NNVB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, vec));
     return NNVB_OK;
 }
 
@@ -400,7 +469,7 @@ int forward_t(cudaStream_t st, const AttnArgs& a) {
     constexpr int TILE = fwd_tile<A>(DP);
     const bool vec = a.D * sizeof(T) % 16 == 0 && rows16(a.q, a.qs, sizeof(T)) && rows16(a.k, a.ks, sizeof(T)) &&
                      rows16(a.v, a.vs, sizeof(T));
-    return launch(attn_fwd_simt_kernel<T, TILE, DP>, ceil_div(a.Lq, TILE) * a.Hq * a.B,
+    return launch(attn_fwd_simt_kernel<T, TILE, DP>, ceil_div(a.Lq, TILE) * a.Hq * a.B, 0,
                   3 * tile_bytes<A>(TILE, DP) + score_bytes<A>(TILE), st, a, vec);
 }
 
@@ -411,8 +480,9 @@ int backward_t(cudaStream_t st, const AttnArgs& a) {
     const bool vec = a.D * sizeof(T) % 16 == 0 && rows16(a.q, a.qs, sizeof(T)) && rows16(a.k, a.ks, sizeof(T)) &&
                      rows16(a.v, a.vs, sizeof(T)) && rows16(a.dout, a.dos, sizeof(T));
     const int smem = 4 * tile_bytes<A>(TILE, DP) + 2 * score_bytes<A>(TILE);
-    NNVB_TRY(launch(attn_dq_simt_kernel<T, TILE, DP>, ceil_div(a.Lq, TILE) * a.Hq * a.B, smem, st, a, vec));
-    return launch(attn_dkv_simt_kernel<T, TILE, DP>, ceil_div(a.Lk, TILE) * a.Hkv * a.B, smem, st, a, vec);
+    NNVB_TRY(launch(attn_dq_simt_kernel<T, TILE, DP>, ceil_div(a.Lq, TILE) * a.Hq * a.B, ceil_div(a.Lk, TILE), smem, st, a, vec));
+    return launch(attn_dkv_simt_kernel<T, TILE, DP>, ceil_div(a.Lk, TILE) * a.Hkv * a.B,
+                  ceil_div(a.Lq, TILE) * (a.Hq / a.Hkv), smem, st, a, vec);
 }
 
 template <typename T>

@@ -70,7 +70,8 @@ struct Work<double, DP> {
             for (int e = 0; e < 4; ++e) o[i][e] = 0;
     }
     __device__ __forceinline__ int row(int i) const { return warp * 16 + g + i * 8; }
-    __device__ __forceinline__ void scores(const double* Q, const double* K) {
+    // rest: states of the tile that count; 8-state tiles behind them are left out
+    __device__ __forceinline__ void scores(const double* Q, const double* K, int rest) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -83,6 +84,7 @@ struct Work<double, DP> {
             const double a[4] = {x.x, y.x, x.y, y.y};
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
+                if (j * 8 >= rest) break;
                 const double2 z = *reinterpret_cast<const double2*>(k + j * 8 * S::LDK + d);
                 const double b[2] = {z.x, z.y};
                 dmma_16x8x8(s[j], a, b);
@@ -105,10 +107,11 @@ struct Work<double, DP> {
             for (int e = 0; e < 4; ++e) o[i][e] *= f[e / 2];
     }
     __device__ __forceinline__ void hand_over(double*) {}          // the weights stay in their registers
-    __device__ __forceinline__ void weigh(const double*, const double* V) {
+    __device__ __forceinline__ void weigh(const double*, const double* V, int rest) {
         const double* v = V + 2 * t * S::LDV + 2 * g;
 #pragma unroll
         for (int k = 0; k < NT; ++k) {
+            if (k * 8 >= rest) break;
             const double a[4] = {s[k][0], s[k][2], s[k][1], s[k][3]};
 #pragma unroll
             for (int j = 0; j < DP / 16; ++j) {
@@ -146,7 +149,7 @@ struct Work<float, DP> {
             for (int e = 0; e < DP / 32; ++e) o[i][e] = both(0.f);
     }
     __device__ __forceinline__ int row(int i) const { return ty * NR + i; }
-    __device__ __forceinline__ void scores(const float* Q, const float* K) {
+    __device__ __forceinline__ void scores(const float* Q, const float* K, int) {
         Pair<float> acc[NR][4];
 #pragma unroll
         for (int i = 0; i < NR; ++i)
@@ -194,10 +197,10 @@ struct Work<float, DP> {
             for (int j = 0; j < 4; ++j) P[row(i) * S::LDP + tx + 16 * j] = s[i][j];
         __syncwarp();                      // a row's weights are read by the warp that wrote them
     }
-    __device__ __forceinline__ void weigh(const float* P, const float* V) {
+    __device__ __forceinline__ void weigh(const float* P, const float* V, int rest) {
         const float *p = P + ty * NR * S::LDP, *v = V + tx * 4;
 #pragma unroll 1
-        for (int k = 0; k < S::BK; k += 4) {
+        for (int k = 0; k < S::BK && k < rest; k += 4) {
             float4 x[NR];
 #pragma unroll
             for (int i = 0; i < NR; ++i) x[i] = *reinterpret_cast<const float4*>(p + i * S::LDP + k);
@@ -261,7 +264,7 @@ attn_fwd_wide_kernel(AttnArgs a, bool vec) {
         load_rows<T, S::BK, DP, S::LDV>(Vs, v, a.vs[1], k0, n, a.D, vec);
         cp_async_wait<1>();
         __syncthreads();
-        w.scores(Qs, Ks);
+        w.scores(Qs, Ks, n - k0);
         __syncthreads();
         if (it + world < steps) load_rows<T, S::BK, DP, S::LDK>(Ks, k, a.ks[1], (it + world) * S::BK, n, a.D, vec);
         else cp_async_commit();
@@ -296,7 +299,7 @@ attn_fwd_wide_kernel(AttnArgs a, bool vec) {
         w.hand_over(Ps);
         cp_async_wait<1>();
         __syncthreads();
-        w.weigh(Ps, Vs);
+        w.weigh(Ps, Vs, rest);
         __syncthreads();
     }
     cp_async_wait<0>();
