@@ -8,14 +8,21 @@
 // S as 16-bit values, and add the row's sum.  The two tiles alternate: while one is in its softmax the other's
 // products run, so the tensor pipe sees S and P V of one tile during the exponentials of the other.
 //
+// Where such blocks are few, a cluster of up to 16 shares the states of one and joins its rows in distributed shared
+// memory.
+//
 // The running maximum m is raised lazily: O is only rescaled when a row's maximum has grown by more than a factor of
 // 2^8 over the m in use, so weights stay below 2^8, which 16-bit P and fp32 sums hold without loss; after the first
 // tiles the rescale is rare.  P is rounded to the tensors' type because the product takes 16-bit operands; its
 // row sum is added in fp32 before the rounding.
+#include <cooperative_groups.h>
+
 #include <mutex>
 
 #include "attention.cuh"
 #include "tcgen05.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace nnvb {
 namespace {
@@ -81,6 +88,12 @@ __device__ __forceinline__ Pair<float> ex2_poly(Pair<float> x) {
     return mul2(y, {__int_as_float((__float_as_int(r.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(r.y) << 23) + 0x3f800000)});
 }
 
+// eight results, one rounding each
+template <typename T>
+__device__ __forceinline__ void store8(T* to, const float (&x)[8]) {
+    *reinterpret_cast<uint4*>(to) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+}
+
 struct TcMaps {
     CUtensorMap q, k, v, dout;
 };
@@ -111,15 +124,20 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
     __shared__ uint64_t full[STAGES], empty[STAGES], q_full, s_ready[2], p_ready[2], o_ready[2], tail, drain;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
+    __shared__ float row_m[2 * ROWS], row_l[2 * ROWS];             // clusters
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = int(cluster.block_rank()), world = int(cluster.num_blocks());
     const int tiles = (a.Lq + 2 * ROWS - 1) / (2 * ROWS);
-    const int q0 = int(blockIdx.x % tiles) * 2 * ROWS;
-    const int h = int(blockIdx.x / tiles % a.Hq), b = int(blockIdx.x / tiles / a.Hq);
+    const int64_t unit = blockIdx.x / world;
+    const int q0 = int(unit % tiles) * 2 * ROWS;
+    const int h = int(unit / tiles % a.Hq), b = int(unit / tiles / a.Hq);
     const int g = h / (a.Hq / a.Hkv);
     const int n = attn_len(a, b);
     const int live = a.Lq - q0 > ROWS ? 2 : 1;             // tiles of positions this block holds
-    const int steps = (n + ROWS - 1) / ROWS;
+    // tiles of states: every world-th is this block's
+    const int all_steps = (n + ROWS - 1) / ROWS, steps = all_steps > rank ? (all_steps - rank + world - 1) / world : 0;
 
     if (threadIdx.x == 0) {
         abort_flag = 0;
@@ -140,7 +158,7 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
     if (warp == 9) {
         // ---- copies -------------------------------------------------------------------------------------------
         const int kb = a.ks[0] ? b : 0, kh = a.ks[2] ? g : 0, vb = a.vs[0] ? b : 0, vh = a.vs[2] ? g : 0;
-        if (lane == 0 && n > 0) {
+        if (lane == 0 && steps > 0) {
             mbar_expect_bytes(&q_full, uint32_t(live) * SM::TILE);
             for (int t = 0; t < live; ++t)
                 load_tile(sq + t * SM::TILE, &maps.q, DP / 64, SM::BOX, q0 + t * ROWS, a.qs[2] ? h : 0, a.qs[0] ? b : 0, &q_full);
@@ -154,13 +172,13 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 unsigned char* dst = ring + s * SM::TILE;
-                const int rest = n - i * ROWS;
+                const int row = (rank + i * world) * ROWS, rest = n - row;
                 // V rows behind the valid states may hold anything, and 0 * NaN is NaN: they are cleared here.  (K needs
                 // nothing: its rows only make scores that are masked.)
                 if (kv == 1 && rest < ROWS && n < a.Lk) {
                     if (lane == 0) {
                         mbar_expect_bytes(&tail, SM::TILE);
-                        load_tile(dst, &maps.v, DP / 64, SM::BOX, i * ROWS, vh, vb, &tail);
+                        load_tile(dst, &maps.v, DP / 64, SM::BOX, row, vh, vb, &tail);
                     }
                     ok = __all_sync(0xffffffffu, mbar_wait_fast(&tail, 0, abort));
                     for (int j = lane; j < (ROWS - rest) * 8 * (DP / 64); j += 32) {
@@ -172,18 +190,18 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
                     if (lane == 0) mbar_arrive(&full[s]);
                 } else if (lane == 0) {
                     mbar_expect_bytes(&full[s], SM::TILE);
-                    load_tile(dst, kv ? &maps.v : &maps.k, DP / 64, SM::BOX, i * ROWS, kv ? vh : kh, kv ? vb : kb, &full[s]);
+                    load_tile(dst, kv ? &maps.v : &maps.k, DP / 64, SM::BOX, row, kv ? vh : kh, kv ? vb : kb, &full[s]);
                 }
             }
         }
         if (!ok && lane == 0) {            // gave up: the copies issued so far still write to this block's memory
-            if (n > 0) mbar_wait(&q_full, 0, 1 << 20);
+            mbar_wait(&q_full, 0, 1 << 20);
             for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j) mbar_wait(&full[j % STAGES], (j / STAGES) & 1, 1 << 20);
         }
     } else if (warp == 8) {
         // ---- products -----------------------------------------------------------------------------------------
         const uint32_t leader = elect_lane();
-        if (n > 0) {
+        if (steps > 0) {
             constexpr uint32_t id_s = mma_idesc(is_bf16<T>, 128, ROWS, false);
             constexpr uint32_t id_o = mma_idesc(is_bf16<T>, 128, DP, true);
             const int ksteps = (a.D + 15) / 16;
@@ -249,7 +267,7 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) tmem_load32(s[j], s_at + j * 32);
             tmem_wait_load();
-            const int rest = n - i * ROWS;
+            const int rest = n - (rank + i * world) * ROWS;
             if (rest < ROWS) {
 #pragma unroll
                 for (int j = 0; j < 128; ++j)
@@ -299,37 +317,95 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_ready[t]);           // one arrival a warp: arrivals on a barrier are served one by one
         }
-        if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait_fast(&o_ready[t], 0, abort));
+        if (ok && steps > 0) {
+            ok = mbar_wait_fast(&o_ready[t], 0, abort);
+            // a cluster's results go over the ring, which the other tile's products read too
+            if (world > 1 && live > 1) ok = ok && mbar_wait_fast(&o_ready[1 - t], 0, abort);
+            ok = __all_sync(0xffffffffu, ok);
+        }
         tmem_fence_after();
-        const float f = !ok ? NAN : (n > 0 ? 1.f / l : 0.f);
-        T* out = static_cast<T*>(const_cast<void*>(a.o)) + int64_t(b) * a.os[0] + int64_t(row) * a.os[1] + int64_t(h) * a.os[2];
+        if (world > 1) {
+            const int r = t * ROWS + (warp % 4) * 32 + lane;
+            if (!ok) l = NAN;
+            row_m[r] = m;
+            row_l[r] = l;
+            float4* mine = reinterpret_cast<float4*>(ring) + r * (DP / 4);
 #pragma unroll 1
-        for (int j = 0; j < DP / 32; ++j) {
-            uint32_t o[32];
-            if (n > 0 && ok) {
-                tmem_load32(o, o_at + j * 32);
-                tmem_wait_load();
-            } else {
+            for (int j = 0; j < DP / 32; ++j) {
+                uint32_t o[32];
+                if (steps > 0) {
+                    tmem_load32(o, o_at + j * 32);
+                    tmem_wait_load();
+                }
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = 0;
+                for (int e = 0; e < 8; ++e) {
+                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (steps > 0)
+                        x = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
+                                        __uint_as_float(o[4 * e + 3]));
+                    mine[(j * 8 + e + r) % (DP / 4)] = x;          // rows turned against each other: one bank a lane
+                }
             }
-            if (row < a.Lq) {
+        } else {
+            const float f = !ok ? NAN : (n > 0 ? 1.f / l : 0.f);
+            T* out = static_cast<T*>(const_cast<void*>(a.o)) + int64_t(b) * a.os[0] + int64_t(row) * a.os[1] + int64_t(h) * a.os[2];
+#pragma unroll 1
+            for (int j = 0; j < DP / 32; ++j) {
+                uint32_t o[32];
+                if (n > 0 && ok) {
+                    tmem_load32(o, o_at + j * 32);
+                    tmem_wait_load();
+                } else {
 #pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    if (j * 32 + e < a.D) {
-                        uint4 w;
-                        w.x = pack2<T>(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f);
-                        w.y = pack2<T>(__uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
-                        w.z = pack2<T>(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 5]) * f);
-                        w.w = pack2<T>(__uint_as_float(o[e + 6]) * f, __uint_as_float(o[e + 7]) * f);
-                        *reinterpret_cast<uint4*>(out + j * 32 + e) = w;
+                    for (int e = 0; e < 32; ++e) o[e] = 0;
+                }
+                if (row < a.Lq) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        if (j * 32 + e < a.D) {
+                            float x[8];
+#pragma unroll
+                            for (int u = 0; u < 8; ++u) x[u] = __uint_as_float(o[e + u]) * f;
+                            store8<T>(out + j * 32 + e, x);
+                        }
                     }
                 }
             }
+            if (a.lse && row < a.Lq)
+                static_cast<float*>(a.lse)[(int64_t(b) * a.Hq + h) * a.Lq + row] =
+                    !ok ? NAN : (n > 0 ? m * float(a.scale) + logf(l) : -INFINITY);
         }
-        if (a.lse && row < a.Lq)
-            static_cast<float*>(a.lse)[(int64_t(b) * a.Hq + h) * a.Lq + row] =
-                !ok ? NAN : (n > 0 ? m * float(a.scale) + logf(l) : -INFINITY);
+    }
+    if (world > 1) {
+        // the blocks of a cluster hold the same rows over different states: each writes a share of the rows, added in
+        // block order
+        cluster.sync();
+        const float c = float(a.scale * LOG2E);
+        for (int i = rank * FWD_THREADS + threadIdx.x; i < live * ROWS * (DP / 8); i += world * FWD_THREADS) {
+            const int r = i / (DP / 8), d = i % (DP / 8) * 8, row = q0 + r;
+            if (row >= a.Lq) continue;
+            float top = -INFINITY, sum = 0.f, x[8] = {};
+            for (int w = 0; w < world; ++w) top = fmaxf(top, *cluster.map_shared_rank(&row_m[r], w));
+            const float base = top == -INFINITY ? 0.f : top;
+            for (int w = 0; w < world; ++w) {
+                const float f = ex2((*cluster.map_shared_rank(&row_m[r], w) - base) * c);
+                sum += *cluster.map_shared_rank(&row_l[r], w) * f;
+                const float4* part = cluster.map_shared_rank(reinterpret_cast<float4*>(ring), w) + r * (DP / 4);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float4 y = part[(d / 4 + u + r) % (DP / 4)];
+                    x[u * 4] += y.x * f; x[u * 4 + 1] += y.y * f; x[u * 4 + 2] += y.z * f; x[u * 4 + 3] += y.w * f;
+                }
+            }
+            const float f = n > 0 ? 1.f / sum : 0.f;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[u] *= f;
+            if (d < a.D)
+                store8<T>(static_cast<T*>(const_cast<void*>(a.o)) + int64_t(b) * a.os[0] + int64_t(row) * a.os[1] + int64_t(h) * a.os[2] + d, x);
+            if (d == 0 && a.lse)
+                static_cast<float*>(a.lse)[(int64_t(b) * a.Hq + h) * a.Lq + row] = n > 0 ? top * float(a.scale) + logf(sum) : -INFINITY;
+        }
+        cluster.sync();                    // nobody leaves while its shared memory is read
     }
     tmem_fence_before();
     __syncthreads();
@@ -414,14 +490,20 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int own_len = KV ? a.Lk : a.Lq, own_heads = KV ? a.Hkv : a.Hq;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = int(cluster.block_rank()), world = int(cluster.num_blocks());
     const int tiles = (own_len + ROWS - 1) / ROWS;
-    const int r0 = int(blockIdx.x % tiles) * ROWS;
-    const int oh = int(blockIdx.x / tiles % own_heads), b = int(blockIdx.x / tiles / own_heads);
+    const int64_t unit = blockIdx.x / world;
+    const int r0 = int(unit % tiles) * ROWS;
+    const int oh = int(unit / tiles % own_heads), b = int(unit / tiles / own_heads);
     const int G = a.Hq / a.Hkv;
     const int n = attn_len(a, b);
     // streamed tiles: positions of all query heads of the group, or valid states
     const int per_head = KV ? (a.Lq + BROWS - 1) / BROWS : (n + BROWS - 1) / BROWS;
-    const int steps = KV ? (r0 < n ? per_head * G : 0) : per_head;
+    const int all_steps = KV ? (r0 < n ? per_head * G : 0) : per_head;
+    // every `share`-th is this block's; rows of up to 128 states stay in one block, which sums P dP over them
+    const int share = all_steps <= 2 ? 1 : world;
+    const int steps = rank < share && all_steps > rank ? (all_steps - rank + share - 1) / share : 0;
 
     if (threadIdx.x == 0) {
         abort_flag = 0;
@@ -461,8 +543,9 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
             if (it >= STAGES) ok = mbar_wait_fast(&empty[s], (it / STAGES - 1) & 1, abort);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            const int sh = KV ? oh * G + it / per_head : oh / G;           // streamed head
-            const int row = it % per_head * BROWS;
+            const int at_step = rank + it * share;
+            const int sh = KV ? oh * G + at_step / per_head : oh / G;      // streamed head
+            const int row = at_step % per_head * BROWS;
             unsigned char* dst = ring + s * 2 * SM::BTILE;
             const int rest = KV ? BROWS : n - row;
             // K rows behind the valid states may hold anything, and 0 * NaN is NaN: they are cleared here.  (V
@@ -567,7 +650,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tmem_fence_after();
             const float* sl = stats + (j % STAGES) * 2 * BROWS + half * 32;
-            const int rest = KV ? 32 : n - j * BROWS - half * 32;          // columns with weight
+            const int rest = KV ? 32 : n - (rank + j * share) * BROWS - half * 32;          // columns with weight
             uint32_t s[32];
             tmem_load32(s, s_at);
             tmem_wait_load();
@@ -578,7 +661,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
                 s[e] = __float_as_uint(!KV && e >= rest ? 0.f : ex2(x.x));
                 s[e + 1] = __float_as_uint(!KV && e + 1 >= rest ? 0.f : ex2(x.y));
             }
-            if (!KV && steps <= 2) {
+            if (!KV && all_steps <= 2) {
                 float sum = 0.f;
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
@@ -634,6 +717,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
         T* out = static_cast<T*>(KV ? (value ? a.dv : a.dk) : a.dq) +
                  (int64_t(b) * own_len * own_heads + int64_t(row) * own_heads + oh) * a.D;
         const uint32_t o_at = lanes + 256 + (value ? 128 : 0);
+        float4* mine = reinterpret_cast<float4*>(base) + ((value ? ROWS : 0) + local) * (DP / 4);
         constexpr int NJ = DP / 32;
         const int j0 = KV ? half * (NJ / 2) : wg, j1 = KV ? j0 + NJ / 2 : (wg < NJ ? wg + 1 : wg);
 #pragma unroll 1
@@ -644,21 +728,47 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
                 tmem_wait_load();
             }
             const bool zero = ok && (steps == 0 || dead);
-            if (row < own_len) {
+            if (world > 1) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float x[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) x[u] = zero ? 0.f : (ok ? __uint_as_float(o[4 * e + u]) * f : NAN);
+                    mine[(j * 8 + e + local) % (DP / 4)] = make_float4(x[0], x[1], x[2], x[3]);
+                }
+            } else if (row < own_len) {
 #pragma unroll
                 for (int e = 0; e < 32; e += 8) {
                     if (j * 32 + e < a.D) {
-                        uint32_t w[4];
+                        float x[8];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float x = __uint_as_float(o[e + 2 * i]) * f, y = __uint_as_float(o[e + 2 * i + 1]) * f;
-                            w[i] = zero ? 0u : pack2<T>(ok ? x : NAN, ok ? y : NAN);
-                        }
-                        *reinterpret_cast<uint4*>(out + j * 32 + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                        for (int u = 0; u < 8; ++u) x[u] = zero ? 0.f : (ok ? __uint_as_float(o[e + u]) * f : NAN);
+                        store8<T>(out + j * 32 + e, x);
                     }
                 }
             }
         }
+    }
+    if (world > 1) {
+        // the blocks' sums over their streamed tiles, added in block order; each writes a share of the rows
+        cluster.sync();
+        constexpr int PARTS = KV ? 2 : 1;
+        for (int i = rank * BWD_THREADS + threadIdx.x; i < PARTS * ROWS * (DP / 8); i += world * BWD_THREADS) {
+            const int pr = i / (DP / 8), r = pr % ROWS, d = i % (DP / 8) * 8, row = r0 + r;
+            if (row >= own_len || d >= a.D) continue;
+            float x[8] = {};
+            for (int w = 0; w < world; ++w) {
+                const float4* part = cluster.map_shared_rank(reinterpret_cast<float4*>(base), w) + pr * (DP / 4);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float4 y = part[(d / 4 + u + r) % (DP / 4)];
+                    x[u * 4] += y.x; x[u * 4 + 1] += y.y; x[u * 4 + 2] += y.z; x[u * 4 + 3] += y.w;
+                }
+            }
+            store8<T>(static_cast<T*>(KV ? (pr >= ROWS ? a.dv : a.dk) : a.dq) +
+                          (int64_t(b) * own_len * own_heads + int64_t(row) * own_heads + oh) * a.D + d, x);
+        }
+        cluster.sync();                    // nobody leaves while its shared memory is read
     }
     tmem_fence_before();
     __syncthreads();
@@ -715,6 +825,32 @@ bool tma_rows(const void* p, const int64_t (&s)[3], int64_t tokens) {
     return tokens <= 1 || s[1] > 0;
 }
 
+// Launches `units` blocks, or clusters of up to 16 where blocks are few and walk over many tiles (`steps`).
+template <typename K, typename... Args>
+int launch_shared(K kernel, int64_t units, int64_t steps, int threads, int smem, cudaStream_t st, Args... args) {
+    int dev = 0, sms = 148;
+    NNVB_CUDA(cudaGetDevice(&dev));
+    NNVB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    int world = 1;
+    while (world < 16 && units * world * 2 <= sms && world * 4 <= steps) world *= 2;
+    NNVB_REQUIRE(units * world < (int64_t(1) << 31), "nnvb_cross_attention: too many tiles (%lld) for one launch", (long long)units);
+    NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (world > 8) NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(units * world));
+    cfg.blockDim = dim3(unsigned(threads));
+    cfg.dynamicSmemBytes = size_t(smem);
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = unsigned(world);
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    NNVB_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    return NNVB_OK;
+}
+
 template <typename T, int DP>
 int forward_t(cudaStream_t st, const AttnArgs& a) {
     using SM = FwdSmem<DP>;
@@ -724,13 +860,8 @@ int forward_t(cudaStream_t st, const AttnArgs& a) {
         NNVB_TRY(make_map(&maps.k, a.dtype, a.k, a.ks, a.D, a.Lk, a.Hkv, a.B, ROWS));
         NNVB_TRY(make_map(&maps.v, a.dtype, a.v, a.vs, a.D, a.Lk, a.Hkv, a.B, ROWS));
     }
-    const int64_t blocks = ceil_div(a.Lq, 2 * ROWS) * a.Hq * a.B;
-    NNVB_REQUIRE(blocks < (int64_t(1) << 31), "nnvb_cross_attention: too many tiles (%lld) for one launch", (long long)blocks);
-    auto kernel = attn_fwd_tc_kernel<T, DP>;
-    NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::BYTES));
-    kernel<<<unsigned(blocks), FWD_THREADS, SM::BYTES, st>>>(maps, a);
-    NNVB_CUDA(cudaGetLastError());
-    return NNVB_OK;
+    return launch_shared(attn_fwd_tc_kernel<T, DP>, ceil_div(a.Lq, 2 * ROWS) * a.Hq * a.B, ceil_div(a.Lk, ROWS), FWD_THREADS,
+                         SM::BYTES, st, maps, a);
 }
 
 template <typename T, int DP>
@@ -739,8 +870,7 @@ int backward_t(cudaStream_t st, const AttnArgs& a) {
     const int64_t LqP = round_up(a.Lq, BROWS);
     const int64_t rows = LqP * a.B * a.Hq;
     const int64_t bq = ceil_div(a.Lq, ROWS) * a.Hq * a.B, bk = ceil_div(a.Lk, ROWS) * a.Hkv * a.B;
-    NNVB_REQUIRE(ceil_div(rows, 16) < (int64_t(1) << 31) && bq < (int64_t(1) << 31) && bk < (int64_t(1) << 31),
-                 "nnvb_cross_attention_backward: too many tiles for one launch");
+    NNVB_REQUIRE(ceil_div(rows, 16) < (int64_t(1) << 31), "nnvb_cross_attention_backward: too many rows (%lld)", (long long)rows);
     attn_stats_tc_kernel<T><<<unsigned(ceil_div(rows, 16)), 256, 0, st>>>(a, int(LqP));
     NNVB_CUDA(cudaGetLastError());
     BwdMaps mq{}, mk{};
@@ -752,15 +882,8 @@ int backward_t(cudaStream_t st, const AttnArgs& a) {
     NNVB_TRY(make_map(&mk.a1, a.dtype, a.v, a.vs, a.D, a.Lk, a.Hkv, a.B, ROWS));
     NNVB_TRY(make_map(&mk.b0, a.dtype, a.q, a.qs, a.D, a.Lq, a.Hq, a.B, BROWS));
     NNVB_TRY(make_map(&mk.b1, a.dtype, a.dout, a.dos, a.D, a.Lq, a.Hq, a.B, BROWS));
-    auto kq = attn_bwd_tc_kernel<T, DP, false>;
-    auto kk = attn_bwd_tc_kernel<T, DP, true>;
-    NNVB_CUDA(cudaFuncSetAttribute(kq, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::BYTES));
-    NNVB_CUDA(cudaFuncSetAttribute(kk, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::BYTES));
-    kq<<<unsigned(bq), BWD_THREADS, SM::BYTES, st>>>(mq, a, int(LqP));
-    NNVB_CUDA(cudaGetLastError());
-    kk<<<unsigned(bk), BWD_THREADS, SM::BYTES, st>>>(mk, a, int(LqP));
-    NNVB_CUDA(cudaGetLastError());
-    return NNVB_OK;
+    NNVB_TRY(launch_shared(attn_bwd_tc_kernel<T, DP, false>, bq, ceil_div(a.Lk, BROWS), BWD_THREADS, SM::BYTES, st, mq, a, int(LqP)));
+    return launch_shared(attn_bwd_tc_kernel<T, DP, true>, bk, LqP / BROWS * (a.Hq / a.Hkv), BWD_THREADS, SM::BYTES, st, mk, a, int(LqP));
 }
 
 }  // namespace

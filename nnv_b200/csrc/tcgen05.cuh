@@ -22,8 +22,11 @@ namespace nnvb {
 // swizzle) is the same for all: a step moves the low word by its bytes / 16.  One thread issues every product of a block,
 // so what it computes per product counts.
 constexpr uint32_t DESC_HIGH = (1024u >> 4) | 1u << 14 | 2u << 29;
-__device__ __forceinline__ uint32_t desc_k_major(uint32_t addr) { return (addr >> 4) | 1u << 16; }
-__device__ __forceinline__ uint32_t desc_mn_major(uint32_t addr, uint32_t tile_bytes) { return (addr >> 4) | (tile_bytes >> 4) << 16; }
+// The address field holds an offset within the SM's shared memory; in a cluster the address of a block's own memory
+// carries the block's rank above it, which would run into the leading stride.
+__device__ __forceinline__ uint32_t desc_address(uint32_t addr) { return (addr & 0x3ffffu) >> 4; }
+__device__ __forceinline__ uint32_t desc_k_major(uint32_t addr) { return desc_address(addr) | 1u << 16; }
+__device__ __forceinline__ uint32_t desc_mn_major(uint32_t addr, uint32_t tile_bytes) { return desc_address(addr) | (tile_bytes >> 4) << 16; }
 
 // 16-bit operands, fp32 accumulator; b_mn: B is MN-major
 __host__ __device__ constexpr uint32_t mma_idesc(bool bf16, int M, int N, bool b_mn) {

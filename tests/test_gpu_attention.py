@@ -101,10 +101,31 @@ def test_few_positions_over_many_states(t, Lq, Lk, G):
 
 
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("B,Lq,Lk,H", [(1, 100, 5000, 1), (1, 300, 2000, 2), (2, 16, 3000, 1)])
-def test_few_rows_over_a_long_axis(t, B, Lq, Lk, H):
-    q, k, v, dout = _data(t, B, Lq, Lk, H, H, 64)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,Lq,Lk,H", [(1, 100, 5000, 1), (1, 300, 2000, 2), (2, 20, 3000, 1), (1, 2000, 300, 1)])
+def test_few_rows_over_a_long_axis(t, B, Lq, Lk, H, D):
+    """Few tiles over many: clusters of blocks share one."""
+    q, k, v, dout = _data(t, B, Lq, Lk, H, H, D)
     _check(t, q, k, v, dout, _lens([Lk - 70] * B))
+
+
+@pytest.mark.parametrize("t", F16)
+@pytest.mark.parametrize("D", [64, 128])
+def test_clusters_with_ragged_lengths(t, D):
+    """Entries whose states do not reach every block of the cluster, 128 and fewer states among them, and none."""
+    q, k, v, dout = _data(t, 5, 40, 3000, 2, 1, D)
+    lengths = _lens([3000, 0, 100, 129, 1000])
+    for b, n in enumerate([3000, 0, 100, 129, 1000]):
+        k[b, n:] = math.nan
+        v[b, n:] = math.nan
+    ref_k, ref_v = k.nan_to_num(), v.nan_to_num()
+    from nnv_b200 import ops
+    out, lse = ops.cross_attention(q, k, v, lengths, return_lse=True)
+    ref = R.attention(q, ref_k, ref_v, lengths, 1 / math.sqrt(D), dout)
+    R.check("out", out, *ref["out"])
+    R.check("lse", lse, *ref["lse"])
+    for name, x in zip(("dq", "dk", "dv"), ops.cross_attention_backward(dout, q, k, v, out, lse, lengths)):
+        R.check(name, x, *ref[name])
 
 
 @pytest.mark.parametrize("t", TYPES)
