@@ -18,6 +18,8 @@ int check_desc(const char* who, const nnvb_attention_desc* d) {
                  (long long)d->kv_len);
     NNVB_REQUIRE(d->q_heads >= 1 && d->kv_heads >= 1 && d->q_heads < I31 && d->q_heads % d->kv_heads == 0,
                  "%s: %lld query heads over %lld state heads", who, (long long)d->q_heads, (long long)d->kv_heads);
+    NNVB_REQUIRE(d->q_len * (d->q_heads / d->kv_heads) < I31, "%s: bad sizes (%lld positions of %lld heads a state head)", who,
+                 (long long)d->q_len, (long long)(d->q_heads / d->kv_heads));
     NNVB_REQUIRE(d->head_dim >= 1 && d->head_dim <= 256, "%s: head size %lld (1..256 supported)", who, (long long)d->head_dim);
     NNVB_REQUIRE(std::isfinite(d->scale) && d->scale > 0, "%s: the factor on the scores must be finite and positive", who);
     for (const int64_t* s : {d->q_stride, d->k_stride, d->v_stride, d->out_stride, d->dout_stride})

@@ -23,6 +23,27 @@ namespace {
 
 constexpr int THREADS = 256;
 
+// Rows are the positions of all query heads that share a state head, heads of a position side by side, so that few
+// positions of grouped heads fill tiles.
+struct Rows {
+    int G, n;                                      // heads of the group, rows
+    const AttnArgs& a;
+    int b, g;
+    __device__ Rows(const AttnArgs& a_, int b_, int g_) : G(a_.Hq / a_.Hkv), n(a_.Lq * (a_.Hq / a_.Hkv)), a(a_), b(b_), g(g_) {}
+    // of a tensor with strides s, from the group's first head
+    __device__ __forceinline__ int64_t at(const int64_t (&s)[3], int r) const {
+        return G == 1 ? r * s[1] : int64_t(r / G) * s[1] + int64_t(r % G) * s[2];
+    }
+    __device__ __forceinline__ int64_t first(const int64_t (&s)[3]) const { return int64_t(b) * s[0] + int64_t(g) * G * s[2]; }
+    // of a [B, Hq, Lq] statistic; of the dense gradient of q
+    __device__ __forceinline__ int64_t stat(int r) const {
+        return G == 1 ? (int64_t(b) * a.Hq + g) * a.Lq + r : (int64_t(b) * a.Hq + g * G + r % G) * a.Lq + r / G;
+    }
+    __device__ __forceinline__ int64_t dense(int r) const {
+        return G == 1 ? ((int64_t(b) * a.Lq + r) * a.Hq + g) * a.D : ((int64_t(b) * a.Lq + r / G) * a.Hq + g * G + r % G) * a.D;
+    }
+};
+
 template <typename A> struct VecOf;
 template <> struct VecOf<float> { static constexpr int N = 4; };
 template <> struct VecOf<double> { static constexpr int N = 2; };
@@ -32,9 +53,10 @@ __device__ __forceinline__ Pack<A, VecOf<A>::N> lds(const A* p) {
     return *reinterpret_cast<const Pack<A, VecOf<A>::N>*>(p);
 }
 
-// rows [r0, r0 + TILE) of a [token] x D slab into s[TILE][DP + pad]; rows at or past n_rows and columns past D are zero
-template <typename T, typename A, int TILE, int DP>
-__device__ void load_tile(A* s, const T* g, int64_t stride, int r0, int n_rows, int D, bool vec) {
+// rows [r0, r0 + TILE) into s[TILE][DP + pad]; row r begins at(r) elements from g; rows at or past n_rows and columns past
+// D are zero
+template <typename T, typename A, int TILE, int DP, typename At>
+__device__ void load_tile(A* s, const T* g, At&& at, int r0, int n_rows, int D, bool vec) {
     constexpr int LD = DP + VecOf<A>::N;
     constexpr int V = 16 / sizeof(T);
     if (vec) {
@@ -42,24 +64,23 @@ __device__ void load_tile(A* s, const T* g, int64_t stride, int r0, int n_rows, 
             const int r = i / (DP / V), c = i % (DP / V) * V;
             Pack<T, V> p;
             const bool in = r0 + r < n_rows && c < D;          // D is a multiple of V here
-            if (in) p = *reinterpret_cast<const Pack<T, V>*>(g + int64_t(r0 + r) * stride + c);
+            if (in) p = *reinterpret_cast<const Pack<T, V>*>(g + at(r0 + r) + c);
 #pragma unroll
             for (int e = 0; e < V; ++e) s[r * LD + c + e] = in ? to_acc(p.v[e]) : A(0);
         }
     } else {
         for (int i = threadIdx.x; i < TILE * DP; i += THREADS) {
             const int r = i / DP, c = i % DP;
-            s[r * LD + c] = r0 + r < n_rows && c < D ? A(to_acc(g[int64_t(r0 + r) * stride + c])) : A(0);
+            s[r * LD + c] = r0 + r < n_rows && c < D ? A(to_acc(g[at(r0 + r) + c])) : A(0);
         }
     }
 }
 
-// acc[i][j] += sum_d X[(ty*M + i)][d] * Y[tx + 16 j][d]
+// acc[i][j] += sum_d X[(ty*M + i)][d] * Y[tx + 16 j][d], d < D
 template <typename A, int TILE, int DP>
-__device__ __forceinline__ void mul_rows(A (&acc)[TILE / 16][TILE / 16], const A* X, const A* Y, int ty, int tx) {
+__device__ __forceinline__ void mul_rows(A (&acc)[TILE / 16][TILE / 16], const A* X, const A* Y, int D, int ty, int tx) {
     constexpr int M = TILE / 16, V = VecOf<A>::N, LD = DP + V;
-#pragma unroll 4
-    for (int d = 0; d < DP; d += V) {
+    auto step = [&](int d) {
         Pack<A, V> x[M], y[M];
 #pragma unroll
         for (int i = 0; i < M; ++i) x[i] = lds<A>(X + (ty * M + i) * LD + d);
@@ -71,6 +92,13 @@ __device__ __forceinline__ void mul_rows(A (&acc)[TILE / 16][TILE / 16], const A
             for (int i = 0; i < M; ++i)
 #pragma unroll
                 for (int j = 0; j < M; ++j) acc[i][j] += x[i].v[e] * y[j].v[e];
+    };
+    if (D > DP - V) {                      // a loop of known length is the faster one
+#pragma unroll 4
+        for (int d = 0; d < DP; d += V) step(d);
+    } else {
+#pragma unroll 2
+        for (int d = 0; d < D; d += V) step(d);
     }
 }
 
@@ -116,35 +144,36 @@ __device__ __forceinline__ void mul_cols_t(A (&acc)[TILE / 16][DP / 16], const A
     }
 }
 
-template <typename T, typename A, int TILE, int DP>
-__device__ __forceinline__ void store_rows(T* g, int64_t stride, int r0, int n_rows, int D, const A (&acc)[TILE / 16][DP / 16],
+template <typename T, typename A, int TILE, int DP, typename At>
+__device__ __forceinline__ void store_rows(T* g, At&& at, int r0, int n_rows, int D, const A (&acc)[TILE / 16][DP / 16],
                                            const A (&f)[TILE / 16], int ty, int tx) {
     constexpr int M = TILE / 16, V = VecOf<A>::N, NC = DP / (16 * V);
 #pragma unroll
     for (int i = 0; i < M; ++i) {
         const int r = r0 + ty * M + i;
+        T* to = g + (r < n_rows ? at(r) : 0);
         if (r < n_rows)
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     const int d = tx * V + 16 * V * c + e;
-                    if (d < D) g[int64_t(r) * stride + d] = from_acc<T, A>(acc[i][c * V + e] * f[i]);
+                    if (d < D) to[d] = from_acc<T, A>(acc[i][c * V + e] * f[i]);
                 }
     }
 }
 
 // The blocks of a cluster have summed shares of the same rows: each leaves its sums in `mine`, [TILE][DP], and writes a
 // share of the total, added in block order.
-template <typename T, typename A, int TILE, int DP>
-__device__ void store_shared(cg::cluster_group& cluster, T* g, int64_t stride, int r0, int n_rows, int D, const A* mine, A f) {
+template <typename T, typename A, int TILE, int DP, typename At>
+__device__ void store_shared(cg::cluster_group& cluster, T* g, At&& at, int r0, int n_rows, int D, const A* mine, A f) {
     const int rank = int(cluster.block_rank()), world = int(cluster.num_blocks());
     for (int i = rank * THREADS + threadIdx.x; i < TILE * DP; i += world * THREADS) {
         const int r = r0 + i / DP, d = i % DP;
         if (r >= n_rows || d >= D) continue;
         A x = 0;
         for (int p = 0; p < world; ++p) x += *cluster.map_shared_rank(mine + i, p);
-        g[int64_t(r) * stride + d] = from_acc<T, A>(x * f);
+        g[at(r) + d] = from_acc<T, A>(x * f);
     }
 }
 template <typename A, int TILE, int DP>
@@ -182,13 +211,13 @@ attn_fwd_simt_kernel(AttnArgs a, bool vec) {
     A* Ks = Qs + TILE * LD;
     A* Vs = Ks + TILE * LD;
     A* Ps = Vs + TILE * LD;
-    const int tiles = (a.Lq + TILE - 1) / TILE;
+    const int tiles = (a.Lq * (a.Hq / a.Hkv) + TILE - 1) / TILE;
     const int q0 = int(blockIdx.x % tiles) * TILE;
-    const int h = int(blockIdx.x / tiles % a.Hq), b = int(blockIdx.x / tiles / a.Hq);
-    const int g = h / (a.Hq / a.Hkv);
+    const int g = int(blockIdx.x / tiles % a.Hkv), b = int(blockIdx.x / tiles / a.Hkv);
+    const Rows rows(a, b, g);
     const int n = attn_len(a, b);
     const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-    const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2];
+    const T* q = static_cast<const T*>(a.q) + rows.first(a.qs);
     const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + g * a.ks[2];
     const T* v = static_cast<const T*>(a.v) + b * a.vs[0] + g * a.vs[2];
     const A c = A(a.scale * LOG2E), ninf = -INFINITY;
@@ -200,14 +229,14 @@ attn_fwd_simt_kernel(AttnArgs a, bool vec) {
 #pragma unroll
         for (int e = 0; e < DP / 16; ++e) o[i][e] = 0;
     }
-    load_tile<T, A, TILE, DP>(Qs, q, a.qs[1], q0, a.Lq, a.D, vec);
+    load_tile<T, A, TILE, DP>(Qs, q, [&](int r) { return rows.at(a.qs, r); }, q0, rows.n, a.D, vec);
     for (int k0 = 0; k0 < n; k0 += TILE) {
         __syncthreads();
-        load_tile<T, A, TILE, DP>(Ks, k, a.ks[1], k0, n, a.D, vec);
-        load_tile<T, A, TILE, DP>(Vs, v, a.vs[1], k0, n, a.D, vec);
+        load_tile<T, A, TILE, DP>(Ks, k, [&](int r) { return r * a.ks[1]; }, k0, n, a.D, vec);
+        load_tile<T, A, TILE, DP>(Vs, v, [&](int r) { return r * a.vs[1]; }, k0, n, a.D, vec);
         __syncthreads();
         A s[M][M] = {};
-        mul_rows<A, TILE, DP>(s, Qs, Ks, ty, tx);
+        mul_rows<A, TILE, DP>(s, Qs, Ks, a.D, ty, tx);
 #pragma unroll
         for (int i = 0; i < M; ++i) {
             A mx = ninf;
@@ -240,11 +269,11 @@ attn_fwd_simt_kernel(AttnArgs a, bool vec) {
     for (int i = 0; i < M; ++i) {
         f[i] = n > 0 ? A(1) / l[i] : A(0);
         const int r = q0 + ty * M + i;
-        if (a.lse && tx == 0 && r < a.Lq)
-            static_cast<A*>(a.lse)[(int64_t(b) * a.Hq + h) * a.Lq + r] = n > 0 ? m[i] / A(LOG2E) + log_acc(l[i]) : ninf;
+        if (a.lse && tx == 0 && r < rows.n)
+            static_cast<A*>(a.lse)[rows.stat(r)] = n > 0 ? m[i] / A(LOG2E) + log_acc(l[i]) : ninf;
     }
-    T* out = static_cast<T*>(const_cast<void*>(a.o)) + b * a.os[0] + h * a.os[2];
-    store_rows<T, A, TILE, DP>(out, a.os[1], q0, a.Lq, a.D, o, f, ty, tx);
+    T* out = static_cast<T*>(const_cast<void*>(a.o)) + rows.first(a.os);
+    store_rows<T, A, TILE, DP>(out, [&](int r) { return rows.at(a.os, r); }, q0, rows.n, a.D, o, f, ty, tx);
 }
 
 template <typename T>
@@ -275,13 +304,13 @@ attn_dq_simt_kernel(AttnArgs a, bool vec) {
     A* Ks = Gs + TILE * LD;
     A* Vs = Ks + TILE * LD;
     A* Ps = Vs + TILE * LD;
-    const int tiles = (a.Lq + TILE - 1) / TILE;
+    const int tiles = (a.Lq * (a.Hq / a.Hkv) + TILE - 1) / TILE;
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = int(cluster.block_rank()), world = int(cluster.num_blocks());
     const int64_t unit = blockIdx.x / world;
     const int q0 = int(unit % tiles) * TILE;
-    const int h = int(unit / tiles % a.Hq), b = int(unit / tiles / a.Hq);
-    const int g = h / (a.Hq / a.Hkv);
+    const int g = int(unit / tiles % a.Hkv), b = int(unit / tiles / a.Hkv);
+    const Rows rows(a, b, g);
     const int n = attn_len(a, b);
     const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
     const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + g * a.ks[2];
@@ -291,23 +320,22 @@ attn_dq_simt_kernel(AttnArgs a, bool vec) {
 #pragma unroll
     for (int i = 0; i < M; ++i) {
         const int r = q0 + ty * M + i;
-        const int64_t at = (int64_t(b) * a.Hq + h) * a.Lq + r;
-        lse[i] = r < a.Lq ? static_cast<const A*>(a.lse)[at] * A(LOG2E) : A(0);
-        dl[i] = r < a.Lq ? static_cast<const A*>(a.delta)[at] : A(0);
+        lse[i] = r < rows.n ? static_cast<const A*>(a.lse)[rows.stat(r)] * A(LOG2E) : A(0);
+        dl[i] = r < rows.n ? static_cast<const A*>(a.delta)[rows.stat(r)] : A(0);
         f[i] = A(a.scale);
 #pragma unroll
         for (int e = 0; e < DP / 16; ++e) acc[i][e] = 0;
     }
-    load_tile<T, A, TILE, DP>(Qs, static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2], a.qs[1], q0, a.Lq, a.D, vec);
-    load_tile<T, A, TILE, DP>(Gs, static_cast<const T*>(a.dout) + b * a.dos[0] + h * a.dos[2], a.dos[1], q0, a.Lq, a.D, vec);
+    load_tile<T, A, TILE, DP>(Qs, static_cast<const T*>(a.q) + rows.first(a.qs), [&](int r) { return rows.at(a.qs, r); }, q0, rows.n, a.D, vec);
+    load_tile<T, A, TILE, DP>(Gs, static_cast<const T*>(a.dout) + rows.first(a.dos), [&](int r) { return rows.at(a.dos, r); }, q0, rows.n, a.D, vec);
     for (int k0 = rank * TILE; k0 < n; k0 += world * TILE) {
         __syncthreads();
-        load_tile<T, A, TILE, DP>(Ks, k, a.ks[1], k0, n, a.D, vec);
-        load_tile<T, A, TILE, DP>(Vs, v, a.vs[1], k0, n, a.D, vec);
+        load_tile<T, A, TILE, DP>(Ks, k, [&](int r) { return r * a.ks[1]; }, k0, n, a.D, vec);
+        load_tile<T, A, TILE, DP>(Vs, v, [&](int r) { return r * a.vs[1]; }, k0, n, a.D, vec);
         __syncthreads();
         A s[M][M] = {}, dp[M][M] = {};
-        mul_rows<A, TILE, DP>(s, Qs, Ks, ty, tx);
-        mul_rows<A, TILE, DP>(dp, Gs, Vs, ty, tx);
+        mul_rows<A, TILE, DP>(s, Qs, Ks, a.D, ty, tx);
+        mul_rows<A, TILE, DP>(dp, Gs, Vs, a.D, ty, tx);
 #pragma unroll
         for (int i = 0; i < M; ++i)
 #pragma unroll
@@ -318,15 +346,16 @@ attn_dq_simt_kernel(AttnArgs a, bool vec) {
         __syncwarp();
         mul_cols<A, TILE, DP>(acc, Ps, Ks, ty, tx);
     }
-    T* dq = static_cast<T*>(a.dq) + (int64_t(b) * a.Lq * a.Hq + h) * a.D;
+    T* dq = static_cast<T*>(a.dq);
+    auto at = [&](int r) { return rows.dense(r); };
     if (world == 1) {
-        store_rows<T, A, TILE, DP>(dq, int64_t(a.Hq) * a.D, q0, a.Lq, a.D, acc, f, ty, tx);
+        store_rows<T, A, TILE, DP>(dq, at, q0, rows.n, a.D, acc, f, ty, tx);
         return;
     }
     __syncthreads();
     leave_rows<A, TILE, DP>(Qs, acc, ty, tx);
     cluster.sync();
-    store_shared<T, A, TILE, DP>(cluster, dq, int64_t(a.Hq) * a.D, q0, a.Lq, a.D, Qs, A(a.scale));
+    store_shared<T, A, TILE, DP>(cluster, dq, at, q0, rows.n, a.D, Qs, A(a.scale));
     cluster.sync();                        // nobody leaves while its shared memory is read
 }
 
@@ -349,7 +378,7 @@ attn_dkv_simt_kernel(AttnArgs a, bool vec) {
     const int64_t unit = blockIdx.x / world;
     const int k0 = int(unit % tiles) * TILE;
     const int g = int(unit / tiles % a.Hkv), b = int(unit / tiles / a.Hkv);
-    const int G = a.Hq / a.Hkv;
+    const Rows rows(a, b, g);
     const int n = attn_len(a, b);
     const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
     const A c = A(a.scale * LOG2E);
@@ -362,29 +391,26 @@ attn_dkv_simt_kernel(AttnArgs a, bool vec) {
         for (int e = 0; e < DP / 16; ++e) { dk[i][e] = 0; dv[i][e] = 0; }
     }
     if (k0 < n) {
-        load_tile<T, A, TILE, DP>(Ks, static_cast<const T*>(a.k) + b * a.ks[0] + g * a.ks[2], a.ks[1], k0, n, a.D, vec);
-        load_tile<T, A, TILE, DP>(Vs, static_cast<const T*>(a.v) + b * a.vs[0] + g * a.vs[2], a.vs[1], k0, n, a.D, vec);
-        const int per_head = (a.Lq + TILE - 1) / TILE;
-        for (int step = rank; step < per_head * G; step += world) {
-            const int h = g * G + step / per_head, q0 = step % per_head * TILE;
-            const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2];
-            const T* go = static_cast<const T*>(a.dout) + b * a.dos[0] + h * a.dos[2];
+        load_tile<T, A, TILE, DP>(Ks, static_cast<const T*>(a.k) + b * a.ks[0] + g * a.ks[2], [&](int r) { return r * a.ks[1]; }, k0, n, a.D, vec);
+        load_tile<T, A, TILE, DP>(Vs, static_cast<const T*>(a.v) + b * a.vs[0] + g * a.vs[2], [&](int r) { return r * a.vs[1]; }, k0, n, a.D, vec);
+        const T* q = static_cast<const T*>(a.q) + rows.first(a.qs);
+        const T* go = static_cast<const T*>(a.dout) + rows.first(a.dos);
+        for (int q0 = rank * TILE; q0 < rows.n; q0 += world * TILE) {
             __syncthreads();
-            load_tile<T, A, TILE, DP>(Qs, q, a.qs[1], q0, a.Lq, a.D, vec);
-            load_tile<T, A, TILE, DP>(Gs, go, a.dos[1], q0, a.Lq, a.D, vec);
+            load_tile<T, A, TILE, DP>(Qs, q, [&](int r) { return rows.at(a.qs, r); }, q0, rows.n, a.D, vec);
+            load_tile<T, A, TILE, DP>(Gs, go, [&](int r) { return rows.at(a.dos, r); }, q0, rows.n, a.D, vec);
             __syncthreads();
             A s[M][M] = {}, dp[M][M] = {};
-            mul_rows<A, TILE, DP>(s, Qs, Ks, ty, tx);
-            mul_rows<A, TILE, DP>(dp, Gs, Vs, ty, tx);
+            mul_rows<A, TILE, DP>(s, Qs, Ks, a.D, ty, tx);
+            mul_rows<A, TILE, DP>(dp, Gs, Vs, a.D, ty, tx);
 #pragma unroll
             for (int i = 0; i < M; ++i) {
                 const int r = q0 + ty * M + i;
-                const int64_t at = (int64_t(b) * a.Hq + h) * a.Lq + r;
-                const A lse = r < a.Lq ? static_cast<const A*>(a.lse)[at] * A(LOG2E) : A(0);
-                const A dl = r < a.Lq ? static_cast<const A*>(a.delta)[at] : A(0);
+                const A lse = r < rows.n ? static_cast<const A*>(a.lse)[rows.stat(r)] * A(LOG2E) : A(0);
+                const A dl = r < rows.n ? static_cast<const A*>(a.delta)[rows.stat(r)] : A(0);
 #pragma unroll
                 for (int j = 0; j < M; ++j) {
-                    const A p = r < a.Lq && k0 + tx + 16 * j < n ? exp_acc(s[i][j] * c - lse) : A(0);
+                    const A p = r < rows.n && k0 + tx + 16 * j < n ? exp_acc(s[i][j] * c - lse) : A(0);
                     Ps[(ty * M + i) * LP + tx + 16 * j] = p;
                     Ss[(ty * M + i) * LP + tx + 16 * j] = p * (dp[i][j] - dl);
                 }
@@ -394,18 +420,19 @@ attn_dkv_simt_kernel(AttnArgs a, bool vec) {
             mul_cols_t<A, TILE, DP>(dk, Ss, Qs, ty, tx);
         }
     }
-    const int64_t base = (int64_t(b) * a.Lk * a.Hkv + g) * a.D, stride = int64_t(a.Hkv) * a.D;
+    const int64_t base = (int64_t(b) * a.Lk * a.Hkv + g) * a.D;
+    auto at = [&](int r) { return int64_t(r) * a.Hkv * a.D; };
     if (world == 1) {
-        store_rows<T, A, TILE, DP>(static_cast<T*>(a.dk) + base, stride, k0, a.Lk, a.D, dk, fk, ty, tx);
-        store_rows<T, A, TILE, DP>(static_cast<T*>(a.dv) + base, stride, k0, a.Lk, a.D, dv, fv, ty, tx);
+        store_rows<T, A, TILE, DP>(static_cast<T*>(a.dk) + base, at, k0, a.Lk, a.D, dk, fk, ty, tx);
+        store_rows<T, A, TILE, DP>(static_cast<T*>(a.dv) + base, at, k0, a.Lk, a.D, dv, fv, ty, tx);
         return;
     }
     __syncthreads();
     leave_rows<A, TILE, DP>(Qs, dk, ty, tx);
     leave_rows<A, TILE, DP>(Gs, dv, ty, tx);
     cluster.sync();
-    store_shared<T, A, TILE, DP>(cluster, static_cast<T*>(a.dk) + base, stride, k0, a.Lk, a.D, Qs, A(a.scale));
-    store_shared<T, A, TILE, DP>(cluster, static_cast<T*>(a.dv) + base, stride, k0, a.Lk, a.D, Gs, A(1));
+    store_shared<T, A, TILE, DP>(cluster, static_cast<T*>(a.dk) + base, at, k0, a.Lk, a.D, Qs, A(a.scale));
+    store_shared<T, A, TILE, DP>(cluster, static_cast<T*>(a.dv) + base, at, k0, a.Lk, a.D, Gs, A(1));
     cluster.sync();                        // nobody leaves while its shared memory is read
 }
 
@@ -469,7 +496,7 @@ int forward_t(cudaStream_t st, const AttnArgs& a) {
     constexpr int TILE = fwd_tile<A>(DP);
     const bool vec = a.D * sizeof(T) % 16 == 0 && rows16(a.q, a.qs, sizeof(T)) && rows16(a.k, a.ks, sizeof(T)) &&
                      rows16(a.v, a.vs, sizeof(T));
-    return launch(attn_fwd_simt_kernel<T, TILE, DP>, ceil_div(a.Lq, TILE) * a.Hq * a.B, 0,
+    return launch(attn_fwd_simt_kernel<T, TILE, DP>, ceil_div(int64_t(a.Lq) * (a.Hq / a.Hkv), TILE) * a.Hkv * a.B, 0,
                   3 * tile_bytes<A>(TILE, DP) + score_bytes<A>(TILE), st, a, vec);
 }
 
@@ -480,9 +507,10 @@ int backward_t(cudaStream_t st, const AttnArgs& a) {
     const bool vec = a.D * sizeof(T) % 16 == 0 && rows16(a.q, a.qs, sizeof(T)) && rows16(a.k, a.ks, sizeof(T)) &&
                      rows16(a.v, a.vs, sizeof(T)) && rows16(a.dout, a.dos, sizeof(T));
     const int smem = 4 * tile_bytes<A>(TILE, DP) + 2 * score_bytes<A>(TILE);
-    NNVB_TRY(launch(attn_dq_simt_kernel<T, TILE, DP>, ceil_div(a.Lq, TILE) * a.Hq * a.B, ceil_div(a.Lk, TILE), smem, st, a, vec));
+    NNVB_TRY(launch(attn_dq_simt_kernel<T, TILE, DP>, ceil_div(int64_t(a.Lq) * (a.Hq / a.Hkv), TILE) * a.Hkv * a.B, ceil_div(a.Lk, TILE), smem, st,
+                    a, vec));
     return launch(attn_dkv_simt_kernel<T, TILE, DP>, ceil_div(a.Lk, TILE) * a.Hkv * a.B,
-                  ceil_div(a.Lq, TILE) * (a.Hq / a.Hkv), smem, st, a, vec);
+                  ceil_div(int64_t(a.Lq) * (a.Hq / a.Hkv), TILE), smem, st, a, vec);
 }
 
 template <typename T>

@@ -1,6 +1,6 @@
 // Attention over an encoder's states, forward, for float and double tensors with head sizes up to 128.
 //
-// A block of four warps takes 64 positions of one head and walks over tiles of states with the running maximum and sum of
+// A block of four warps takes 64 rows, positions of the query heads that share a state head, and walks over tiles of states with the running maximum and sum of
 // each row's softmax.  K and V tiles arrive by cp.async in a buffer each: V while the scores are computed, the next K
 // while the weights meet V.
 //   double  tensor cores (mma.sync f64 m16n8k8): a warp has 16 rows.  The order of the contraction is free, so channels
@@ -34,21 +34,22 @@ struct WideShape {
     static constexpr int BYTES = (NQ + NK + NV + NP) * int(sizeof(T));
 };
 
-// rows r0 .. r0 + ROWS of a [token] x D slab; rows from n_rows on and columns from D on become 0.  vec: asynchronous
-template <typename T, int ROWS, int DP, int LD>
-__device__ __forceinline__ void load_rows(T* s, const T* g, int64_t stride, int r0, int n_rows, int D, bool vec) {
+// rows r0 .. r0 + ROWS; rows from n_rows on and columns from D on become 0.  at(r): where row r begins, in elements from g.
+// vec: asynchronous
+template <typename T, int ROWS, int DP, int LD, typename At>
+__device__ __forceinline__ void load_rows(T* s, const T* g, At&& at, int r0, int n_rows, int D, bool vec) {
     constexpr int V = 16 / sizeof(T), P = DP / V;
     if (vec) {
 #pragma unroll 4
         for (int i = threadIdx.x; i < ROWS * P; i += THREADS) {
             const int r = i / P, c = i % P * V;
             const bool in = r0 + r < n_rows && c < D;              // D is a multiple of V
-            cp_async16(s + r * LD + c, g + (in ? int64_t(r0 + r) * stride + c : 0), in ? 16 : 0);
+            cp_async16(s + r * LD + c, g + (in ? at(r0 + r) + c : 0), in ? 16 : 0);
         }
     } else {
         for (int i = threadIdx.x; i < ROWS * DP; i += THREADS) {
             const int r = i / DP, c = i % DP;
-            s[r * LD + c] = r0 + r < n_rows && c < D ? g[int64_t(r0 + r) * stride + c] : T(0);
+            s[r * LD + c] = r0 + r < n_rows && c < D ? g[at(r0 + r) + c] : T(0);
         }
     }
     cp_async_commit();
@@ -241,12 +242,18 @@ attn_fwd_wide_kernel(AttnArgs a, bool vec) {
     __shared__ T all_m[BQ], all_l[BQ];
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = int(cluster.block_rank()), world = int(cluster.num_blocks());
-    const int tiles = (a.Lq + BQ - 1) / BQ;
+    // rows: the positions of all query heads that share a state head, heads of a position side by side
+    const int G = a.Hq / a.Hkv, rows = a.Lq * G;
+    const int tiles = (rows + BQ - 1) / BQ;
     const int64_t unit = blockIdx.x / world;
     const int q0 = int(unit % tiles) * BQ;
-    const int h = int(unit / tiles % a.Hq), b = int(unit / tiles / a.Hq);
-    const int g = h / (a.Hq / a.Hkv);
+    const int g = int(unit / tiles % a.Hkv), b = int(unit / tiles / a.Hkv);
     const int n = attn_len(a, b);
+    auto q_at = [&](int r) { return G == 1 ? r * a.qs[1] : int64_t(r / G) * a.qs[1] + int64_t(r % G) * a.qs[2]; };
+    auto o_at = [&](int r) { return G == 1 ? r * a.os[1] : int64_t(r / G) * a.os[1] + int64_t(r % G) * a.os[2]; };
+    auto k_at = [&](int r) { return int64_t(r) * a.ks[1]; };
+    auto v_at = [&](int r) { return int64_t(r) * a.vs[1]; };
+    auto lse_at = [&](int r) { return (int64_t(b) * a.Hq + g * G + r % G) * a.Lq + r / G; };
     const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + g * a.ks[2];
     const T* v = static_cast<const T*>(a.v) + b * a.vs[0] + g * a.vs[2];
     const T c = T(a.scale * LOG2E), ninf = -INFINITY;
@@ -256,17 +263,17 @@ attn_fwd_wide_kernel(AttnArgs a, bool vec) {
 #pragma unroll
     for (int i = 0; i < NR; ++i) { m[i] = ninf; l[i] = 0; }
     if (rank < steps) {
-        load_rows<T, BQ, DP, S::LDQ>(Qs, static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2], a.qs[1], q0, a.Lq, a.D, vec);
-        load_rows<T, S::BK, DP, S::LDK>(Ks, k, a.ks[1], rank * S::BK, n, a.D, vec);
+        load_rows<T, BQ, DP, S::LDQ>(Qs, static_cast<const T*>(a.q) + b * a.qs[0] + int64_t(g) * G * a.qs[2], q_at, q0, rows, a.D, vec);
+        load_rows<T, S::BK, DP, S::LDK>(Ks, k, k_at, rank * S::BK, n, a.D, vec);
     }
     for (int it = rank; it < steps; it += world) {
         const int k0 = it * S::BK;
-        load_rows<T, S::BK, DP, S::LDV>(Vs, v, a.vs[1], k0, n, a.D, vec);
+        load_rows<T, S::BK, DP, S::LDV>(Vs, v, v_at, k0, n, a.D, vec);
         cp_async_wait<1>();
         __syncthreads();
         w.scores(Qs, Ks, n - k0);
         __syncthreads();
-        if (it + world < steps) load_rows<T, S::BK, DP, S::LDK>(Ks, k, a.ks[1], (it + world) * S::BK, n, a.D, vec);
+        if (it + world < steps) load_rows<T, S::BK, DP, S::LDK>(Ks, k, k_at, (it + world) * S::BK, n, a.D, vec);
         else cp_async_commit();
         T top[NR], f[NR], base[NR];
 #pragma unroll
@@ -307,21 +314,22 @@ attn_fwd_wide_kernel(AttnArgs a, bool vec) {
     for (int i = 0; i < NR; ++i)
 #pragma unroll
         for (int o = W::LANES / 2; o > 0; o >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o, 32);
-    const int64_t lse0 = (int64_t(b) * a.Hq + h) * a.Lq + q0;
-    T* out = static_cast<T*>(const_cast<void*>(a.o)) + b * a.os[0] + int64_t(q0) * a.os[1] + h * a.os[2];
+    T* out = static_cast<T*>(const_cast<void*>(a.o)) + b * a.os[0] + int64_t(g) * G * a.os[2];
     const bool first = threadIdx.x % W::LANES == 0;
     if (world == 1) {
         T f[NR];
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
             f[i] = n > 0 ? T(1) / l[i] : T(0);
-            const int r = w.row(i);
-            if (a.lse && first && q0 + r < a.Lq)
-                static_cast<T*>(a.lse)[lse0 + r] = n > 0 ? m[i] / T(LOG2E) + log_acc(l[i]) : ninf;
+            const int r = q0 + w.row(i);
+            if (a.lse && first && r < rows)
+                static_cast<T*>(a.lse)[lse_at(r)] = n > 0 ? m[i] / T(LOG2E) + log_acc(l[i]) : ninf;
         }
+        T* to[NR];
+#pragma unroll
+        for (int i = 0; i < NR; ++i) to[i] = q0 + w.row(i) < rows ? out + o_at(q0 + w.row(i)) : nullptr;
         w.each_out([&](int i, int d, T x) {
-            const int r = w.row(i);
-            if (q0 + r < a.Lq && d < a.D) out[int64_t(r) * a.os[1] + d] = x * f[i];
+            if (to[i] && d < a.D) to[i][d] = x * f[i];
         });
         return;
     }
@@ -336,7 +344,7 @@ attn_fwd_wide_kernel(AttnArgs a, bool vec) {
     cluster.sync();
     for (int i = rank * THREADS + threadIdx.x; i < BQ * DP; i += world * THREADS) {
         const int r = i / DP, d = i % DP;
-        if (q0 + r >= a.Lq) continue;
+        if (q0 + r >= rows) continue;
         T top = ninf, sum = 0, x = 0;
         for (int p = 0; p < world; ++p) {
             const T y = *cluster.map_shared_rank(&all_m[r], p);
@@ -348,8 +356,8 @@ attn_fwd_wide_kernel(AttnArgs a, bool vec) {
             sum += *cluster.map_shared_rank(&all_l[r], p) * f;
             x += *cluster.map_shared_rank(&mine[i], p) * f;
         }
-        if (d < a.D) out[int64_t(r) * a.os[1] + d] = n > 0 ? x / sum : T(0);
-        if (d == 0 && a.lse) static_cast<T*>(a.lse)[lse0 + r] = n > 0 ? top / T(LOG2E) + log_acc(sum) : ninf;
+        if (d < a.D) out[o_at(q0 + r) + d] = n > 0 ? x / sum : T(0);
+        if (d == 0 && a.lse) static_cast<T*>(a.lse)[lse_at(q0 + r)] = n > 0 ? top / T(LOG2E) + log_acc(sum) : ninf;
     }
     cluster.sync();                        // nobody leaves while its shared memory is read
 }
@@ -362,7 +370,7 @@ int wide_t(cudaStream_t st, const AttnArgs& a) {
     for (auto* s : {a.qs, a.ks, a.vs})
         for (int i = 0; i < 3; ++i) vec = vec && s[i] * e % 16 == 0;
     for (const void* p : {a.q, a.k, a.v}) vec = vec && reinterpret_cast<uintptr_t>(p) % 16 == 0;
-    const int64_t units = ceil_div(a.Lq, BQ) * a.Hq * a.B, steps = ceil_div(a.Lk, S::BK);
+    const int64_t units = ceil_div(int64_t(a.Lq) * (a.Hq / a.Hkv), BQ) * a.Hkv * a.B, steps = ceil_div(a.Lk, S::BK);
     int dev = 0, sms = 148;
     NNVB_CUDA(cudaGetDevice(&dev));
     NNVB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
