@@ -455,8 +455,8 @@ int nnvb_layer_norm_forward(void* stream, int dtype, int64_t rows, int64_t cols,
                             void* rstd);
 /* Gradients of the same: dx [rows, cols], dscale and doffset [cols] (each may be
  * NULL).  mean, rstd are the forward call's.  With dscale or doffset the call needs
- * nnvb_layer_norm_workspace bytes of 16-byte aligned workspace; its contents need
- * no preparation.  The sums over rows are added in a fixed order. */
+ * nnvb_layer_norm_workspace bytes of 16-byte aligned workspace (0 for small tensors:
+ * NULL then); its contents need no preparation.  The sums over rows are added in a fixed order. */
 int64_t nnvb_layer_norm_workspace(int dtype, int64_t rows, int64_t cols);
 int nnvb_layer_norm_backward(void* stream, int dtype, int64_t rows, int64_t cols, const void* dy, int64_t lddy,
                              const void* x, int64_t ldx, const void* scale, const void* mean, const void* rstd, void* dx,

@@ -76,22 +76,24 @@ __device__ void load_tile(A* s, const T* g, At&& at, int r0, int n_rows, int D, 
     }
 }
 
-// acc[i][j] += sum_d X[(ty*M + i)][d] * Y[tx + 16 j][d], d < D
+// acc[i][j] += sum_d X[(ty*M + i)][d] * Y[tx + 16 j][d], d < D; rows of X from nx on and of Y from ny on do not count
 template <typename A, int TILE, int DP>
-__device__ __forceinline__ void mul_rows(A (&acc)[TILE / 16][TILE / 16], const A* X, const A* Y, int D, int ty, int tx) {
+__device__ __forceinline__ void mul_rows(A (&acc)[TILE / 16][TILE / 16], const A* X, const A* Y, int D, int nx, int ny, int ty, int tx) {
     constexpr int M = TILE / 16, V = VecOf<A>::N, LD = DP + V;
+    if (int(threadIdx.x / 32) * 2 * M >= nx) return;       // none of this warp's rows
     auto step = [&](int d) {
         Pack<A, V> x[M], y[M];
 #pragma unroll
         for (int i = 0; i < M; ++i) x[i] = lds<A>(X + (ty * M + i) * LD + d);
 #pragma unroll
-        for (int j = 0; j < M; ++j) y[j] = lds<A>(Y + (tx + 16 * j) * LD + d);
+        for (int j = 0; j < M; ++j)
+            if (16 * j < ny) {
+                y[j] = lds<A>(Y + (tx + 16 * j) * LD + d);
 #pragma unroll
-        for (int e = 0; e < V; ++e)
+                for (int e = 0; e < V; ++e)
 #pragma unroll
-            for (int i = 0; i < M; ++i)
-#pragma unroll
-                for (int j = 0; j < M; ++j) acc[i][j] += x[i].v[e] * y[j].v[e];
+                    for (int i = 0; i < M; ++i) acc[i][j] += x[i].v[e] * y[j].v[e];
+            }
     };
     if (D > DP - V) {                      // a loop of known length is the faster one
 #pragma unroll 4
@@ -102,12 +104,12 @@ __device__ __forceinline__ void mul_rows(A (&acc)[TILE / 16][TILE / 16], const A
     }
 }
 
-// acc[i][c] += sum_k P[ty*M + i][k] * Y[k][column c of this thread];  thread columns: V at tx*V + 16*V*c
+// acc[i][c] += sum_k P[ty*M + i][k] * Y[k][column c of this thread], k < n;  thread columns: V at tx*V + 16*V*c
 template <typename A, int TILE, int DP>
-__device__ __forceinline__ void mul_cols(A (&acc)[TILE / 16][DP / 16], const A* P, const A* Y, int ty, int tx) {
+__device__ __forceinline__ void mul_cols(A (&acc)[TILE / 16][DP / 16], const A* P, const A* Y, int n, int ty, int tx) {
     constexpr int M = TILE / 16, V = VecOf<A>::N, LD = DP + V, LP = TILE + V, NC = DP / (16 * V);
 #pragma unroll 2
-    for (int k = 0; k < TILE; k += V) {
+    for (int k = 0; k < TILE && k < n; k += V) {
         Pack<A, V> p[M];
 #pragma unroll
         for (int i = 0; i < M; ++i) p[i] = lds<A>(P + (ty * M + i) * LP + k);
@@ -124,12 +126,13 @@ __device__ __forceinline__ void mul_cols(A (&acc)[TILE / 16][DP / 16], const A* 
     }
 }
 
-// acc[i][c] += sum_q P[q][ty*M + i] * Y[q][column c of this thread]
+// acc[i][c] += sum_q P[q][ty*M + i] * Y[q][column c of this thread], q < n; rows of the result from nr on do not count
 template <typename A, int TILE, int DP>
-__device__ __forceinline__ void mul_cols_t(A (&acc)[TILE / 16][DP / 16], const A* P, const A* Y, int ty, int tx) {
+__device__ __forceinline__ void mul_cols_t(A (&acc)[TILE / 16][DP / 16], const A* P, const A* Y, int n, int nr, int ty, int tx) {
     constexpr int M = TILE / 16, V = VecOf<A>::N, LD = DP + V, LP = TILE + V, NC = DP / (16 * V);
+    if (int(threadIdx.x / 32) * 2 * M >= nr) return;       // none of this warp's rows
 #pragma unroll 4
-    for (int q = 0; q < TILE; ++q) {
+    for (int q = 0; q < TILE && q < n; ++q) {
         A p[M];
 #pragma unroll
         for (int i = 0; i < M; ++i) p[i] = P[q * LP + ty * M + i];
@@ -236,7 +239,7 @@ attn_fwd_simt_kernel(AttnArgs a, bool vec) {
         load_tile<T, A, TILE, DP>(Vs, v, [&](int r) { return r * a.vs[1]; }, k0, n, a.D, vec);
         __syncthreads();
         A s[M][M] = {};
-        mul_rows<A, TILE, DP>(s, Qs, Ks, a.D, ty, tx);
+        mul_rows<A, TILE, DP>(s, Qs, Ks, a.D, rows.n - q0, n - k0, ty, tx);
 #pragma unroll
         for (int i = 0; i < M; ++i) {
             A mx = ninf;
@@ -262,7 +265,7 @@ attn_fwd_simt_kernel(AttnArgs a, bool vec) {
             for (int e = 0; e < DP / 16; ++e) o[i][e] *= f;
         }
         __syncwarp();                     // a warp reads back only the rows its own threads wrote
-        mul_cols<A, TILE, DP>(o, Ps, Vs, ty, tx);
+        mul_cols<A, TILE, DP>(o, Ps, Vs, n - k0, ty, tx);
     }
     A f[M];
 #pragma unroll
@@ -334,8 +337,8 @@ attn_dq_simt_kernel(AttnArgs a, bool vec) {
         load_tile<T, A, TILE, DP>(Vs, v, [&](int r) { return r * a.vs[1]; }, k0, n, a.D, vec);
         __syncthreads();
         A s[M][M] = {}, dp[M][M] = {};
-        mul_rows<A, TILE, DP>(s, Qs, Ks, a.D, ty, tx);
-        mul_rows<A, TILE, DP>(dp, Gs, Vs, a.D, ty, tx);
+        mul_rows<A, TILE, DP>(s, Qs, Ks, a.D, rows.n - q0, n - k0, ty, tx);
+        mul_rows<A, TILE, DP>(dp, Gs, Vs, a.D, rows.n - q0, n - k0, ty, tx);
 #pragma unroll
         for (int i = 0; i < M; ++i)
 #pragma unroll
@@ -344,7 +347,7 @@ attn_dq_simt_kernel(AttnArgs a, bool vec) {
                 Ps[(ty * M + i) * LP + tx + 16 * j] = p * (dp[i][j] - dl[i]);
             }
         __syncwarp();
-        mul_cols<A, TILE, DP>(acc, Ps, Ks, ty, tx);
+        mul_cols<A, TILE, DP>(acc, Ps, Ks, n - k0, ty, tx);
     }
     T* dq = static_cast<T*>(a.dq);
     auto at = [&](int r) { return rows.dense(r); };
@@ -401,8 +404,8 @@ attn_dkv_simt_kernel(AttnArgs a, bool vec) {
             load_tile<T, A, TILE, DP>(Gs, go, [&](int r) { return rows.at(a.dos, r); }, q0, rows.n, a.D, vec);
             __syncthreads();
             A s[M][M] = {}, dp[M][M] = {};
-            mul_rows<A, TILE, DP>(s, Qs, Ks, a.D, ty, tx);
-            mul_rows<A, TILE, DP>(dp, Gs, Vs, a.D, ty, tx);
+            mul_rows<A, TILE, DP>(s, Qs, Ks, a.D, rows.n - q0, n - k0, ty, tx);
+            mul_rows<A, TILE, DP>(dp, Gs, Vs, a.D, rows.n - q0, n - k0, ty, tx);
 #pragma unroll
             for (int i = 0; i < M; ++i) {
                 const int r = q0 + ty * M + i;
@@ -416,8 +419,8 @@ attn_dkv_simt_kernel(AttnArgs a, bool vec) {
                 }
             }
             __syncthreads();
-            mul_cols_t<A, TILE, DP>(dv, Ps, Gs, ty, tx);
-            mul_cols_t<A, TILE, DP>(dk, Ss, Qs, ty, tx);
+            mul_cols_t<A, TILE, DP>(dv, Ps, Gs, rows.n - q0, n - k0, ty, tx);
+            mul_cols_t<A, TILE, DP>(dk, Ss, Qs, rows.n - q0, n - k0, ty, tx);
         }
     }
     const int64_t base = (int64_t(b) * a.Lk * a.Hkv + g) * a.D;

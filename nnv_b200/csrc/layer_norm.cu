@@ -16,8 +16,11 @@
 // a group's barriers stop no other group.  About 16 elements per thread spread what a row costs besides its elements;
 // with fewer the instruction issue is the bound, not memory.  A thread keeps its columns for all rows, so the weights,
 // and the sums over rows for their gradients, stay in registers; they leave a block as one partial row, and a second
-// kernel adds the partial rows in a fixed order: no atomics, the same bits every time.
+// kernel adds the partial rows in a fixed order: no atomics, the same bits every time.  Small tensors are given to one
+// cluster of up to 16 blocks, which adds its blocks' sums in distributed shared memory: one launch and no workspace.
 // Sums are held in float (double for double).
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <initializer_list>
 #include <type_traits>
@@ -25,6 +28,8 @@
 #include "common.cuh"
 #include "mma_f64.cuh"
 #include "tensor_types.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace nnvb {
 namespace {
@@ -99,6 +104,7 @@ struct LnTile {
     int cols;
     int R, tensor_bytes;                         // rows of a tile; bytes of one tensor's rows in a stage
     int mode;
+    void *dscale, *doffset;                      // one cluster of blocks: where it writes the weights' gradients itself
 };
 
 template <typename T, int VEC, int TPR, int N, bool BWD, int MINB>
@@ -337,10 +343,12 @@ ln_tile_kernel(const __grid_constant__ LnTile p) {
         for (int i = 0; i < LN_STAGES; ++i) mbar_wait(&full[i], phase, 1 << 20);
 
     if constexpr (BWD) {
-        if (!p.partial) return;
+        const bool whole = p.dscale || p.doffset;
+        if (!p.partial && !whole) return;
         // the groups' sums, added in group order, one access of columns at a time through the ring
         A* buf = reinterpret_cast<A*>(ring);
-        A* ps = static_cast<A*>(p.partial) + int64_t(blockIdx.x) * 2 * cols;
+        A* own = buf + LN_THREADS * VEC;        // a cluster's blocks keep their sums in shared memory, behind that
+        A* ps = whole ? own : static_cast<A*>(p.partial) + int64_t(blockIdx.x) * 2 * cols;
         const A bad = ok ? A(0) : A(NAN);
 #pragma unroll
         for (int k = 0; k < 2 * N; ++k) {
@@ -361,6 +369,18 @@ ln_tile_kernel(const __grid_constant__ LnTile p) {
                     ps[(k & 1) * int64_t(cols) + c] = sum;
                 }
             }
+        }
+        if (whole) {
+            cg::cluster_group cluster = cg::this_cluster();
+            cluster.sync();
+            const int rank = int(cluster.block_rank()), world = int(cluster.num_blocks());
+            for (int c = rank * LN_THREADS + tid; c < 2 * cols; c += world * LN_THREADS) {
+                A sum = 0;
+                for (int w = 0; w < world; ++w) sum += *cluster.map_shared_rank(own + c, w);
+                T* to = static_cast<T*>(c < cols ? p.dscale : p.doffset);
+                if (to) to[c < cols ? c : c - cols] = from_acc<T, A>(sum);
+            }
+            cluster.sync();                     // nobody leaves while its shared memory is read
         }
     }
 }
@@ -482,6 +502,7 @@ struct LnArgs {
     void *out, *mean, *rstd;
     void* partial;
     int grid;               // backward: blocks
+    void *dscale, *doffset;
 };
 
 int sm_count() {
@@ -498,10 +519,14 @@ int sm_count() {
 
 constexpr int LN_MAX_PARTS = 2 * 148;        // partial rows of the weights' gradients: blocks that fit at once
 
+// Backward of tensors up to this size runs in one cluster: its 16 SMs take about as long as a second launch does.
+bool ln_in_cluster(int64_t rows, int64_t cols) { return rows * cols <= 512 * 1024 && cols <= 4096; }
+
 template <typename T, int VEC, int TPR, int N, bool BWD, int MINB>
 int ln_tile(LnArgs& a, int mode) {
     constexpr int GROUPS = LN_THREADS / TPR, TENSORS = BWD ? 2 : 1;
-    const int64_t slots = std::min(sm_count(), 148) * MINB;
+    const bool cluster = BWD && (a.dscale || a.doffset) && ln_in_cluster(a.rows, a.cols);
+    const int64_t slots = cluster ? 16 : std::min(sm_count(), 148) * MINB;
     const int64_t pitch = a.cols * int64_t(sizeof(T));
     LnTile p{};
     p.rows = a.rows; p.cols = int(a.cols);
@@ -519,10 +544,30 @@ int ln_tile(LnArgs& a, int mode) {
     p.n_tiles = ceil_div(a.rows, R);
     p.tensor_bytes = int(round_up(R * pitch + 32, 128));
     using A = typename AccOf<T>::type;
-    const int smem = std::max<int>(LN_STAGES * p.tensor_bytes * TENSORS, BWD ? LN_THREADS * VEC * int(sizeof(A)) : 0);
+    const int sums = BWD ? (LN_THREADS * VEC + (cluster ? 2 * p.cols : 0)) * int(sizeof(A)) : 0;
+    const int smem = std::max<int>(LN_STAGES * p.tensor_bytes * TENSORS, sums);
     a.grid = int(std::min<int64_t>(p.n_tiles, slots));
     auto kernel = ln_tile_kernel<T, VEC, TPR, N, BWD, MINB>;
     NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (cluster) {
+        int world = 1;
+        while (world < a.grid) world *= 2;
+        p.dscale = a.dscale; p.doffset = a.doffset;
+        if (world > 8) NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(unsigned(world));
+        cfg.blockDim = dim3(LN_THREADS);
+        cfg.dynamicSmemBytes = size_t(smem);
+        cfg.stream = a.st;
+        cudaLaunchAttribute at{};
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = unsigned(world);
+        at.val.clusterDim.y = at.val.clusterDim.z = 1;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+        NNVB_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+        return NNVB_OK;
+    }
     kernel<<<unsigned(a.grid), LN_THREADS, smem, a.st>>>(p);
     NNVB_CUDA(cudaGetLastError());
     return NNVB_OK;
@@ -587,6 +632,7 @@ template <typename T>
 int ln_backward_t(LnArgs a, void* dscale, void* doffset) {
     using A = typename AccOf<T>::type;
     bool done;
+    a.dscale = dscale; a.doffset = doffset;
     NNVB_TRY((ln_run<T, true>(a, &done)));
     if (!done) {
         ln_backward_wide_kernel<T><<<unsigned(a.rows), 1024, 0, a.st>>>(
@@ -639,7 +685,7 @@ int nnvb_layer_norm_forward(void* stream, int dtype, int64_t rows, int64_t cols,
     if (rows == 0) return NNVB_OK;
     NNVB_REQUIRE(x && y, "nnvb_layer_norm_forward: NULL pointer");
     LnArgs a{static_cast<cudaStream_t>(stream), rows, cols, nullptr, x, scale, offset, 0, ldx, ldy, eps, y, mean, rstd,
-             nullptr, 0};
+             nullptr, 0, nullptr, nullptr};
     switch (dtype) {
         case NNVB_F64: return ln_forward_t<double>(a);
         case NNVB_F32: return ln_forward_t<float>(a);
@@ -649,7 +695,7 @@ int nnvb_layer_norm_forward(void* stream, int dtype, int64_t rows, int64_t cols,
 }
 
 int64_t nnvb_layer_norm_workspace(int dtype, int64_t rows, int64_t cols) {
-    if (dtype_bytes(dtype) == 0 || rows < 0 || cols < 1) return 0;
+    if (dtype_bytes(dtype) == 0 || rows < 0 || cols < 1 || ln_in_cluster(rows, cols)) return 0;
     return std::min<int64_t>(std::max<int64_t>(rows, 1), LN_MAX_PARTS) * 2 * cols * (dtype == NNVB_F64 ? 8 : 4);
 }
 
@@ -667,7 +713,7 @@ int nnvb_layer_norm_backward(void* stream, int dtype, int64_t rows, int64_t cols
         return NNVB_OK;
     }
     NNVB_REQUIRE(dy && x && mean && rstd && dx, "nnvb_layer_norm_backward: NULL pointer");
-    const bool weights = dscale || doffset;
+    const bool weights = (dscale || doffset) && !ln_in_cluster(rows, cols);
     if (weights) {
         NNVB_REQUIRE(workspace && workspace_bytes >= nnvb_layer_norm_workspace(dtype, rows, cols) &&
                          reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
@@ -675,7 +721,7 @@ int nnvb_layer_norm_backward(void* stream, int dtype, int64_t rows, int64_t cols
                      (long long)nnvb_layer_norm_workspace(dtype, rows, cols));
     }
     LnArgs a{st, rows, cols, dy, x, scale, nullptr, lddy, ldx, lddx, 0.0, dx, const_cast<void*>(mean),
-             const_cast<void*>(rstd), weights ? workspace : nullptr, 0};
+             const_cast<void*>(rstd), weights ? workspace : nullptr, 0, nullptr, nullptr};
     switch (dtype) {
         case NNVB_F64: return ln_backward_t<double>(a, dscale, doffset);
         case NNVB_F32: return ln_backward_t<float>(a, dscale, doffset);

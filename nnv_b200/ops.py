@@ -22,6 +22,7 @@ from . import _lib as L
 __all__ = ["layer_norm", "layer_norm_backward", "cross_attention", "cross_attention_backward"]
 
 _DTYPES = {torch.float64: L.F64, torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
+_entries = {}
 _DESC = struct.Struct("ii6qd15q")              # nnvb_attention_desc
 # the current stream as an address, without a Stream object per call (a fifth of a small call's host time)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
@@ -71,7 +72,9 @@ def _like(t):
 
 def _launch(dev, name, *args):
     """Call a library entry on torch's current stream of device ``dev``, with that device current."""
-    fn = getattr(L.load(), name)
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(L.load(), name)
     if torch.cuda.current_device() == dev:
         status = fn(_raw_stream(dev), *args)
     else:
@@ -141,13 +144,13 @@ def layer_norm_backward(dy, x, scale, mean, rstd):
     xr, rows, ldx = _rows(x, cols)
     gr, _, ldg = _rows(dy, cols)
     dx = _like(x)
-    dscale = x.new_empty(cols)
+    dscale = x.new_empty(cols) if scale is None else torch.empty_like(scale)
     doffset = torch.empty_like(dscale)
     nbytes = L.load().nnvb_layer_norm_workspace(kind, rows, cols)
-    ws = mean.new_empty(nbytes // mean.element_size())
+    ws = mean.new_empty(nbytes // mean.element_size()) if nbytes else None
     _launch(x.get_device(), "nnvb_layer_norm_backward", kind, rows, cols, gr.data_ptr(), ldg, xr.data_ptr(), ldx,
             _ptr(scale), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), cols, dscale.data_ptr(), doffset.data_ptr(),
-            ws.data_ptr(), nbytes)
+            _ptr(ws), nbytes)
     return dx, dscale, doffset
 
 

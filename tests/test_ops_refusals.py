@@ -71,9 +71,13 @@ def test_layer_norm_refuses():
     assert fwd(None, _lib.F32, 2, 8, None, 8, FAKE, FAKE, 1e-5, FAKE, 8, None, None) == _lib.NNVB_E_ARG
     assert fwd(None, _lib.F32, 0, 8, None, 8, None, None, 1e-5, None, 8, None, None) == _lib.NNVB_OK
     bwd = lib.nnvb_layer_norm_backward
-    need = lib.nnvb_layer_norm_workspace(_lib.F32, 2, 8)
-    assert need >= 2 * 8 * 4
-    assert bwd(None, _lib.F32, 2, 8, FAKE, 8, FAKE, 8, FAKE, FAKE, FAKE, FAKE, 8, FAKE, FAKE, FAKE, need - 1) == _lib.NNVB_E_ARG
+    need = lib.nnvb_layer_norm_workspace(_lib.F32, 1000, 1024)
+    assert need >= 2 * 1024 * 4
+    for ws, n in ((FAKE, need - 1), (FAKE + 4, need), (None, need)):
+        assert bwd(None, _lib.F32, 1000, 1024, FAKE, 1024, FAKE, 1024, FAKE, FAKE, FAKE, FAKE, 1024, FAKE, FAKE, ws, n) == _lib.NNVB_E_ARG
+        assert b"workspace" in lib.nnvb_last_error()
+    assert lib.nnvb_layer_norm_workspace(_lib.F32, 2, 8) == 0                  # small tensors need none
+    need = 0
     assert bwd(None, _lib.F32, 2, 8, FAKE, 8, FAKE, 8, FAKE, None, FAKE, FAKE, 8, FAKE, FAKE, FAKE, need) == _lib.NNVB_E_ARG
     assert bwd(None, _lib.F32, 2, 8, FAKE, 6, FAKE, 8, FAKE, FAKE, FAKE, FAKE, 8, FAKE, FAKE, FAKE, need) == _lib.NNVB_E_ARG
 
