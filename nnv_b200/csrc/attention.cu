@@ -113,7 +113,13 @@ int nnvb_cross_attention_backward(void* stream, const nnvb_attention_desc* d, co
     a.dq = dq; a.dk = dk; a.dv = dv; a.delta = workspace;
     if (attn_tc_takes_backward(a)) return attn_backward_tc(st, a);
     NNVB_TRY(attn_delta(st, a));
-    return attn_backward_simt(st, a);
+    // Large problems have the wide kernels' throughput (8 x 512 x 1024 x 8 x 64 double: 1.5 against 2.5 ms; 8 x 1024 x 2048 x 16 x
+    // 64 float: 6.3 against 7.4 ms).  With fewer tiles than SMs on one side the blocks of twice as many threads are the
+    // faster ones (4 x 6 x 13 float: 40 against 54 us; 1 x 573 x 8: 74 against 104 us).
+    const int64_t heads = int64_t(a.B) * a.Hkv, rows = int64_t(a.Lq) * (a.Hq / a.Hkv);
+    const bool wide = (a.dtype == NNVB_F64 || a.dtype == NNVB_F32) && a.D <= 128 && ceil_div(rows, 64) * heads >= 148 &&
+                      ceil_div(a.Lk, 64) * heads >= 148;
+    return wide ? attn_backward_wide(st, a) : attn_backward_simt(st, a);
 }
 
 }  // extern "C"

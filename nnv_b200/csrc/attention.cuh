@@ -41,6 +41,7 @@ bool attn_rows_takes(const AttnArgs& a);
 int attn_forward_rows(cudaStream_t st, const AttnArgs& a);
 // float and double, head size up to 128
 int attn_forward_wide(cudaStream_t st, const AttnArgs& a);
+int attn_backward_wide(cudaStream_t st, const AttnArgs& a);      // needs attn_delta's result
 // 16-bit types on the tensor cores; head size a multiple of 8 up to 128, 16-byte aligned rows
 bool attn_tc_takes_forward(const AttnArgs& a);
 int attn_forward_tc(cudaStream_t st, const AttnArgs& a);

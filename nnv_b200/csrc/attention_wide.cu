@@ -1,6 +1,6 @@
-// Attention over an encoder's states, forward, for float and double tensors with head sizes up to 128.
+// Attention over an encoder's states for float and double tensors with head sizes up to 128.
 //
-// A block of four warps takes 64 rows, positions of the query heads that share a state head, and walks over tiles of states with the running maximum and sum of
+// Forward.  A block of four warps takes 64 rows, positions of the query heads that share a state head, and walks over tiles of states with the running maximum and sum of
 // each row's softmax.  K and V tiles arrive by cp.async in a buffer each: V while the scores are computed, the next K
 // while the weights meet V.
 //   double  tensor cores (mma.sync f64 m16n8k8): a warp has 16 rows.  The order of the contraction is free, so channels
@@ -25,10 +25,10 @@ namespace {
 constexpr int BQ = 64, THREADS = 128;
 
 // Row strides (elements) that spread the loads of a warp over all banks.
-template <typename T, int DP>
+template <typename T, int DP, int BK_ = 0>
 struct WideShape {
     static constexpr bool F64 = sizeof(T) == 8;
-    static constexpr int BK = F64 && DP == 128 ? 32 : 64;          // states of a tile
+    static constexpr int BK = BK_ ? BK_ : (F64 && DP == 128 ? 32 : 64);        // states of a tile (backward: rows streamed)
     static constexpr int LDQ = F64 ? DP + 8 : DP + 4, LDK = LDQ, LDV = F64 ? DP + 2 : DP + 4, LDP = BK + 4;
     static constexpr int NQ = BQ * LDQ, NK = BK * LDK, NV = BK * LDV, NP = F64 ? 0 : BQ * LDP;
     static constexpr int BYTES = (NQ + NK + NV + NP) * int(sizeof(T));
@@ -56,11 +56,11 @@ __device__ __forceinline__ void load_rows(T* s, const T* g, At&& at, int r0, int
 }
 
 // A warp's or thread's part of the tile: scores and output of its rows.  Row of index i, and the type's products.
-template <typename T, int DP> struct Work;
+template <typename T, int DP, int BK = 0> struct Work;
 
-template <int DP>
-struct Work<double, DP> {
-    using S = WideShape<double, DP>;
+template <int DP, int BK_>
+struct Work<double, DP, BK_> {
+    using S = WideShape<double, DP, BK_>;
     static constexpr int NR = 2, NT = S::BK / 8;                   // rows of a lane; 8-state tiles
     double s[NT][4], o[DP / 8][4];
     int warp, g, t;
@@ -72,13 +72,14 @@ struct Work<double, DP> {
     }
     __device__ __forceinline__ int row(int i) const { return warp * 16 + g + i * 8; }
     // rest: states of the tile that count; 8-state tiles behind them are left out
+    template <int LDY = S::LDK>
     __device__ __forceinline__ void scores(const double* Q, const double* K, int rest) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[j][e] = 0;
         const double* q = Q + row(0) * S::LDQ + 2 * t;
-        const double* k = K + g * S::LDK + 2 * t;
+        const double* k = K + g * LDY + 2 * t;
 #pragma unroll 4
         for (int d = 0; d < DP; d += 8) {
             const double2 x = *reinterpret_cast<const double2*>(q + d), y = *reinterpret_cast<const double2*>(q + 8 * S::LDQ + d);
@@ -86,7 +87,7 @@ struct Work<double, DP> {
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 if (j * 8 >= rest) break;
-                const double2 z = *reinterpret_cast<const double2*>(k + j * 8 * S::LDK + d);
+                const double2 z = *reinterpret_cast<const double2*>(k + j * 8 * LDY + d);
                 const double b[2] = {z.x, z.y};
                 dmma_16x8x8(s[j], a, b);
             }
@@ -99,6 +100,14 @@ struct Work<double, DP> {
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) f(e / 2, j * 8 + 2 * t + e % 2, s[j][e]);
+    }
+    // f(row index, state of the tile, value, the other's value)
+    template <typename F>
+    __device__ __forceinline__ void each(Work& y, F&& f) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f(e / 2, j * 8 + 2 * t + e % 2, s[j][e], y.s[j][e]);
     }
     static constexpr int LANES = 4;                                // neighbouring lanes that share a row
     __device__ __forceinline__ void scale_out(const double (&f)[NR]) {
@@ -136,9 +145,9 @@ struct Work<double, DP> {
     }
 };
 
-template <int DP>
-struct Work<float, DP> {
-    using S = WideShape<float, DP>;
+template <int DP, int BK_>
+struct Work<float, DP, BK_> {
+    using S = WideShape<float, DP, BK_>;
     static constexpr int NR = 8;
     float s[NR][4];
     Pair<float> o[NR][DP / 32];
@@ -150,18 +159,19 @@ struct Work<float, DP> {
             for (int e = 0; e < DP / 32; ++e) o[i][e] = both(0.f);
     }
     __device__ __forceinline__ int row(int i) const { return ty * NR + i; }
+    template <int LDY = S::LDK>
     __device__ __forceinline__ void scores(const float* Q, const float* K, int) {
         Pair<float> acc[NR][4];
 #pragma unroll
         for (int i = 0; i < NR; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[i][j] = both(0.f);
-        const float *q = Q + ty * NR * S::LDQ, *k = K + tx * S::LDK;
+        const float *q = Q + ty * NR * S::LDQ, *k = K + tx * LDY;
 #pragma unroll 2
         for (int d = 0; d < DP; d += 4) {
             float4 y[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(k + 16 * j * S::LDK + d);
+            for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(k + 16 * j * LDY + d);
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
                 const float4 x = *reinterpret_cast<const float4*>(q + i * S::LDQ + d);
@@ -183,6 +193,13 @@ struct Work<float, DP> {
         for (int i = 0; i < NR; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) f(i, tx + 16 * j, s[i][j]);
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(Work& y, F&& f) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f(i, tx + 16 * j, s[i][j], y.s[i][j]);
     }
     static constexpr int LANES = 16;
     __device__ __forceinline__ void scale_out(const float (&f)[NR]) {
@@ -362,30 +379,188 @@ attn_fwd_wide_kernel(AttnArgs a, bool vec) {
     cluster.sync();                        // nobody leaves while its shared memory is read
 }
 
+// ---------------------------------------------------------------------------
+// Backward, with the roles of the tensor-core kernels: a block keeps 64 rows (positions for dQ, states for dK and dV), streams
+// tiles of the other side, and sums its rows' gradients in registers in a fixed order.  Streamed tiles are the second
+// operand of the scores and of the gradients, so their row stride suits both.
+
 template <typename T, int DP>
-int wide_t(cudaStream_t st, const AttnArgs& a) {
-    using S = WideShape<T, DP>;
-    const int64_t e = sizeof(T);
+struct BwdWide {
+    static constexpr bool F64 = sizeof(T) == 8;
+    static constexpr int BK = F64 ? (DP == 128 ? 16 : 32) : 64;
+    using S = WideShape<T, DP, BK>;
+    static constexpr int NA = BQ * S::LDQ, NB = BK * S::LDV;
+    static constexpr int BYTES = (2 * NA + 2 * NB + S::NP + 2 * BK) * int(sizeof(T));
+    // dK and dV of 128 channels in double do not fit the registers together: one pass each
+    static constexpr bool APART = F64 && DP == 128;
+};
+
+constexpr int BOTH = 0, ONLY_V = 1, ONLY_K = 2;
+
+template <typename T, int DP, bool KV, int WHICH>
+__global__ void __launch_bounds__(THREADS)
+attn_bwd_wide_kernel(AttnArgs a, bool vec) {
+    using H = BwdWide<T, DP>;
+    using S = typename H::S;
+    using W = Work<T, DP, H::BK>;
+    constexpr int NR = W::NR, BK = H::BK;
+    extern __shared__ __align__(128) unsigned char raw[];
+    T* A0 = reinterpret_cast<T*>(raw);
+    T *A1 = A0 + H::NA, *B0 = A1 + H::NA, *B1 = B0 + H::NB, *Ps = B1 + H::NB, *col_l = Ps + S::NP, *col_d = col_l + BK;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = int(cluster.block_rank()), world = int(cluster.num_blocks());
+    const int G = a.Hq / a.Hkv, rows = a.Lq * G;
+    const int own = KV ? a.Lk : rows;
+    const int tiles = (own + BQ - 1) / BQ;
+    const int64_t unit = blockIdx.x / world;
+    const int r0 = int(unit % tiles) * BQ;
+    const int g = int(unit / tiles % a.Hkv), b = int(unit / tiles / a.Hkv);
+    const int n = attn_len(a, b);
+    const int own_n = KV ? n : rows, other_n = KV ? rows : n;
+    const int steps = r0 < own_n ? (other_n + BK - 1) / BK : 0;
+    auto at = [&](const int64_t (&s)[3], int r) { return G == 1 ? r * s[1] : int64_t(r / G) * s[1] + int64_t(r % G) * s[2]; };
+    auto q_at = [&](int r) { return at(a.qs, r); };
+    auto g_at = [&](int r) { return at(a.dos, r); };
+    auto k_at = [&](int r) { return int64_t(r) * a.ks[1]; };
+    auto v_at = [&](int r) { return int64_t(r) * a.vs[1]; };
+    auto stat_at = [&](int r) {
+        return G == 1 ? (int64_t(b) * a.Hq + g) * a.Lq + r : (int64_t(b) * a.Hq + g * G + r % G) * a.Lq + r / G;
+    };
+    const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + int64_t(g) * G * a.qs[2];
+    const T* go = static_cast<const T*>(a.dout) + b * a.dos[0] + int64_t(g) * G * a.dos[2];
+    const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + g * a.ks[2];
+    const T* v = static_cast<const T*>(a.v) + b * a.vs[0] + g * a.vs[2];
+    const T *lse = static_cast<const T*>(a.lse), *delta = static_cast<const T*>(a.delta);
+    const T c = T(a.scale * LOG2E);
+    auto load0 = [&](int it) {
+        if (it >= steps) { cp_async_commit(); return; }
+        if constexpr (KV) load_rows<T, BK, DP, S::LDV>(B0, q, q_at, it * BK, rows, a.D, vec);
+        else load_rows<T, BK, DP, S::LDV>(B0, k, k_at, it * BK, n, a.D, vec);
+    };
+    auto load1 = [&](int it) {
+        if (it >= steps) { cp_async_commit(); return; }
+        if constexpr (KV) load_rows<T, BK, DP, S::LDV>(B1, go, g_at, it * BK, rows, a.D, vec);
+        else load_rows<T, BK, DP, S::LDV>(B1, v, v_at, it * BK, n, a.D, vec);
+    };
+    const bool busy = r0 + int(threadIdx.x / 32) * 16 < own_n;    // a warp has 16 rows
+    W x, y;                                // S (then P) with dV; dP (then dS) with dK or dQ
+    T row_l[NR], row_d[NR];
+    if (rank < steps) {
+        if constexpr (KV) {
+            load_rows<T, BQ, DP, S::LDQ>(A0, k, k_at, r0, n, a.D, vec);
+            load_rows<T, BQ, DP, S::LDQ>(A1, v, v_at, r0, n, a.D, vec);
+        } else {
+            load_rows<T, BQ, DP, S::LDQ>(A0, q, q_at, r0, rows, a.D, vec);
+            load_rows<T, BQ, DP, S::LDQ>(A1, go, g_at, r0, rows, a.D, vec);
+        }
+        load0(rank);
+        load1(rank);
+    }
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+        const int r = r0 + x.row(i);
+        row_l[i] = !KV && r < rows ? lse[stat_at(r)] * T(LOG2E) : T(0);
+        row_d[i] = !KV && r < rows ? delta[stat_at(r)] : T(0);
+    }
+    for (int it = rank; it < steps; it += world) {
+        const int rest = other_n - it * BK;
+        if (KV)
+            for (int j = threadIdx.x; j < BK && j < rest; j += THREADS) {
+                col_l[j] = lse[stat_at(it * BK + j)] * T(LOG2E);
+                col_d[j] = delta[stat_at(it * BK + j)];
+            }
+        cp_async_wait<0>();
+        __syncthreads();
+        if (busy) x.template scores<S::LDV>(A0, B0, rest);
+        if (WHICH != ONLY_V && busy) y.template scores<S::LDV>(A1, B1, rest);
+        if (!KV) {
+            __syncthreads();
+            load1(it + world);
+        }
+        if (busy) x.each(y, [&](int i, int j, T& p, T& d) {
+            const T l = KV ? (j < rest ? col_l[j] : T(0)) : row_l[i];
+            p = j < rest ? exp_acc(p * c - l) : T(0);
+            if (WHICH != ONLY_V) d = j < rest ? p * (d - (KV ? col_d[j] : row_d[i])) : T(0);
+        });
+        if (KV && WHICH != ONLY_K && busy) {
+            x.hand_over(Ps);
+            x.weigh(Ps, B1, rest);
+        }
+        if (KV) {
+            __syncthreads();
+            load1(it + world);
+        }
+        if (WHICH != ONLY_V && busy) {
+            y.hand_over(Ps);
+            y.weigh(Ps, B0, rest);
+        }
+        __syncthreads();
+        load0(it + world);
+    }
+    cp_async_wait<0>();
+    auto dense_at = [&](int r) {
+        return KV ? ((int64_t(b) * a.Lk + r) * a.Hkv + g) * a.D
+                  : (G == 1 ? ((int64_t(b) * a.Lq + r) * a.Hq + g) * a.D : ((int64_t(b) * a.Lq + r / G) * a.Hq + g * G + r % G) * a.D);
+    };
+    T *out_y = static_cast<T*>(KV ? a.dk : a.dq), *out_x = static_cast<T*>(a.dv);
+    if (world == 1) {
+        int64_t to[NR];
+#pragma unroll
+        for (int i = 0; i < NR; ++i) to[i] = r0 + x.row(i) < own ? dense_at(r0 + x.row(i)) : -1;
+        if (WHICH != ONLY_V)
+            y.each_out([&](int i, int d, T z) {
+                if (to[i] >= 0 && d < a.D) out_y[to[i] + d] = r0 + x.row(i) < own_n ? z * T(a.scale) : T(0);
+            });
+        if (KV && WHICH != ONLY_K)
+            x.each_out([&](int i, int d, T z) {
+                if (to[i] >= 0 && d < a.D) out_x[to[i] + d] = r0 + x.row(i) < own_n ? z : T(0);
+            });
+        return;
+    }
+    __syncthreads();
+    static_assert(BQ * DP <= H::NA, "");
+    if (WHICH != ONLY_V) y.each_out([&](int i, int d, T z) { A0[x.row(i) * DP + d] = z; });
+    if (KV && WHICH != ONLY_K) x.each_out([&](int i, int d, T z) { A1[x.row(i) * DP + d] = z; });
+    cluster.sync();
+    for (int i = rank * THREADS + threadIdx.x; i < BQ * DP; i += world * THREADS) {
+        const int r = r0 + i / DP, d = i % DP;
+        if (r >= own || d >= a.D) continue;
+        T sum_y = 0, sum_x = 0;
+        for (int w = 0; w < world; ++w) {
+            if (WHICH != ONLY_V) sum_y += *cluster.map_shared_rank(A0 + i, w);
+            if (KV && WHICH != ONLY_K) sum_x += *cluster.map_shared_rank(A1 + i, w);
+        }
+        const bool in = r < own_n;
+        if (WHICH != ONLY_V) out_y[dense_at(r) + d] = in ? sum_y * T(a.scale) : T(0);
+        if (KV && WHICH != ONLY_K) out_x[dense_at(r) + d] = in ? sum_x : T(0);
+    }
+    cluster.sync();                        // nobody leaves while its shared memory is read
+}
+
+// 16-byte accesses on every row?
+bool wide_rows16(const AttnArgs& a, int64_t e, bool backward) {
     bool vec = a.D * e % 16 == 0;
-    for (auto* s : {a.qs, a.ks, a.vs})
+    for (auto* s : {a.qs, a.ks, a.vs, backward ? a.dos : a.qs})
         for (int i = 0; i < 3; ++i) vec = vec && s[i] * e % 16 == 0;
-    for (const void* p : {a.q, a.k, a.v}) vec = vec && reinterpret_cast<uintptr_t>(p) % 16 == 0;
-    const int64_t units = ceil_div(int64_t(a.Lq) * (a.Hq / a.Hkv), BQ) * a.Hkv * a.B, steps = ceil_div(a.Lk, S::BK);
+    for (const void* p : {a.q, a.k, a.v, backward ? a.dout : a.q}) vec = vec && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+    return vec;
+}
+
+// `units` blocks, or clusters of up to 16 where blocks are few: those share the `steps` tiles a block walks over, two each at least
+template <typename K>
+int launch_wide(K kernel, int64_t units, int64_t steps, int per_sm, int smem, cudaStream_t st, const AttnArgs& a, bool vec) {
     int dev = 0, sms = 148;
     NNVB_CUDA(cudaGetDevice(&dev));
     NNVB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    // a cluster's blocks each take two tiles of states at least
     int world = 1;
-    while (world < 16 && units * world * 2 <= int64_t(sms) * 2 && world * 4 <= steps) world *= 2;
-    NNVB_REQUIRE(units * world < (int64_t(1) << 31), "nnvb_cross_attention_forward: too many tiles (%lld) for one launch",
-                 (long long)units);
-    auto kernel = attn_fwd_wide_kernel<T, DP>;
-    NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
+    while (world < 16 && units * world * 2 <= int64_t(sms) * per_sm && world * 4 <= steps) world *= 2;
+    NNVB_REQUIRE(units * world < (int64_t(1) << 31), "nnvb_cross_attention: too many tiles (%lld) for one launch", (long long)units);
+    NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     if (world > 8) NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(units * world));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = S::BYTES;
+    cfg.dynamicSmemBytes = size_t(smem);
     cfg.stream = st;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeClusterDimension;
@@ -397,11 +572,41 @@ int wide_t(cudaStream_t st, const AttnArgs& a) {
     return NNVB_OK;
 }
 
+template <typename T, int DP>
+int wide_backward_t(cudaStream_t st, const AttnArgs& a) {
+    using H = BwdWide<T, DP>;
+    const bool vec = wide_rows16(a, sizeof(T), true);
+    const int64_t rows = int64_t(a.Lq) * (a.Hq / a.Hkv), heads = int64_t(a.Hkv) * a.B;
+    const int per_sm = H::BYTES <= 113 * 1024 ? 2 : 1;
+    const int64_t uk = ceil_div(a.Lk, BQ) * heads, sk = ceil_div(rows, H::BK);
+    NNVB_TRY(launch_wide(attn_bwd_wide_kernel<T, DP, false, BOTH>, ceil_div(rows, BQ) * heads, ceil_div(a.Lk, H::BK), per_sm,
+                         H::BYTES, st, a, vec));
+    if constexpr (H::APART) {
+        NNVB_TRY(launch_wide(attn_bwd_wide_kernel<T, DP, true, ONLY_V>, uk, sk, per_sm, H::BYTES, st, a, vec));
+        return launch_wide(attn_bwd_wide_kernel<T, DP, true, ONLY_K>, uk, sk, per_sm, H::BYTES, st, a, vec);
+    } else {
+        return launch_wide(attn_bwd_wide_kernel<T, DP, true, BOTH>, uk, sk, per_sm, H::BYTES, st, a, vec);
+    }
+}
+
+template <typename T, int DP>
+int wide_t(cudaStream_t st, const AttnArgs& a) {
+    using S = WideShape<T, DP>;
+    const bool vec = wide_rows16(a, sizeof(T), false);
+    return launch_wide(attn_fwd_wide_kernel<T, DP>, ceil_div(int64_t(a.Lq) * (a.Hq / a.Hkv), BQ) * a.Hkv * a.B,
+                       ceil_div(a.Lk, S::BK), 2, S::BYTES, st, a, vec);
+}
+
 }  // namespace
 
 int attn_forward_wide(cudaStream_t st, const AttnArgs& a) {
     if (a.dtype == NNVB_F64) return a.D <= 64 ? wide_t<double, 64>(st, a) : wide_t<double, 128>(st, a);
     return a.D <= 64 ? wide_t<float, 64>(st, a) : wide_t<float, 128>(st, a);
+}
+
+int attn_backward_wide(cudaStream_t st, const AttnArgs& a) {
+    if (a.dtype == NNVB_F64) return a.D <= 64 ? wide_backward_t<double, 64>(st, a) : wide_backward_t<double, 128>(st, a);
+    return a.D <= 64 ? wide_backward_t<float, 64>(st, a) : wide_backward_t<float, 128>(st, a);
 }
 
 }  // namespace nnvb

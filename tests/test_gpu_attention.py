@@ -109,6 +109,14 @@ def test_few_rows_over_a_long_axis(t, B, Lq, Lk, H, D):
     _check(t, q, k, v, dout, _lens([Lk - 70] * B))
 
 
+@pytest.mark.parametrize("t", [torch.float64, torch.float32])
+@pytest.mark.parametrize("D", [64, 80, 128])
+def test_many_tiles_in_single_and_double(t, D):
+    """Enough tiles on both sides for the large problems' kernels; grouped heads, ragged lengths, odd sizes."""
+    q, k, v, dout = _data(t, 10, 99, 70, 16, 8, D)
+    _check(t, q, k, v, dout, _lens([70, 0, 1, 64, 65, 33, 70, 12, 69, 3]))
+
+
 @pytest.mark.parametrize("t", F16)
 @pytest.mark.parametrize("D", [64, 128])
 def test_clusters_with_ragged_lengths(t, D):
