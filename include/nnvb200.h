@@ -3,7 +3,8 @@
  * (estimated-bounds) reachability path of NNV.
  *
  * Everything crosses this boundary as plain pointers and sizes.  All floating
- * point is IEEE double; all tensors use MATLAB's column-major layout, i.e. an
+ * point is IEEE double (the operators on device tensors at the end of this file
+ * take other types too); all tensors use MATLAB's column-major layout, i.e. an
  * image-shaped set is V[h + H*(w + W*(c + C*j))] for predicate column j
  * (j = 0 is the centre), exactly what mxGetDoubles returns for the reference's
  * ImageStar.V.  Indices are 0-based here; the MEX gateway converts.

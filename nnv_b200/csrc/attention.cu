@@ -21,7 +21,10 @@ int check_desc(const char* who, const nnvb_attention_desc* d) {
     NNVB_REQUIRE(d->q_len * (d->q_heads / d->kv_heads) < I31, "%s: bad sizes (%lld positions of %lld heads a state head)", who,
                  (long long)d->q_len, (long long)(d->q_heads / d->kv_heads));
     NNVB_REQUIRE(d->head_dim >= 1 && d->head_dim <= 256, "%s: head size %lld (1..256 supported)", who, (long long)d->head_dim);
-    NNVB_REQUIRE(std::isfinite(d->scale) && d->scale > 0, "%s: the factor on the scores must be finite and positive", who);
+    // in the type of the sums, where it is folded with log2 e
+    const double c = d->scale * LOG2E;
+    NNVB_REQUIRE(std::isfinite(c) && c > 0 && (d->dtype == NNVB_F64 || (std::isfinite(float(c)) && float(c) > 0)),
+                 "%s: the factor on the scores must be finite and positive", who);
     for (const int64_t* s : {d->q_stride, d->k_stride, d->v_stride, d->out_stride, d->dout_stride})
         for (int i = 0; i < 3; ++i) NNVB_REQUIRE(s[i] >= 0, "%s: negative stride", who);
     return NNVB_OK;

@@ -15,6 +15,9 @@
 // 2^8 over the m in use, so weights stay below 2^8, which 16-bit P and fp32 sums hold without loss; after the first
 // tiles the rescale is rare.  P is rounded to the tensors' type because the product takes 16-bit operands; its
 // row sum is added in fp32 before the rounding.
+//
+// Every wait is bounded (about 0.2 s): a block whose hand-over breaks stops issuing, waits for its own copies and products
+// to end, frees its tensor memory and writes its rows as NaN.
 #include <cooperative_groups.h>
 
 #include <mutex>
@@ -26,8 +29,6 @@ namespace cg = cooperative_groups;
 
 namespace nnvb {
 namespace {
-
-__device__ unsigned long long g_timeouts;         // waits given up (a broken hand-over; the rows are written as NaN)
 
 constexpr int ROWS = 128;                          // rows of a tile of positions, states of a tile
 constexpr int FWD_THREADS = 320;
@@ -409,7 +410,6 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
     }
     tmem_fence_before();
     __syncthreads();
-    if (threadIdx.x == 0 && abort_flag) atomicAdd(&g_timeouts, 1ull);
     if (warp == 8) tmem_free(tmem, 512);
 }
 
@@ -772,7 +772,6 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
     }
     tmem_fence_before();
     __syncthreads();
-    if (threadIdx.x == 0 && abort_flag) atomicAdd(&g_timeouts, 1ull);
     if (warp == 16) tmem_free(tmem, 512);
 }
 

@@ -10,7 +10,7 @@
 //         nnvb200_mex('destroy', h)
 //
 // layers(i) has the fields of the reference's layer objects: Type ('conv2d', 'fc',
-// 'bn', 'avgpool', 'relu'), Weights, Bias, PaddingSize, Stride, DilationFactor,
+// 'bn', 'avgpool', 'relu', 'layernorm', 'attention'), Weights, Bias, PaddingSize, Stride, DilationFactor,
 // PoolSize, TrainedMean, TrainedVariance, Scale, Offset, Epsilon
 // (code/nnv/engine/nn/layers/Conv2DLayer.m:84-144, FullyConnectedLayer.m:56-66,
 //  BatchNormalizationLayer.m:72-77, AveragePooling2DLayer.m:109-131).
@@ -136,6 +136,34 @@ void create_net(int nlhs, mxArray* plhs[], int nrhs, const mxArray* prhs[], Err&
             d.avgpool_divisor = (dv && dv[0] != 0.0) ? NNVB_POOL_DIV_WINDOW : NNVB_POOL_DIV_INSIDE;
         } else if (type == "relu") {
             d.type = NNVB_LAYER_RELU;
+        } else if (type == "layernorm") {      // evaluated only; Scale and Offset may be left empty
+            d.type = NNVB_LAYER_LAYERNORM;
+            size_t ns = 0, no = 0;
+            const double* ch = field_doubles(prhs[1], i, "NumChannels", &n, e);
+            d.bn_scale = field_doubles(prhs[1], i, "Scale", &ns, e);
+            d.bn_offset = field_doubles(prhs[1], i, "Offset", &no, e);
+            if (ch) d.cout = (int32_t)ch[0];
+            if (!ch || (d.bn_scale && ns != (size_t)d.cout) || (d.bn_offset && no != (size_t)d.cout)) {
+                e.fail("NNVB200:layer", "layernorm needs NumChannels, and Scale and Offset of that size"); break;
+            }
+            const double* eps = field_doubles(prhs[1], i, "Epsilon", &n, e);
+            d.bn_eps = eps ? eps[0] : 1e-5;
+        } else if (type == "attention") {      // evaluated only; Keys, Values [channels, state heads, states]
+            d.type = NNVB_LAYER_ATTENTION;
+            const mxArray* kx = mxGetField(prhs[1], i, "Keys");
+            const mxArray* vx = mxGetField(prhs[1], i, "Values");
+            const double* heads = field_doubles(prhs[1], i, "NumHeads", &n, e);
+            if (!kx || !vx || !heads || !mxIsDouble(kx) || !mxIsDouble(vx) ||
+                mxGetNumberOfElements(kx) != mxGetNumberOfElements(vx)) {
+                e.fail("NNVB200:layer", "attention needs NumHeads, and double Keys and Values of one size"); break;
+            }
+            const mwSize nd = mxGetNumberOfDimensions(kx);
+            const mwSize* dm = mxGetDimensions(kx);
+            d.cin = (int32_t)dm[0]; d.kw = (int32_t)dm[1]; d.cout = nd > 2 ? (int32_t)dm[2] : 1;
+            d.kh = (int32_t)heads[0];
+            d.W = mxGetDoubles(kx); d.b = mxGetDoubles(vx);
+            const double* sc = field_doubles(prhs[1], i, "AttentionScale", &n, e);
+            d.bn_eps = sc ? sc[0] : 0.0;
         } else {
             e.fail("NNVB200:layer", "layer type '" + type + "' is outside the approx-star path of this engine");
         }

@@ -30,7 +30,8 @@ def test_descriptor_layout():
     ({"dtype": 7}, "element type"), ({"batch": -1}, "bad sizes"), ({"kv_len": 1 << 31}, "bad sizes"),
     ({"q_len": 1 << 30}, "bad sizes"),
     ({"q_heads": 7}, "heads"), ({"kv_heads": 0}, "heads"), ({"head_dim": 0}, "head size"), ({"head_dim": 257}, "head size"),
-    ({"scale": 0.0}, "factor"), ({"scale": float("nan")}, "factor"), ({"k_stride": (-1, 0, 0)}, "negative stride"),
+    ({"scale": 0.0}, "factor"), ({"scale": float("nan")}, "factor"), ({"scale": 1e300}, "factor"),
+    ({"scale": 1e-60}, "factor"), ({"k_stride": (-1, 0, 0)}, "negative stride"),
     ({"out_stride": (384, 128, 8)}, "overlap"), ({"out_stride": (0, 128, 16)}, "overlap")])
 def test_attention_forward_refuses(change, word):
     lib = _lib.load()
