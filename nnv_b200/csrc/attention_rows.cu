@@ -63,8 +63,8 @@ attn_rows_kernel(AttnArgs a) {
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = int(cluster.block_rank()), world = int(cluster.num_blocks());
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int64_t unit = blockIdx.x / world;                       // batch entry and state head
-    const int g = int(unit % a.Hkv), b = int(unit / a.Hkv);
+    const int unit = int(blockIdx.x) / world;                       // batch entry and state head
+    const int g = unit % a.Hkv, b = unit / a.Hkv;
     const int G = a.Hq / a.Hkv, rows = G * a.Lq;
     const int n = attn_len(a, b);
     const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + g * a.ks[2];
@@ -334,8 +334,8 @@ attn_rows_mma_kernel(AttnArgs a) {
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = int(cluster.block_rank()), world = int(cluster.num_blocks());
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, gr = lane / 4, tq = lane % 4;
-    const int64_t unit = blockIdx.x / world;
-    const int g = int(unit % a.Hkv), b = int(unit / a.Hkv);
+    const int unit = int(blockIdx.x) / world;
+    const int g = unit % a.Hkv, b = unit / a.Hkv;
     const int G = a.Hq / a.Hkv, rows = G * a.Lq;
     const int n = attn_len(a, b);
     const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + g * a.ks[2];

@@ -310,9 +310,9 @@ attn_dq_simt_kernel(AttnArgs a, bool vec) {
     const int tiles = (a.Lq * (a.Hq / a.Hkv) + TILE - 1) / TILE;
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = int(cluster.block_rank()), world = int(cluster.num_blocks());
-    const int64_t unit = blockIdx.x / world;
-    const int q0 = int(unit % tiles) * TILE;
-    const int g = int(unit / tiles % a.Hkv), b = int(unit / tiles / a.Hkv);
+    const int unit = int(blockIdx.x) / world;
+    const int q0 = unit % tiles * TILE;
+    const int g = unit / tiles % a.Hkv, b = unit / tiles / a.Hkv;
     const Rows rows(a, b, g);
     const int n = attn_len(a, b);
     const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
@@ -378,9 +378,9 @@ attn_dkv_simt_kernel(AttnArgs a, bool vec) {
     const int tiles = (a.Lk + TILE - 1) / TILE;
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = int(cluster.block_rank()), world = int(cluster.num_blocks());
-    const int64_t unit = blockIdx.x / world;
-    const int k0 = int(unit % tiles) * TILE;
-    const int g = int(unit / tiles % a.Hkv), b = int(unit / tiles / a.Hkv);
+    const int unit = int(blockIdx.x) / world;
+    const int k0 = unit % tiles * TILE;
+    const int g = unit / tiles % a.Hkv, b = unit / tiles / a.Hkv;
     const Rows rows(a, b, g);
     const int n = attn_len(a, b);
     const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;

@@ -99,10 +99,12 @@ struct TcMaps {
     CUtensorMap q, k, v, dout;
 };
 
-// coordinates of a head in a map; a broadcast dimension is stored as one entry
-__device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* m, int boxes, int box_bytes, int row, int head, int batch,
+// Rows of positions are those of 2^gs query heads that share a state head, heads of a position side by side: few positions
+// of grouped heads fill tiles, and K and V are read once for them.  A map's dimensions are channel, head, token, batch
+// entry; a broadcast dimension is stored as one entry.
+__device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* m, int boxes, int box_bytes, int token, int head, int batch,
                                           uint64_t* bar) {
-    for (int i = 0; i < boxes; ++i) tma_load_4d(static_cast<char*>(dst) + i * box_bytes, m, i * 64, row, head, batch, bar);
+    for (int i = 0; i < boxes; ++i) tma_load_4d(static_cast<char*>(dst) + i * box_bytes, m, i * 64, head, token, batch, bar);
 }
 
 template <int DP>
@@ -115,7 +117,7 @@ struct FwdSmem {
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
-attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
+attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
     using SM = FwdSmem<DP>;
     constexpr int STAGES = SM::STAGES;
     extern __shared__ unsigned char raw[];
@@ -130,13 +132,21 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = int(cluster.block_rank()), world = int(cluster.num_blocks());
-    const int tiles = (a.Lq + 2 * ROWS - 1) / (2 * ROWS);
-    const int64_t unit = blockIdx.x / world;
-    const int q0 = int(unit % tiles) * 2 * ROWS;
-    const int h = int(unit / tiles % a.Hq), b = int(unit / tiles / a.Hq);
+    const int rows = a.Lq << gs, groups = a.Hq >> gs, in_group = (1 << gs) - 1;
+    const int tiles = (rows + 2 * ROWS - 1) / (2 * ROWS);
+    const int unit = int(blockIdx.x) / world;
+    const int q0 = unit % tiles * 2 * ROWS;
+    const int h = (unit / tiles % groups) << gs, b = unit / tiles / groups;      // h: the group's first head
     const int g = h / (a.Hq / a.Hkv);
     const int n = attn_len(a, b);
-    const int live = a.Lq - q0 > ROWS ? 2 : 1;             // tiles of positions this block holds
+    const int live = rows - q0 > ROWS ? 2 : 1;             // tiles of rows this block holds
+    auto out_at = [&](int row) {
+        return static_cast<T*>(const_cast<void*>(a.o)) + int64_t(b) * a.os[0] + int64_t(row >> gs) * a.os[1] +
+               int64_t(h + (row & in_group)) * a.os[2];
+    };
+    auto lse_at = [&](int row) {
+        return static_cast<float*>(a.lse) + (int64_t(b) * a.Hq + h + (row & in_group)) * a.Lq + (row >> gs);
+    };
     // tiles of states: every world-th is this block's
     const int all_steps = (n + ROWS - 1) / ROWS, steps = all_steps > rank ? (all_steps - rank + world - 1) / world : 0;
 
@@ -162,7 +172,7 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
         if (lane == 0 && steps > 0) {
             mbar_expect_bytes(&q_full, uint32_t(live) * SM::TILE);
             for (int t = 0; t < live; ++t)
-                load_tile(sq + t * SM::TILE, &maps.q, DP / 64, SM::BOX, q0 + t * ROWS, a.qs[2] ? h : 0, a.qs[0] ? b : 0, &q_full);
+                load_tile(sq + t * SM::TILE, &maps.q, DP / 64, SM::BOX, (q0 + t * ROWS) >> gs, a.qs[2] ? h : 0, a.qs[0] ? b : 0, &q_full);
         }
         int it = 0;
         bool ok = true;
@@ -264,22 +274,27 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
             ok = mbar_wait_fast(&s_ready[t], i & 1, abort);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tmem_fence_after();
-            uint32_t s[4][32];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) tmem_load32(s[j], s_at + j * 32);
-            tmem_wait_load();
             const int rest = n - (rank + i * world) * ROWS;
-            if (rest < ROWS) {
+            // S is read twice, 32 columns at a time: all 128 would not fit the registers beside the rest
+            uint32_t s[2][32];
+            auto masked = [&](uint32_t (&x)[32], int j) {
+                if (rest < (j + 1) * 32) {
 #pragma unroll
-                for (int j = 0; j < 128; ++j)
-                    if (j >= rest) s[j / 32][j % 32] = 0xff800000u;        // -inf
-            }
+                    for (int e = 0; e < 32; ++e)
+                        if (j * 32 + e >= rest) x[e] = 0xff800000u;        // -inf
+                }
+            };
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            tmem_load32(s[0], s_at);
 #pragma unroll
-            for (int j = 0; j < 128; j += 8)
+            for (int j = 0; j < 4; ++j) {
+                tmem_wait_load(s[j % 2]);
+                if (j < 3) tmem_load32(s[(j + 1) % 2], s_at + (j + 1) * 32);
+                masked(s[j % 2], j);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    mx[e] = max3(mx[e], __uint_as_float(s[(j + 2 * e) / 32][(j + 2 * e) % 32]), __uint_as_float(s[(j + 2 * e) / 32][(j + 2 * e) % 32 + 1]));
+                for (int e = 0; e < 32; e += 2) mx[e / 2 % 4] = max3(mx[e / 2 % 4], __uint_as_float(s[j % 2][e]), __uint_as_float(s[j % 2][e + 1]));
+            }
+            tmem_load32(s[0], s_at);
             const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
             const bool raise = m == -INFINITY ? top > m : (top - m) * c > 8.f;
             if (i == 0) {
@@ -292,7 +307,7 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
                 for (int j = 0; j < DP / 32; ++j) {
                     uint32_t o[32];
                     tmem_load32(o, o_at + j * 32);
-                    tmem_wait_load();
+                    tmem_wait_load(o);
 #pragma unroll
                     for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
                     tmem_store32(o_at + j * 32, o);
@@ -302,14 +317,18 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
             Pair<float> sum[2] = {both(0.f), both(0.f)};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
+                tmem_wait_load(s[j % 2]);
+                if (j < 3) tmem_load32(s[(j + 1) % 2], s_at + (j + 1) * 32);
+                masked(s[j % 2], j);
                 uint32_t p[16];
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
-                    Pair<float> x = fma2({__uint_as_float(s[j][e]), __uint_as_float(s[j][e + 1])}, both(c), both(-mc));
+                    Pair<float> x = fma2({__uint_as_float(s[j % 2][e]), __uint_as_float(s[j % 2][e + 1])}, both(c), both(-mc));
                     x = e % 16 < EMULATED ? ex2_poly(x) : Pair<float>{ex2(x.x), ex2(x.y)};
                     sum[e / 2 % 2] = add2(sum[e / 2 % 2], x);
                     p[e / 2] = pack2<T>(x.x, x.y);
                 }
+                // over columns 16 j .. 16 j + 15 of S, which have been read by now
                 tmem_store16(s_at + j * 16, p);
             }
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
@@ -336,7 +355,7 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
                 uint32_t o[32];
                 if (steps > 0) {
                     tmem_load32(o, o_at + j * 32);
-                    tmem_wait_load();
+                    tmem_wait_load(o);
                 }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -349,18 +368,18 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
             }
         } else {
             const float f = !ok ? NAN : (n > 0 ? 1.f / l : 0.f);
-            T* out = static_cast<T*>(const_cast<void*>(a.o)) + int64_t(b) * a.os[0] + int64_t(row) * a.os[1] + int64_t(h) * a.os[2];
+            T* out = out_at(row);
 #pragma unroll 1
             for (int j = 0; j < DP / 32; ++j) {
                 uint32_t o[32];
                 if (n > 0 && ok) {
                     tmem_load32(o, o_at + j * 32);
-                    tmem_wait_load();
+                    tmem_wait_load(o);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) o[e] = 0;
                 }
-                if (row < a.Lq) {
+                if (row < rows) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) {
                         if (j * 32 + e < a.D) {
@@ -372,9 +391,8 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
                     }
                 }
             }
-            if (a.lse && row < a.Lq)
-                static_cast<float*>(a.lse)[(int64_t(b) * a.Hq + h) * a.Lq + row] =
-                    !ok ? NAN : (n > 0 ? m * float(a.scale) + logf(l) : -INFINITY);
+            if (a.lse && row < rows)
+                *lse_at(row) = !ok ? NAN : (n > 0 ? m * float(a.scale) + logf(l) : -INFINITY);
         }
     }
     if (world > 1) {
@@ -384,7 +402,7 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
         const float c = float(a.scale * LOG2E);
         for (int i = rank * FWD_THREADS + threadIdx.x; i < live * ROWS * (DP / 8); i += world * FWD_THREADS) {
             const int r = i / (DP / 8), d = i % (DP / 8) * 8, row = q0 + r;
-            if (row >= a.Lq) continue;
+            if (row >= rows) continue;
             float top = -INFINITY, sum = 0.f, x[8] = {};
             for (int w = 0; w < world; ++w) top = fmaxf(top, *cluster.map_shared_rank(&row_m[r], w));
             const float base = top == -INFINITY ? 0.f : top;
@@ -401,10 +419,8 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a) {
             const float f = n > 0 ? 1.f / sum : 0.f;
 #pragma unroll
             for (int u = 0; u < 8; ++u) x[u] *= f;
-            if (d < a.D)
-                store8<T>(static_cast<T*>(const_cast<void*>(a.o)) + int64_t(b) * a.os[0] + int64_t(row) * a.os[1] + int64_t(h) * a.os[2] + d, x);
-            if (d == 0 && a.lse)
-                static_cast<float*>(a.lse)[(int64_t(b) * a.Hq + h) * a.Lq + row] = n > 0 ? top * float(a.scale) + logf(sum) : -INFINITY;
+            if (d < a.D) store8<T>(out_at(row) + d, x);
+            if (d == 0 && a.lse) *lse_at(row) = n > 0 ? top * float(a.scale) + logf(sum) : -INFINITY;
         }
         cluster.sync();                    // nobody leaves while its shared memory is read
     }
@@ -449,33 +465,35 @@ struct BwdMaps {
     CUtensorMap a0, a1, b0, b1;
 };
 
-// stats: [B, Hq, LqP] lse' then the same of delta; LqP = Lq rounded up to 64, the rows behind Lq hold +inf and 0
+// stats: [B, groups of heads, RowsP] lse' then the same of delta, a group's rows rounded up to 64: those behind hold +inf and 0
 template <typename T>
 __global__ void __launch_bounds__(256)
-attn_stats_tc_kernel(AttnArgs a, int LqP) {
+attn_stats_tc_kernel(AttnArgs a, int RowsP, int gs) {
     const int lane = threadIdx.x % 16;
-    const int64_t i = int64_t(blockIdx.x) * 16 + threadIdx.x / 16;     // ((b * LqP) + r) * Hq + h
-    const bool live = i < int64_t(a.B) * LqP * a.Hq;
-    const int h = int(i % a.Hq), r = int(i / a.Hq % LqP), b = int(i / a.Hq / LqP);
+    const int64_t i = int64_t(blockIdx.x) * 16 + threadIdx.x / 16;
+    const int groups = a.Hq >> gs;
+    const int64_t count = int64_t(a.B) * groups * RowsP;
+    const int row = int(i % RowsP), b = int(i / RowsP / groups);
+    const int h = (int(i / RowsP % groups) << gs) + (row & ((1 << gs) - 1)), r = row >> gs;
+    const bool live = i < count && r < a.Lq;
     float s = 0.f;
-    if (live && r < a.Lq && lane * 8 < a.D) {
+    if (live && lane * 8 < a.D) {
         const auto o = *reinterpret_cast<const Pack<T, 8>*>(static_cast<const T*>(a.o) + b * a.os[0] + r * a.os[1] + h * a.os[2] + lane * 8);
         const auto d = *reinterpret_cast<const Pack<T, 8>*>(static_cast<const T*>(a.dout) + b * a.dos[0] + r * a.dos[1] + h * a.dos[2] + lane * 8);
 #pragma unroll
         for (int e = 0; e < 8; ++e) s += to_acc(o.v[e]) * to_acc(d.v[e]);
     }
     for (int w = 8; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w, 32);
-    if (live && lane == 0) {
+    if (i < count && lane == 0) {
         float* st = static_cast<float*>(a.delta);
-        const int64_t at = (int64_t(b) * a.Hq + h) * LqP + r;
-        st[at] = r < a.Lq ? static_cast<const float*>(a.lse)[(int64_t(b) * a.Hq + h) * a.Lq + r] * float(LOG2E) : INFINITY;
-        st[int64_t(a.B) * a.Hq * LqP + at] = s;
+        st[i] = live ? static_cast<const float*>(a.lse)[(int64_t(b) * a.Hq + h) * a.Lq + r] * float(LOG2E) : INFINITY;
+        st[count + i] = s;
     }
 }
 
 template <typename T, int DP, bool KV>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
-attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
+attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, int gs) {
     using SM = BwdSmem<DP>;
     constexpr int STAGES = SM::STAGES;
     extern __shared__ unsigned char raw[];
@@ -489,17 +507,19 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
     __shared__ float row_sum[4][ROWS];
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int own_len = KV ? a.Lk : a.Lq, own_heads = KV ? a.Hkv : a.Hq;
+    // rows and heads (dQ: groups of 2^gs) of this pass
+    const int rows = a.Lq << gs, groups = a.Hq >> gs;
+    const int own_len = KV ? a.Lk : rows, own_heads = KV ? a.Hkv : groups;
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = int(cluster.block_rank()), world = int(cluster.num_blocks());
     const int tiles = (own_len + ROWS - 1) / ROWS;
-    const int64_t unit = blockIdx.x / world;
-    const int r0 = int(unit % tiles) * ROWS;
-    const int oh = int(unit / tiles % own_heads), b = int(unit / tiles / own_heads);
-    const int G = a.Hq / a.Hkv;
+    const int unit = int(blockIdx.x) / world;
+    const int r0 = unit % tiles * ROWS;
+    const int oh = unit / tiles % own_heads, b = unit / tiles / own_heads;
+    const int G = (a.Hq / a.Hkv) >> gs;                    // groups that share a state head
     const int n = attn_len(a, b);
-    // streamed tiles: positions of all query heads of the group, or valid states
-    const int per_head = KV ? (a.Lq + BROWS - 1) / BROWS : (n + BROWS - 1) / BROWS;
+    // streamed tiles: rows of the groups that share the state head, or valid states
+    const int per_head = KV ? (rows + BROWS - 1) / BROWS : (n + BROWS - 1) / BROWS;
     const int all_steps = KV ? (r0 < n ? per_head * G : 0) : per_head;
     // every `share`-th is this block's; rows of up to 128 states stay in one block, which sums P dP over them
     const int share = all_steps <= 2 ? 1 : world;
@@ -522,19 +542,27 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
     tmem_fence_after();
     constexpr uint32_t tmem = 0;           // all 512 columns are this block's, so they start at column 0
     volatile int* abort = &abort_flag;
+    // Weights of many states are small, and fp16 loses bits below 2^-14: they enter dV's product times 2^12.
+    constexpr float P_SCALE = is_bf16<T> ? 1.f : 4096.f;
     // Tensor memory, columns: tile in flight t at 128 t: S 0..63, dP 64..127; the accumulators of dQ / dK at 256 and of
     // dV at 384.  The two warpgroups of a tile own 32 columns of S and of dP each and put their 16-bit operands there:
     // P over the lower half of their columns of S, the rest of dS over the upper half, dS over the lower half of dP.
     const float* st_lse = static_cast<const float*>(a.delta);
-    float* st_delta = static_cast<float*>(a.delta) + int64_t(a.B) * a.Hq * LqP;
+    float* st_delta = static_cast<float*>(a.delta) + int64_t(a.B) * groups * RowsP;
+    // where row r of a gradient begins
+    auto grad_at = [&](int r) {
+        return KV ? ((int64_t(b) * a.Lk + r) * a.Hkv + oh) * a.D
+                  : ((int64_t(b) * a.Lq + (r >> gs)) * a.Hq + (oh << gs) + (r & ((1 << gs) - 1))) * a.D;
+    };
 
     if (warp == 17) {
         // ---- copies -------------------------------------------------------------------------------------------
         const int64_t *as0 = KV ? a.ks : a.qs, *as1 = KV ? a.vs : a.dos, *bs0 = KV ? a.qs : a.ks, *bs1 = KV ? a.dos : a.vs;
         if (lane == 0 && steps > 0) {
             mbar_expect_bytes(&a_full, 2 * SM::ATILE);
-            load_tile(res, &maps.a0, DP / 64, SM::ABOX, r0, as0[2] ? oh : 0, as0[0] ? b : 0, &a_full);
-            load_tile(res + SM::ATILE, &maps.a1, DP / 64, SM::ABOX, r0, as1[2] ? oh : 0, as1[0] ? b : 0, &a_full);
+            const int ah = KV ? oh : oh << gs, token = KV ? r0 : r0 >> gs;
+            load_tile(res, &maps.a0, DP / 64, SM::ABOX, token, as0[2] ? ah : 0, as0[0] ? b : 0, &a_full);
+            load_tile(res + SM::ATILE, &maps.a1, DP / 64, SM::ABOX, token, as1[2] ? ah : 0, as1[0] ? b : 0, &a_full);
         }
         int it = 0;
         bool ok = true;
@@ -544,7 +572,8 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const int at_step = rank + it * share;
-            const int sh = KV ? oh * G + at_step / per_head : oh / G;      // streamed head
+            const int sh = KV ? oh * G + at_step / per_head : oh / G;      // streamed group or state head
+            const int bh = KV ? sh << gs : sh;
             const int row = at_step % per_head * BROWS;
             unsigned char* dst = ring + s * 2 * SM::BTILE;
             const int rest = KV ? BROWS : n - row;
@@ -554,10 +583,11 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
             uint64_t* bar = clear ? &tail : &full[s];
             if (lane == 0) {
                 mbar_expect_bytes(bar, 2 * SM::BTILE + (KV ? SM::STATS : 0));
-                load_tile(dst, &maps.b0, DP / 64, SM::BBOX, row, bs0[2] ? sh : 0, bs0[0] ? b : 0, bar);
-                load_tile(dst + SM::BTILE, &maps.b1, DP / 64, SM::BBOX, row, bs1[2] ? sh : 0, bs1[0] ? b : 0, bar);
+                const int token = KV ? row >> gs : row;
+                load_tile(dst, &maps.b0, DP / 64, SM::BBOX, token, bs0[2] ? bh : 0, bs0[0] ? b : 0, bar);
+                load_tile(dst + SM::BTILE, &maps.b1, DP / 64, SM::BBOX, token, bs1[2] ? bh : 0, bs1[0] ? b : 0, bar);
                 if (KV) {
-                    const int64_t at = (int64_t(b) * a.Hq + sh) * LqP + row;
+                    const int64_t at = (int64_t(b) * groups + sh) * RowsP + row;
                     bulk_copy_g2s(stats + s * 2 * BROWS, st_lse + at, BROWS * 4, bar);
                     bulk_copy_g2s(stats + s * 2 * BROWS + BROWS, st_delta + at, BROWS * 4, bar);
                 }
@@ -639,9 +669,10 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
         const int local = (warp % 4) * 32 + lane, row = r0 + local;
         const float c = float(a.scale * LOG2E);
         float my_lse = 0.f, my_delta = 0.f;
-        if (!KV && row < a.Lq) {
-            my_lse = st_lse[(int64_t(b) * a.Hq + oh) * LqP + row];
-            my_delta = st_delta[(int64_t(b) * a.Hq + oh) * LqP + row];
+        const int64_t my_at = (int64_t(b) * groups + oh) * RowsP + row;
+        if (!KV && row < rows) {
+            my_lse = st_lse[my_at];
+            my_delta = st_delta[my_at];
         }
         bool ok = true;
         for (int j = t; j < steps; j += 2) {
@@ -653,7 +684,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
             const int rest = KV ? 32 : n - (rank + j * share) * BROWS - half * 32;          // columns with weight
             uint32_t s[32];
             tmem_load32(s, s_at);
-            tmem_wait_load();
+            tmem_wait_load(s);
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
                 const Pair<float> lse = KV ? *reinterpret_cast<const Pair<float>*>(sl + e) : both(my_lse);
@@ -667,7 +698,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
                 for (int g = 0; g < 2; ++g) {
                     uint32_t d[16];
                     tmem_load16(d, d_at + g * 16);
-                    tmem_wait_load();
+                    tmem_wait_load(d);
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
                         if (g * 16 + e < rest) sum += __uint_as_float(s[g * 16 + e]) * __uint_as_float(d[e]);
@@ -679,13 +710,13 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
                 if (!ok) break;
                 my_delta = row_sum[0][local] + row_sum[1][local];
                 if (steps == 2) my_delta += row_sum[2][local] + row_sum[3][local];
-                if (wg == 0 && row < a.Lq) st_delta[(int64_t(b) * a.Hq + oh) * LqP + row] = my_delta;     // for the pass over dK, dV
+                if (wg == 0 && row < rows) st_delta[my_at] = my_delta;     // for the pass over dK, dV
             }
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 uint32_t d[16], p[8], hi[8], lo[8];
                 tmem_load16(d, d_at + g * 16);
-                tmem_wait_load();
+                tmem_wait_load(d);
 #pragma unroll
                 for (int e = 0; e < 16; e += 2) {
                     const int col = g * 16 + e;
@@ -694,7 +725,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
                     Pair<float> ds = mul2(pv, add2(Pair<float>{__uint_as_float(d[e]), __uint_as_float(d[e + 1])}, Pair<float>{-dl.x, -dl.y}));
                     if (!KV && col >= rest) ds.x = 0.f;                    // dP there may be 0 * NaN
                     if (!KV && col + 1 >= rest) ds.y = 0.f;
-                    if (KV) p[e / 2] = pack2<T>(pv.x, pv.y);
+                    if (KV) p[e / 2] = pack2<T>(pv.x * P_SCALE, pv.y * P_SCALE);
                     hi[e / 2] = pack2<T>(ds.x, ds.y);
                     ds = add2(ds, Pair<float>{-unpack_lo<T>(hi[e / 2]), -unpack_hi<T>(hi[e / 2])});
                     lo[e / 2] = pack2<T>(ds.x, ds.y);
@@ -713,9 +744,8 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
         // dK: warpgroups 0 and 1, dV: 2 and 3, half of the columns each; dQ: every warpgroup a chunk of 32
         const bool value = KV && t == 1;
         const bool dead = KV && row >= n;                  // states without weight: their rows of S may hold anything
-        const float f = !ok ? NAN : (value ? 1.f : float(a.scale));
-        T* out = static_cast<T*>(KV ? (value ? a.dv : a.dk) : a.dq) +
-                 (int64_t(b) * own_len * own_heads + int64_t(row) * own_heads + oh) * a.D;
+        const float f = !ok ? NAN : (value ? 1.f / P_SCALE : float(a.scale));
+        T* out = static_cast<T*>(KV ? (value ? a.dv : a.dk) : a.dq) + grad_at(row);
         const uint32_t o_at = lanes + 256 + (value ? 128 : 0);
         float4* mine = reinterpret_cast<float4*>(base) + ((value ? ROWS : 0) + local) * (DP / 4);
         constexpr int NJ = DP / 32;
@@ -725,7 +755,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
             uint32_t o[32];
             if (steps > 0 && ok) {
                 tmem_load32(o, o_at + j * 32);
-                tmem_wait_load();
+                tmem_wait_load(o);
             }
             const bool zero = ok && (steps == 0 || dead);
             if (world > 1) {
@@ -765,8 +795,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int LqP) {
                     x[u * 4] += y.x; x[u * 4 + 1] += y.y; x[u * 4 + 2] += y.z; x[u * 4 + 3] += y.w;
                 }
             }
-            store8<T>(static_cast<T*>(KV ? (pr >= ROWS ? a.dv : a.dk) : a.dq) +
-                          (int64_t(b) * own_len * own_heads + int64_t(row) * own_heads + oh) * a.D + d, x);
+            store8<T>(static_cast<T*>(KV ? (pr >= ROWS ? a.dv : a.dk) : a.dq) + grad_at(row) + d, x);
         }
         cluster.sync();                    // nobody leaves while its shared memory is read
     }
@@ -794,18 +823,18 @@ EncodeFn encode_fn() {
     return fn;
 }
 
-// Boxes of 64 elements x `rows` tokens of one head; a dimension with stride 0 (broadcast, or of one entry) has one entry.
+// Boxes of 64 elements x 2^gs heads x `rows` / 2^gs tokens; a dimension with stride 0 (broadcast, or of one entry) has one entry.
 int make_map(CUtensorMap* m, int dtype, const void* p, const int64_t (&s)[3], int64_t D, int64_t tokens, int64_t heads,
-             int64_t batch, int rows) {
+             int64_t batch, int rows, int gs) {
     EncodeFn fn = encode_fn();
     if (!fn) {
         set_error("nnvb_cross_attention: the CUDA driver does not offer cuTensorMapEncodeTiled");
         return NNVB_E_CUDA;
     }
-    const cuuint64_t dims[4] = {cuuint64_t(D), cuuint64_t(tokens), cuuint64_t(s[2] ? heads : 1), cuuint64_t(s[0] ? batch : 1)};
+    const cuuint64_t dims[4] = {cuuint64_t(D), cuuint64_t(s[2] ? heads : 1), cuuint64_t(tokens), cuuint64_t(s[0] ? batch : 1)};
     auto stride = [](int64_t e) { return cuuint64_t(e ? e * 2 : 16); };
-    const cuuint64_t strides[3] = {stride(s[1]), stride(s[2]), stride(s[0])};
-    const cuuint32_t box[4] = {64, cuuint32_t(rows), 1, 1}, one[4] = {1, 1, 1, 1};
+    const cuuint64_t strides[3] = {stride(s[2]), stride(s[1]), stride(s[0])};
+    const cuuint32_t box[4] = {64, cuuint32_t(1) << gs, cuuint32_t(rows >> gs), 1}, one[4] = {1, 1, 1, 1};
     const CUresult r = fn(m, dtype == NNVB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                           const_cast<void*>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -814,6 +843,15 @@ int make_map(CUtensorMap* m, int dtype, const void* p, const int64_t (&s)[3], in
         return NNVB_E_CUDA;
     }
     return NNVB_OK;
+}
+
+// Heads of a group whose positions are packed into rows: the largest power of two that divides the group, at most a
+// streamed tile's 64 rows; tensors whose heads are broadcast are not packed.
+int pack_shift(const AttnArgs& a, bool backward) {
+    int gs = 0;
+    if (a.qs[2] == 0 || (backward && a.dos[2] == 0)) return 0;
+    while (gs < 6 && (a.Hq / a.Hkv) % (2 << gs) == 0) ++gs;
+    return gs;
 }
 
 // rows TMA can read: 16-byte aligned, strides a multiple of 16 bytes below 2^40; tokens must not be broadcast
@@ -831,7 +869,8 @@ int launch_shared(K kernel, int64_t units, int64_t steps, int threads, int smem,
     NNVB_CUDA(cudaGetDevice(&dev));
     NNVB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     int world = 1;
-    while (world < 16 && units * world * 2 <= sms && world * 4 <= steps) world *= 2;
+    const int most = units <= 4 ? 16 : 8;              // a GPC has room for one cluster of 16 such blocks
+    while (world < most && units * world * 2 <= sms && world * 4 <= steps) world *= 2;
     NNVB_REQUIRE(units * world < (int64_t(1) << 31), "nnvb_cross_attention: too many tiles (%lld) for one launch", (long long)units);
     NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     if (world > 8) NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
@@ -854,35 +893,38 @@ template <typename T, int DP>
 int forward_t(cudaStream_t st, const AttnArgs& a) {
     using SM = FwdSmem<DP>;
     TcMaps maps{};
-    NNVB_TRY(make_map(&maps.q, a.dtype, a.q, a.qs, a.D, a.Lq, a.Hq, a.B, ROWS));
+    const int gs = pack_shift(a, false);
+    NNVB_TRY(make_map(&maps.q, a.dtype, a.q, a.qs, a.D, a.Lq, a.Hq, a.B, ROWS, gs));
     if (a.Lk > 0) {
-        NNVB_TRY(make_map(&maps.k, a.dtype, a.k, a.ks, a.D, a.Lk, a.Hkv, a.B, ROWS));
-        NNVB_TRY(make_map(&maps.v, a.dtype, a.v, a.vs, a.D, a.Lk, a.Hkv, a.B, ROWS));
+        NNVB_TRY(make_map(&maps.k, a.dtype, a.k, a.ks, a.D, a.Lk, a.Hkv, a.B, ROWS, 0));
+        NNVB_TRY(make_map(&maps.v, a.dtype, a.v, a.vs, a.D, a.Lk, a.Hkv, a.B, ROWS, 0));
     }
-    return launch_shared(attn_fwd_tc_kernel<T, DP>, ceil_div(a.Lq, 2 * ROWS) * a.Hq * a.B, ceil_div(a.Lk, ROWS), FWD_THREADS,
-                         SM::BYTES, st, maps, a);
+    return launch_shared(attn_fwd_tc_kernel<T, DP>, ceil_div(int64_t(a.Lq) << gs, 2 * ROWS) * (a.Hq >> gs) * a.B,
+                         ceil_div(a.Lk, ROWS), FWD_THREADS, SM::BYTES, st, maps, a, gs);
 }
 
 template <typename T, int DP>
 int backward_t(cudaStream_t st, const AttnArgs& a) {
     using SM = BwdSmem<DP>;
-    const int64_t LqP = round_up(a.Lq, BROWS);
-    const int64_t rows = LqP * a.B * a.Hq;
-    const int64_t bq = ceil_div(a.Lq, ROWS) * a.Hq * a.B, bk = ceil_div(a.Lk, ROWS) * a.Hkv * a.B;
-    NNVB_REQUIRE(ceil_div(rows, 16) < (int64_t(1) << 31), "nnvb_cross_attention_backward: too many rows (%lld)", (long long)rows);
-    attn_stats_tc_kernel<T><<<unsigned(ceil_div(rows, 16)), 256, 0, st>>>(a, int(LqP));
+    const int gs = pack_shift(a, true);
+    const int64_t rows = int64_t(a.Lq) << gs, groups = a.Hq >> gs, RowsP = round_up(rows, BROWS);
+    const int64_t count = RowsP * a.B * groups;
+    NNVB_REQUIRE(ceil_div(count, 16) < (int64_t(1) << 31), "nnvb_cross_attention_backward: too many rows (%lld)", (long long)count);
+    attn_stats_tc_kernel<T><<<unsigned(ceil_div(count, 16)), 256, 0, st>>>(a, int(RowsP), gs);
     NNVB_CUDA(cudaGetLastError());
     BwdMaps mq{}, mk{};
-    NNVB_TRY(make_map(&mq.a0, a.dtype, a.q, a.qs, a.D, a.Lq, a.Hq, a.B, ROWS));
-    NNVB_TRY(make_map(&mq.a1, a.dtype, a.dout, a.dos, a.D, a.Lq, a.Hq, a.B, ROWS));
-    NNVB_TRY(make_map(&mq.b0, a.dtype, a.k, a.ks, a.D, a.Lk, a.Hkv, a.B, BROWS));
-    NNVB_TRY(make_map(&mq.b1, a.dtype, a.v, a.vs, a.D, a.Lk, a.Hkv, a.B, BROWS));
-    NNVB_TRY(make_map(&mk.a0, a.dtype, a.k, a.ks, a.D, a.Lk, a.Hkv, a.B, ROWS));
-    NNVB_TRY(make_map(&mk.a1, a.dtype, a.v, a.vs, a.D, a.Lk, a.Hkv, a.B, ROWS));
-    NNVB_TRY(make_map(&mk.b0, a.dtype, a.q, a.qs, a.D, a.Lq, a.Hq, a.B, BROWS));
-    NNVB_TRY(make_map(&mk.b1, a.dtype, a.dout, a.dos, a.D, a.Lq, a.Hq, a.B, BROWS));
-    NNVB_TRY(launch_shared(attn_bwd_tc_kernel<T, DP, false>, bq, ceil_div(a.Lk, BROWS), BWD_THREADS, SM::BYTES, st, mq, a, int(LqP)));
-    return launch_shared(attn_bwd_tc_kernel<T, DP, true>, bk, LqP / BROWS * (a.Hq / a.Hkv), BWD_THREADS, SM::BYTES, st, mk, a, int(LqP));
+    NNVB_TRY(make_map(&mq.a0, a.dtype, a.q, a.qs, a.D, a.Lq, a.Hq, a.B, ROWS, gs));
+    NNVB_TRY(make_map(&mq.a1, a.dtype, a.dout, a.dos, a.D, a.Lq, a.Hq, a.B, ROWS, gs));
+    NNVB_TRY(make_map(&mq.b0, a.dtype, a.k, a.ks, a.D, a.Lk, a.Hkv, a.B, BROWS, 0));
+    NNVB_TRY(make_map(&mq.b1, a.dtype, a.v, a.vs, a.D, a.Lk, a.Hkv, a.B, BROWS, 0));
+    NNVB_TRY(make_map(&mk.a0, a.dtype, a.k, a.ks, a.D, a.Lk, a.Hkv, a.B, ROWS, 0));
+    NNVB_TRY(make_map(&mk.a1, a.dtype, a.v, a.vs, a.D, a.Lk, a.Hkv, a.B, ROWS, 0));
+    NNVB_TRY(make_map(&mk.b0, a.dtype, a.q, a.qs, a.D, a.Lq, a.Hq, a.B, BROWS, gs));
+    NNVB_TRY(make_map(&mk.b1, a.dtype, a.dout, a.dos, a.D, a.Lq, a.Hq, a.B, BROWS, gs));
+    NNVB_TRY(launch_shared(attn_bwd_tc_kernel<T, DP, false>, ceil_div(rows, ROWS) * groups * a.B, ceil_div(a.Lk, BROWS), BWD_THREADS,
+                           SM::BYTES, st, mq, a, int(RowsP), gs));
+    return launch_shared(attn_bwd_tc_kernel<T, DP, true>, ceil_div(a.Lk, ROWS) * a.Hkv * a.B,
+                         RowsP / BROWS * ((a.Hq / a.Hkv) >> gs), BWD_THREADS, SM::BYTES, st, mk, a, int(RowsP), gs);
 }
 
 }  // namespace

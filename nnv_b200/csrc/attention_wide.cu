@@ -262,9 +262,9 @@ attn_fwd_wide_kernel(AttnArgs a, bool vec) {
     // rows: the positions of all query heads that share a state head, heads of a position side by side
     const int G = a.Hq / a.Hkv, rows = a.Lq * G;
     const int tiles = (rows + BQ - 1) / BQ;
-    const int64_t unit = blockIdx.x / world;
-    const int q0 = int(unit % tiles) * BQ;
-    const int g = int(unit / tiles % a.Hkv), b = int(unit / tiles / a.Hkv);
+    const int unit = int(blockIdx.x) / world;
+    const int q0 = unit % tiles * BQ;
+    const int g = unit / tiles % a.Hkv, b = unit / tiles / a.Hkv;
     const int n = attn_len(a, b);
     auto q_at = [&](int r) { return G == 1 ? r * a.qs[1] : int64_t(r / G) * a.qs[1] + int64_t(r % G) * a.qs[2]; };
     auto o_at = [&](int r) { return G == 1 ? r * a.os[1] : int64_t(r / G) * a.os[1] + int64_t(r % G) * a.os[2]; };
@@ -412,9 +412,9 @@ attn_bwd_wide_kernel(AttnArgs a, bool vec) {
     const int G = a.Hq / a.Hkv, rows = a.Lq * G;
     const int own = KV ? a.Lk : rows;
     const int tiles = (own + BQ - 1) / BQ;
-    const int64_t unit = blockIdx.x / world;
-    const int r0 = int(unit % tiles) * BQ;
-    const int g = int(unit / tiles % a.Hkv), b = int(unit / tiles / a.Hkv);
+    const int unit = int(blockIdx.x) / world;
+    const int r0 = unit % tiles * BQ;
+    const int g = unit / tiles % a.Hkv, b = unit / tiles / a.Hkv;
     const int n = attn_len(a, b);
     const int own_n = KV ? n : rows, other_n = KV ? rows : n;
     const int steps = r0 < own_n ? (other_n + BK - 1) / BK : 0;

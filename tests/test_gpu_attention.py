@@ -145,6 +145,32 @@ def test_large_scores_and_a_rising_maximum(t):
     _check(t, q, k, v, dout, None)
 
 
+@pytest.mark.parametrize("Lq,Lk", [(2, 3000), (200, 4000)])
+def test_small_weights_keep_their_bits_in_half_precision(Lq, Lk):
+    """Weights around 1/Lk, many below the smallest normal fp16: dv to the rounding of its terms and of its own, without
+    the absolute error that subnormal weights would add (2^-25 each, the allowance of the other tests)."""
+    from nnv_b200 import ops
+    q, k, v, dout = _data(torch.float16, 1, Lq, Lk, 2, 2, 64, spread=2.0)
+    out, lse = ops.cross_attention(q, k, v, return_lse=True)
+    dv = ops.cross_attention_backward(dout, q, k, v, out, lse)[2]
+    want, _ = R.attention(q, k, v, None, 0.125, dout)["dv"]
+    s = torch.einsum("bqhd,bkhd->bhqk", q.double(), k.double()) * 0.125
+    spread = torch.einsum("bhqk,bqhd->bkhd", s.softmax(-1), dout.double().abs()).cpu().numpy()
+    # rounding of each weight (half a step, 2^-11) and fp32 arithmetic (a 16th of it at most), then dv's own rounding,
+    # which is absolute (2^-25) where dv itself is below the smallest normal number
+    R.check("dv", dv, want, 2.0 ** -11 * (1 + 1 / 16) * spread + 2.0 ** -11 * abs(want) + 2.0 ** -25)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("Hq,Hkv,Lq", [(8, 2, 9), (12, 2, 50), (64, 1, 3), (128, 1, 5), (4, 2, 200)])
+def test_grouped_heads_share_tiles(t, Hq, Hkv, Lq):
+    """Groups of 4, 6, 64, 128 and 2 heads: positions of a group's heads are rows of one tile."""
+    q, k, v, dout = _data(t, 2, Lq, 150, Hq, Hkv, 64)
+    _check(t, q, k, v, dout, _lens([150, 61]))
+    one = q[:, :, :1].expand(-1, -1, Hq, -1)                   # a broadcast query head is not packed
+    out, lse = _check(t, one, k, v, dout, _lens([150, 61]))
+
+
 @pytest.mark.parametrize("t", TYPES)
 def test_scale_and_strided_views(t):
     from nnv_b200 import ops
