@@ -31,7 +31,7 @@ namespace nnvb {
 namespace {
 
 constexpr int ROWS = 128;                          // rows of a tile of positions, states of a tile
-constexpr int FWD_THREADS = 320;
+constexpr int FWD_THREADS = 384;
 constexpr int EMULATED = 4;                        // of 16 exponentials run on the FMA pipe (0: 460 us, 4: 459, 6: 474 at
                                                    // 8 x 2048 x 4096 x 16 x 128; 416, 387, 407 with 64 channels)
 
@@ -166,233 +166,233 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
     constexpr uint32_t tmem = 0;           // all 512 columns are this block's, so they start at column 0
     volatile int* abort = &abort_flag;
 
-    if (warp == 9) {
-        // ---- copies -------------------------------------------------------------------------------------------
-        const int kb = a.ks[0] ? b : 0, kh = a.ks[2] ? g : 0, vb = a.vs[0] ? b : 0, vh = a.vs[2] ? g : 0;
-        if (lane == 0 && steps > 0) {
-            mbar_expect_bytes(&q_full, uint32_t(live) * SM::TILE);
-            for (int t = 0; t < live; ++t)
-                load_tile(sq + t * SM::TILE, &maps.q, DP / 64, SM::BOX, (q0 + t * ROWS) >> gs, a.qs[2] ? h : 0, a.qs[0] ? b : 0, &q_full);
-        }
-        int it = 0;
-        bool ok = true;
-        for (int i = 0; i < steps && ok; ++i) {
-            for (int kv = 0; kv < 2; ++kv, ++it) {
-                const int s = it % STAGES;
-                if (it >= STAGES) ok = mbar_wait_fast(&empty[s], (it / STAGES - 1) & 1, abort);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                unsigned char* dst = ring + s * SM::TILE;
-                const int row = (rank + i * world) * ROWS, rest = n - row;
-                // V rows behind the valid states may hold anything, and 0 * NaN is NaN: they are cleared here.  (K needs
-                // nothing: its rows only make scores that are masked.)
-                if (kv == 1 && rest < ROWS && n < a.Lk) {
-                    if (lane == 0) {
-                        mbar_expect_bytes(&tail, SM::TILE);
-                        load_tile(dst, &maps.v, DP / 64, SM::BOX, row, vh, vb, &tail);
-                    }
-                    ok = __all_sync(0xffffffffu, mbar_wait_fast(&tail, 0, abort));
-                    for (int j = lane; j < (ROWS - rest) * 8 * (DP / 64); j += 32) {
-                        const int box = j / ((ROWS - rest) * 8), r = j % ((ROWS - rest) * 8);
-                        *reinterpret_cast<uint4*>(dst + box * SM::BOX + rest * 128 + r * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    async_proxy_fence();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&full[s]);
-                } else if (lane == 0) {
-                    mbar_expect_bytes(&full[s], SM::TILE);
-                    load_tile(dst, kv ? &maps.v : &maps.k, DP / 64, SM::BOX, row, kv ? vh : kh, kv ? vb : kb, &full[s]);
-                }
+    // 384 threads at 168 registers = 256 at 208 + 128 at 88: a softmax thread holds a row of 128 scores (8 x 2048 x 4096 x
+    // 16 x 128: 522 us; 567 with 168 registers and the scores read twice, 550 with them spilled)
+    if (warp >= 8) {
+        reg_dealloc<88>();
+        if (warp == 9) {
+            // ---- copies -------------------------------------------------------------------------------------------
+            const int kb = a.ks[0] ? b : 0, kh = a.ks[2] ? g : 0, vb = a.vs[0] ? b : 0, vh = a.vs[2] ? g : 0;
+            if (lane == 0 && steps > 0) {
+                mbar_expect_bytes(&q_full, uint32_t(live) * SM::TILE);
+                for (int t = 0; t < live; ++t)
+                    load_tile(sq + t * SM::TILE, &maps.q, DP / 64, SM::BOX, (q0 + t * ROWS) >> gs, a.qs[2] ? h : 0, a.qs[0] ? b : 0, &q_full);
             }
-        }
-        if (!ok && lane == 0) {            // gave up: the copies issued so far still write to this block's memory
-            mbar_wait(&q_full, 0, 1 << 20);
-            for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j) mbar_wait(&full[j % STAGES], (j / STAGES) & 1, 1 << 20);
-        }
-    } else if (warp == 8) {
-        // ---- products -----------------------------------------------------------------------------------------
-        const uint32_t leader = elect_lane();
-        if (steps > 0) {
-            constexpr uint32_t id_s = mma_idesc(is_bf16<T>, 128, ROWS, false);
-            constexpr uint32_t id_o = mma_idesc(is_bf16<T>, 128, DP, true);
-            const int ksteps = (a.D + 15) / 16;
-            const uint32_t q_addr = smem_u32(sq), r_addr = smem_u32(ring);
-            auto scores = [&](int t, int s) {
-                const uint32_t qd = desc_k_major(q_addr + t * SM::TILE), kd = desc_k_major(r_addr + s * SM::TILE);
-#pragma unroll
-                for (int k = 0; k < DP / 16; ++k) {
-                    const uint32_t off = ((k / 4) * SM::BOX + (k % 4) * 32) >> 4;
-                    if (k < ksteps) mma_ss(leader, tmem + t * 128, qd + off, kd + off, id_s, k > 0);
-                }
-                mma_commit(leader, &s_ready[t]);
-            };
-            bool ok = warp_wait(&q_full, 0, abort) && warp_wait(&full[0], 0, abort);
-            if (ok) {
-                for (int t = 0; t < live; ++t) scores(t, 0);
-                mma_commit(leader, &empty[0]);
-            }
+            int it = 0;
+            bool ok = true;
             for (int i = 0; i < steps && ok; ++i) {
-                const int vi = 2 * i + 1, ki = 2 * i + 2;
-                const bool next = i + 1 < steps;
-                ok = warp_wait(&full[vi % STAGES], (vi / STAGES) & 1, abort);
-                if (ok && next) ok = warp_wait(&full[ki % STAGES], (ki / STAGES) & 1, abort);
-                for (int t = 0; t < live && ok; ++t) {
-                    ok = warp_wait(&p_ready[t], i & 1, abort);
+                for (int kv = 0; kv < 2; ++kv, ++it) {
+                    const int s = it % STAGES;
+                    if (it >= STAGES) ok = mbar_wait_fast(&empty[s], (it / STAGES - 1) & 1, abort);
+                    ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    tmem_fence_after();
-                    const uint32_t vd = desc_mn_major(r_addr + (vi % STAGES) * SM::TILE, SM::BOX);
-#pragma unroll
-                    for (int k = 0; k < ROWS / 16; ++k)
-                        mma_ts(leader, tmem + 256 + t * 128, tmem + t * 128 + k * 8, vd + k * (2048 >> 4), id_o, i > 0 || k > 0);
-                    // S of the next states goes over P of these: products issued by one thread run in order
-                    if (next) scores(t, ki % STAGES);
-                    else mma_commit(leader, &o_ready[t]);
+                    unsigned char* dst = ring + s * SM::TILE;
+                    const int row = (rank + i * world) * ROWS, rest = n - row;
+                    // V rows behind the valid states may hold anything, and 0 * NaN is NaN: they are cleared here.  (K needs
+                    // nothing: its rows only make scores that are masked.)
+                    if (kv == 1 && rest < ROWS && n < a.Lk) {
+                        if (lane == 0) {
+                            mbar_expect_bytes(&tail, SM::TILE);
+                            load_tile(dst, &maps.v, DP / 64, SM::BOX, row, vh, vb, &tail);
+                        }
+                        ok = __all_sync(0xffffffffu, mbar_wait_fast(&tail, 0, abort));
+                        for (int j = lane; j < (ROWS - rest) * 8 * (DP / 64); j += 32) {
+                            const int box = j / ((ROWS - rest) * 8), r = j % ((ROWS - rest) * 8);
+                            *reinterpret_cast<uint4*>(dst + box * SM::BOX + rest * 128 + r * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        async_proxy_fence();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&full[s]);
+                    } else if (lane == 0) {
+                        mbar_expect_bytes(&full[s], SM::TILE);
+                        load_tile(dst, kv ? &maps.v : &maps.k, DP / 64, SM::BOX, row, kv ? vh : kh, kv ? vb : kb, &full[s]);
+                    }
                 }
+            }
+            if (!ok && lane == 0) {            // gave up: the copies issued so far still write to this block's memory
+                mbar_wait(&q_full, 0, 1 << 20);
+                for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j) mbar_wait(&full[j % STAGES], (j / STAGES) & 1, 1 << 20);
+            }
+        } else if (warp == 8) {
+            // ---- products -----------------------------------------------------------------------------------------
+            const uint32_t leader = elect_lane();
+            if (steps > 0) {
+                constexpr uint32_t id_s = mma_idesc(is_bf16<T>, 128, ROWS, false);
+                constexpr uint32_t id_o = mma_idesc(is_bf16<T>, 128, DP, true);
+                const int ksteps = (a.D + 15) / 16;
+                const uint32_t q_addr = smem_u32(sq), r_addr = smem_u32(ring);
+                auto scores = [&](int t, int s) {
+                    const uint32_t qd = desc_k_major(q_addr + t * SM::TILE), kd = desc_k_major(r_addr + s * SM::TILE);
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) {
+                        const uint32_t off = ((k / 4) * SM::BOX + (k % 4) * 32) >> 4;
+                        if (k < ksteps) mma_ss(leader, tmem + t * 128, qd + off, kd + off, id_s, k > 0);
+                    }
+                    mma_commit(leader, &s_ready[t]);
+                };
+                bool ok = warp_wait(&q_full, 0, abort) && warp_wait(&full[0], 0, abort);
                 if (ok) {
-                    mma_commit(leader, &empty[vi % STAGES]);
-                    if (next) mma_commit(leader, &empty[ki % STAGES]);
+                    for (int t = 0; t < live; ++t) scores(t, 0);
+                    mma_commit(leader, &empty[0]);
+                }
+                for (int i = 0; i < steps && ok; ++i) {
+                    const int vi = 2 * i + 1, ki = 2 * i + 2;
+                    const bool next = i + 1 < steps;
+                    ok = warp_wait(&full[vi % STAGES], (vi / STAGES) & 1, abort);
+                    if (ok && next) ok = warp_wait(&full[ki % STAGES], (ki / STAGES) & 1, abort);
+                    for (int t = 0; t < live && ok; ++t) {
+                        ok = warp_wait(&p_ready[t], i & 1, abort);
+                        if (!ok) break;
+                        tmem_fence_after();
+                        const uint32_t vd = desc_mn_major(r_addr + (vi % STAGES) * SM::TILE, SM::BOX);
+#pragma unroll
+                        for (int k = 0; k < ROWS / 16; ++k)
+                            mma_ts(leader, tmem + 256 + t * 128, tmem + t * 128 + k * 8, vd + k * (2048 >> 4), id_o, i > 0 || k > 0);
+                        // S of the next states goes over P of these: products issued by one thread run in order
+                        if (next) scores(t, ki % STAGES);
+                        else mma_commit(leader, &o_ready[t]);
+                    }
+                    if (ok) {
+                        mma_commit(leader, &empty[vi % STAGES]);
+                        if (next) mma_commit(leader, &empty[ki % STAGES]);
+                    }
+                }
+                // the last commit has arrived: nothing touches this block's barriers after it has left
+                if (ok) ok = warp_wait(&empty[(2 * steps - 1) % STAGES], ((2 * steps - 1) / STAGES) & 1, abort);
+                if (!ok) {                     // gave up: nothing may still write to the tensor memory that is freed below
+                    mma_commit(leader, &drain);
+                    mbar_wait(&drain, 0, 1 << 20);
                 }
             }
-            // the last commit has arrived: nothing touches this block's barriers after it has left
-            if (ok) ok = warp_wait(&empty[(2 * steps - 1) % STAGES], ((2 * steps - 1) / STAGES) & 1, abort);
-            if (!ok) {                     // gave up: nothing may still write to the tensor memory that is freed below
-                mma_commit(leader, &drain);
-                mbar_wait(&drain, 0, 1 << 20);
-            }
+            __syncwarp();
         }
-        __syncwarp();
-    } else if (warp / 4 < live) {
-        // ---- softmax: one row per thread ------------------------------------------------------------------------
-        const int t = warp / 4;
-        const uint32_t lanes = tmem + (uint32_t(warp % 4) << 21);
-        const uint32_t s_at = lanes + t * 128, o_at = lanes + 256 + t * 128;
-        const int row = q0 + t * ROWS + (warp % 4) * 32 + lane;
-        const float c = float(a.scale * LOG2E);
-        float m = -INFINITY, l = 0.f;      // m: the maximum in use, of the scores without the factor
-        bool ok = true;
-        for (int i = 0; i < steps; ++i) {
-            ok = mbar_wait_fast(&s_ready[t], i & 1, abort);
-            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-            tmem_fence_after();
-            const int rest = n - (rank + i * world) * ROWS;
-            // S is read twice, 32 columns at a time: all 128 would not fit the registers beside the rest
-            uint32_t s[2][32];
-            auto masked = [&](uint32_t (&x)[32], int j) {
-                if (rest < (j + 1) * 32) {
+    } else {
+        reg_alloc<208>();
+        if (warp / 4 < live) {
+            // ---- softmax: one row per thread ------------------------------------------------------------------------
+            const int t = warp / 4;
+            const uint32_t lanes = tmem + (uint32_t(warp % 4) << 21);
+            const uint32_t s_at = lanes + t * 128, o_at = lanes + 256 + t * 128;
+            const int row = q0 + t * ROWS + (warp % 4) * 32 + lane;
+            const float c = float(a.scale * LOG2E);
+            float m = -INFINITY, l = 0.f;      // m: the maximum in use, of the scores without the factor
+            bool ok = true;
+            for (int i = 0; i < steps; ++i) {
+                ok = mbar_wait_fast(&s_ready[t], i & 1, abort);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                tmem_fence_after();
+                const int rest = n - (rank + i * world) * ROWS;
+                uint32_t s[4][32];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (j * 32 + e >= rest) x[e] = 0xff800000u;        // -inf
+                for (int j = 0; j < 4; ++j) tmem_load32(s[j], s_at + j * 32);
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    tmem_wait_load(s[j]);
+                    if (rest < (j + 1) * 32) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (j * 32 + e >= rest) s[j][e] = 0xff800000u;        // -inf
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) mx[e / 2 % 4] = max3(mx[e / 2 % 4], __uint_as_float(s[j][e]), __uint_as_float(s[j][e + 1]));
                 }
-            };
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            tmem_load32(s[0], s_at);
+                const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+                const bool raise = m == -INFINITY ? top > m : (top - m) * c > 8.f;
+                if (i == 0) {
+                    m = top;
+                } else if (__any_sync(0xffffffffu, raise)) {
+                    const float f = raise ? (m == -INFINITY ? 0.f : ex2((m - top) * c)) : 1.f;
+                    if (raise) m = top;
+                    l *= f;
+#pragma unroll 1
+                    for (int j = 0; j < DP / 32; ++j) {
+                        uint32_t o[32];
+                        tmem_load32(o, o_at + j * 32);
+                        tmem_wait_load(o);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                tmem_wait_load(s[j % 2]);
-                if (j < 3) tmem_load32(s[(j + 1) % 2], s_at + (j + 1) * 32);
-                masked(s[j % 2], j);
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_store32(o_at + j * 32, o);
+                    }
+                }
+                const float mc = m == -INFINITY ? 0.f : m * c;
+                Pair<float> sum[2] = {both(0.f), both(0.f)};
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) mx[e / 2 % 4] = max3(mx[e / 2 % 4], __uint_as_float(s[j % 2][e]), __uint_as_float(s[j % 2][e + 1]));
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t p[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        Pair<float> x = fma2({__uint_as_float(s[j][e]), __uint_as_float(s[j][e + 1])}, both(c), both(-mc));
+                        x = e % 16 < EMULATED ? ex2_poly(x) : Pair<float>{ex2(x.x), ex2(x.y)};
+                        sum[e / 2 % 2] = add2(sum[e / 2 % 2], x);
+                        p[e / 2] = pack2<T>(x.x, x.y);
+                    }
+                    // over columns 16 j .. 16 j + 15 of S, which have been read by now
+                    tmem_store16(s_at + j * 16, p);
+                }
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                tmem_wait_store();
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_ready[t]);           // one arrival a warp: arrivals on a barrier are served one by one
             }
-            tmem_load32(s[0], s_at);
-            const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
-            const bool raise = m == -INFINITY ? top > m : (top - m) * c > 8.f;
-            if (i == 0) {
-                m = top;
-            } else if (__any_sync(0xffffffffu, raise)) {
-                const float f = raise ? (m == -INFINITY ? 0.f : ex2((m - top) * c)) : 1.f;
-                if (raise) m = top;
-                l *= f;
+            if (ok && steps > 0) {
+                ok = mbar_wait_fast(&o_ready[t], 0, abort);
+                // a cluster's results go over the ring, which the other tile's products read too
+                if (world > 1 && live > 1) ok = ok && mbar_wait_fast(&o_ready[1 - t], 0, abort);
+                ok = __all_sync(0xffffffffu, ok);
+            }
+            tmem_fence_after();
+            if (world > 1) {
+                const int r = t * ROWS + (warp % 4) * 32 + lane;
+                if (!ok) l = NAN;
+                row_m[r] = m;
+                row_l[r] = l;
+                float4* mine = reinterpret_cast<float4*>(ring) + r * (DP / 4);
 #pragma unroll 1
                 for (int j = 0; j < DP / 32; ++j) {
                     uint32_t o[32];
-                    tmem_load32(o, o_at + j * 32);
-                    tmem_wait_load(o);
+                    if (steps > 0) {
+                        tmem_load32(o, o_at + j * 32);
+                        tmem_wait_load(o);
+                    }
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                    tmem_store32(o_at + j * 32, o);
+                    for (int e = 0; e < 8; ++e) {
+                        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (steps > 0)
+                            x = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
+                                            __uint_as_float(o[4 * e + 3]));
+                        mine[(j * 8 + e + r) % (DP / 4)] = x;          // rows turned against each other: one bank a lane
+                    }
                 }
-            }
-            const float mc = m == -INFINITY ? 0.f : m * c;
-            Pair<float> sum[2] = {both(0.f), both(0.f)};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                tmem_wait_load(s[j % 2]);
-                if (j < 3) tmem_load32(s[(j + 1) % 2], s_at + (j + 1) * 32);
-                masked(s[j % 2], j);
-                uint32_t p[16];
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    Pair<float> x = fma2({__uint_as_float(s[j % 2][e]), __uint_as_float(s[j % 2][e + 1])}, both(c), both(-mc));
-                    x = e % 16 < EMULATED ? ex2_poly(x) : Pair<float>{ex2(x.x), ex2(x.y)};
-                    sum[e / 2 % 2] = add2(sum[e / 2 % 2], x);
-                    p[e / 2] = pack2<T>(x.x, x.y);
-                }
-                // over columns 16 j .. 16 j + 15 of S, which have been read by now
-                tmem_store16(s_at + j * 16, p);
-            }
-            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-            tmem_wait_store();
-            tmem_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_ready[t]);           // one arrival a warp: arrivals on a barrier are served one by one
-        }
-        if (ok && steps > 0) {
-            ok = mbar_wait_fast(&o_ready[t], 0, abort);
-            // a cluster's results go over the ring, which the other tile's products read too
-            if (world > 1 && live > 1) ok = ok && mbar_wait_fast(&o_ready[1 - t], 0, abort);
-            ok = __all_sync(0xffffffffu, ok);
-        }
-        tmem_fence_after();
-        if (world > 1) {
-            const int r = t * ROWS + (warp % 4) * 32 + lane;
-            if (!ok) l = NAN;
-            row_m[r] = m;
-            row_l[r] = l;
-            float4* mine = reinterpret_cast<float4*>(ring) + r * (DP / 4);
+            } else {
+                const float f = !ok ? NAN : (n > 0 ? 1.f / l : 0.f);
+                T* out = out_at(row);
 #pragma unroll 1
-            for (int j = 0; j < DP / 32; ++j) {
-                uint32_t o[32];
-                if (steps > 0) {
-                    tmem_load32(o, o_at + j * 32);
-                    tmem_wait_load(o);
-                }
+                for (int j = 0; j < DP / 32; ++j) {
+                    uint32_t o[32];
+                    if (n > 0 && ok) {
+                        tmem_load32(o, o_at + j * 32);
+                        tmem_wait_load(o);
+                    } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (steps > 0)
-                        x = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
-                                        __uint_as_float(o[4 * e + 3]));
-                    mine[(j * 8 + e + r) % (DP / 4)] = x;          // rows turned against each other: one bank a lane
-                }
-            }
-        } else {
-            const float f = !ok ? NAN : (n > 0 ? 1.f / l : 0.f);
-            T* out = out_at(row);
-#pragma unroll 1
-            for (int j = 0; j < DP / 32; ++j) {
-                uint32_t o[32];
-                if (n > 0 && ok) {
-                    tmem_load32(o, o_at + j * 32);
-                    tmem_wait_load(o);
-                } else {
+                        for (int e = 0; e < 32; ++e) o[e] = 0;
+                    }
+                    if (row < rows) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0;
-                }
-                if (row < rows) {
+                        for (int e = 0; e < 32; e += 8) {
+                            if (j * 32 + e < a.D) {
+                                float x[8];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        if (j * 32 + e < a.D) {
-                            float x[8];
-#pragma unroll
-                            for (int u = 0; u < 8; ++u) x[u] = __uint_as_float(o[e + u]) * f;
-                            store8<T>(out + j * 32 + e, x);
+                                for (int u = 0; u < 8; ++u) x[u] = __uint_as_float(o[e + u]) * f;
+                                store8<T>(out + j * 32 + e, x);
+                            }
                         }
                     }
                 }
+                if (a.lse && row < rows)
+                    *lse_at(row) = !ok ? NAN : (n > 0 ? m * float(a.scale) + logf(l) : -INFINITY);
             }
-            if (a.lse && row < rows)
-                *lse_at(row) = !ok ? NAN : (n > 0 ? m * float(a.scale) + logf(l) : -INFINITY);
         }
     }
     if (world > 1) {
