@@ -124,7 +124,7 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
     unsigned char* base = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
     unsigned char* sq = base;
     unsigned char* ring = base + 2 * SM::TILE;
-    __shared__ uint64_t full[STAGES], empty[STAGES], q_full, s_ready[2], p_ready[2], o_ready[2], tail, drain;
+    __shared__ uint64_t full[STAGES], empty[STAGES], q_full, s_ready[2], p_ready[2][2], o_ready[2], tail, drain;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     __shared__ float row_m[2 * ROWS], row_l[2 * ROWS];             // clusters
@@ -156,7 +156,11 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
         mbar_init(&q_full, 1);
         mbar_init(&tail, 1);
         mbar_init(&drain, 1);
-        for (int t = 0; t < 2; ++t) { mbar_init(&s_ready[t], 1); mbar_init(&p_ready[t], 4); mbar_init(&o_ready[t], 1); }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&s_ready[t], 1);
+            mbar_init(&o_ready[t], 1);
+            for (int half = 0; half < 2; ++half) mbar_init(&p_ready[t][half], 4);
+        }
         mbar_init_fence();
     }
     if (warp == 8) tmem_alloc(&tmem_slot, 512);
@@ -241,13 +245,17 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
                     ok = warp_wait(&full[vi % STAGES], (vi / STAGES) & 1, abort);
                     if (ok && next) ok = warp_wait(&full[ki % STAGES], (ki / STAGES) & 1, abort);
                     for (int t = 0; t < live && ok; ++t) {
-                        ok = warp_wait(&p_ready[t], i & 1, abort);
-                        if (!ok) break;
-                        tmem_fence_after();
                         const uint32_t vd = desc_mn_major(r_addr + (vi % STAGES) * SM::TILE, SM::BOX);
 #pragma unroll
-                        for (int k = 0; k < ROWS / 16; ++k)
-                            mma_ts(leader, tmem + 256 + t * 128, tmem + t * 128 + k * 8, vd + k * (2048 >> 4), id_o, i > 0 || k > 0);
+                        for (int half = 0; half < 2; ++half) {         // the first half runs while the second's exponentials do
+                            ok = ok && warp_wait(&p_ready[t][half], i & 1, abort);
+                            if (!ok) break;
+                            tmem_fence_after();
+#pragma unroll
+                            for (int k = half * ROWS / 32; k < (half + 1) * ROWS / 32; ++k)
+                                mma_ts(leader, tmem + 256 + t * 128, tmem + t * 128 + k * 8, vd + k * (2048 >> 4), id_o, i > 0 || k > 0);
+                        }
+                        if (!ok) break;
                         // S of the next states goes over P of these: products issued by one thread run in order
                         if (next) scores(t, ki % STAGES);
                         else mma_commit(leader, &o_ready[t]);
@@ -329,12 +337,14 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
                     }
                     // over columns 16 j .. 16 j + 15 of S, which have been read by now
                     tmem_store16(s_at + j * 16, p);
+                    if (j % 2) {
+                        tmem_wait_store();
+                        tmem_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&p_ready[t][j / 2]);    // one arrival a warp: arrivals on a barrier are served one by one
+                    }
                 }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-                tmem_wait_store();
-                tmem_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_ready[t]);           // one arrival a warp: arrivals on a barrier are served one by one
             }
             if (ok && steps > 0) {
                 ok = mbar_wait_fast(&o_ready[t], 0, abort);
