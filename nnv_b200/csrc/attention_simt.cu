@@ -13,8 +13,10 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attention.cuh"
+#include "mma_f64.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -54,12 +56,21 @@ __device__ __forceinline__ Pack<A, VecOf<A>::N> lds(const A* p) {
 }
 
 // rows [r0, r0 + TILE) into s[TILE][DP + pad]; row r begins at(r) elements from g; rows at or past n_rows and columns past
-// D are zero
+// D are zero.  vec: rows of float and double arrive asynchronously
 template <typename T, typename A, int TILE, int DP, typename At>
 __device__ void load_tile(A* s, const T* g, At&& at, int r0, int n_rows, int D, bool vec) {
     constexpr int LD = DP + VecOf<A>::N;
     constexpr int V = 16 / sizeof(T);
-    if (vec) {
+    if (vec && std::is_same<T, A>::value) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < TILE * (DP / V); i += THREADS) {
+            const int r = i / (DP / V), c = i % (DP / V) * V;
+            const bool in = r0 + r < n_rows && c < D;
+            cp_async16(s + r * LD + c, g + (in ? at(r0 + r) + c : 0), in ? 16 : 0);
+        }
+        cp_async_commit();
+    } else if (vec) {
+#pragma unroll 4
         for (int i = threadIdx.x; i < TILE * (DP / V); i += THREADS) {
             const int r = i / (DP / V), c = i % (DP / V) * V;
             Pack<T, V> p;
@@ -237,6 +248,7 @@ attn_fwd_simt_kernel(AttnArgs a, bool vec) {
         __syncthreads();
         load_tile<T, A, TILE, DP>(Ks, k, [&](int r) { return r * a.ks[1]; }, k0, n, a.D, vec);
         load_tile<T, A, TILE, DP>(Vs, v, [&](int r) { return r * a.vs[1]; }, k0, n, a.D, vec);
+        cp_async_wait<0>();
         __syncthreads();
         A s[M][M] = {};
         mul_rows<A, TILE, DP>(s, Qs, Ks, a.D, rows.n - q0, n - k0, ty, tx);
@@ -267,6 +279,7 @@ attn_fwd_simt_kernel(AttnArgs a, bool vec) {
         __syncwarp();                     // a warp reads back only the rows its own threads wrote
         mul_cols<A, TILE, DP>(o, Ps, Vs, n - k0, ty, tx);
     }
+    cp_async_wait<0>();
     A f[M];
 #pragma unroll
     for (int i = 0; i < M; ++i) {
@@ -335,6 +348,7 @@ attn_dq_simt_kernel(AttnArgs a, bool vec) {
         __syncthreads();
         load_tile<T, A, TILE, DP>(Ks, k, [&](int r) { return r * a.ks[1]; }, k0, n, a.D, vec);
         load_tile<T, A, TILE, DP>(Vs, v, [&](int r) { return r * a.vs[1]; }, k0, n, a.D, vec);
+        cp_async_wait<0>();
         __syncthreads();
         A s[M][M] = {}, dp[M][M] = {};
         mul_rows<A, TILE, DP>(s, Qs, Ks, a.D, rows.n - q0, n - k0, ty, tx);
@@ -349,6 +363,7 @@ attn_dq_simt_kernel(AttnArgs a, bool vec) {
         __syncwarp();
         mul_cols<A, TILE, DP>(acc, Ps, Ks, n - k0, ty, tx);
     }
+    cp_async_wait<0>();
     T* dq = static_cast<T*>(a.dq);
     auto at = [&](int r) { return rows.dense(r); };
     if (world == 1) {
@@ -402,6 +417,7 @@ attn_dkv_simt_kernel(AttnArgs a, bool vec) {
             __syncthreads();
             load_tile<T, A, TILE, DP>(Qs, q, [&](int r) { return rows.at(a.qs, r); }, q0, rows.n, a.D, vec);
             load_tile<T, A, TILE, DP>(Gs, go, [&](int r) { return rows.at(a.dos, r); }, q0, rows.n, a.D, vec);
+            cp_async_wait<0>();
             __syncthreads();
             A s[M][M] = {}, dp[M][M] = {};
             mul_rows<A, TILE, DP>(s, Qs, Ks, a.D, rows.n - q0, n - k0, ty, tx);
@@ -423,6 +439,7 @@ attn_dkv_simt_kernel(AttnArgs a, bool vec) {
             mul_cols_t<A, TILE, DP>(dk, Ss, Qs, rows.n - q0, n - k0, ty, tx);
         }
     }
+    cp_async_wait<0>();
     const int64_t base = (int64_t(b) * a.Lk * a.Hkv + g) * a.D;
     auto at = [&](int r) { return int64_t(r) * a.Hkv * a.D; };
     if (world == 1) {
