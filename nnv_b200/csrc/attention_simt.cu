@@ -478,15 +478,15 @@ constexpr int bwd_tile(int dp) {
     return 16;
 }
 
-// `steps`: tiles a block walks over; where there are few blocks a cluster of up to 16 shares them, two each at least
+// `per_sm`: blocks an SM holds.  `steps`: tiles a block walks over; where there are few blocks a cluster of up to 16 shares them, two each at least
 template <typename K>
-int launch(K kernel, int64_t units, int64_t steps, int smem, cudaStream_t st, const AttnArgs& a, bool vec) {
+int launch(K kernel, int64_t units, int64_t steps, int smem, int per_sm, cudaStream_t st, const AttnArgs& a, bool vec) {
     if (units <= 0) return NNVB_OK;
     int dev = 0, sms = 148;
     NNVB_CUDA(cudaGetDevice(&dev));
     NNVB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     int world = 1;
-    while (world < 16 && units * world * 2 <= sms && world * 4 <= steps) world *= 2;
+    while (world < 16 && units * world * 2 <= int64_t(sms) * per_sm && world * 4 <= steps) world *= 2;
     NNVB_REQUIRE(units * world < (int64_t(1) << 31), "nnvb_cross_attention: too many tiles (%lld) for one launch", (long long)units);
     NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     if (world > 8) NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
@@ -517,20 +517,28 @@ int forward_t(cudaStream_t st, const AttnArgs& a) {
     const bool vec = a.D * sizeof(T) % 16 == 0 && rows16(a.q, a.qs, sizeof(T)) && rows16(a.k, a.ks, sizeof(T)) &&
                      rows16(a.v, a.vs, sizeof(T));
     return launch(attn_fwd_simt_kernel<T, TILE, DP>, ceil_div(int64_t(a.Lq) * (a.Hq / a.Hkv), TILE) * a.Hkv * a.B, 0,
-                  3 * tile_bytes<A>(TILE, DP) + score_bytes<A>(TILE), st, a, vec);
+                  3 * tile_bytes<A>(TILE, DP) + score_bytes<A>(TILE), 1, st, a, vec);
+}
+
+template <typename T, int DP, int TILE>
+int backward_tiles(cudaStream_t st, const AttnArgs& a) {
+    using A = typename AccOf<T>::type;
+    const bool vec = a.D * sizeof(T) % 16 == 0 && rows16(a.q, a.qs, sizeof(T)) && rows16(a.k, a.ks, sizeof(T)) &&
+                     rows16(a.v, a.vs, sizeof(T)) && rows16(a.dout, a.dos, sizeof(T));
+    constexpr int SMEM = 4 * tile_bytes<A>(TILE, DP) + 2 * score_bytes<A>(TILE), PER_SM = SMEM <= SMEM_MAX / 2 ? 2 : 1;
+    const int64_t tq = ceil_div(int64_t(a.Lq) * (a.Hq / a.Hkv), TILE), tk = ceil_div(a.Lk, TILE), heads = int64_t(a.Hkv) * a.B;
+    NNVB_TRY(launch(attn_dq_simt_kernel<T, TILE, DP>, tq * heads, tk, SMEM, PER_SM, st, a, vec));
+    return launch(attn_dkv_simt_kernel<T, TILE, DP>, tk * heads, tq, SMEM, PER_SM, st, a, vec);
 }
 
 template <typename T, int DP>
 int backward_t(cudaStream_t st, const AttnArgs& a) {
-    using A = typename AccOf<T>::type;
-    constexpr int TILE = bwd_tile<A>(DP);
-    const bool vec = a.D * sizeof(T) % 16 == 0 && rows16(a.q, a.qs, sizeof(T)) && rows16(a.k, a.ks, sizeof(T)) &&
-                     rows16(a.v, a.vs, sizeof(T)) && rows16(a.dout, a.dos, sizeof(T));
-    const int smem = 4 * tile_bytes<A>(TILE, DP) + 2 * score_bytes<A>(TILE);
-    NNVB_TRY(launch(attn_dq_simt_kernel<T, TILE, DP>, ceil_div(int64_t(a.Lq) * (a.Hq / a.Hkv), TILE) * a.Hkv * a.B, ceil_div(a.Lk, TILE), smem, st,
-                    a, vec));
-    return launch(attn_dkv_simt_kernel<T, TILE, DP>, ceil_div(a.Lk, TILE) * a.Hkv * a.B,
-                  ceil_div(int64_t(a.Lq) * (a.Hq / a.Hkv), TILE), smem, st, a, vec);
+    constexpr int TILE = bwd_tile<typename AccOf<T>::type>(DP);
+    if constexpr (TILE > 32 && sizeof(T) >= 4) {
+        const int64_t rows = int64_t(a.Lq) * (a.Hq / a.Hkv);
+        if (std::min<int64_t>(a.Lk, rows) <= 32) return backward_tiles<T, DP, 32>(st, a);
+    }
+    return backward_tiles<T, DP, TILE>(st, a);
 }
 
 template <typename T>
