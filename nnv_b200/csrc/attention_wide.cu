@@ -71,9 +71,9 @@ struct Work<double, DP, BK_> {
             for (int e = 0; e < 4; ++e) o[i][e] = 0;
     }
     __device__ __forceinline__ int row(int i) const { return warp * 16 + g + i * 8; }
-    // rest: states of the tile that count; 8-state tiles behind them are left out
+    // rest: states of the tile that count; 8-state tiles behind them are left out, and channels from D on
     template <int LDY = S::LDK>
-    __device__ __forceinline__ void scores(const double* Q, const double* K, int rest) {
+    __device__ __forceinline__ void scores(const double* Q, const double* K, int rest, int D) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -82,6 +82,7 @@ struct Work<double, DP, BK_> {
         const double* k = K + g * LDY + 2 * t;
 #pragma unroll 4
         for (int d = 0; d < DP; d += 8) {
+            if (d >= D) break;
             const double2 x = *reinterpret_cast<const double2*>(q + d), y = *reinterpret_cast<const double2*>(q + 8 * S::LDQ + d);
             const double a[4] = {x.x, y.x, x.y, y.y};
 #pragma unroll
@@ -117,7 +118,7 @@ struct Work<double, DP, BK_> {
             for (int e = 0; e < 4; ++e) o[i][e] *= f[e / 2];
     }
     __device__ __forceinline__ void hand_over(double*) {}          // the weights stay in their registers
-    __device__ __forceinline__ void weigh(const double*, const double* V, int rest) {
+    __device__ __forceinline__ void weigh(const double*, const double* V, int rest, int D) {
         const double* v = V + 2 * t * S::LDV + 2 * g;
 #pragma unroll
         for (int k = 0; k < NT; ++k) {
@@ -125,6 +126,7 @@ struct Work<double, DP, BK_> {
             const double a[4] = {s[k][0], s[k][2], s[k][1], s[k][3]};
 #pragma unroll
             for (int j = 0; j < DP / 16; ++j) {
+                if (j * 16 >= D) break;
                 const double2 x = *reinterpret_cast<const double2*>(v + k * 8 * S::LDV + j * 16);
                 const double2 y = *reinterpret_cast<const double2*>(v + (k * 8 + 1) * S::LDV + j * 16);
                 const double b0[2] = {x.x, y.x}, b1[2] = {x.y, y.y};
@@ -160,7 +162,7 @@ struct Work<float, DP, BK_> {
     }
     __device__ __forceinline__ int row(int i) const { return ty * NR + i; }
     template <int LDY = S::LDK>
-    __device__ __forceinline__ void scores(const float* Q, const float* K, int) {
+    __device__ __forceinline__ void scores(const float* Q, const float* K, int, int D) {
         Pair<float> acc[NR][4];
 #pragma unroll
         for (int i = 0; i < NR; ++i)
@@ -169,6 +171,7 @@ struct Work<float, DP, BK_> {
         const float *q = Q + ty * NR * S::LDQ, *k = K + tx * LDY;
 #pragma unroll 2
         for (int d = 0; d < DP; d += 4) {
+            if (d >= D) break;
             float4 y[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(k + 16 * j * LDY + d);
@@ -215,7 +218,7 @@ struct Work<float, DP, BK_> {
             for (int j = 0; j < 4; ++j) P[row(i) * S::LDP + tx + 16 * j] = s[i][j];
         __syncwarp();                      // a row's weights are read by the warp that wrote them
     }
-    __device__ __forceinline__ void weigh(const float* P, const float* V, int rest) {
+    __device__ __forceinline__ void weigh(const float* P, const float* V, int rest, int) {
         const float *p = P + ty * NR * S::LDP, *v = V + tx * 4;
 #pragma unroll 1
         for (int k = 0; k < S::BK && k < rest; k += 4) {
@@ -288,7 +291,7 @@ attn_fwd_wide_kernel(AttnArgs a, bool vec) {
         load_rows<T, S::BK, DP, S::LDV>(Vs, v, v_at, k0, n, a.D, vec);
         cp_async_wait<1>();
         __syncthreads();
-        w.scores(Qs, Ks, n - k0);
+        w.scores(Qs, Ks, n - k0, a.D);
         __syncthreads();
         if (it + world < steps) load_rows<T, S::BK, DP, S::LDK>(Ks, k, k_at, (it + world) * S::BK, n, a.D, vec);
         else cp_async_commit();
@@ -323,7 +326,7 @@ attn_fwd_wide_kernel(AttnArgs a, bool vec) {
         w.hand_over(Ps);
         cp_async_wait<1>();
         __syncthreads();
-        w.weigh(Ps, Vs, rest);
+        w.weigh(Ps, Vs, rest, a.D);
         __syncthreads();
     }
     cp_async_wait<0>();
@@ -471,8 +474,8 @@ attn_bwd_wide_kernel(AttnArgs a, bool vec) {
             }
         cp_async_wait<0>();
         __syncthreads();
-        if (busy) x.template scores<S::LDV>(A0, B0, rest);
-        if (WHICH != ONLY_V && busy) y.template scores<S::LDV>(A1, B1, rest);
+        if (busy) x.template scores<S::LDV>(A0, B0, rest, a.D);
+        if (WHICH != ONLY_V && busy) y.template scores<S::LDV>(A1, B1, rest, a.D);
         if (!KV) {
             __syncthreads();
             load1(it + world);
@@ -484,7 +487,7 @@ attn_bwd_wide_kernel(AttnArgs a, bool vec) {
         });
         if (KV && WHICH != ONLY_K && busy) {
             x.hand_over(Ps);
-            x.weigh(Ps, B1, rest);
+            x.weigh(Ps, B1, rest, a.D);
         }
         if (KV) {
             __syncthreads();
@@ -492,7 +495,7 @@ attn_bwd_wide_kernel(AttnArgs a, bool vec) {
         }
         if (WHICH != ONLY_V && busy) {
             y.hand_over(Ps);
-            y.weigh(Ps, B0, rest);
+            y.weigh(Ps, B0, rest, a.D);
         }
         __syncthreads();
         load0(it + world);
