@@ -117,14 +117,14 @@ int nnvb_cross_attention_backward(void* stream, const nnvb_attention_desc* d, co
     if (attn_tc_takes_backward(a)) return attn_backward_tc(st, a);
     NNVB_TRY(attn_delta(st, a));
     // Large problems have the wide kernels' throughput (8 x 512 x 1024 x 8 x 64 double: 1.5 against 2.5 ms; 8 x 1024 x 2048 x 16 x
-    // 64 float: 6.3 against 7.4 ms).  Where one side is short, or with fewer tiles than SMs, the blocks of twice as many
-    // threads on smaller tiles are the faster ones (2 x 3582 x 8 x 8 x 4 x 64 double: 0.79 against 0.94 ms); of heads with more
-    // than 64 channels, whose wide kernels have a block an SM, with few tiles on either side (2 x 562 x 2855 x 2 x 128 float:
-    // 0.80 against 0.96 ms with larger tiles).
+    // 64 float: 6.3 against 7.4 ms).  Where one side is short, or tiles are fewer than the SMs need, the blocks of twice as many
+    // threads on smaller tiles are the faster ones (2 x 3582 x 8 x 8 x 4 x 64 double: 0.79 against 0.94 ms).  More than 64
+    // float channels leave a wide block alone on its SM: there both of its kernels need the tiles (4 x 148 x 677 x 12 x 96
+    // float, 144 and 528 tiles: 342 wide, 377 us not; 2 x 127 x 198 x 16 x 2 x 80 double: 352 and 435).
     const int64_t heads = int64_t(a.B) * a.Hkv, rows = int64_t(a.Lq) * (a.Hq / a.Hkv);
     const int64_t tq = ceil_div(rows, 64) * heads, tk = ceil_div(a.Lk, 64) * heads;
     const bool wide = (a.dtype == NNVB_F64 || a.dtype == NNVB_F32) && a.D <= 128 && std::min<int64_t>(rows, a.Lk) > 32 &&
-                      (a.D <= 64 ? std::max(tq, tk) : std::min(tq, tk)) >= 148;
+                      (a.D <= 64 || a.dtype == NNVB_F64 ? std::max(tq, tk) : std::min(tq, tk)) >= 100;
     return wide ? attn_backward_wide(st, a) : attn_backward_simt(st, a);
 }
 
