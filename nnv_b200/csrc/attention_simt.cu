@@ -1,5 +1,6 @@
-// Attention over an encoder's states on the CUDA cores: double and float tensors, and the 16-bit layouts the
-// tensor-core kernels do not take (head sizes over 128, rows that are not 16-byte aligned).
+// Attention over an encoder's states on the CUDA cores: the layouts the tensor-core kernels do not
+// take (16-bit rows that are not 16-byte aligned, heads of more than 128 channels in any type), and the backward pass
+// of small or one-sided problems in float and double.
 //
 //   forward   one pass over the states with the running maximum m and sum l of each row's softmax:
 //             m' = max(m, max_j S_j), p_j = exp(S_j - m'), l' = l exp(m - m') + sum p_j, O' = O exp(m - m') + p V
@@ -9,7 +10,10 @@
 //
 // A block of 256 threads holds TILE x TILE scores, 16 x 16 threads with (TILE/16)^2 scores each, operands in shared
 // memory in the type sums are held in, rows padded by 16 bytes so that the 16-byte loads of neighbouring rows
-// fall on different banks.  Bound by the FMA pipe: a 4 x 4 register tile needs 8 16-byte loads for 64 FMAs.
+// fall on different banks.  With 64 rows a 4 x 4 register tile needs 8 16-byte loads for 64 FMAs.
+// Problems with a short side are bound by the latency of a step (load, products, exponentials, products; a short side also
+// leaves warps of the products over it idle), so two blocks share an SM: 18 x 1618 x 8 x 2 x 2 x 128 float 392 us, 2 x 3178 x
+// 19 x 2 x 4 x 96 double 681 us.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -523,16 +527,24 @@ int forward_t(cudaStream_t st, const AttnArgs& a) {
                   3 * tile_bytes<A>(TILE, DP) + score_bytes<A>(TILE), 1, st, a, vec);
 }
 
-template <typename T, int DP>
-int backward_t(cudaStream_t st, const AttnArgs& a) {
+template <typename T, int DP, int TILE>
+int backward_tiles(cudaStream_t st, const AttnArgs& a) {
     using A = typename AccOf<T>::type;
     const bool vec = a.D * sizeof(T) % 16 == 0 && rows16(a.q, a.qs, sizeof(T)) && rows16(a.k, a.ks, sizeof(T)) &&
                      rows16(a.v, a.vs, sizeof(T)) && rows16(a.dout, a.dos, sizeof(T));
-    constexpr int TILE = bwd_tile<T>(DP);
     constexpr int SMEM = 4 * tile_bytes<A>(TILE, DP) + 2 * score_bytes<A>(TILE), PER_SM = SMEM <= SMEM_MAX / 2 ? 2 : 1;
     const int64_t tq = ceil_div(int64_t(a.Lq) * (a.Hq / a.Hkv), TILE), tk = ceil_div(a.Lk, TILE), heads = int64_t(a.Hkv) * a.B;
     NNVB_TRY(launch(attn_dq_simt_kernel<T, TILE, DP>, tq * heads, tk, SMEM, PER_SM, st, a, vec));
     return launch(attn_dkv_simt_kernel<T, TILE, DP>, tk * heads, tq, SMEM, PER_SM, st, a, vec);
+}
+
+// 128 double channels leave room for two blocks with 16 rows, which suits a side no longer (13 x 239 x 13 x 16 x 2 x 96: 716 us
+// with 32 rows, 524 with 16; 14 x 1686 x 21 x 2 x 128: 373 and 527)
+template <typename T, int DP>
+int backward_t(cudaStream_t st, const AttnArgs& a) {
+    if constexpr (sizeof(T) == 8 && DP == 128)
+        if (std::min<int64_t>(a.Lk, int64_t(a.Lq) * (a.Hq / a.Hkv)) <= 16) return backward_tiles<T, DP, 16>(st, a);
+    return backward_tiles<T, DP, bwd_tile<T>(DP)>(st, a);
 }
 
 template <typename T>

@@ -1,7 +1,7 @@
 // Attention over an encoder's states on the tensor cores: bf16 and fp16 tensors with head sizes up to 128 whose rows
 // TMA can read (16-byte aligned, sizes a multiple of 8).
 //
-// Forward.  A block of ten warps takes 256 positions of one head as two tiles of 128 rows and walks over the states in
+// Forward.  A block of twelve warps takes 256 positions of one head as two tiles of 128 rows and walks over the states in
 // tiles of 128.  Warp 9 copies Q once and the K and V tiles through a ring of shared-memory stages (TMA); warp 8
 // issues the products: S = Q K^T into tensor memory, then O += P V with P read from tensor memory and O kept there.
 // Warps 0-3 and 4-7 hold one row of a tile per thread: read S, take the row's maximum, write P = exp2(c S - c m) over
@@ -15,6 +15,12 @@
 // 2^8 over the m in use, so weights stay below 2^8, which 16-bit P and fp32 sums hold without loss; after the first
 // tiles the rescale is rare.  P is rounded to the tensors' type because the product takes 16-bit operands; its
 // row sum is added in fp32 before the rounding.
+//
+// Bound by the products at long lengths: Q K^T reads both operands from shared memory, 8 KB for each 64 cycles of the
+// tensor pipe, all that shared memory delivers.  8 x 2048 x 4096 x 16 x 128 bf16: 509 us, 1.08 PFLOP/s.
+//
+// A block takes an SM's registers whole (the backward kernels 55 of 64 K), so no other block of this kind waits for its
+// tensor memory while it waits for the rest of its cluster.
 //
 // Every wait is bounded (about 0.2 s): a block whose hand-over breaks stops issuing, waits for its own copies and products
 // to end, frees its tensor memory and writes its rows as NaN.
@@ -32,8 +38,9 @@ namespace {
 
 constexpr int ROWS = 128;                          // rows of a tile of positions, states of a tile
 constexpr int FWD_THREADS = 384;
-constexpr int EMULATED = 4;                        // of 16 exponentials run on the FMA pipe (0: 460 us, 4: 459, 6: 474 at
-                                                   // 8 x 2048 x 4096 x 16 x 128; 416, 387, 407 with 64 channels)
+constexpr int EMULATED = 4;                        // of 16 exponentials run on the FMA pipe (0: 44.7 us, 2: 43.5, 4: 42.7,
+                                                   // 6: 45.9 at 8 x 1024 x 1024 x 8 x 128; 511, 509, 509, 520 at
+                                                   // 8 x 2048 x 4096 x 16 x 128, where the products bound)
 
 template <typename T> constexpr bool is_bf16 = false;
 template <> constexpr bool is_bf16<__nv_bfloat16> = true;

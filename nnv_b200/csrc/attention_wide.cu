@@ -557,6 +557,10 @@ int launch_wide(K kernel, int64_t units, int64_t steps, int per_sm, int smem, cu
     NNVB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     int world = 1;
     while (world < 16 && units * world * 2 <= int64_t(sms) * per_sm && world * 4 <= steps) world *= 2;
+    // or where the last blocks would leave many SMs idle: the longest sum of an SM's blocks counts
+    auto longest = [&](int w) { return double(ceil_div(units * w, sms)) / w; };
+    for (int w = 2; world == 1 && w <= 4 && w * 4 <= steps; w *= 2)
+        if (longest(w) < 0.9 * longest(1)) world = w;
     NNVB_REQUIRE(units * world < (int64_t(1) << 31), "nnvb_cross_attention: too many tiles (%lld) for one launch", (long long)units);
     NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     if (world > 8) NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
