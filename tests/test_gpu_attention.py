@@ -272,6 +272,56 @@ def test_on_another_stream_and_captured(t):
         assert torch.equal(o, out) and torch.equal(s, step) and all(torch.equal(a, b) for a, b in zip(g, ref))
 
 
+@pytest.mark.parametrize("t", [torch.float64, torch.float32])
+@pytest.mark.parametrize("D", [40, 64, 96, 128])
+@pytest.mark.parametrize("Lq,Lk", [(300, 8), (300, 16), (150, 17), (150, 32), (150, 33), (10, 700), (17, 700), (33, 700)])
+def test_one_short_side_in_single_and_double(t, D, Lq, Lk):
+    q, k, v, dout = _data(t, 3, Lq, Lk, 2, 1, D)
+    _check(t, q, k, v, dout, _lens([Lk, Lk // 2, 0]))
+
+
+@pytest.mark.parametrize("t", [torch.float64, torch.float32])
+@pytest.mark.parametrize("Lq,Lk", [(40, 600), (600, 40)])
+def test_tiles_split_where_blocks_do_not_come_out_even(t, Lq, Lk):
+    q, k, v, dout = _data(t, 10, Lq, Lk, 16, 16, 64)
+    _check(t, q, k, v, dout, _lens([Lk, 0, 1, Lk - 1, 65, 64, 63, 17, Lk, 5]) if Lk > 64 else None)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("Lq,Lk,D", [(1, 40, 64), (24, 40, 64), (24, 40, 136)])
+def test_offsets_past_32_bits(t, Lq, Lk, D):
+    """Tokens so far apart that the last one begins more than 2^31 elements behind the first, in every operand."""
+    q, k, v, dout = _data(t, 1, Lq, Lk, 2, 2, D)
+    step = (1 << 31) // (Lk - 4) // 64 * 64
+    far = torch.empty(step * Lk, dtype=t, device="cuda")
+    views = [far.as_strided((1, n, 2, D), (step * Lk, step, D, 1), i * 1024) for i, n in enumerate((Lk, Lk, Lq, Lq))]
+    for a, b in zip(views, (k, v, q, dout)):
+        a.copy_(b)
+    assert step * (Lk - 1) > 1 << 31
+    _check(t, views[2], views[0], views[1], views[3], None)
+
+
+def test_two_streams_at_once():
+    from nnv_b200 import ops
+    sets = [_data(torch.bfloat16, 1, 300, 2000, 2, 2, 128), _data(torch.float16, 1, 500, 1500, 4, 1, 64),
+            _data(torch.float32, 1, 100, 900, 2, 2, 64)]
+
+    def work(q, k, v, dout):
+        out, lse = ops.cross_attention(q, k, v, return_lse=True)
+        return (out, ops.cross_attention(q[:, :1], k, v), *ops.cross_attention_backward(dout, q, k, v, out, lse))
+    want = [work(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for _ in range(5):
+        for s, st in zip(sets, streams):
+            with torch.cuda.stream(st):
+                got.append(work(*s))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % len(sets)]))
+
+
 def test_shapes_that_do_not_fit_are_refused():
     from nnv_b200 import ops
     q, k, v, dout = _data(torch.bfloat16, 2, 3, 4, 4, 2, 16)

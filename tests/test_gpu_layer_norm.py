@@ -93,6 +93,24 @@ def test_strided_and_misaligned_rows(cut):
     R.check("y", ops.layer_norm(z), want, tol)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,cols", [(20, 256), (600, 72)])
+def test_rows_past_32_bits(t, rows, cols):
+    """Rows so far apart that the last one begins more than 2^31 elements behind the first."""
+    from nnv_b200 import ops
+    x, dy = _rows(t, rows, cols), _rows(t, rows, cols, 2, 0.0)
+    s, o = _weights(t, cols)
+    step = (1 << 31) // (rows - 3) // 64 * 64
+    far = torch.empty(step * rows, dtype=t, device="cuda")
+    xf, df = (far.as_strided((rows, cols), (step, 1), i * 1024) for i in range(2))
+    xf.copy_(x)
+    df.copy_(dy)
+    y, mean, rstd = ops.layer_norm(xf, s, o, 1e-5, return_stats=True)
+    assert torch.equal(y, ops.layer_norm(x, s, o, 1e-5))
+    assert all(torch.equal(a, b) for a, b in zip(ops.layer_norm_backward(df, xf, s, mean, rstd),
+                                                 ops.layer_norm_backward(dy, x, s, mean, rstd)))
+
+
 def test_large_mean_keeps_the_variance():
     from nnv_b200 import ops
     x = _rows(torch.float32, 9, 1000, mean=1e4)
