@@ -17,6 +17,7 @@ struct AttnArgs {
     double scale;
     int B, Lq, Lk, Hq, Hkv, D;
     int dtype;
+    int longest_first;             // few rows: batch entries in the order of their lengths
 };
 
 // valid states of batch entry b

@@ -301,6 +301,17 @@ def test_offsets_past_32_bits(t, Lq, Lk, D):
     _check(t, views[2], views[0], views[1], views[3], None)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("B,Lk", [(70, 1150), (128, 2100), (129, 300)])
+def test_large_batches_of_single_positions(t, B, Lk):
+    q, k, v, dout = _data(t, B, 1, Lk, 8, 8, 16)
+    g = torch.Generator().manual_seed(5)
+    lengths = torch.randint(0, Lk + 1, (B,), generator=g).tolist()
+    lengths[:6] = [0, 0, Lk, Lk, 77, 77]
+    out, _ = _check(t, q, k, v, dout, _lens(lengths), backward=False)
+    assert torch.equal(out[:2], torch.zeros_like(out[:2]))
+
+
 def test_two_streams_at_once():
     from nnv_b200 import ops
     sets = [_data(torch.bfloat16, 1, 300, 2000, 2, 2, 128), _data(torch.float16, 1, 500, 1500, 4, 1, 64),
