@@ -84,7 +84,10 @@ int nnvb_cross_attention_forward(void* stream, const nnvb_attention_desc* d, con
 int64_t nnvb_cross_attention_workspace(const nnvb_attention_desc* d) {
     if (!d || d->batch < 0 || d->q_len < 0 || d->q_heads < 0) return 0;
     // delta, and for the tensor cores the log-sum-exp beside it, in rows padded to a tile
-    return d->batch * d->q_heads * round_up(d->q_len, 64) * 8;
+    const int64_t rows = d->batch * d->q_heads * round_up(d->q_len, 64), stats = rows * 8;
+    if (d->dtype != NNVB_F16 || d->kv_heads < 0 || d->kv_len < 0) return stats;
+    // the norms that bound dS: of dO's rows and of V's states, one of 16
+    return stats + round_up((rows / 16 + d->batch * d->kv_heads * ceil_div(d->kv_len, 16)) * 4, 16);
 }
 
 int nnvb_cross_attention_backward(void* stream, const nnvb_attention_desc* d, const void* dout, const void* q,

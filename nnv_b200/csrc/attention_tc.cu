@@ -460,6 +460,10 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
 // arithmetic: two warpgroups per tile in flight, one row and half of its 64 columns per thread (with one warpgroup per
 // tile the products waited for it: a quarter of the tensor pipe's cycles were used).
 //
+// fp16 holds 2^-24 to 65504, dS anything from the product of two small gradients up to |dP| of large ones: it is lifted by a
+// power of two that its bound |dS| <= 2 max |dO_i| max |v_j| (Euclidean norms, P <= 1) puts below 2^15, and the gradient is
+// divided by it again.  With two terms that leaves 2^-40 of the bound.  dQ takes the norm of 16 of its rows of dO, dK of all.
+//
 // Roundings: P is rounded to the tensors' type, as in the forward pass.  dS enters its product as the sum of two
 // 16-bit values (its rounding and the rounding of what is left), an eighth and a ninth product: its rounding error
 // would be as large as that of storing dQ and dK, and the terms of dS cancel in their row sums.  delta comes from the
@@ -483,24 +487,54 @@ struct BwdMaps {
     CUtensorMap a0, a1, b0, b1;
 };
 
-// stats: [B, groups of heads, RowsP] lse' then the same of delta, a group's rows rounded up to 64: those behind hold +inf and 0
+// The largest squared norm among the 16 rows of a block, 16 lanes a row.
+__device__ __forceinline__ void block_largest(float s, float* to) {
+    __shared__ float part[8];
+    for (int w = 8; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w, 32);
+    s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, 16, 32));
+    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 8; ++w) s = fmaxf(s, part[w]);
+        *to = s;
+    }
+}
+
+// stats: [B, groups of heads, RowsP] lse' then the same of delta, a group's rows rounded up to 64: those behind hold +inf and 0.
+// fp16: then the largest squared norm of dO of every 16 rows, and of V of every 16 states (blocks from row_blocks on).
 template <typename T>
 __global__ void __launch_bounds__(256)
-attn_stats_tc_kernel(AttnArgs a, int RowsP, int gs) {
+attn_stats_tc_kernel(AttnArgs a, int RowsP, int gs, unsigned row_blocks) {
     const int lane = threadIdx.x % 16;
-    const int64_t i = int64_t(blockIdx.x) * 16 + threadIdx.x / 16;
     const int groups = a.Hq >> gs;
     const int64_t count = int64_t(a.B) * groups * RowsP;
+    if (!is_bf16<T> && blockIdx.x >= row_blocks) {
+        const int chunks = (a.Lk + 15) / 16, at = int(blockIdx.x - row_blocks);
+        const int j = at % chunks * 16 + threadIdx.x / 16, g = at / chunks % a.Hkv, b = at / chunks / a.Hkv;
+        float s = 0.f;
+        if (j < attn_len(a, b) && lane * 8 < a.D) {
+            const auto v = *reinterpret_cast<const Pack<T, 8>*>(static_cast<const T*>(a.v) + b * a.vs[0] + j * a.vs[1] + g * a.vs[2] + lane * 8);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s += to_acc(v.v[e]) * to_acc(v.v[e]);
+        }
+        block_largest(s, static_cast<float*>(a.delta) + 2 * count + count / 16 + at);
+        return;
+    }
+    const int64_t i = int64_t(blockIdx.x) * 16 + threadIdx.x / 16;
     const int row = int(i % RowsP), b = int(i / RowsP / groups);
     const int h = (int(i / RowsP % groups) << gs) + (row & ((1 << gs) - 1)), r = row >> gs;
     const bool live = i < count && r < a.Lq;
-    float s = 0.f;
+    float s = 0.f, norm = 0.f;
     if (live && lane * 8 < a.D) {
         const auto o = *reinterpret_cast<const Pack<T, 8>*>(static_cast<const T*>(a.o) + b * a.os[0] + r * a.os[1] + h * a.os[2] + lane * 8);
         const auto d = *reinterpret_cast<const Pack<T, 8>*>(static_cast<const T*>(a.dout) + b * a.dos[0] + r * a.dos[1] + h * a.dos[2] + lane * 8);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s += to_acc(o.v[e]) * to_acc(d.v[e]);
+        for (int e = 0; e < 8; ++e) {
+            s += to_acc(o.v[e]) * to_acc(d.v[e]);
+            norm += to_acc(d.v[e]) * to_acc(d.v[e]);
+        }
     }
+    if (!is_bf16<T>) block_largest(norm, static_cast<float*>(a.delta) + 2 * count + blockIdx.x);
     for (int w = 8; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w, 32);
     if (i < count && lane == 0) {
         float* st = static_cast<float*>(a.delta);
@@ -509,11 +543,20 @@ attn_stats_tc_kernel(AttnArgs a, int RowsP, int gs) {
     }
 }
 
+// The power of two that lifts values of at most `bound` to below 2^15, and its inverse.
+__device__ __forceinline__ void ds_factor(float bound, float* up, float* down) {
+    if (!(bound > 0.f && bound < INFINITY)) return;          // nothing to lift, or results that are not finite anyway
+    const int e = (__float_as_int(bound) >> 23) - 127;       // a bound of fp16 norms: 2^-48 .. 2^42
+    *up = __int_as_float((127 + 14 - e) << 23);
+    *down = __int_as_float((127 - 14 + e) << 23);
+}
+
 template <typename T, int DP, bool KV>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
 attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, int gs) {
     using SM = BwdSmem<DP>;
     constexpr int STAGES = SM::STAGES;
+    constexpr bool SCALED = !is_bf16<T>;
     extern __shared__ unsigned char raw[];
     unsigned char* base = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
     unsigned char* res = base;                             // A0, A1
@@ -523,6 +566,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     __shared__ float row_sum[4][ROWS];
+    __shared__ float norms[2][BWD_THREADS / 32];
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     // rows and heads (dQ: groups of 2^gs) of this pass
@@ -555,6 +599,24 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
         mbar_init_fence();
     }
     if (warp == 16) tmem_alloc(&tmem_slot, 512);
+    if (SCALED) {                          // the largest squared norms of V's valid states and (dK) of dO's rows
+        const float* of_do = static_cast<const float*>(a.delta) + 2 * int64_t(a.B) * groups * RowsP;
+        const float* of_v = of_do + int64_t(a.B) * groups * (RowsP / 16);
+        const int chunks = (a.Lk + 15) / 16;
+        float x[2] = {0.f, 0.f};
+        if (steps > 0) {
+            of_v += (int64_t(b) * a.Hkv + (KV ? oh : oh / G)) * chunks;
+            for (int i = threadIdx.x; i < (n + 15) / 16; i += BWD_THREADS) x[0] = fmaxf(x[0], of_v[i]);
+            if (KV) {
+                of_do += (int64_t(b) * groups + oh * G) * (RowsP / 16);
+                for (int64_t i = threadIdx.x; i < int64_t(G) * (RowsP / 16); i += BWD_THREADS) x[1] = fmaxf(x[1], of_do[i]);
+            }
+        }
+        for (int w = 16; w > 0; w >>= 1)
+            for (int i = 0; i < 2; ++i) x[i] = fmaxf(x[i], __shfl_xor_sync(0xffffffffu, x[i], w, 32));
+        if (lane == 0)
+            for (int i = 0; i < 2; ++i) norms[i][warp] = x[i];
+    }
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
@@ -692,6 +754,16 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
             my_lse = st_lse[my_at];
             my_delta = st_delta[my_at];
         }
+        float up = 1.f, down = 1.f;        // fp16: what dS is multiplied with, and the inverse
+        if (SCALED) {
+            float of_v = 0.f, of_do = 0.f;
+            for (int w = 0; w < BWD_THREADS / 32; ++w) {
+                of_v = fmaxf(of_v, norms[0][w]);
+                of_do = fmaxf(of_do, norms[1][w]);
+            }
+            if (!KV && row < rows) of_do = st_delta[int64_t(a.B) * groups * RowsP + my_at / 16];
+            ds_factor(2.f * sqrtf(of_v * of_do), &up, &down);
+        }
         bool ok = true;
         for (int j = t; j < steps; j += 2) {
             ok = mbar_wait_fast(&full[j % STAGES], (j / STAGES) & 1, abort) &&
@@ -740,7 +812,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
                     const int col = g * 16 + e;
                     const Pair<float> dl = KV ? *reinterpret_cast<const Pair<float>*>(sl + BROWS + col) : both(my_delta);
                     const Pair<float> pv{__uint_as_float(s[col]), __uint_as_float(s[col + 1])};
-                    Pair<float> ds = mul2(pv, add2(Pair<float>{__uint_as_float(d[e]), __uint_as_float(d[e + 1])}, Pair<float>{-dl.x, -dl.y}));
+                    Pair<float> ds = mul2(SCALED ? mul2(pv, both(up)) : pv, add2(Pair<float>{__uint_as_float(d[e]), __uint_as_float(d[e + 1])}, Pair<float>{-dl.x, -dl.y}));
                     if (!KV && col >= rest) ds.x = 0.f;                    // dP there may be 0 * NaN
                     if (!KV && col + 1 >= rest) ds.y = 0.f;
                     if (KV) p[e / 2] = pack2<T>(pv.x * P_SCALE, pv.y * P_SCALE);
@@ -762,7 +834,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
         // dK: warpgroups 0 and 1, dV: 2 and 3, half of the columns each; dQ: every warpgroup a chunk of 32
         const bool value = KV && t == 1;
         const bool dead = KV && row >= n;                  // states without weight: their rows of S may hold anything
-        const float f = !ok ? NAN : (value ? 1.f / P_SCALE : float(a.scale));
+        const float f = !ok ? NAN : (value ? 1.f / P_SCALE : float(a.scale) * down);
         T* out = static_cast<T*>(KV ? (value ? a.dv : a.dk) : a.dq) + grad_at(row);
         const uint32_t o_at = lanes + 256 + (value ? 128 : 0);
         float4* mine = reinterpret_cast<float4*>(base) + ((value ? ROWS : 0) + local) * (DP / 4);
@@ -927,8 +999,9 @@ int backward_t(cudaStream_t st, const AttnArgs& a) {
     const int gs = pack_shift(a, true);
     const int64_t rows = int64_t(a.Lq) << gs, groups = a.Hq >> gs, RowsP = round_up(rows, BROWS);
     const int64_t count = RowsP * a.B * groups;
-    NNVB_REQUIRE(ceil_div(count, 16) < (int64_t(1) << 31), "nnvb_cross_attention_backward: too many rows (%lld)", (long long)count);
-    attn_stats_tc_kernel<T><<<unsigned(ceil_div(count, 16)), 256, 0, st>>>(a, int(RowsP), gs);
+    const int64_t row_blocks = count / 16, blocks = row_blocks + (is_bf16<T> ? 0 : ceil_div(a.Lk, 16) * a.Hkv * a.B);
+    NNVB_REQUIRE(blocks < (int64_t(1) << 31), "nnvb_cross_attention_backward: too many rows (%lld)", (long long)blocks * 16);
+    attn_stats_tc_kernel<T><<<unsigned(blocks), 256, 0, st>>>(a, int(RowsP), gs, unsigned(row_blocks));
     NNVB_CUDA(cudaGetLastError());
     BwdMaps mq{}, mk{};
     NNVB_TRY(make_map(&mq.a0, a.dtype, a.q, a.qs, a.D, a.Lq, a.Hq, a.B, ROWS, gs));

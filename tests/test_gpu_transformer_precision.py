@@ -1,0 +1,67 @@
+"""What 16-bit attention must not lose: gradients over the whole range of their type.
+
+The gradients' measure is the error's relative 2-norm, row by row, beside the same measure of the
+exact gradient rounded once to its type.  dq and dk are sums of dS = P (dP - delta) times 16-bit inputs in 32 bits, so
+that rounding is the only one of 2^-9 (bf16) or 2^-12 (fp16) root mean square.  All others are of 32-bit values, of
+random sign, and together at most half of it: sqrt(1 + 1/4) = 1.12 times the storage rounding.  One rounding of dS to
+16 bits, or of the output that delta is taken from, adds as much as the storage itself: 1.41 times.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+LIMIT = 1.12
+
+
+def _data(t, B, Lq, Lk, Hq, Hkv, D, seed=0, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+
+    def r(*s):
+        return torch.randn(*s, generator=g, dtype=torch.float64)
+    return (spread * r(B, Lq, Hq, D)).to(t), r(B, Lk, Hkv, D).to(t), r(B, Lk, Hkv, D).to(t), r(B, Lq, Hq, D)
+
+
+def _formula(q, k, v, dout):
+    """(dq, dk) in 64 bits on the CPU."""
+    q, k, v, dout = (x.double() for x in (q, k, v, dout))
+    B, Lq, Hq, D = q.shape
+    Hkv = k.shape[2]
+    qg, dg = (x.view(B, Lq, Hkv, Hq // Hkv, D) for x in (q, dout))
+    p = (torch.einsum("bqhgd,bkhd->bhgqk", qg, k) / math.sqrt(D)).softmax(-1)
+    dp = torch.einsum("bqhgd,bkhd->bhgqk", dg, v)
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True)) / math.sqrt(D)
+    return torch.einsum("bhgqk,bkhd->bqhgd", ds, k).reshape(q.shape), torch.einsum("bhgqk,bqhgd->bkhd", ds, qg)
+
+
+def _row_error(x, want):
+    e = (x.double() - want).norm(dim=-1) / want.norm(dim=-1).clamp_min(1e-300)
+    return float(e.square().mean().sqrt())
+
+
+def _check_gradients(q, k, v, dout):
+    from nnv_b200 import ops
+    t = q.dtype
+    want = _formula(q, k, v, dout)
+    dev = [x.cuda() for x in (q, k, v, dout)]
+    out, lse = ops.cross_attention(*dev[:3], return_lse=True)
+    got = ops.cross_attention_backward(dev[3], *dev[:3], out, lse)
+    for name, a, b in zip(("dq", "dk"), got, want):
+        a = a.cpu()
+        assert a.isfinite().all(), name
+        err, store = _row_error(a, b), _row_error(b.to(t), b)
+        assert err <= LIMIT * store, "%s: %.3g, storage rounding %.3g" % (name, err, store)
+
+
+@pytest.mark.parametrize("size", [1e-4, 1e-3, 1e-2, 1.0, 1e3])
+@pytest.mark.parametrize("Lq,Lk,D", [(200, 100, 64), (200, 4000, 64), (130, 1500, 128)])
+def test_half_precision_gradients_of_any_size(size, Lq, Lk, D):
+    q, k, v, dout = _data(torch.float16, 1, Lq, Lk, 2, 1, D, spread=1.5)
+    _check_gradients(q, k, v, (size * dout).half())
+
+
+def test_half_precision_gradients_behind_the_type():
+    """dS up to 99675, beyond fp16, where dq and dk stay below 60000."""
+    q, k, v, dout = _data(torch.float16, 1, 64, 16, 1, 1, 64, seed=8, spread=1.5)
+    _check_gradients(q, k, v, (12000 * dout).clamp(-46560, 46560).half())
