@@ -448,12 +448,13 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
 
 // ---------------------------------------------------------------------------
 // Backward.  P = exp2(c S - lse'), dS = P (dP - delta) with lse' = lse log2 e.  One kernel serves both passes:
-//   dQ       resident Q and dO (128 positions), streamed K and V:   S = Q K^T,  dP = dO V^T,  dQ += dS K
+//   dQ       resident Q and dO (128 positions), streamed K and V:   S = Q K^T,  dP = dO V^T,  dQ += dS K,  W += P K
 //   dK, dV   resident K and V (128 states), streamed Q and dO of every query head of the group:
 //            S^T = K Q^T,  dP^T = V dO^T,  dV += P^T dO,  dK += dS^T Q
 // so each gradient row is summed in tensor memory by one block, in a fixed order.  Separate passes compute S and dP
-// twice: seven products a pair instead of the five of one pass that would add to dQ atomically.  Bound by the products:
-// 4 x 2048 x 2048 x 16 x 128 bf16, 621 us, 0.55 PFLOP/s counted as five products, 1.0 as the nine that run.
+// twice: eight products a pair instead of the five of one pass that would add to dQ atomically, ten with the second terms of
+// dS.  Bound by the products and the shared memory that feeds them: 4 x 2048 x 2048 x 16 x 128 bf16, 680 us, 0.51 PFLOP/s
+// counted as five products, 1.0 as the ten that run.
 //
 // Streamed tiles have 64 rows, which lets two of them be in flight in tensor memory beside 128 x 128 accumulators;
 // they serve as K-major operand of S and dP and as MN-major operand of the gradients.  Sixteen warps do the softmax
@@ -467,8 +468,10 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
 // Roundings: P is rounded to the tensors' type, as in the forward pass.  dS enters its product as the sum of two
 // 16-bit values (its rounding and the rounding of what is left), an eighth and a ninth product: its rounding error
 // would be as large as that of storing dQ and dK, and the terms of dS cancel in their row sums.  delta comes from the
-// stored output, whose rounding weighs little once a row attends to many states; entries of up to 128 states, where
-// the pass over dQ holds whole rows of P and dP in tensor memory, take the exact sum of P dP instead.
+// stored output (delta0), and where a row's weight lies on a few states its rounding is larger than dP - delta: the error
+// of dq would be 7.2e-3 instead of 1.7e-3 for bf16 queries of 16 sigma over 129 states.  So the dQ pass sums what dS with
+// delta0 misses, e = sum_j P (dP - delta0), takes it back as dQ - e W at its end and leaves delta0 + e for the
+// other pass.  P's rounding enters e W in second order only.
 
 constexpr int BROWS = 64;                          // rows of a streamed tile
 constexpr int BWD_SOFT = 512;                      // threads of the softmax arithmetic
@@ -487,10 +490,11 @@ struct BwdMaps {
     CUtensorMap a0, a1, b0, b1;
 };
 
-// The largest squared norm among the 16 rows of a block, 16 lanes a row.
+constexpr int V_CHUNK = 64;                        // states whose largest norm is kept
+
+// The largest of a block's 16 values, which 16 lanes each hold.
 __device__ __forceinline__ void block_largest(float s, float* to) {
     __shared__ float part[8];
-    for (int w = 8; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w, 32);
     s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, 16, 32));
     if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = s;
     __syncthreads();
@@ -500,8 +504,11 @@ __device__ __forceinline__ void block_largest(float s, float* to) {
     }
 }
 
-// stats: [B, groups of heads, RowsP] lse' then the same of delta, a group's rows rounded up to 64: those behind hold +inf and 0.
-// fp16: then the largest squared norm of dO of every 16 rows, and of V of every 16 states (blocks from row_blocks on).
+// fp16 loses bits below 2^-14: weights enter their products times 2^12.
+template <typename T> constexpr float P_SHIFT = is_bf16<T> ? 0.f : 12.f;
+
+// stats: [B, groups of heads, RowsP] lse' (less P_SHIFT) then the same of delta, a group's rows rounded up to 64: those behind hold +inf and 0.
+// fp16: then the largest squared norm of dO of every 16 rows, and of V of every V_CHUNK states (blocks from row_blocks on).
 template <typename T>
 __global__ void __launch_bounds__(256)
 attn_stats_tc_kernel(AttnArgs a, int RowsP, int gs, unsigned row_blocks) {
@@ -509,13 +516,21 @@ attn_stats_tc_kernel(AttnArgs a, int RowsP, int gs, unsigned row_blocks) {
     const int groups = a.Hq >> gs;
     const int64_t count = int64_t(a.B) * groups * RowsP;
     if (!is_bf16<T> && blockIdx.x >= row_blocks) {
-        const int chunks = (a.Lk + 15) / 16, at = int(blockIdx.x - row_blocks);
-        const int j = at % chunks * 16 + threadIdx.x / 16, g = at / chunks % a.Hkv, b = at / chunks / a.Hkv;
+        const int chunks = (a.Lk + V_CHUNK - 1) / V_CHUNK, at = int(blockIdx.x - row_blocks);
+        const int j0 = at % chunks * V_CHUNK + threadIdx.x / 16, g = at / chunks % a.Hkv, b = at / chunks / a.Hkv, n = attn_len(a, b);
+        const T* v = static_cast<const T*>(a.v) + b * a.vs[0] + g * a.vs[2] + lane * 8;
         float s = 0.f;
-        if (j < attn_len(a, b) && lane * 8 < a.D) {
-            const auto v = *reinterpret_cast<const Pack<T, 8>*>(static_cast<const T*>(a.v) + b * a.vs[0] + j * a.vs[1] + g * a.vs[2] + lane * 8);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s += to_acc(v.v[e]) * to_acc(v.v[e]);
+        for (int i = 0; i < V_CHUNK / 16; ++i) {
+            const int j = j0 + 16 * i;
+            float x = 0.f;
+            if (j < n && lane * 8 < a.D) {
+                const auto y = *reinterpret_cast<const Pack<T, 8>*>(v + j * a.vs[1]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x += to_acc(y.v[e]) * to_acc(y.v[e]);
+            }
+            for (int w = 8; w > 0; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w, 32);
+            s = fmaxf(s, x);
         }
         block_largest(s, static_cast<float*>(a.delta) + 2 * count + count / 16 + at);
         return;
@@ -534,11 +549,14 @@ attn_stats_tc_kernel(AttnArgs a, int RowsP, int gs, unsigned row_blocks) {
             norm += to_acc(d.v[e]) * to_acc(d.v[e]);
         }
     }
+    for (int w = 8; w > 0; w >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, w, 32);
+        if (!is_bf16<T>) norm += __shfl_xor_sync(0xffffffffu, norm, w, 32);
+    }
     if (!is_bf16<T>) block_largest(norm, static_cast<float*>(a.delta) + 2 * count + blockIdx.x);
-    for (int w = 8; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w, 32);
     if (i < count && lane == 0) {
         float* st = static_cast<float*>(a.delta);
-        st[i] = live ? static_cast<const float*>(a.lse)[(int64_t(b) * a.Hq + h) * a.Lq + r] * float(LOG2E) : INFINITY;
+        st[i] = live ? static_cast<const float*>(a.lse)[(int64_t(b) * a.Hq + h) * a.Lq + r] * float(LOG2E) - P_SHIFT<T> : INFINITY;
         st[count + i] = s;
     }
 }
@@ -562,11 +580,11 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
     unsigned char* res = base;                             // A0, A1
     unsigned char* ring = base + 2 * SM::ATILE;            // B0, B1 per stage
     float* stats = reinterpret_cast<float*>(ring + STAGES * 2 * SM::BTILE);
-    __shared__ uint64_t full[STAGES], empty[STAGES], a_full, s_ready[2], p_ready[2], o_ready, x_ready, tail, drain;
+    __shared__ uint64_t full[STAGES], empty[STAGES], a_full, s_ready[2], p_ready[2], o_ready, tail, drain;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
-    __shared__ float row_sum[4][ROWS];
-    __shared__ float norms[2][BWD_THREADS / 32];
+    __shared__ float row_sum[4][ROWS], row_miss[ROWS];
+    __shared__ float factor;
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     // rows and heads (dQ: groups of 2^gs) of this pass
@@ -583,15 +601,13 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
     // streamed tiles: rows of the groups that share the state head, or valid states
     const int per_head = KV ? (rows + BROWS - 1) / BROWS : (n + BROWS - 1) / BROWS;
     const int all_steps = KV ? (r0 < n ? per_head * G : 0) : per_head;
-    // every `share`-th is this block's; rows of up to 128 states stay in one block, which sums P dP over them
-    const int share = all_steps <= 2 ? 1 : world;
-    const int steps = rank < share && all_steps > rank ? (all_steps - rank + share - 1) / share : 0;
+    // every world-th is this block's
+    const int steps = all_steps > rank ? (all_steps - rank + world - 1) / world : 0;
 
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         mbar_init(&a_full, 1);
-        mbar_init(&x_ready, steps > 1 ? 16 : 8);
         mbar_init(&o_ready, 1);
         mbar_init(&tail, 1);
         mbar_init(&drain, 1);
@@ -599,33 +615,14 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
         mbar_init_fence();
     }
     if (warp == 16) tmem_alloc(&tmem_slot, 512);
-    if (SCALED) {                          // the largest squared norms of V's valid states and (dK) of dO's rows
-        const float* of_do = static_cast<const float*>(a.delta) + 2 * int64_t(a.B) * groups * RowsP;
-        const float* of_v = of_do + int64_t(a.B) * groups * (RowsP / 16);
-        const int chunks = (a.Lk + 15) / 16;
-        float x[2] = {0.f, 0.f};
-        if (steps > 0) {
-            of_v += (int64_t(b) * a.Hkv + (KV ? oh : oh / G)) * chunks;
-            for (int i = threadIdx.x; i < (n + 15) / 16; i += BWD_THREADS) x[0] = fmaxf(x[0], of_v[i]);
-            if (KV) {
-                of_do += (int64_t(b) * groups + oh * G) * (RowsP / 16);
-                for (int64_t i = threadIdx.x; i < int64_t(G) * (RowsP / 16); i += BWD_THREADS) x[1] = fmaxf(x[1], of_do[i]);
-            }
-        }
-        for (int w = 16; w > 0; w >>= 1)
-            for (int i = 0; i < 2; ++i) x[i] = fmaxf(x[i], __shfl_xor_sync(0xffffffffu, x[i], w, 32));
-        if (lane == 0)
-            for (int i = 0; i < 2; ++i) norms[i][warp] = x[i];
-    }
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
     constexpr uint32_t tmem = 0;           // all 512 columns are this block's, so they start at column 0
     volatile int* abort = &abort_flag;
-    // Weights of many states are small, and fp16 loses bits below 2^-14: they enter dV's product times 2^12.
-    constexpr float P_SCALE = is_bf16<T> ? 1.f : 4096.f;
+    constexpr float P_SCALE = is_bf16<T> ? 1.f : 4096.f;           // 2^P_SHIFT
     // Tensor memory, columns: tile in flight t at 128 t: S 0..63, dP 64..127; the accumulators of dQ / dK at 256 and of
-    // dV at 384.  The two warpgroups of a tile own 32 columns of S and of dP each and put their 16-bit operands there:
+    // W / dV at 384.  The two warpgroups of a tile own 32 columns of S and of dP each and put their 16-bit operands there:
     // P over the lower half of their columns of S, the rest of dS over the upper half, dS over the lower half of dP.
     const float* st_lse = static_cast<const float*>(a.delta);
     float* st_delta = static_cast<float*>(a.delta) + int64_t(a.B) * groups * RowsP;
@@ -651,7 +648,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
             if (it >= STAGES) ok = mbar_wait_fast(&empty[s], (it / STAGES - 1) & 1, abort);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            const int at_step = rank + it * share;
+            const int at_step = rank + it * world;
             const int sh = KV ? oh * G + at_step / per_head : oh / G;      // streamed group or state head
             const int bh = KV ? sh << gs : sh;
             const int row = at_step % per_head * BROWS;
@@ -727,7 +724,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
                     const uint32_t at = d + (k / 2) * 32 + (k % 2) * 8;
                     mma_ts(leader, tmem + 256, at + 64, b0 + k * (2048 >> 4), id_g, j > 0 || k > 0);
                     mma_ts(leader, tmem + 256, at + 16, b0 + k * (2048 >> 4), id_g, true);
-                    if (KV) mma_ts(leader, tmem + 384, at, b1 + k * (2048 >> 4), id_g, j > 0 || k > 0);
+                    mma_ts(leader, tmem + 384, at, (KV ? b1 : b0) + k * (2048 >> 4), id_g, j > 0 || k > 0);
                 }
                 mma_commit(leader, &empty[j % STAGES]);
             }
@@ -754,16 +751,31 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
             my_lse = st_lse[my_at];
             my_delta = st_delta[my_at];
         }
-        float up = 1.f, down = 1.f;        // fp16: what dS is multiplied with, and the inverse
-        if (SCALED) {
-            float of_v = 0.f, of_do = 0.f;
-            for (int w = 0; w < BWD_THREADS / 32; ++w) {
-                of_v = fmaxf(of_v, norms[0][w]);
-                of_do = fmaxf(of_do, norms[1][w]);
+        // fp16: what dS (beside P's 2^P_SHIFT) is multiplied with and divided by; the dQ pass leaves delta times dK's factor
+        float up = 1.f, down = 1.f, head_up = 1.f;
+        if (SCALED && all_steps > 0) {
+            const int sh = KV ? oh : oh / G;
+            const int64_t chunks = (a.Lk + V_CHUNK - 1) / V_CHUNK, row_chunks = int64_t(G) * (RowsP / 16);
+            const float* of_rows = st_delta + int64_t(a.B) * groups * RowsP;
+            const float* of_states = of_rows + int64_t(a.B) * a.Hkv * row_chunks + (int64_t(b) * a.Hkv + sh) * chunks;
+            float v = 0.f, d = 0.f;
+            for (int i = lane; i < (n + V_CHUNK - 1) / V_CHUNK; i += 32) v = fmaxf(v, of_states[i]);
+            for (int64_t i = lane; i < row_chunks; i += 32) d = fmaxf(d, of_rows[(int64_t(b) * a.Hkv + sh) * row_chunks + i]);
+            for (int w = 16; w > 0; w >>= 1) {
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, w, 32));
+                d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, w, 32));
             }
-            if (!KV && row < rows) of_do = st_delta[int64_t(a.B) * groups * RowsP + my_at / 16];
-            ds_factor(2.f * sqrtf(of_v * of_do), &up, &down);
+            ds_factor(2.f * sqrtf(v * d), &up, &down);
+            head_up = up *= 1.f / P_SCALE;
+            if (!KV) {
+                up = down = 1.f;
+                if (row < rows) ds_factor(2.f * sqrtf(v * of_rows[my_at / 16]), &up, &down);
+                up *= 1.f / P_SCALE;
+            }
         }
+        if (threadIdx.x == 0) factor = head_up;
+        const float up_delta = up * my_delta;
+        Pair<float> miss = both(0.f);
         bool ok = true;
         for (int j = t; j < steps; j += 2) {
             ok = mbar_wait_fast(&full[j % STAGES], (j / STAGES) & 1, abort) &&
@@ -771,7 +783,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tmem_fence_after();
             const float* sl = stats + (j % STAGES) * 2 * BROWS + half * 32;
-            const int rest = KV ? 32 : n - (rank + j * share) * BROWS - half * 32;          // columns with weight
+            const int rest = KV ? 32 : n - (rank + j * world) * BROWS - half * 32;          // columns with weight
             uint32_t s[32];
             tmem_load32(s, s_at);
             tmem_wait_load(s);
@@ -782,26 +794,6 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
                 s[e] = __float_as_uint(!KV && e >= rest ? 0.f : ex2(x.x));
                 s[e + 1] = __float_as_uint(!KV && e + 1 >= rest ? 0.f : ex2(x.y));
             }
-            if (!KV && all_steps <= 2) {
-                float sum = 0.f;
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    uint32_t d[16];
-                    tmem_load16(d, d_at + g * 16);
-                    tmem_wait_load(d);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (g * 16 + e < rest) sum += __uint_as_float(s[g * 16 + e]) * __uint_as_float(d[e]);
-                }
-                row_sum[wg][local] = sum;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&x_ready);
-                ok = __all_sync(0xffffffffu, mbar_wait_fast(&x_ready, 0, abort));
-                if (!ok) break;
-                my_delta = row_sum[0][local] + row_sum[1][local];
-                if (steps == 2) my_delta += row_sum[2][local] + row_sum[3][local];
-                if (wg == 0 && row < rows) st_delta[my_at] = my_delta;     // for the pass over dK, dV
-            }
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 uint32_t d[16], p[8], hi[8], lo[8];
@@ -810,17 +802,20 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
 #pragma unroll
                 for (int e = 0; e < 16; e += 2) {
                     const int col = g * 16 + e;
-                    const Pair<float> dl = KV ? *reinterpret_cast<const Pair<float>*>(sl + BROWS + col) : both(my_delta);
                     const Pair<float> pv{__uint_as_float(s[col]), __uint_as_float(s[col + 1])};
-                    Pair<float> ds = mul2(SCALED ? mul2(pv, both(up)) : pv, add2(Pair<float>{__uint_as_float(d[e]), __uint_as_float(d[e + 1])}, Pair<float>{-dl.x, -dl.y}));
+                    const Pair<float> dp{__uint_as_float(d[e]), __uint_as_float(d[e + 1])};
+                    // dl: fp16: delta times the factor
+                    const Pair<float> dl = KV ? *reinterpret_cast<const Pair<float>*>(sl + BROWS + col) : both(up_delta);
+                    Pair<float> ds = mul2(pv, SCALED ? fma2(dp, both(up), Pair<float>{-dl.x, -dl.y}) : add2(dp, Pair<float>{-dl.x, -dl.y}));
                     if (!KV && col >= rest) ds.x = 0.f;                    // dP there may be 0 * NaN
                     if (!KV && col + 1 >= rest) ds.y = 0.f;
-                    if (KV) p[e / 2] = pack2<T>(pv.x * P_SCALE, pv.y * P_SCALE);
+                    if (!KV) miss = add2(miss, ds);
+                    p[e / 2] = pack2<T>(pv.x, pv.y);
                     hi[e / 2] = pack2<T>(ds.x, ds.y);
                     ds = add2(ds, Pair<float>{-unpack_lo<T>(hi[e / 2]), -unpack_hi<T>(hi[e / 2])});
                     lo[e / 2] = pack2<T>(ds.x, ds.y);
                 }
-                if (KV) tmem_store8(s_at + g * 8, p);
+                tmem_store8(s_at + g * 8, p);
                 tmem_store8(s_at + 16 + g * 8, lo);
                 tmem_store8(d_at + g * 8, hi);
             }
@@ -831,9 +826,19 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
         }
         if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait_fast(&o_ready, 0, abort));
         tmem_fence_after();
+        float e = 0.f;                                     // dQ: what delta0 misses
+        if (!KV) {
+            row_sum[wg][local] = ok ? (miss.x + miss.y) * down : NAN;
+            named_bar_sync(1, BWD_SOFT);
+            e = (row_sum[0][local] + row_sum[1][local]) + (row_sum[2][local] + row_sum[3][local]);
+            if (wg == 0) row_miss[local] = e;
+            if (wg == 0 && world == 1 && row < rows) st_delta[my_at] = (my_delta + e) * head_up;
+        }
         // dK: warpgroups 0 and 1, dV: 2 and 3, half of the columns each; dQ: every warpgroup a chunk of 32
         const bool value = KV && t == 1;
         const bool dead = KV && row >= n;                  // states without weight: their rows of S may hold anything
+        const bool zero = ok && (steps == 0 || dead);
+        const float fw = float(a.scale) / P_SCALE;
         const float f = !ok ? NAN : (value ? 1.f / P_SCALE : float(a.scale) * down);
         T* out = static_cast<T*>(KV ? (value ? a.dv : a.dk) : a.dq) + grad_at(row);
         const uint32_t o_at = lanes + 256 + (value ? 128 : 0);
@@ -847,23 +852,36 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
                 tmem_load32(o, o_at + j * 32);
                 tmem_wait_load(o);
             }
-            const bool zero = ok && (steps == 0 || dead);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(zero ? 0.f : (ok ? __uint_as_float(o[i]) * f : NAN));
+            if (!KV) {
+                uint32_t w[32];
+                if (steps > 0 && ok) {
+                    tmem_load32(w, o_at + 128 + j * 32);
+                    tmem_wait_load(w);
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float x = zero ? 0.f : (ok ? __uint_as_float(w[i]) * fw : NAN);
+                    if (world > 1) w[i] = __float_as_uint(x);
+                    else o[i] = __float_as_uint(__uint_as_float(o[i]) - e * x);
+                }
+                if (world > 1)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        (mine + ROWS * (DP / 4))[(j * 8 + i + local) % (DP / 4)] = *reinterpret_cast<const float4*>(w + 4 * i);
+            }
             if (world > 1) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float x[4];
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) x[u] = zero ? 0.f : (ok ? __uint_as_float(o[4 * e + u]) * f : NAN);
-                    mine[(j * 8 + e + local) % (DP / 4)] = make_float4(x[0], x[1], x[2], x[3]);
-                }
+                for (int i = 0; i < 8; ++i) mine[(j * 8 + i + local) % (DP / 4)] = *reinterpret_cast<const float4*>(o + 4 * i);
             } else if (row < own_len) {
 #pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    if (j * 32 + e < a.D) {
+                for (int i = 0; i < 32; i += 8) {
+                    if (j * 32 + i < a.D) {
                         float x[8];
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) x[u] = zero ? 0.f : (ok ? __uint_as_float(o[e + u]) * f : NAN);
-                        store8<T>(out + j * 32 + e, x);
+                        for (int u = 0; u < 8; ++u) x[u] = __uint_as_float(o[i + u]);
+                        store8<T>(out + j * 32 + i, x);
                     }
                 }
             }
@@ -873,17 +891,29 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
         // the blocks' sums over their streamed tiles, added in block order; each writes a share of the rows
         cluster.sync();
         constexpr int PARTS = KV ? 2 : 1;
-        for (int i = rank * BWD_THREADS + threadIdx.x; i < PARTS * ROWS * (DP / 8); i += world * BWD_THREADS) {
-            const int pr = i / (DP / 8), r = pr % ROWS, d = i % (DP / 8) * 8, row = r0 + r;
-            if (row >= own_len || d >= a.D) continue;
-            float x[8] = {};
+        auto joined = [&](float (&x)[8], int pr, int d) {
             for (int w = 0; w < world; ++w) {
                 const float4* part = cluster.map_shared_rank(reinterpret_cast<float4*>(base), w) + pr * (DP / 4);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const float4 y = part[(d / 4 + u + r) % (DP / 4)];
+                    const float4 y = part[(d / 4 + u + pr) % (DP / 4)];
                     x[u * 4] += y.x; x[u * 4 + 1] += y.y; x[u * 4 + 2] += y.z; x[u * 4 + 3] += y.w;
                 }
+            }
+        };
+        for (int i = rank * BWD_THREADS + threadIdx.x; i < PARTS * ROWS * (DP / 8); i += world * BWD_THREADS) {
+            const int pr = i / (DP / 8), r = pr % ROWS, d = i % (DP / 8) * 8, row = r0 + r;
+            if (row >= own_len || d >= a.D) continue;
+            float x[8] = {};
+            joined(x, pr, d);
+            if (!KV) {
+                float w[8] = {}, e = 0.f;
+                joined(w, ROWS + r, d);
+                for (int k = 0; k < world; ++k) e += *cluster.map_shared_rank(&row_miss[r], k);
+#pragma unroll
+                for (int u = 0; u < 8; ++u) x[u] -= e * w[u];
+                float* delta = st_delta + (int64_t(b) * groups + oh) * RowsP + row;
+                if (d == 0) *delta = (*delta + e) * factor;
             }
             store8<T>(static_cast<T*>(KV ? (pr >= ROWS ? a.dv : a.dk) : a.dq) + grad_at(row) + d, x);
         }
@@ -999,7 +1029,7 @@ int backward_t(cudaStream_t st, const AttnArgs& a) {
     const int gs = pack_shift(a, true);
     const int64_t rows = int64_t(a.Lq) << gs, groups = a.Hq >> gs, RowsP = round_up(rows, BROWS);
     const int64_t count = RowsP * a.B * groups;
-    const int64_t row_blocks = count / 16, blocks = row_blocks + (is_bf16<T> ? 0 : ceil_div(a.Lk, 16) * a.Hkv * a.B);
+    const int64_t row_blocks = count / 16, blocks = row_blocks + (is_bf16<T> ? 0 : ceil_div(a.Lk, V_CHUNK) * a.Hkv * a.B);
     NNVB_REQUIRE(blocks < (int64_t(1) << 31), "nnvb_cross_attention_backward: too many rows (%lld)", (long long)blocks * 16);
     attn_stats_tc_kernel<T><<<unsigned(blocks), 256, 0, st>>>(a, int(RowsP), gs, unsigned(row_blocks));
     NNVB_CUDA(cudaGetLastError());

@@ -1,7 +1,8 @@
-"""What 16-bit attention must not lose: gradients over the whole range of their type.
+"""What 16-bit attention must not lose: gradients over the whole range of their type, gradients of peaked rows.
 
-The gradients' measure is the error's relative 2-norm, row by row, beside the same measure of the
-exact gradient rounded once to its type.  dq and dk are sums of dS = P (dP - delta) times 16-bit inputs in 32 bits, so
+The gradients' measure is the error's relative 2-norm, row by row where no row is peaked, beside the same measure of the
+exact gradient rounded once to its type.  (A row whose weight lies on one state has a dq around 1 - P; sums in 32 bits
+leave 2^-24 of delta there, so its own relative error has no bound.)  dq and dk are sums of dS = P (dP - delta) times 16-bit inputs in 32 bits, so
 that rounding is the only one of 2^-9 (bf16) or 2^-12 (fp16) root mean square.  All others are of 32-bit values, of
 random sign, and together at most half of it: sqrt(1 + 1/4) = 1.12 times the storage rounding.  One rounding of dS to
 16 bits, or of the output that delta is taken from, adds as much as the storage itself: 1.41 times.
@@ -12,6 +13,7 @@ import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
+F16 = [torch.bfloat16, torch.float16]
 LIMIT = 1.12
 
 
@@ -40,7 +42,11 @@ def _row_error(x, want):
     return float(e.square().mean().sqrt())
 
 
-def _check_gradients(q, k, v, dout):
+def _error(x, want):
+    return float((x.double() - want).norm() / want.norm())
+
+
+def _check_gradients(q, k, v, dout, measure=_row_error):
     from nnv_b200 import ops
     t = q.dtype
     want = _formula(q, k, v, dout)
@@ -50,7 +56,7 @@ def _check_gradients(q, k, v, dout):
     for name, a, b in zip(("dq", "dk"), got, want):
         a = a.cpu()
         assert a.isfinite().all(), name
-        err, store = _row_error(a, b), _row_error(b.to(t), b)
+        err, store = measure(a, b), measure(b.to(t), b)
         assert err <= LIMIT * store, "%s: %.3g, storage rounding %.3g" % (name, err, store)
 
 
@@ -65,3 +71,20 @@ def test_half_precision_gradients_behind_the_type():
     """dS up to 99675, beyond fp16, where dq and dk stay below 60000."""
     q, k, v, dout = _data(torch.float16, 1, 64, 16, 1, 1, 64, seed=8, spread=1.5)
     _check_gradients(q, k, v, (12000 * dout).clamp(-46560, 46560).half())
+
+
+def test_half_precision_gradients_of_uneven_rows():
+    """Positions whose gradients differ by 2^20, none at all among them, and states whose values differ by 2^10."""
+    q, k, v, dout = _data(torch.float16, 2, 150, 700, 4, 2, 64, spread=1.5)
+    dout *= torch.logspace(-10, 10, 150, base=2.0)[None, :, None, None]
+    v = (v.double() * torch.logspace(5, -5, 700, base=2.0)[None, :, None, None]).half()
+    dout[:, 7] = 0
+    _check_gradients(q, k, v, dout.half())
+
+
+@pytest.mark.parametrize("t", F16)
+@pytest.mark.parametrize("spread", [1.0, 4.0, 16.0])
+@pytest.mark.parametrize("Lq,Lk,H", [(150, 128, 2), (150, 129, 2), (100, 4096, 1), (600, 300, 16)])
+def test_gradients_of_peaked_rows(t, spread, Lq, Lk, H):
+    q, k, v, dout = _data(t, 1, Lq, Lk, H, 1, 64, spread=spread)
+    _check_gradients(q, k, v, dout.to(t), _error)
