@@ -312,7 +312,8 @@ attn_delta_kernel(AttnArgs a) {
     if (lane == 0) static_cast<A*>(a.delta)[(int64_t(b) * a.Hq + h) * a.Lq + r] = s;
 }
 
-// dQ: a block per tile of positions
+// dQ: a block per tile of positions.  16-bit types: delta from the stored output would carry its rounding, which is larger
+// than dP - delta where a row's weight lies on a few states; a first walk sums P dP instead and leaves it for dK.
 template <typename T, int TILE, int DP>
 __global__ void __launch_bounds__(THREADS)
 attn_dq_simt_kernel(AttnArgs a, bool vec) {
@@ -341,29 +342,64 @@ attn_dq_simt_kernel(AttnArgs a, bool vec) {
     for (int i = 0; i < M; ++i) {
         const int r = q0 + ty * M + i;
         lse[i] = r < rows.n ? static_cast<const A*>(a.lse)[rows.stat(r)] * A(LOG2E) : A(0);
-        dl[i] = r < rows.n ? static_cast<const A*>(a.delta)[rows.stat(r)] : A(0);
+        dl[i] = sizeof(T) > 2 && r < rows.n ? static_cast<const A*>(a.delta)[rows.stat(r)] : A(0);
         f[i] = A(a.scale);
 #pragma unroll
         for (int e = 0; e < DP / 16; ++e) acc[i][e] = 0;
     }
     load_tile<T, A, TILE, DP>(Qs, static_cast<const T*>(a.q) + rows.first(a.qs), [&](int r) { return rows.at(a.qs, r); }, q0, rows.n, a.D, vec);
     load_tile<T, A, TILE, DP>(Gs, static_cast<const T*>(a.dout) + rows.first(a.dos), [&](int r) { return rows.at(a.dos, r); }, q0, rows.n, a.D, vec);
-    for (int k0 = rank * TILE; k0 < n; k0 += world * TILE) {
+    // P and dP of the tile of states from k0 on
+    auto products = [&](int k0, A (&p)[M][M], A (&dp)[M][M]) {
         __syncthreads();
         load_tile<T, A, TILE, DP>(Ks, k, [&](int r) { return r * a.ks[1]; }, k0, n, a.D, vec);
         load_tile<T, A, TILE, DP>(Vs, v, [&](int r) { return r * a.vs[1]; }, k0, n, a.D, vec);
         cp_async_wait<0>();
         __syncthreads();
-        A s[M][M] = {}, dp[M][M] = {};
-        mul_rows<A, TILE, DP>(s, Qs, Ks, a.D, rows.n - q0, n - k0, ty, tx);
+        mul_rows<A, TILE, DP>(p, Qs, Ks, a.D, rows.n - q0, n - k0, ty, tx);
         mul_rows<A, TILE, DP>(dp, Gs, Vs, a.D, rows.n - q0, n - k0, ty, tx);
 #pragma unroll
         for (int i = 0; i < M; ++i)
 #pragma unroll
-            for (int j = 0; j < M; ++j) {
-                const A p = k0 + tx + 16 * j < n ? exp_acc(s[i][j] * c - lse[i]) : A(0);
-                Ps[(ty * M + i) * LP + tx + 16 * j] = p * (dp[i][j] - dl[i]);
+            for (int j = 0; j < M; ++j) p[i][j] = k0 + tx + 16 * j < n ? exp_acc(p[i][j] * c - lse[i]) : A(0);
+    };
+    if constexpr (sizeof(T) == 2) {
+        for (int k0 = rank * TILE; k0 < n; k0 += world * TILE) {
+            A p[M][M] = {}, dp[M][M] = {};
+            products(k0, p, dp);
+#pragma unroll
+            for (int i = 0; i < M; ++i)
+#pragma unroll
+                for (int j = 0; j < M; ++j)
+                    if (k0 + tx + 16 * j < n) dl[i] += p[i][j] * dp[i][j];
+        }
+        __shared__ A sums[TILE];
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            dl[i] = sum16(dl[i]);
+            if (world > 1 && tx == 0) sums[ty * M + i] = dl[i];
+        }
+        if (world > 1) {
+            cluster.sync();
+#pragma unroll
+            for (int i = 0; i < M; ++i) {
+                dl[i] = 0;
+                for (int w = 0; w < world; ++w) dl[i] += *cluster.map_shared_rank(sums + ty * M + i, w);
             }
+        }
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            const int r = q0 + ty * M + i;
+            if (rank == 0 && tx == 0 && r < rows.n) static_cast<A*>(a.delta)[rows.stat(r)] = dl[i];
+        }
+    }
+    for (int k0 = rank * TILE; k0 < n; k0 += world * TILE) {
+        A p[M][M] = {}, dp[M][M] = {};
+        products(k0, p, dp);
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+#pragma unroll
+            for (int j = 0; j < M; ++j) Ps[(ty * M + i) * LP + tx + 16 * j] = p[i][j] * (dp[i][j] - dl[i]);
         __syncwarp();
         mul_cols<A, TILE, DP>(acc, Ps, Ks, n - k0, ty, tx);
     }
@@ -575,9 +611,7 @@ int attn_delta(cudaStream_t st, const AttnArgs& a) {
     NNVB_REQUIRE(blocks < (int64_t(1) << 31), "nnvb_cross_attention_backward: too many rows (%lld)", (long long)rows);
     switch (a.dtype) {
         case NNVB_F64: attn_delta_kernel<double><<<unsigned(blocks), 256, 0, st>>>(a); break;
-        case NNVB_F32: attn_delta_kernel<float><<<unsigned(blocks), 256, 0, st>>>(a); break;
-        case NNVB_BF16: attn_delta_kernel<__nv_bfloat16><<<unsigned(blocks), 256, 0, st>>>(a); break;
-        default: attn_delta_kernel<__half><<<unsigned(blocks), 256, 0, st>>>(a); break;
+        default: attn_delta_kernel<float><<<unsigned(blocks), 256, 0, st>>>(a); break;
     }
     NNVB_CUDA(cudaGetLastError());
     return NNVB_OK;

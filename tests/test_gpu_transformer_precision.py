@@ -88,3 +88,12 @@ def test_half_precision_gradients_of_uneven_rows():
 def test_gradients_of_peaked_rows(t, spread, Lq, Lk, H):
     q, k, v, dout = _data(t, 1, Lq, Lk, H, 1, 64, spread=spread)
     _check_gradients(q, k, v, dout.to(t), _error)
+
+
+@pytest.mark.parametrize("t", F16)
+@pytest.mark.parametrize("spread", [4.0, 16.0])
+@pytest.mark.parametrize("Lq,Lk,H,D", [(60, 400, 6, 136), (300, 70, 2, 256), (20, 3000, 1, 66)])
+def test_gradients_of_peaked_rows_in_other_layouts(t, spread, Lq, Lk, H, D):
+    """Heads that the tensor cores do not take: more than 128 channels, rows that are not whole 16-byte pieces."""
+    q, k, v, dout = _data(t, 1, Lq, Lk, H, 1, D, spread=spread)
+    _check_gradients(q, k, v, dout.to(t), _error)
