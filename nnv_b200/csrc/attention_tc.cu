@@ -79,11 +79,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // 2^x on the FMA pipe, for a share of the weights: the exponential unit takes 16 a cycle, half of what the tensor pipe
 // needs of them.  x = i + f with f in [-1/2, 1/2]; 2^f by the polynomial of degree 4 that interpolates it at the
-// Chebyshev points (relative error below 5e-6, a 500th of P's rounding), times 2^i.  x <= 8 here; below
-// -125 the result is about 2^-125 instead of less.
+// Chebyshev points (relative error below 5e-6, a 500th of P's rounding), times 2^i.  x <= 8 here.  From -126.5 down, -inf
+// included, i is -127, whose bits as a float's exponent are those of 0: the same flush to zero as ex2's.
 __device__ __forceinline__ Pair<float> ex2_poly(Pair<float> x) {
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-125.f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-125.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.f));
     const float magic = 12582912.f;                    // 1.5 * 2^23: adding it rounds to an integer in the low bits
     const Pair<float> r = add2(x, both(magic));
     const Pair<float> f = add2(x, mul2(add2(r, both(-magic)), both(-1.f)));

@@ -1,4 +1,5 @@
-"""What 16-bit attention must not lose: gradients over the whole range of their type, gradients of peaked rows.
+"""What 16-bit attention must not lose: gradients over the whole range of their type, gradients of peaked rows, and
+scores of -inf.
 
 The gradients' measure is the error's relative 2-norm, row by row where no row is peaked, beside the same measure of the
 exact gradient rounded once to its type.  (A row whose weight lies on one state has a dq around 1 - P; sums in 32 bits
@@ -11,6 +12,8 @@ import math
 
 import pytest
 import torch
+
+import transformer_reference as R
 
 pytestmark = pytest.mark.gpu
 F16 = [torch.bfloat16, torch.float16]
@@ -97,3 +100,24 @@ def test_gradients_of_peaked_rows_in_other_layouts(t, spread, Lq, Lk, H, D):
     """Heads that the tensor cores do not take: more than 128 channels, rows that are not whole 16-byte pieces."""
     q, k, v, dout = _data(t, 1, Lq, Lk, H, 1, D, spread=spread)
     _check_gradients(q, k, v, dout.to(t), _error)
+
+
+@pytest.mark.parametrize("t", F16)
+@pytest.mark.parametrize("Lq,Lk,D", [(130, 300, 64), (300, 1000, 128), (50, 5000, 64), (2, 300, 64)])
+def test_scores_of_minus_infinity_weigh_nothing(t, Lq, Lk, D):
+    from nnv_b200 import ops
+    q, k, v, _ = _data(t, 1, Lq, Lk, 2, 2, D)
+    q = q.abs()
+    keep = torch.ones(Lk, dtype=torch.bool)
+    keep[100::3] = False
+    k[:, ~keep] = -math.inf
+    big = torch.finfo(t).max
+    v[:, ~keep] = big
+    out, lse = ops.cross_attention(q.cuda(), k.cuda(), v.cuda(), return_lse=True)
+    ref = R.attention(q, k[:, keep], v[:, keep], None, 1 / math.sqrt(D))
+    R.check("out", out, *ref["out"])
+    R.check("lse", lse, *ref["lse"])
+    k[:] = -math.inf                           # softmax of nothing but -inf: 0 / 0
+    v[:] = 1
+    out, lse = ops.cross_attention(q.cuda(), k.cuda(), v.cuda(), return_lse=True)
+    assert out.isnan().all() and (lse == -math.inf).all()
