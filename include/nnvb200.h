@@ -471,7 +471,8 @@ int nnvb_layer_norm_backward(void* stream, int dtype, int64_t rows, int64_t cols
  * n_b on are not read into any result, whatever they hold; with n_b = 0 the rows of
  * `out` are 0 and lse is -inf.  A valid score of -inf (from infinite q or k) has
  * weight 0; where all valid scores of a row are -inf its softmax is 0 / 0: `out` is
- * NaN, lse -inf.  A tensor's element (b, token, head, d) lies at
+ * NaN, lse -inf.  fp16 takes scores of magnitude up to 2^25 (beyond, the rounding of a
+ * 32-bit score can lift a weight past the type's end).  A tensor's element (b, token, head, d) lies at
  * b*stride[0] + token*stride[1] + head*stride[2] + d; strides are in elements and
  * not negative; inputs may have any (0 broadcasts), `out` must not overlap itself.
  * head_dim 1..256; q_heads a multiple of kv_heads. */

@@ -10,7 +10,8 @@
 // whatever the arithmetic does) and multiplies with warp-wide mma.sync: rows fill one 16-row tile, tcgen05's smallest has
 // 64 or 128, and at this bound its rate would not show.  Products with the FMA pipe took 50 instructions a state, which
 // was the bound; these take 6.  Weights enter P V as the sum of two 16-bit values, because a few rows' rounding errors do
-// not average out: with up to eight rows the second value rides in the tile's idle rows.
+// not average out: with up to eight rows the second value rides in the tile's idle rows.  In fp16 they carry a factor 2^14,
+// so that those below 2^-14 keep their bits too.
 //
 // float and double: states go straight into registers, products run on the FMA pipe with two terms an instruction.
 //
@@ -19,6 +20,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attention.cuh"
 #include "mma_f64.cuh"
@@ -363,6 +365,7 @@ attn_rows_mma_kernel(AttnArgs a) {
     unsigned char* ring = rings + warp * RING * 2 * BLOCK;
     const uint32_t ring_at = smem_u32(ring);
     const float c = float(a.scale * LOG2E);
+    constexpr float SHIFT = std::is_same<T, __half>::value ? 14.f : 0.f;
 
     const int blocks = (n + KEYS - 1) / KEYS, stride = world * WARPS, first = rank * WARPS + warp;
     // block `blk` into stage s; states behind the valid ones and channels behind the last become 0
@@ -450,7 +453,7 @@ attn_rows_mma_kernel(AttnArgs a) {
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    p[t][h * 2 + e] = t * 8 + tq * 2 + e < rest ? exp2f(sc[t][h * 2 + e] - base) : 0.f;
+                    p[t][h * 2 + e] = t * 8 + tq * 2 + e < rest ? exp2f(sc[t][h * 2 + e] - base + SHIFT) : 0.f;
                     sum += p[t][h * 2 + e];
                 }
             l[h] = l[h] * f + sum;
@@ -533,7 +536,7 @@ attn_rows_mma_kernel(AttnArgs a) {
             static_cast<T*>(const_cast<void*>(a.o))[b * a.os[0] + tok * a.os[1] + h * a.os[2] + d] =
                 from_acc<T, float>(n > 0 ? x / sum : 0.f);
         if (d == 0 && a.lse)
-            static_cast<float*>(a.lse)[(int64_t(b) * a.Hq + h) * a.Lq + tok] = n > 0 ? top / float(LOG2E) + logf(sum) : -INFINITY;
+            static_cast<float*>(a.lse)[(int64_t(b) * a.Hq + h) * a.Lq + tok] = n > 0 ? (top - SHIFT) / float(LOG2E) + logf(sum) : -INFINITY;
     }
     cluster.sync();                        // nobody leaves while its shared memory is read
 }

@@ -14,7 +14,8 @@
 // The running maximum m is raised lazily: O is only rescaled when a row's maximum has grown by more than a factor of
 // 2^8 over the m in use, so weights stay below 2^8, which 16-bit P and fp32 sums hold without loss; after the first
 // tiles the rescale is rare.  P is rounded to the tensors' type because the product takes 16-bit operands; its
-// row sum is added in fp32 before the rounding.
+// row sum is added in fp32 before the rounding.  fp16 P carries a factor 2^7, up to the type's end: without it weights
+// below 2^-14 lose bits, which shows where one state outweighs the others and its V does not matter.
 //
 // Bound by the products at long lengths: Q K^T reads both operands from shared memory, 8 KB for each 64 cycles of the
 // tensor pipe, all that shared memory delivers.  8 x 2048 x 4096 x 16 x 128 bf16: 509 us, 1.08 PFLOP/s.
@@ -79,7 +80,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // 2^x on the FMA pipe, for a share of the weights: the exponential unit takes 16 a cycle, half of what the tensor pipe
 // needs of them.  x = i + f with f in [-1/2, 1/2]; 2^f by the polynomial of degree 4 that interpolates it at the
-// Chebyshev points (relative error below 5e-6, a 500th of P's rounding), times 2^i.  x <= 8 here.  From -126.5 down, -inf
+// Chebyshev points (relative error below 5e-6, a 500th of P's rounding), times 2^i.  x <= 15 here.  From -126.5 down, -inf
 // included, i is -127, whose bits as a float's exponent are those of 0: the same flush to zero as ex2's.
 __device__ __forceinline__ Pair<float> ex2_poly(Pair<float> x) {
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.f));
@@ -290,7 +291,10 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
             const uint32_t s_at = lanes + t * 128, o_at = lanes + 256 + t * 128;
             const int row = q0 + t * ROWS + (warp % 4) * 32 + lane;
             const float c = float(a.scale * LOG2E);
-            float m = -INFINITY, l = 0.f;      // m: the maximum in use, of the scores without the factor
+            // m: the maximum in use, of the scores without the factor; fp16: less 7 powers of two, except where scores are so
+            // large (2^20) that the rounding of m c would take P past the type's end
+            const float below = fminf(7.f / c, 3e38f), large = 1048576.f / c;
+            float m = -INFINITY, l = 0.f;
             bool ok = true;
             for (int i = 0; i < steps; ++i) {
                 ok = mbar_wait_fast(&s_ready[t], i & 1, abort);
@@ -312,7 +316,8 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) mx[e / 2 % 4] = max3(mx[e / 2 % 4], __uint_as_float(s[j][e]), __uint_as_float(s[j][e + 1]));
                 }
-                const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+                float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+                if (!is_bf16<T> && fabsf(top) < large) top -= below;
                 const bool raise = m == -INFINITY ? top > m : (top - m) * c > 8.f;
                 if (i == 0) {
                     m = top;

@@ -1,5 +1,5 @@
-"""What 16-bit attention must not lose: gradients over the whole range of their type, gradients of peaked rows, and
-scores of -inf.
+"""What 16-bit attention must not lose: gradients over the whole range of their type, gradients of peaked rows, weights
+of states that an outweighing one leaves small, and scores of -inf.
 
 The gradients' measure is the error's relative 2-norm, row by row where no row is peaked, beside the same measure of the
 exact gradient rounded once to its type.  (A row whose weight lies on one state has a dq around 1 - P; sums in 32 bits
@@ -121,3 +121,44 @@ def test_scores_of_minus_infinity_weigh_nothing(t, Lq, Lk, D):
     v[:] = 1
     out, lse = ops.cross_attention(q.cuda(), k.cuda(), v.cuda(), return_lse=True)
     assert out.isnan().all() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("Lq", [1, 4, 100])
+def test_half_precision_keeps_small_weights_beside_an_outweighing_state(Lq):
+    """One state holds nearly all weight and no value: the others' weights, around 2^-26 of it, make the output."""
+    from nnv_b200 import ops
+    t, Lk, D = torch.float16, 3000, 64
+    q, k, v, _ = _data(t, 1, Lq, Lk, 1, 1, D)
+    q[..., 0], k[..., 0] = 8.0, 0.0            # scores: 8 k_0 / 8 plus sigma 1 of the other channels
+    k[:, 0] = 0
+    k[:, 0, :, 0] = 18.0                       # e^18 = 2^26 times the others
+    v[:, 1:] = 1000 * v[:, 1:].abs()
+    v[:, 0] = 0
+    out = ops.cross_attention(q.cuda(), k.cuda(), v.cuda()).cpu().double()
+    p = (torch.einsum("bqhd,bkhd->bhqk", q.double(), k.double()) / 8).softmax(-1)
+    want = torch.einsum("bhqk,bkhd->bqhd", p, v.double())
+    # half a step of fp16 for each weight and for the output, fp32 arithmetic a 16th of that
+    tol = 2.0 ** -11 * (2 + 1 / 16) * want
+    R.check("out", out, want.numpy(), tol.numpy())
+
+
+@pytest.mark.parametrize("t,size", [(torch.bfloat16, 300.0), (torch.bfloat16, 3000.0), (torch.bfloat16, 10000.0),
+                                    (torch.float16, 300.0), (torch.float16, 3000.0)])
+@pytest.mark.parametrize("Lq,Lk", [(2, 500), (200, 500), (100, 4000)])
+def test_scores_of_millions_pick_a_state(t, size, Lq, Lk):
+    """Scores of 1e5 to 1e9 whose rounding in 32 bits is up to dozens of powers of two, and gaps far wider than that: each
+    row is the value of its largest score, to the roundings of a weight and of the output."""
+    from nnv_b200 import ops
+    q, k, v, _ = _data(t, 1, Lq, Lk, 2, 2, 64, spread=size)
+    k = (size * k.double()).to(t)
+    assert q.isfinite().all() and k.isfinite().all()
+    s = torch.einsum("bqhd,bkhd->bhqk", q.double(), k.double()) / 8
+    two = s.topk(2, -1).values
+    clear = (two[..., 0] - two[..., 1]) > 64 * 2.0 ** -24 * torch.einsum("bqhd,bkhd->bhqk", q.double().abs(), k.double().abs()).amax(-1) / 8 + 40
+    assert clear.double().mean() > 0.8
+    out = ops.cross_attention(q.cuda(), k.cuda(), v.cuda()).cpu()
+    assert out.isfinite().all()
+    want = torch.stack([v[0, s[0, h].argmax(-1), h] for h in range(2)], 1)[None]
+    # m c is rounded, so the weight is not quite 1: its own rounding to 16 bits is a half step, the output's another
+    near = (out.double() - want.double()).abs() <= 2.02 * R.half_step(t) * want.double().abs()
+    assert (near.all(-1) | ~clear.transpose(1, 2)).all()
