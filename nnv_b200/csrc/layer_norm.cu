@@ -520,6 +520,11 @@ int sm_count() {
     return n[dev];
 }
 
+// Shared memory that any call may need: every stage's tiles, or a cluster's sums.  The limit of a kernel belongs to the
+// process, so every call sets this value; with its own need, a call with few rows could lower the limit between another
+// thread's setting and its launch.
+constexpr int LN_SMEM = 200 * 1024;
+
 constexpr int LN_MAX_PARTS = 2 * 148;        // partial rows of the weights' gradients: blocks that fit at once
 
 // Backward of tensors up to this size runs in one cluster: its 16 SMs take about as long as a second launch does.
@@ -539,7 +544,7 @@ int ln_tile(LnArgs& a, int mode) {
     p.eps = a.eps;
     p.mode = mode;
     // as many rounds of all groups as a stage holds, but no more rows than spread over all blocks
-    const int64_t budget = (MINB == 2 ? 100 : 200) * 1024 / LN_STAGES;
+    const int64_t budget = LN_SMEM / LN_STAGES / (MINB == 2 ? 2 : 1);
     int64_t R = (budget - 32 * TENSORS - 256) / (TENSORS * pitch);
     R = std::min<int64_t>(R, ceil_div(a.rows, slots));
     R = R >= GROUPS ? R / GROUPS * GROUPS : std::max<int64_t>(R, 1);
@@ -551,7 +556,8 @@ int ln_tile(LnArgs& a, int mode) {
     const int smem = std::max<int>(LN_STAGES * p.tensor_bytes * TENSORS, sums);
     a.grid = int(std::min<int64_t>(p.n_tiles, slots));
     auto kernel = ln_tile_kernel<T, VEC, TPR, N, BWD, MINB>;
-    NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    NNVB_REQUIRE(smem <= LN_SMEM, "nnvb_layer_norm: rows of %lld columns need %d bytes of shared memory", (long long)a.cols, smem);
+    NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LN_SMEM));
     if (cluster) {
         int world = 1;
         while (world < a.grid) world *= 2;
@@ -593,7 +599,7 @@ int ln_by_width(LnArgs& a, int mode, bool* done) {
     if (c <= 512 * E) return ln_tile<T, VEC, 512, N, BWD, M>(a, mode);
     // the ring holds a row per stage at least
     const int64_t row = round_up(c * int64_t(sizeof(T)) + 32, 128) * (BWD ? 2 : 1);
-    if (c <= 512 * 2 * E && row * LN_STAGES <= 200 * 1024) return ln_tile<T, VEC, 512, 2 * N, BWD, M>(a, mode);
+    if (c <= 512 * 2 * E && row * LN_STAGES <= LN_SMEM) return ln_tile<T, VEC, 512, 2 * N, BWD, M>(a, mode);
     *done = false;
     return NNVB_OK;
 }
