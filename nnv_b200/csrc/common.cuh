@@ -119,6 +119,9 @@ void conv_arrange_weights(const ConvGeom& g, const double* W, double* dst, int b
 // (column j at cin + j*cin_stride, window wh_in x ww_in), read instead of Vin.  Vout may be null when pack is
 // given: the output then exists in compact form only.
 int conv_win_wait_timeouts(cudaStream_t st, int* out);
+// nnvb_layer_norm_forward on doubles; *gave_up (device) becomes 1 when a bounded wait ran out, whose rows are NaN
+int layer_norm_rows(cudaStream_t st, int64_t rows, int64_t cols, const double* x, int64_t ld, const double* scale,
+                    const double* offset, double eps, double* y, int* gave_up);
 int launch_conv_win(cudaStream_t st, const ConvGeom& g, const ConvWeights& w, const ChanAffine& bn, const RowMask& mask,
                     const ColWindows& win, int wh_in, int ww_in, int64_t col_base, const double* Vin, int64_t ld_in,
                     double* Vout, int64_t ld_out, int64_t ncols, double* pack, bool* done, int64_t* launches,

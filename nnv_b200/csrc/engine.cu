@@ -122,12 +122,13 @@ struct WorkBufs {
     DevBuf pack2[2];                     // compact (window-only, channel-fastest) storage of the windowed cohorts: a layer
                                          // reads one buffer and writes the other
     DevBuf hs_G, hs_g, hs_q, hs_margin, hs_r, hs_roff, hs_val, hs_scale, hs_bound, wit[2];   // halfspace tests
+    DevBuf gave_up;                      // evaluation: int, 1 when a bounded wait of a layer norm ran out
     std::vector<std::unique_ptr<ReluLayerRecord>> relu;
     void release() {
         DevBuf* bufs[] = {&col_q, &pl, &pu, &col_pos, &box, &qcol_off[0], &qcol_off[1], &qcol_idx[0], &qcol_idx[1],
                           &chunk_beg, &chunk_end, &q_chunk_off, &partial, &sums, &lb, &ub, &state, &state_cf, &rank, &blk_cross,
                           &q_cross, &q_dead, &q_new_off, &gen_off, &tmp, &fcg, &winsort, &hot_idx, &hot_scale, &pack2[0], &pack2[1], &hs_G, &hs_g, &hs_q, &hs_margin, &hs_r,
-                          &hs_roff, &hs_val, &hs_scale, &hs_bound, &wit[0], &wit[1]};
+                          &hs_roff, &hs_val, &hs_scale, &hs_bound, &wit[0], &wit[1], &gave_up};
         for (DevBuf* d : bufs) d->release();
         for (auto& r : relu) r->release();
         relu.clear();
@@ -801,10 +802,20 @@ int nnvb_net_evaluate(nnvb_net* net, int64_t n_points, const double* X, double* 
                                     sizeof(double) * N0, size_t(n), cudaMemcpyHostToDevice, st));
         double* out = nullptr;
         int64_t ldx = 0;
+        int gave_up = 0;
+        if (net->evaluate_only) {
+            NNVB_TRY(wk->gave_up.ensure(sizeof(int), st));
+            NNVB_CUDA(cudaMemsetAsync(wk->gave_up.p, 0, sizeof(int), st));
+        }
         NNVB_TRY(forward_points(net, wk, nullptr, n, nullptr, &out, &ldx, nullptr, nullptr, nullptr));
+        if (net->evaluate_only) NNVB_CUDA(cudaMemcpyAsync(&gave_up, wk->gave_up.p, sizeof(int), cudaMemcpyDeviceToHost, st));
         NNVB_CUDA(cudaMemcpy2DAsync(Y + p0 * Nout, sizeof(double) * Nout, out, sizeof(double) * ldx,
                                     sizeof(double) * Nout, size_t(n), cudaMemcpyDeviceToHost, st));
         NNVB_TRY(sync(ctx));
+        if (gave_up) {
+            set_error("nnvb_net_evaluate: a bounded wait inside a layer normalisation ran out; the results are not valid");
+            return NNVB_E_CUDA;
+        }
     }
     return NNVB_OK;
 }
@@ -2118,12 +2129,12 @@ int output_ranges(nnvb_batch* b) {
 
 // One column of n points holds T positions of L.cols entries each.  When the columns follow one another without
 // padding, or hold one position each, all positions are rows of one call.
-int layer_norm_points(cudaStream_t st, const Layer& L, const double* X, int64_t ld, double* Y, int64_t n, int64_t* launches) {
+int layer_norm_points(cudaStream_t st, const Layer& L, const double* X, int64_t ld, double* Y, int64_t n, int* gave_up,
+                      int64_t* launches) {
     const int64_t T = L.Ho * L.Wo * L.Co / L.cols;
     auto rows = [&](const double* x, double* y, int64_t count, int64_t stride) {
         ++*launches;
-        return nnvb_layer_norm_forward(st, NNVB_F64, count, L.cols, x, stride, L.bn_scale, L.bn_offset, L.eps, y, stride,
-                                       nullptr, nullptr);
+        return layer_norm_rows(st, count, L.cols, x, stride, L.bn_scale, L.bn_offset, L.eps, y, gave_up);
     };
     if (T == 1) return rows(X, Y, n, ld);
     if (ld == T * L.cols) return rows(X, Y, n * T, L.cols);
@@ -2194,7 +2205,7 @@ int forward_points(nnvb_net* net, WorkBufs* wk, nnvb_batch* b, int n, const int3
                 NNVB_TRY(launch_bn_f64(st, bn, L.H * L.W, N, cur, ld, n, n, &ctx->launches));
             }
         } else if (L.type == NNVB_LAYER_LAYERNORM) {
-            NNVB_TRY(layer_norm_points(st, L, cur, ld, oth, n, &ctx->launches));
+            NNVB_TRY(layer_norm_points(st, L, cur, ld, oth, n, wk->gave_up.as<int>(), &ctx->launches));
             std::swap(cur, oth);
         } else if (L.type == NNVB_LAYER_ATTENTION) {
             NNVB_TRY(attention_points(st, L, cur, ld, oth, n, &ctx->launches));

@@ -108,6 +108,7 @@ struct LnTile {
     int R, tensor_bytes;                         // rows of a tile; bytes of one tensor's rows in a stage
     int mode;
     void *dscale, *doffset;                      // one cluster of blocks: where it writes the weights' gradients itself
+    int* gave_up;                                // set to 1 when a bounded wait ran out; may be NULL
 };
 
 template <typename T, int VEC, int TPR, int N, bool BWD, int MINB>
@@ -119,7 +120,7 @@ ln_tile_kernel(const __grid_constant__ LnTile p) {
     constexpr bool AGAIN = N * VEC * sizeof(A) > 64;       // wide rows: 16-bit values are converted again, not kept
     extern __shared__ __align__(128) unsigned char ring[];
     __shared__ uint64_t full[LN_STAGES], empty[LN_STAGES];
-    __shared__ int abort_flag;
+    __shared__ int abort_flag, asked[LN_STAGES];           // requests of a stage
     __shared__ __align__(16) A red[4][32];
     const int tid = threadIdx.x;
     const int cols = p.cols, R = p.R;
@@ -147,6 +148,7 @@ ln_tile_kernel(const __grid_constant__ LnTile p) {
         }
     };
     auto request = [&](int64_t tile, int s) {              // one thread
+        ++asked[s];
         unsigned char* dst = ring + s * stage_bytes;
         mbar_expect_bytes(&full[s], bytes_of(tile) * (BWD ? 2 : 1));
         copy(x, p.ldx, tile, dst, &full[s]);
@@ -155,7 +157,7 @@ ln_tile_kernel(const __grid_constant__ LnTile p) {
 
     if (tid == 0) {
         abort_flag = 0;
-        for (int s = 0; s < LN_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], LN_THREADS / 32); }
+        for (int s = 0; s < LN_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], LN_THREADS / 32); asked[s] = 0; }
         mbar_init_fence();
         if (p.mode != LN_PLAIN)
             for (int s = 0; s < LN_STAGES; ++s)
@@ -198,7 +200,8 @@ ln_tile_kernel(const __grid_constant__ LnTile p) {
     int flip = 0, s = 0;
     uint32_t phase = 0;
     bool ok = true;
-    // A failed wait changes no control flow: the groups' barriers need every thread.  The results become NaN.
+    // A failed wait changes no control flow: the groups' barriers need every thread.  Its thread adds NaN to its group's
+    // sums, so the row's results and statistics become NaN whatever the others of the group have seen.
     for (int64_t tile = blockIdx.x; tile < p.n_tiles; tile += gridDim.x) {
         unsigned char* st = ring + s * stage_bytes;
         const int n = rows_of(tile);
@@ -239,7 +242,7 @@ ln_tile_kernel(const __grid_constant__ LnTile p) {
             for (int i = 0; i < N; ++i)
                 if (has(i)) px[i] = *reinterpret_cast<const P*>(sx + (t + i * TPR) * VEC);
             if constexpr (!BWD) {
-                U sum = one(0);
+                U sum = one(ok ? A(0) : A(NAN));
 #pragma unroll
                 for (int i = 0; i < N; ++i)
                     if (has(i))
@@ -257,12 +260,11 @@ ln_tile_kernel(const __grid_constant__ LnTile p) {
                             dev = fma2(d, d, dev);
                         }
                     }
-                A rstd = rsqrt_acc(group_sum1<TPR>(across(dev), red, flip) * inv_n + eps);
+                const A rstd = rsqrt_acc(group_sum1<TPR>(across(dev), red, flip) * inv_n + eps);
                 if (live && t == 0) {
                     if (p.mean) static_cast<A*>(p.mean)[row] = mean;
                     if (p.rstd) static_cast<A*>(p.rstd)[row] = rstd;
                 }
-                if (!ok) rstd = A(NAN);
 #pragma unroll
                 for (int i = 0; i < N; ++i)
                     if (has(i)) {
@@ -288,7 +290,7 @@ ln_tile_kernel(const __grid_constant__ LnTile p) {
                     if (has(i)) pg[i] = *reinterpret_cast<const P*>(sg + (t + i * TPR) * VEC);
                 const A mu = live ? __ldg(static_cast<const A*>(p.mean) + row) : A(0);
                 const A rs = live ? __ldg(static_cast<const A*>(p.rstd) + row) : A(0);
-                U s1 = one(0), s2 = one(0);
+                U s1 = one(ok ? A(0) : A(NAN)), s2 = s1;
 #pragma unroll
                 for (int i = 0; i < N; ++i)
                     if (has(i)) {
@@ -342,8 +344,10 @@ ln_tile_kernel(const __grid_constant__ LnTile p) {
         }
         if (++s == LN_STAGES) { s = 0; phase ^= 1; }
     }
+    if (!ok && p.gave_up) *p.gave_up = 1;
     if (!ok && tid == 0)                        // gave up: copies may still be on their way into this block's memory
-        for (int i = 0; i < LN_STAGES; ++i) mbar_wait(&full[i], phase, 1 << 20);
+        for (int i = 0; i < LN_STAGES; ++i)
+            if (asked[i] > 0) mbar_wait(&full[i], (asked[i] - 1) & 1, 1 << 20);
 
     if constexpr (BWD) {
         const bool whole = p.dscale || p.doffset;
@@ -506,6 +510,7 @@ struct LnArgs {
     void* partial;
     int grid;               // backward: blocks
     void *dscale, *doffset;
+    int* gave_up;
 };
 
 int sm_count() {
@@ -543,6 +548,7 @@ int ln_tile(LnArgs& a, int mode) {
     p.out = a.out; p.mean = a.mean; p.rstd = a.rstd; p.partial = a.partial;
     p.eps = a.eps;
     p.mode = mode;
+    p.gave_up = a.gave_up;
     // as many rounds of all groups as a stage holds, but no more rows than spread over all blocks
     const int64_t budget = LN_SMEM / LN_STAGES / (MINB == 2 ? 2 : 1);
     int64_t R = (budget - 32 * TENSORS - 256) / (TENSORS * pitch);
@@ -680,11 +686,10 @@ int64_t dtype_bytes(int dtype) {
 
 using namespace nnvb;
 
-extern "C" {
+namespace {
 
-int nnvb_layer_norm_forward(void* stream, int dtype, int64_t rows, int64_t cols, const void* x, int64_t ldx,
-                            const void* scale, const void* offset, double eps, void* y, int64_t ldy, void* mean,
-                            void* rstd) {
+int ln_forward(cudaStream_t st, int dtype, int64_t rows, int64_t cols, const void* x, int64_t ldx, const void* scale,
+               const void* offset, double eps, void* y, int64_t ldy, void* mean, void* rstd, int* gave_up) {
     NNVB_REQUIRE(dtype_bytes(dtype) > 0, "nnvb_layer_norm_forward: unknown element type %d", dtype);
     NNVB_REQUIRE(rows >= 0 && cols >= 1 && rows < (int64_t(1) << 31) && cols < (int64_t(1) << 31),
                  "nnvb_layer_norm_forward: bad sizes (rows=%lld, cols=%lld)", (long long)rows, (long long)cols);
@@ -693,14 +698,28 @@ int nnvb_layer_norm_forward(void* stream, int dtype, int64_t rows, int64_t cols,
     NNVB_REQUIRE(eps >= 0 && eps < 1e30, "nnvb_layer_norm_forward: eps must be finite and not negative");
     if (rows == 0) return NNVB_OK;
     NNVB_REQUIRE(x && y, "nnvb_layer_norm_forward: NULL pointer");
-    LnArgs a{static_cast<cudaStream_t>(stream), rows, cols, nullptr, x, scale, offset, 0, ldx, ldy, eps, y, mean, rstd,
-             nullptr, 0, nullptr, nullptr};
+    LnArgs a{st, rows, cols, nullptr, x, scale, offset, 0, ldx, ldy, eps, y, mean, rstd, nullptr, 0, nullptr, nullptr, gave_up};
     switch (dtype) {
         case NNVB_F64: return ln_forward_t<double>(a);
         case NNVB_F32: return ln_forward_t<float>(a);
         case NNVB_BF16: return ln_forward_t<__nv_bfloat16>(a);
         default: return ln_forward_t<__half>(a);
     }
+}
+
+}  // namespace
+
+int nnvb::layer_norm_rows(cudaStream_t st, int64_t rows, int64_t cols, const double* x, int64_t ld, const double* scale,
+                          const double* offset, double eps, double* y, int* gave_up) {
+    return ln_forward(st, NNVB_F64, rows, cols, x, ld, scale, offset, eps, y, ld, nullptr, nullptr, gave_up);
+}
+
+extern "C" {
+
+int nnvb_layer_norm_forward(void* stream, int dtype, int64_t rows, int64_t cols, const void* x, int64_t ldx,
+                            const void* scale, const void* offset, double eps, void* y, int64_t ldy, void* mean,
+                            void* rstd) {
+    return ln_forward(static_cast<cudaStream_t>(stream), dtype, rows, cols, x, ldx, scale, offset, eps, y, ldy, mean, rstd, nullptr);
 }
 
 int64_t nnvb_layer_norm_workspace(int dtype, int64_t rows, int64_t cols) {
@@ -730,7 +749,7 @@ int nnvb_layer_norm_backward(void* stream, int dtype, int64_t rows, int64_t cols
                      (long long)nnvb_layer_norm_workspace(dtype, rows, cols));
     }
     LnArgs a{st, rows, cols, dy, x, scale, nullptr, lddy, ldx, lddx, 0.0, dx, const_cast<void*>(mean),
-             const_cast<void*>(rstd), weights ? workspace : nullptr, 0, nullptr, nullptr};
+             const_cast<void*>(rstd), weights ? workspace : nullptr, 0, nullptr, nullptr, nullptr};
     switch (dtype) {
         case NNVB_F64: return ln_backward_t<double>(a, dscale, doffset);
         case NNVB_F32: return ln_backward_t<float>(a, dscale, doffset);
