@@ -191,7 +191,7 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
                     load_tile(sq + t * SM::TILE, &maps.q, DP / 64, SM::BOX, (q0 + t * ROWS) >> gs, a.qs[2] ? h : 0, a.qs[0] ? b : 0, &q_full);
             }
             int it = 0;
-            bool ok = true;
+            bool ok = true, cleared = false;
             for (int i = 0; i < steps && ok; ++i) {
                 for (int kv = 0; kv < 2; ++kv, ++it) {
                     const int s = it % STAGES;
@@ -207,6 +207,7 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
                             mbar_expect_bytes(&tail, SM::TILE);
                             load_tile(dst, &maps.v, DP / 64, SM::BOX, row, vh, vb, &tail);
                         }
+                        cleared = true;
                         ok = __all_sync(0xffffffffu, mbar_wait_fast(&tail, 0, abort));
                         for (int j = lane; j < (ROWS - rest) * 8 * (DP / 64); j += 32) {
                             const int box = j / ((ROWS - rest) * 8), r = j % ((ROWS - rest) * 8);
@@ -221,10 +222,14 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
                     }
                 }
             }
-            if (!ok && lane == 0) {            // gave up: the copies issued so far still write to this block's memory
+            // A block does not leave while a copy writes to its memory.  The products have waited for all of them, unless some
+            // warp gave up.
+            if (lane == 0 && steps > 0) {
                 mbar_wait(&q_full, 0, 1 << 20);
+                if (cleared) mbar_wait(&tail, 0, 1 << 20);
                 for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j) mbar_wait(&full[j % STAGES], (j / STAGES) & 1, 1 << 20);
             }
+            __syncwarp();
         } else if (warp == 8) {
             // ---- products -----------------------------------------------------------------------------------------
             const uint32_t leader = elect_lane();
@@ -647,8 +652,8 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
             load_tile(res + SM::ATILE, &maps.a1, DP / 64, SM::ABOX, token, as1[2] ? ah : 0, as1[0] ? b : 0, &a_full);
         }
         int it = 0;
-        bool ok = true;
-        for (; it < steps; ++it) {
+        bool ok = true, cleared = false;
+        for (; it < steps && ok; ++it) {
             const int s = it % STAGES;
             if (it >= STAGES) ok = mbar_wait_fast(&empty[s], (it / STAGES - 1) & 1, abort);
             ok = __all_sync(0xffffffffu, ok);
@@ -675,6 +680,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
                 }
             }
             if (clear) {
+                cleared = true;
                 ok = __all_sync(0xffffffffu, mbar_wait_fast(&tail, 0, abort));
                 const int pieces = KV ? 8 : (BROWS - rest) * 8;
                 for (int j = lane; j < pieces * (DP / 64); j += 32) {
@@ -686,10 +692,12 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
                 if (lane == 0) mbar_arrive(&full[s]);
             }
         }
-        if (!ok && lane == 0) {            // gave up: the copies issued so far still write to this block's memory
+        if (lane == 0 && steps > 0) {      // a block does not leave while a copy writes to its memory
             mbar_wait(&a_full, 0, 1 << 20);
+            if (cleared) mbar_wait(&tail, 0, 1 << 20);
             for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j) mbar_wait(&full[j % STAGES], (j / STAGES) & 1, 1 << 20);
         }
+        __syncwarp();
     } else if (warp == 16) {
         // ---- products -----------------------------------------------------------------------------------------
         const uint32_t leader = elect_lane();
