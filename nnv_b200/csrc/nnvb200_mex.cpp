@@ -21,6 +21,7 @@
 // mexAtExit tears it down.  MATLAB's 1-based target label becomes 0-based here.
 #include "mex.h"
 
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <string>
@@ -36,6 +37,7 @@ struct NetHandle {
     nnvb_net* net = nullptr;
     nnvb_batch* last = nullptr;   // results of the most recent reach
     int64_t shape[3] = {0, 0, 0};
+    int64_t n_in = 0;             // entries of an input
 };
 std::vector<NetHandle*> g_nets;
 
@@ -70,6 +72,16 @@ const double* field_doubles(const mxArray* s, mwIndex i, const char* name, size_
     if (!mxIsDouble(f) || mxIsComplex(f)) { e.fail("NNVB200:type", std::string(name) + " must be a real double array"); return nullptr; }
     if (n) *n = mxGetNumberOfElements(f);
     return mxGetDoubles(f);
+}
+
+// a whole number from 1 on out of a field; false (with the error set) where it is none
+bool whole(const double* v, const char* name, int32_t* out, Err& e) {
+    if (!v || !(v[0] >= 1 && v[0] <= 2147483647.0 && v[0] == std::floor(v[0]))) {
+        e.fail("NNVB200:layer", std::string(name) + " must be a whole number from 1 on");
+        return false;
+    }
+    *out = (int32_t)v[0];
+    return true;
 }
 
 void fill_ints(const double* src, size_t n, int32_t* dst, size_t want, int32_t dflt) {
@@ -142,9 +154,9 @@ void create_net(int nlhs, mxArray* plhs[], int nrhs, const mxArray* prhs[], Err&
             const double* ch = field_doubles(prhs[1], i, "NumChannels", &n, e);
             d.bn_scale = field_doubles(prhs[1], i, "Scale", &ns, e);
             d.bn_offset = field_doubles(prhs[1], i, "Offset", &no, e);
-            if (ch) d.cout = (int32_t)ch[0];
-            if (!ch || (d.bn_scale && ns != (size_t)d.cout) || (d.bn_offset && no != (size_t)d.cout)) {
-                e.fail("NNVB200:layer", "layernorm needs NumChannels, and Scale and Offset of that size"); break;
+            if (!whole(ch, "layernorm NumChannels", &d.cout, e)) break;
+            if ((d.bn_scale && ns != (size_t)d.cout) || (d.bn_offset && no != (size_t)d.cout)) {
+                e.fail("NNVB200:layer", "layernorm needs Scale and Offset of the size NumChannels"); break;
             }
             const double* eps = field_doubles(prhs[1], i, "Epsilon", &n, e);
             d.bn_eps = eps ? eps[0] : 1e-5;
@@ -153,14 +165,14 @@ void create_net(int nlhs, mxArray* plhs[], int nrhs, const mxArray* prhs[], Err&
             const mxArray* kx = mxGetField(prhs[1], i, "Keys");
             const mxArray* vx = mxGetField(prhs[1], i, "Values");
             const double* heads = field_doubles(prhs[1], i, "NumHeads", &n, e);
-            if (!kx || !vx || !heads || !mxIsDouble(kx) || !mxIsDouble(vx) ||
-                mxGetNumberOfElements(kx) != mxGetNumberOfElements(vx)) {
-                e.fail("NNVB200:layer", "attention needs NumHeads, and double Keys and Values of one size"); break;
+            const mwSize nd = kx ? mxGetNumberOfDimensions(kx) : 0;
+            const mwSize* dm = kx ? mxGetDimensions(kx) : nullptr;
+            if (!kx || !vx || !mxIsDouble(kx) || !mxIsDouble(vx) || mxIsComplex(kx) || mxIsComplex(vx) || nd > 3 ||
+                mxGetNumberOfDimensions(vx) != nd || std::memcmp(dm, mxGetDimensions(vx), nd * sizeof(mwSize)) != 0) {
+                e.fail("NNVB200:layer", "attention needs real double Keys and Values of one size [channels, heads, states]"); break;
             }
-            const mwSize nd = mxGetNumberOfDimensions(kx);
-            const mwSize* dm = mxGetDimensions(kx);
+            if (!whole(heads, "attention NumHeads", &d.kh, e)) break;
             d.cin = (int32_t)dm[0]; d.kw = (int32_t)dm[1]; d.cout = nd > 2 ? (int32_t)dm[2] : 1;
-            d.kh = (int32_t)heads[0];
             d.W = mxGetDoubles(kx); d.b = mxGetDoubles(vx);
             const double* sc = field_doubles(prhs[1], i, "AttentionScale", &n, e);
             d.bn_eps = sc ? sc[0] : 0.0;
@@ -182,6 +194,7 @@ void create_net(int nlhs, mxArray* plhs[], int nrhs, const mxArray* prhs[], Err&
             "nnvb_net_create");
     if (e.set) { delete h; return; }
     nnvb_net_out_shape(h->net, h->shape);
+    h->n_in = (int64_t)hwc[0] * (int64_t)hwc[1] * (int64_t)hwc[2];
     g_nets.push_back(h);
     if (nlhs > 0) plhs[0] = mxCreateDoubleScalar((double)g_nets.size());
 }
@@ -275,6 +288,7 @@ void evaluate(int nlhs, mxArray* plhs[], int nrhs, const mxArray* prhs[], Err& e
     NetHandle* h = get_handle(prhs[1], e);
     if (!h) return;
     const size_t n = mxGetN(prhs[2]);
+    if ((int64_t)mxGetM(prhs[2]) != h->n_in || n < 1) { e.fail("NNVB200:args", "evaluate: X must have one column per input, of as many rows as an input has entries"); return; }
     const size_t n_out = (size_t)(h->shape[0] * h->shape[1] * h->shape[2]);
     mxArray* Y = mxCreateDoubleMatrix((mwSize)n_out, (mwSize)n, mxREAL);
     e.check(nnvb_net_evaluate(h->net, (int64_t)n, mxGetDoubles(prhs[2]), mxGetDoubles(Y)), "nnvb_net_evaluate");
