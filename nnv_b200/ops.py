@@ -5,7 +5,8 @@ with their gradients.
 ``nn.AttentionLayer``; this module is for hosts that keep their tensors on the GPU (torch).  Every function
 checks its arguments (``ValueError`` / ``TypeError`` before anything is launched), allocates its outputs,
 enqueues its kernels on torch's current stream of the tensors' device and returns without waiting.  Gradients are
-explicit calls: the forward functions do not record for autograd.
+explicit calls: the forward functions do not record for autograd, and refuse tensors that require a gradient while
+it records (call them under ``torch.no_grad()``), because that gradient would be lost.
 
 Element types: float64, float32, bfloat16, float16, one type per call.  Statistics (mean, rstd, log-sum-exp) are
 float32, or float64 with float64 tensors; sums are held in that type and a result is rounded once when stored.
@@ -26,6 +27,13 @@ _entries = {}
 _DESC = struct.Struct("ii6qd15q")              # nnvb_attention_desc
 # the current stream as an address, without a Stream object per call (a fifth of a small call's host time)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _explicit(*tensors):
+    """Refuses what autograd would record: its backward pass would silently stop here."""
+    if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in tensors):
+        raise ValueError("a tensor requires a gradient, which these operators do not record for autograd: call them under "
+                         "torch.no_grad() and take the gradients from the _backward function")
 
 
 def _kind(name, t):
@@ -115,6 +123,7 @@ def layer_norm(x, scale=None, offset=None, eps=1e-5, return_stats=False):
 
     ``scale`` and ``offset`` (one entry per column) may be None.  With ``return_stats`` the rows' mean and
     1/sqrt(var + eps) come back too, shaped like ``x`` without its last dimension: what the backward call takes."""
+    _explicit(x, scale, offset)
     kind, cols = _ln_input(x)
     scale, offset = _weight("scale", scale, cols, x), _weight("offset", offset, cols, x)
     eps = float(eps)
@@ -198,6 +207,7 @@ def cross_attention(q, k, v, lengths=None, scale=None, return_lse=False):
     gives the valid states of each batch entry, clipped to 0..Lk; what the others hold has no effect.  Rows
     without a valid state are zero.  ``scale`` defaults to 1/sqrt(D).  Tensors may be strided views.  With
     ``return_lse`` the log-sum-exp [B, Hq, Lq] of each row's scores comes back too (-inf without states)."""
+    _explicit(q, k, v)
     q, k, v, lengths, head = _attn(q, k, v, lengths, scale)
     out = _like(q)
     so = out.stride()
