@@ -162,3 +162,15 @@ def test_scores_of_millions_pick_a_state(t, size, Lq, Lk):
     # m c is rounded, so the weight is not quite 1: its own rounding to 16 bits is a half step, the output's another
     near = (out.double() - want.double()).abs() <= 2.02 * R.half_step(t) * want.double().abs()
     assert (near.all(-1) | ~clear.transpose(1, 2)).all()
+
+
+@pytest.mark.parametrize("t", F16)
+@pytest.mark.parametrize("Lq,G,Lk,D", [(1, 1, 900, 64), (1, 8, 4097, 128), (4, 4, 300, 64), (3, 5, 2000, 96)])
+def test_few_rows_round_only_what_they_store(t, Lq, G, Lk, D):
+    """Weights as two 16-bit terms: one would add as much as the storage rounding (1.41 times it)."""
+    from nnv_b200 import ops
+    q, k, v, _ = _data(t, 4, Lq, Lk, 2 * G, 2, D, spread=1.5)
+    out = ops.cross_attention(q.cuda(), k.cuda(), v.cuda()).cpu()
+    p = (torch.einsum("bqhgd,bkhd->bhgqk", q.double().view(4, Lq, 2, G, D), k.double()) / math.sqrt(D)).softmax(-1)
+    want = torch.einsum("bhgqk,bkhd->bqhgd", p, v.double()).reshape(out.shape)
+    assert _error(out, want) <= LIMIT * _error(want.to(t), want)
