@@ -541,12 +541,6 @@ attn_rows_mma_kernel(AttnArgs a) {
     cluster.sync();                        // nobody leaves while its shared memory is read
 }
 
-int sm_count_now() {
-    int dev = 0, n = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    return n < 1 ? 148 : n;
-}
-
 // Blocks per state head: a power of two (others leave SMs of a cluster's group idle: 8 x 2 x 4096 x 8 x 2 x 128 float, 74 us with 8,
 // 90 with 6) up to 16, at least two blocks of states a warp, and at most a third more blocks than `per_sm` an SM: more
 // would run as a second round (16 x 1 x 2048 x 8 x 4 x 128 bf16: 36 us with 4, 30 with 2).  Sixteen blocks with a large ring
@@ -554,7 +548,7 @@ int sm_count_now() {
 template <typename K>
 int launch_rows(K kernel, cudaStream_t st, const AttnArgs& a, int keys, int per_sm, int smem) {
     const int64_t units = int64_t(a.B) * a.Hkv;
-    const int64_t sms = sm_count_now(), blocks = sms * per_sm * 4 / 3, most = ceil_div(a.Lk, keys * WARPS * 2);
+    const int64_t sms = sm_count(), blocks = sms * per_sm * 4 / 3, most = ceil_div(a.Lk, keys * WARPS * 2);
     int world = 1;
     while (world < (smem > 64 * 1024 && units * 16 > sms ? 8 : 16) && world < most && units * world * 2 <= blocks) world *= 2;
     NNVB_REQUIRE(units * world < (int64_t(1) << 31), "nnvb_cross_attention_forward: too many state heads (%lld) for one launch",

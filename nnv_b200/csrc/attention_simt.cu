@@ -525,9 +525,7 @@ constexpr int bwd_tile(int dp) {
 template <typename K>
 int launch(K kernel, int64_t units, int64_t steps, int smem, int per_sm, cudaStream_t st, const AttnArgs& a, bool vec) {
     if (units <= 0) return NNVB_OK;
-    int dev = 0, sms = 148;
-    NNVB_CUDA(cudaGetDevice(&dev));
-    NNVB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    const int sms = sm_count();
     int world = 1;
     while (world < 16 && units * world * 2 <= int64_t(sms) * per_sm && world * 4 <= steps) world *= 2;
     NNVB_REQUIRE(units * world < (int64_t(1) << 31), "nnvb_cross_attention: too many tiles (%lld) for one launch", (long long)units);
@@ -585,8 +583,9 @@ int backward_t(cudaStream_t st, const AttnArgs& a) {
 
 template <typename T>
 int by_head(cudaStream_t st, const AttnArgs& a, bool backward) {
-    if (a.D <= 64) return backward ? backward_t<T, 64>(st, a) : forward_t<T, 64>(st, a);
-    if (a.D <= 128) return backward ? backward_t<T, 128>(st, a) : forward_t<T, 128>(st, a);
+    if (a.D <= 128 && backward) return a.D <= 64 ? backward_t<T, 64>(st, a) : backward_t<T, 128>(st, a);
+    if constexpr (sizeof(T) == 2)          // float and double forward: attention_wide.cu
+        if (a.D <= 128) return a.D <= 64 ? forward_t<T, 64>(st, a) : forward_t<T, 128>(st, a);
     return backward ? backward_t<T, 256>(st, a) : forward_t<T, 256>(st, a);
 }
 

@@ -104,7 +104,7 @@ __device__ __forceinline__ void store8(T* to, const float (&x)[8]) {
 }
 
 struct TcMaps {
-    CUtensorMap q, k, v, dout;
+    CUtensorMap q, k, v;
 };
 
 // Rows of positions are those of 2^gs query heads that share a state head, heads of a position side by side: few positions
@@ -181,7 +181,7 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
     // 384 threads at 168 registers = 256 at 208 + 128 at 88: a softmax thread holds a row of 128 scores (8 x 2048 x 4096 x
     // 16 x 128: 522 us; 567 with 168 registers and the scores read twice, 550 with them spilled)
     if (warp >= 8) {
-        reg_dealloc<88>();
+        setmaxnreg_dec<88>();
         if (warp == 9) {
             // ---- copies -------------------------------------------------------------------------------------------
             const int kb = a.ks[0] ? b : 0, kh = a.ks[2] ? g : 0, vb = a.vs[0] ? b : 0, vh = a.vs[2] ? g : 0;
@@ -288,7 +288,7 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
             __syncwarp();
         }
     } else {
-        reg_alloc<208>();
+        setmaxnreg_inc<208>();
         if (warp / 4 < live) {
             // ---- softmax: one row per thread ------------------------------------------------------------------------
             const int t = warp / 4;
@@ -682,7 +682,7 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
             if (clear) {
                 cleared = true;
                 ok = __all_sync(0xffffffffu, mbar_wait_fast(&tail, 0, abort));
-                const int pieces = KV ? 8 : (BROWS - rest) * 8;
+                const int pieces = (BROWS - rest) * 8;
                 for (int j = lane; j < pieces * (DP / 64); j += 32) {
                     const int box = j / pieces, r = j % pieces;
                     *reinterpret_cast<uint4*>(dst + box * SM::BBOX + rest * 128 + r * 16) = make_uint4(0, 0, 0, 0);
@@ -998,9 +998,7 @@ bool tma_rows(const void* p, const int64_t (&s)[3], int64_t tokens) {
 // Launches `units` blocks, or clusters of up to 16 where blocks are few and walk over many tiles (`steps`).
 template <typename K, typename... Args>
 int launch_shared(K kernel, int64_t units, int64_t steps, int threads, int smem, cudaStream_t st, Args... args) {
-    int dev = 0, sms = 148;
-    NNVB_CUDA(cudaGetDevice(&dev));
-    NNVB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    const int sms = sm_count();
     int world = 1;
     const int most = units <= 4 ? 16 : 8;              // a GPC has room for one cluster of 16 such blocks
     while (world < most && units * world * 2 <= sms && world * 4 <= steps) world *= 2;

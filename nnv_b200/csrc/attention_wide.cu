@@ -555,9 +555,7 @@ bool wide_rows16(const AttnArgs& a, int64_t e, bool backward) {
 // `units` blocks, or clusters of up to 16 where blocks are few: those share the `steps` tiles a block walks over, two each at least
 template <typename K>
 int launch_wide(K kernel, int64_t units, int64_t steps, int per_sm, int smem, cudaStream_t st, const AttnArgs& a, bool vec) {
-    int dev = 0, sms = 148;
-    NNVB_CUDA(cudaGetDevice(&dev));
-    NNVB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    const int sms = sm_count();
     int world = 1;
     while (world < 16 && units * world * 2 <= int64_t(sms) * per_sm && world * 4 <= steps) world *= 2;
     // or where the last blocks would leave many SMs idle: the longest sum of an SM's blocks counts

@@ -36,6 +36,9 @@ void set_error(const char* fmt, ...);
         }                               \
     } while (0)
 
+// Multiprocessors of the current device (148 where the runtime does not tell).
+int sm_count();
+
 // Bytes of an element of an nnvb_dtype; 0 for any other value.
 int64_t dtype_bytes(int dtype);
 

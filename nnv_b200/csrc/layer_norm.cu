@@ -25,6 +25,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <atomic>
 #include <initializer_list>
 #include <type_traits>
 
@@ -111,8 +112,8 @@ struct LnTile {
     int* gave_up;                                // set to 1 when a bounded wait ran out; may be NULL
 };
 
-template <typename T, int VEC, int TPR, int N, bool BWD, int MINB>
-__global__ void __launch_bounds__(LN_THREADS, MINB)
+template <typename T, int VEC, int TPR, int N, bool BWD>
+__global__ void __launch_bounds__(LN_THREADS, 1)
 ln_tile_kernel(const __grid_constant__ LnTile p) {
     using A = typename AccOf<T>::type;
     using P = Pack<T, VEC>;
@@ -513,33 +514,21 @@ struct LnArgs {
     int* gave_up;
 };
 
-int sm_count() {
-    static int n[64] = {0};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-    if (n[dev] == 0) {
-        int v = 0;
-        if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v < 1) v = 148;
-        n[dev] = v;
-    }
-    return n[dev];
-}
-
 // Shared memory that any call may need: every stage's tiles, or a cluster's sums.  The limit of a kernel belongs to the
 // process, so every call sets this value; with its own need, a call with few rows could lower the limit between another
 // thread's setting and its launch.
 constexpr int LN_SMEM = 200 * 1024;
 
-constexpr int LN_MAX_PARTS = 2 * 148;        // partial rows of the weights' gradients: blocks that fit at once
+constexpr int LN_MAX_PARTS = 2 * 148;        // partial rows of the weights' gradients: the most slices of rows (wide rows)
 
 // Backward of tensors up to this size runs in one cluster: its 16 SMs take about as long as a second launch does.
 bool ln_in_cluster(int64_t rows, int64_t cols) { return rows * cols <= 512 * 1024 && cols <= 4096; }
 
-template <typename T, int VEC, int TPR, int N, bool BWD, int MINB>
+template <typename T, int VEC, int TPR, int N, bool BWD>
 int ln_tile(LnArgs& a, int mode) {
     constexpr int GROUPS = LN_THREADS / TPR, TENSORS = BWD ? 2 : 1;
     const bool cluster = BWD && (a.dscale || a.doffset) && ln_in_cluster(a.rows, a.cols);
-    const int64_t slots = cluster ? 16 : std::min(sm_count(), 148) * MINB;
+    const int64_t slots = cluster ? 16 : std::min(sm_count(), 148);
     const int64_t pitch = a.cols * int64_t(sizeof(T));
     LnTile p{};
     p.rows = a.rows; p.cols = int(a.cols);
@@ -550,7 +539,7 @@ int ln_tile(LnArgs& a, int mode) {
     p.mode = mode;
     p.gave_up = a.gave_up;
     // as many rounds of all groups as a stage holds, but no more rows than spread over all blocks
-    const int64_t budget = LN_SMEM / LN_STAGES / (MINB == 2 ? 2 : 1);
+    const int64_t budget = LN_SMEM / LN_STAGES;
     int64_t R = (budget - 32 * TENSORS - 256) / (TENSORS * pitch);
     R = std::min<int64_t>(R, ceil_div(a.rows, slots));
     R = R >= GROUPS ? R / GROUPS * GROUPS : std::max<int64_t>(R, 1);
@@ -561,7 +550,7 @@ int ln_tile(LnArgs& a, int mode) {
     const int sums = BWD ? (LN_THREADS * VEC + (cluster ? 2 * p.cols : 0)) * int(sizeof(A)) : 0;
     const int smem = std::max<int>(LN_STAGES * p.tensor_bytes * TENSORS, sums);
     a.grid = int(std::min<int64_t>(p.n_tiles, slots));
-    auto kernel = ln_tile_kernel<T, VEC, TPR, N, BWD, MINB>;
+    auto kernel = ln_tile_kernel<T, VEC, TPR, N, BWD>;
     NNVB_REQUIRE(smem <= LN_SMEM, "nnvb_layer_norm: rows of %lld columns need %d bytes of shared memory", (long long)a.cols, smem);
     NNVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LN_SMEM));
     if (cluster) {
@@ -592,20 +581,19 @@ int ln_tile(LnArgs& a, int mode) {
 template <typename T, int VEC, bool BWD>
 int ln_by_width(LnArgs& a, int mode, bool* done) {
     constexpr int E = sizeof(T) == 8 ? 8 : 16, N = E / VEC;
-    constexpr int M = 1;
     const int64_t c = a.cols;
     *done = true;
-    if (c <= 8 * E / 2) return ln_tile<T, VEC, 8, N / 2, BWD, M>(a, mode);
-    if (c <= 8 * E) return ln_tile<T, VEC, 8, N, BWD, M>(a, mode);
-    if (c <= 32 * E / 2) return ln_tile<T, VEC, 32, N / 2, BWD, M>(a, mode);
-    if (c <= 32 * E) return ln_tile<T, VEC, 32, N, BWD, M>(a, mode);
-    if (c <= 64 * E) return ln_tile<T, VEC, 64, N, BWD, M>(a, mode);
-    if (c <= 128 * E) return ln_tile<T, VEC, 128, N, BWD, M>(a, mode);
-    if (c <= 256 * E) return ln_tile<T, VEC, 256, N, BWD, M>(a, mode);
-    if (c <= 512 * E) return ln_tile<T, VEC, 512, N, BWD, M>(a, mode);
+    if (c <= 8 * E / 2) return ln_tile<T, VEC, 8, N / 2, BWD>(a, mode);
+    if (c <= 8 * E) return ln_tile<T, VEC, 8, N, BWD>(a, mode);
+    if (c <= 32 * E / 2) return ln_tile<T, VEC, 32, N / 2, BWD>(a, mode);
+    if (c <= 32 * E) return ln_tile<T, VEC, 32, N, BWD>(a, mode);
+    if (c <= 64 * E) return ln_tile<T, VEC, 64, N, BWD>(a, mode);
+    if (c <= 128 * E) return ln_tile<T, VEC, 128, N, BWD>(a, mode);
+    if (c <= 256 * E) return ln_tile<T, VEC, 256, N, BWD>(a, mode);
+    if (c <= 512 * E) return ln_tile<T, VEC, 512, N, BWD>(a, mode);
     // the ring holds a row per stage at least
     const int64_t row = round_up(c * int64_t(sizeof(T)) + 32, 128) * (BWD ? 2 : 1);
-    if (c <= 512 * 2 * E && row * LN_STAGES <= LN_SMEM) return ln_tile<T, VEC, 512, 2 * N, BWD, M>(a, mode);
+    if (c <= 512 * 2 * E && row * LN_STAGES <= LN_SMEM) return ln_tile<T, VEC, 512, 2 * N, BWD>(a, mode);
     *done = false;
     return NNVB_OK;
 }
@@ -672,6 +660,18 @@ int ln_backward_t(LnArgs a, void* dscale, void* doffset) {
 }
 
 }  // namespace
+
+int sm_count() {
+    static std::atomic<int> known[64];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    n = known[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) n = 148;
+        known[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
 
 int64_t dtype_bytes(int dtype) {
     switch (dtype) {

@@ -87,9 +87,6 @@ __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* r) {
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
-// Registers of a warpgroup's threads, moved within what the block was launched with: every warp of the group calls it.
-template <int N> __device__ __forceinline__ void reg_alloc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" : : "n"(N)); }
-template <int N> __device__ __forceinline__ void reg_dealloc() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" : : "n"(N)); }
 
 // The registers of a load hold their values from this wait on: they pass through it, so that no use moves in front of it.
 __device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[32]) {
@@ -167,9 +164,6 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
             smem_u32(dst)),
         "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
         : "memory");
-}
-__device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) {
-    asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory");
 }
 
 }  // namespace nnvb
