@@ -804,14 +804,24 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
             for (int e = 0; e < 32; e += 2) {
                 const Pair<float> lse = KV ? *reinterpret_cast<const Pair<float>*>(sl + e) : both(my_lse);
                 const Pair<float> x = fma2({__uint_as_float(s[e]), __uint_as_float(s[e + 1])}, both(c), {-lse.x, -lse.y});
-                s[e] = __float_as_uint(!KV && e >= rest ? 0.f : ex2(x.x));
-                s[e + 1] = __float_as_uint(!KV && e + 1 >= rest ? 0.f : ex2(x.y));
+                s[e] = __float_as_uint(ex2(x.x));
+                s[e + 1] = __float_as_uint(ex2(x.y));
+            }
+            if (!KV && rest < 32) {                        // the last tile: S and dP may hold anything there
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    if (e >= rest) s[e] = 0;
             }
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 uint32_t d[16], p[8], hi[8], lo[8];
                 tmem_load16(d, d_at + g * 16);
                 tmem_wait_load(d);
+                if (!KV && rest < 32) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (g * 16 + e >= rest) d[e] = 0;
+                }
 #pragma unroll
                 for (int e = 0; e < 16; e += 2) {
                     const int col = g * 16 + e;
@@ -820,8 +830,6 @@ attn_bwd_tc_kernel(const __grid_constant__ BwdMaps maps, AttnArgs a, int RowsP, 
                     // dl: fp16: delta times the factor
                     const Pair<float> dl = KV ? *reinterpret_cast<const Pair<float>*>(sl + BROWS + col) : both(up_delta);
                     Pair<float> ds = mul2(pv, SCALED ? fma2(dp, both(up), Pair<float>{-dl.x, -dl.y}) : add2(dp, Pair<float>{-dl.x, -dl.y}));
-                    if (!KV && col >= rest) ds.x = 0.f;                    // dP there may be 0 * NaN
-                    if (!KV && col + 1 >= rest) ds.y = 0.f;
                     if (!KV) miss = add2(miss, ds);
                     p[e / 2] = pack2<T>(pv.x, pv.y);
                     hi[e / 2] = pack2<T>(ds.x, ds.y);
