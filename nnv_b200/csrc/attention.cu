@@ -118,7 +118,7 @@ int nnvb_cross_attention_backward(void* stream, const nnvb_attention_desc* d, co
     a.dout = dout; a.q = q; a.k = k; a.v = v; a.o = out; a.lse = const_cast<void*>(lse); a.lengths = lengths;
     a.dq = dq; a.dk = dk; a.dv = dv; a.delta = workspace;
     if (attn_tc_takes_backward(a)) return attn_backward_tc(st, a);
-    if (a.dtype == NNVB_F64 || a.dtype == NNVB_F32) NNVB_TRY(attn_delta(st, a));
+    NNVB_TRY(attn_delta(st, a));
     // Large problems have the wide kernels' throughput (8 x 512 x 1024 x 8 x 64 double: 1.5 against 2.5 ms; 8 x 1024 x 2048 x 16 x
     // 64 float: 6.3 against 7.4 ms).  Where one side is short, or tiles are fewer than the SMs need, the blocks of twice as many
     // threads on smaller tiles are the faster ones (2 x 3582 x 8 x 8 x 4 x 64 double: 0.79 against 0.94 ms).  More than 64

@@ -48,6 +48,6 @@ bool attn_tc_takes_forward(const AttnArgs& a);
 int attn_forward_tc(cudaStream_t st, const AttnArgs& a);
 bool attn_tc_takes_backward(const AttnArgs& a);
 int attn_backward_tc(cudaStream_t st, const AttnArgs& a);
-int attn_delta(cudaStream_t st, const AttnArgs& a);               // float and double
+int attn_delta(cudaStream_t st, const AttnArgs& a);
 
 }  // namespace nnvb
