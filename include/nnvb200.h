@@ -444,7 +444,10 @@ int nnvb_estimate_ranges_noalloc(void* stream, int64_t N, int64_t P, const doubl
  * `dtype` is the element type of every tensor of a call except the statistics
  * (mean, rstd, lse), which are float for the 16- and 32-bit types and double for
  * NNVB_F64.  Sums are held in the type of the statistics; a result is rounded
- * once when it is stored. */
+ * once when it is stored.  16-bit attention on the tensor cores (head sizes a
+ * multiple of 8 up to 128, 16-byte aligned rows) also rounds the weights P once to
+ * the tensors' type: before they meet V where a state head has more than 16 rows,
+ * and before they meet dO in the gradient dv. */
 typedef enum { NNVB_F64 = 0, NNVB_F32 = 1, NNVB_BF16 = 2, NNVB_F16 = 3 } nnvb_dtype;
 
 /* y = (x - mean) * rstd * scale + offset for each of `rows` rows of `cols`

@@ -17,8 +17,9 @@
 // row sum is added in fp32 before the rounding.  fp16 P carries a factor 2^7, up to the type's end: without it weights
 // below 2^-14 lose bits, which shows where one state outweighs the others and its V does not matter.
 //
-// Bound by the products at long lengths: Q K^T reads both operands from shared memory, 8 KB for each 64 cycles of the
-// tensor pipe, all that shared memory delivers.  8 x 2048 x 4096 x 16 x 128 bf16: 509 us, 1.08 PFLOP/s.
+// At long lengths the tensor pipe and shared memory need 1024 cycles each for a tile of states (Q K^T reads 8 KB for each 64
+// cycles of the pipe, all that shared memory delivers), and each is busy 0.61 of the time while all SMs have blocks; the
+// rest goes to the hand-overs between products and exponentials.  8 x 2048 x 4096 x 16 x 128 bf16: 525 us, 1.05 PFLOP/s.
 //
 // A block takes an SM's registers whole (the backward kernels 55 of 64 K), so no other block of this kind waits for its
 // tensor memory while it waits for the rest of its cluster.
@@ -40,8 +41,8 @@ namespace {
 constexpr int ROWS = 128;                          // rows of a tile of positions, states of a tile
 constexpr int FWD_THREADS = 384;
 constexpr int EMULATED = 4;                        // of 16 exponentials run on the FMA pipe (0: 44.7 us, 2: 43.5, 4: 42.7,
-                                                   // 6: 45.9 at 8 x 1024 x 1024 x 8 x 128; 511, 509, 509, 520 at
-                                                   // 8 x 2048 x 4096 x 16 x 128, where the products bound)
+                                                   // 6: 45.9 at 8 x 1024 x 1024 x 8 x 128; within 2 % of one another
+                                                   // at 8 x 2048 x 4096 x 16 x 128)
 
 template <typename T> constexpr bool is_bf16 = false;
 template <> constexpr bool is_bf16<__nv_bfloat16> = true;
@@ -179,7 +180,7 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
     volatile int* abort = &abort_flag;
 
     // 384 threads at 168 registers = 256 at 208 + 128 at 88: a softmax thread holds a row of 128 scores (8 x 2048 x 4096 x
-    // 16 x 128: 522 us; 567 with 168 registers and the scores read twice, 550 with them spilled)
+    // 16 x 128: with 168 registers 9 % slower and the scores read twice, 5 % slower with them spilled)
     if (warp >= 8) {
         setmaxnreg_dec<88>();
         if (warp == 9) {
@@ -463,8 +464,9 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
 //            S^T = K Q^T,  dP^T = V dO^T,  dV += P^T dO,  dK += dS^T Q
 // so each gradient row is summed in tensor memory by one block, in a fixed order.  Separate passes compute S and dP
 // twice: eight products a pair instead of the five of one pass that would add to dQ atomically, ten with the second terms of
-// dS.  Bound by the products and the shared memory that feeds them: 4 x 2048 x 2048 x 16 x 128 bf16, 680 us, 0.51 PFLOP/s
-// counted as five products, 1.0 as the ten that run.
+// dS.  A streamed tile of 64 rows of 128 channels takes 1280 cycles of the tensor pipe and moves 176 KB through shared memory,
+// 1375 cycles; the pipe is busy 0.60 of the time in both passes.  4 x 2048 x 2048 x 16 x 128 bf16: 650 us, 0.53 PFLOP/s
+// counted as five products, 1.06 as the ten that run.
 //
 // Streamed tiles have 64 rows, which lets two of them be in flight in tensor memory beside 128 x 128 accumulators;
 // they serve as K-major operand of S and dP and as MN-major operand of the gradients.  Sixteen warps do the softmax
@@ -476,8 +478,8 @@ attn_fwd_tc_kernel(const __grid_constant__ TcMaps maps, AttnArgs a, int gs) {
 // divided by it again.  With two terms that leaves 2^-40 of the bound.  dQ takes the norm of 16 of its rows of dO, dK of all.
 //
 // Roundings: P is rounded to the tensors' type, as in the forward pass.  dS enters its product as the sum of two
-// 16-bit values (its rounding and the rounding of what is left), an eighth and a ninth product: its rounding error
-// would be as large as that of storing dQ and dK, and the terms of dS cancel in their row sums.  delta comes from the
+// 16-bit values (its rounding and the rounding of what is left): its rounding error would be as large as that of storing dQ
+// and dK, and the terms of dS cancel in their row sums.  delta comes from the
 // stored output (delta0), and where a row's weight lies on a few states its rounding is larger than dP - delta: the error
 // of dq would be 7.2e-3 instead of 1.7e-3 for bf16 queries of 16 sigma over 129 states.  So the dQ pass sums what dS with
 // delta0 misses, e = sum_j P (dP - delta0), takes it back as dQ - e W at its end and leaves delta0 + e for the

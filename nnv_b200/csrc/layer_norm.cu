@@ -4,7 +4,7 @@
 //   backward  g = dy * scale,   dx = r (g - mean_j g - z mean_j(g z)),
 //             dscale = sum_rows dy z,   doffset = sum_rows dy
 //
-// Both directions are bound by memory: forward reads x and writes y, backward reads x and dy and writes dx.  So the rows
+// Both directions have memory as their floor: forward reads x and writes y, backward reads x and dy and writes dx.  So the rows
 // pass through shared memory: blocks stay on the SMs and walk over tiles of rows, and the copy engine (cp.async.bulk)
 // keeps the tiles ahead on their way while a tile is worked on, whatever the arithmetic waits for.  A tile of dense rows
 // is one copy, so rows of any width move at full speed; rows that are not whole 16-byte pieces are only read element by
@@ -20,7 +20,8 @@
 // cluster of up to 16 blocks, which adds its blocks' sums in distributed shared memory: one launch and no workspace.
 // Sums are held in float (double for double).
 //
-// 16384 x 8192 bf16: forward 133 us (4.0 TB/s), backward 189 us (4.3 TB/s); 197000 x 192 double: forward 106 us (5.7 TB/s; a copy
+// Double reaches that floor; in 16 bits a wide row's sums in series are the bound, with one row in work an SM (HBM at 0.44 of
+// its nominal peak, 1.9 instructions a cycle).  16384 x 8192 bf16: forward 133 us (4.0 TB/s), backward 189 us (4.3 TB/s); 197000 x 192 double: forward 106 us (5.7 TB/s; a copy
 // has 6.55).  8 x 768 bf16: 10 us a call, the issue from the host.
 #include <cooperative_groups.h>
 

@@ -10,6 +10,8 @@ it records (call them under ``torch.no_grad()``), because that gradient would be
 
 Element types: float64, float32, bfloat16, float16, one type per call.  Statistics (mean, rstd, log-sum-exp) are
 float32, or float64 with float64 tensors; sums are held in that type and a result is rounded once when stored.
+16-bit attention of more than a few rows also rounds the softmax weights once, before they meet v, or dout in the
+gradient dv.  A row whose valid scores are all -inf is NaN; float16 takes scores up to 2^25 in magnitude.
 """
 from __future__ import annotations
 
