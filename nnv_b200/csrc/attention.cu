@@ -86,8 +86,8 @@ int64_t nnvb_cross_attention_workspace(const nnvb_attention_desc* d) {
     // delta, and for the tensor cores the log-sum-exp beside it, in rows padded to a tile
     const int64_t rows = d->batch * d->q_heads * round_up(d->q_len, 64), stats = rows * 8;
     if (d->dtype != NNVB_F16 || d->kv_heads < 0 || d->kv_len < 0) return stats;
-    // the norms that bound dS: of dO's rows and of V's states, one of 16
-    return stats + round_up((rows / 16 + d->batch * d->kv_heads * ceil_div(d->kv_len, 16)) * 4, 16);
+    // the norms that bound dS: of dO's rows, one of 16, and of V's states
+    return stats + round_up((rows / 16 + d->batch * d->kv_heads * ceil_div(d->kv_len, V_CHUNK)) * 4, 16);
 }
 
 int nnvb_cross_attention_backward(void* stream, const nnvb_attention_desc* d, const void* dout, const void* q,

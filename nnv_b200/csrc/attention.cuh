@@ -32,6 +32,8 @@ __device__ __forceinline__ double exp_acc(double x) { return exp2(x); }
 __device__ __forceinline__ float log_acc(float x) { return logf(x); }
 __device__ __forceinline__ double log_acc(double x) { return log(x); }
 
+constexpr int V_CHUNK = 64;                        // fp16 backward: states whose largest norm is kept
+
 constexpr double LOG2E = 1.4426950408889634074;
 
 // any type, head size up to 256, any strides

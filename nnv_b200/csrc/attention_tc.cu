@@ -502,8 +502,6 @@ struct BwdMaps {
     CUtensorMap a0, a1, b0, b1;
 };
 
-constexpr int V_CHUNK = 64;                        // states whose largest norm is kept
-
 // The largest of a block's 16 values, which 16 lanes each hold.
 __device__ __forceinline__ void block_largest(float s, float* to) {
     __shared__ float part[8];

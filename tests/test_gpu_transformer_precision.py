@@ -174,3 +174,29 @@ def test_few_rows_round_only_what_they_store(t, Lq, G, Lk, D):
     p = (torch.einsum("bqhgd,bkhd->bhgqk", q.double().view(4, Lq, 2, G, D), k.double()) / math.sqrt(D)).softmax(-1)
     want = torch.einsum("bhgqk,bkhd->bqhgd", p, v.double()).reshape(out.shape)
     assert _error(out, want) <= LIMIT * _error(want.to(t), want)
+
+
+def test_half_precision_backward_captured_twice():
+    """Two graphs with a workspace each, replayed in turn on inputs whose size changes between replays."""
+    from nnv_b200 import ops
+    q, k, v, dout = _data(torch.float16, 2, 200, 400, 4, 2, 64, spread=2.0)
+    q, k, v, dout = q.cuda(), k.cuda(), v.cuda(), dout.half().cuda()
+    graphs = []
+    for i in range(2):
+        q_, d_ = q.clone(), dout.clone()
+        ops.cross_attention(q_, k, v)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out, lse = ops.cross_attention(q_, k, v, return_lse=True)
+            grads = ops.cross_attention_backward(d_, q_, k, v, out, lse)
+        graphs.append((graph, q_, d_, grads))
+    for size in (1.0, 2.0 ** -12, 2.0 ** 9):
+        for i, (graph, q_, d_, grads) in enumerate(graphs):
+            d_.copy_(dout * size * (i + 1))
+            graph.replay()
+        torch.cuda.synchronize()
+        for graph, q_, d_, grads in graphs:
+            out, lse = ops.cross_attention(q_, k, v, return_lse=True)
+            assert all(torch.equal(a, b) for a, b in zip(grads, ops.cross_attention_backward(d_, q_, k, v, out, lse)))
+            assert all(g.isfinite().all() and g.any() for g in grads)
